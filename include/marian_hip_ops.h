@@ -2,7 +2,7 @@
  * marian_hip_ops.h - C ABI of the float32 operators that sit between the int8 GEMMs of a
  * transformer decode step (same library and conventions as marian_hip_int8.h: device pointers,
  * caller-owned buffers, nothing retained, work enqueued on `stream`, status codes, no
- * synchronisation).  All tensors are dense row-major fp32; pointers need 4-byte alignment only
+ * synchronisation).  Tensors are dense row-major fp32 where nothing else is said; pointers need 4-byte alignment only
  * (16-byte aligned rows take a vector path).  In-place operation (out == in) is allowed for
  * layer_norm, softmax and logsoftmax.
  */
@@ -282,6 +282,155 @@ int marian_hip_logsoftmax_nbest_beams(const float* logits, const float* rowAdd, 
  * function here it does not synchronise; the C++ wrapper adds the reference's stream synchronisation.
  */
 int marian_hip_fill(void* begin, int64_t count, int elem_bytes, uint64_t pattern, void* stream);
+
+/*
+ * Keys and values in 8 bits: rotary positions, a cache that is quantized as it is written, and attention over it
+ * for single tokens, chains and trees of drafted ones.  No counterpart in the reference, whose decoder state is
+ * float32 (src/models/transformer.h:683-700) and whose positions are added to the embeddings.
+ *
+ * Activations are float32, float16 or bfloat16 ("type"), [sequences, heads, n, dk] with the values between two
+ * sequences, heads and positions given (three strides, in values, whole multiples of 16 bytes), so that rows of an
+ * affine call are read as they are.  16-byte aligned; dk a multiple of 16 from 16 to 256.
+ */
+#define MARIAN_HIP_FLOAT32 0
+#define MARIAN_HIP_FLOAT16 1
+#define MARIAN_HIP_BFLOAT16 2
+
+/*
+ * The cache: for each of sequences * heads entries `capacity` rows of dk codes and a float32 scale each, dense:
+ * k, v: [sequences, heads, capacity, dk], k_scale, v_scale: [sequences, heads, capacity].  A value is code * scale.
+ *   MARIAN_HIP_CACHE_INT8: codes are whole numbers -127 .. 127, scale = largest magnitude of the row / 127;
+ *   MARIAN_HIP_CACHE_E4M3: codes are floats of 4 exponent and 3 mantissa bits up to 448, scale = largest / 448.
+ * A code is the exact quotient value * 127 / largest (448) rounded to the nearest, ties to even.  A row of zeros
+ * has scale 0.  A row that holds an infinity or NaN has zeros for codes and a NaN scale: everything that reads it
+ * is NaN, and nothing that does not read it.
+ *   heads <= 4096, sequences <= 65535, capacity * dk < 2^31; k and v 16-byte, scales 4-byte aligned.
+ */
+#define MARIAN_HIP_CACHE_INT8 0
+#define MARIAN_HIP_CACHE_E4M3 1
+typedef struct marian_hip_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t sequences, heads, capacity, dk;
+  int format;
+} marian_hip_kv_cache;
+
+/*
+ * The new tokens of a step: n for each sequence.
+ *   lens: int32 [sequences] on the device, the positions of each sequence that are settled already (values outside
+ *   0 .. capacity are taken as the nearer end).  New token i of sequence s has row lens[s] + i of the cache.
+ *   counts: null, or int32 [sequences]: only the first counts[s] of the n are there (0 .. n; others are taken as the
+ *   nearer end).
+ *   parents: null - the new tokens follow one another (a prompt, or one token) - or int32 [sequences, n]: a tree of
+ *   drafted tokens, n <= MARIAN_HIP_TREE_MAX.  parents[s, i] is the drafted token that token i continues, or -1: the
+ *   last settled one.  A parent does not come behind its child: a value at or past i, or below -1, stands for -1.
+ */
+#define MARIAN_HIP_TREE_MAX 64
+typedef struct marian_hip_drafts {
+  const int32_t* lens;
+  const int32_t* counts;
+  const int32_t* parents;
+  int64_t n;
+} marian_hip_drafts;
+
+/*
+ * Rotary positions: the first `dims` values of a row (a multiple of 8, up to dk) are dims / 2 pairs, pair p being
+ * values (p, p + dims / 2), or (2 p, 2 p + 1) where interleaved; at position t it is turned by t * turns[p] * 2^-64
+ * whole turns and multiplied by magnitude:
+ *   (a, b) -> magnitude * (a cos - b sin, a sin + b cos).
+ * Turns are whole numbers mod 2^64, so the angle of a far position is as exact as that of a near one.
+ *   turns: uint64 [dims / 2] on the device, made by marian_hip_rotary_turns on the host.
+ */
+typedef struct marian_hip_rotation {
+  const uint64_t* turns;
+  int64_t dims;
+  double magnitude;
+  int interleaved;
+} marian_hip_rotation;
+
+/*
+ * The turns of a model: pair p turns by base^(-2 p / dims) radians a position, changed for contexts `factor` times
+ * as long as the model was made for:
+ *   MARIAN_HIP_ROTARY_LINEAR: all divided by factor;
+ *   MARIAN_HIP_ROTARY_BASE: base * factor^(dims / (dims - 2)) in place of base;
+ *   MARIAN_HIP_ROTARY_BANDS: pairs that turn less than `slow` times in `original` positions are divided by factor, those
+ *   that turn more than `fast` times stay, between them a linear mixture (Peng et al., "YaRN", 2023); magnitude
+ *   0.1 ln(factor) + 1.
+ * host_turns: dims / 2 values in HOST memory; host_magnitude: one.  No HIP call is made.
+ * base > 1, factor >= 1; BASE: dims >= 4; BANDS: original >= 1, 0 <= slow < fast.
+ */
+#define MARIAN_HIP_ROTARY_PLAIN 0
+#define MARIAN_HIP_ROTARY_LINEAR 1
+#define MARIAN_HIP_ROTARY_BASE 2
+#define MARIAN_HIP_ROTARY_BANDS 3
+int marian_hip_rotary_turns(uint64_t* host_turns, double* host_magnitude, int64_t dims, double base, int scaling,
+                            double factor, int64_t original, double slow, double fast);
+
+/*
+ * out = x turned by its positions: x and out [sequences, heads, n, dk].
+ *   positions: int32 on the device: [sequences], row i of a sequence being at positions[s] + i, or, with
+ *   each != 0, [sequences, n].  Positions may be negative.
+ * out is x itself (same strides), or shares no memory with it (MARIAN_HIP_ERR_ALIAS).
+ */
+int marian_hip_rotary(const void* x, const int64_t* x_strides, void* out, const int64_t* out_strides, int type,
+                      int64_t sequences, int64_t heads, int64_t n, int64_t dk, const int32_t* positions, int each,
+                      const marian_hip_rotation* rotation, void* stream);
+
+/*
+ * Writes the keys and values of the new tokens into the cache, in one launch with the rotation of keys and queries:
+ *   k, v: [sequences, heads, n, dk]; rotation: null, or what k (and q) is turned by, token i of sequence s standing at
+ *   position lens[s] + the number of drafted tokens it descends from (a chain: lens[s] + i).
+ *   q: null, or queries [sequences, q_heads, n, dk], turned the same way into q_out (q itself with the same strides, or
+ *   apart from all else); without a rotation they are copied.  Rows of q_out at or past counts[s] are zeros.
+ * Keys are turned in 64-bit arithmetic, rounded to float32 and quantized.  Rows of the cache other than those
+ * of the counts[s] new tokens, and of tokens that do not fit (at or past capacity, which are dropped), stay as they are.
+ * lens, counts and parents are only read.
+ */
+int marian_hip_cache_append(const marian_hip_kv_cache* cache, const marian_hip_drafts* drafts, const void* k,
+                            const int64_t* k_strides, const void* v, const int64_t* v_strides, int type,
+                            const marian_hip_rotation* rotation, const void* q, const int64_t* q_strides, int64_t q_heads,
+                            void* q_out, const int64_t* q_out_strides, void* stream);
+
+/*
+ * Reads rows of the cache back: k_out, v_out [sequences, heads, n, dk], dense, of `type`; row i is position
+ * first[s] + i (first: int32 [sequences] on the device).  Positions outside 0 .. capacity give zeros.
+ */
+int marian_hip_cache_read(const marian_hip_kv_cache* cache, const int32_t* first, int64_t n, void* k_out, void* v_out,
+                          int type, void* stream);
+
+/*
+ * Attention of the new tokens over the cache they have been written to: q and out [sequences, q_heads, n, dk],
+ * q_heads a multiple of the cache's heads (query head h reads head h / (q_heads / heads)):
+ *   out = softmax(scale * q . key) value
+ * over the settled positions of the sequence, the token itself and the drafted tokens it descends from.
+ * Positions that a token does not see are not read into its result, whatever they hold.  A token that sees nothing (it
+ * and all before it past the capacity) gives zeros, and so do rows at or past counts[s].  out shares no memory with q
+ * or the cache.  scale: finite, above zero.
+ * Products and sums are float32.  Of float16 and bfloat16 queries, weights enter the product with the values in
+ * 11 bits, of float32 ones in 22, relative to the largest weight times scale of value of a tile; the sum of the weights is exact.
+ * A sequence's positions are split over workgroups where there are few of them, by the lengths of all
+ * sequences: the last bits of a result depend on the batch it is in, and not on the order of anything.
+ *   workspace: at least marian_hip_cache_attention_workspace_bytes(...) bytes, 256-byte aligned (0 bytes: may be
+ *   null), which marian_hip_cache_attention_workspace_init clears once after allocating (a kernel: it may be
+ *   recorded).  One workspace serves one stream, like that of marian_hip_nbest_beams.
+ */
+size_t marian_hip_cache_attention_workspace_bytes(int64_t sequences, int64_t heads, int64_t q_heads, int64_t n, int64_t dk);
+int marian_hip_cache_attention_workspace_init(void* workspace, size_t workspace_bytes, void* stream);
+int marian_hip_cache_attention(const marian_hip_kv_cache* cache, const marian_hip_drafts* drafts, const void* q,
+                               const int64_t* q_strides, int64_t q_heads, int type, float scale, void* out,
+                               const int64_t* out_strides, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The accepted ones of the drafted tokens become settled: for j < accepted[s] the keys and values of drafted token
+ * path[s, j] move to row lens[s] + j, all of a sequence read before any is written.
+ *   path: int32 [sequences, path_len], path_len <= MARIAN_HIP_TREE_MAX; accepted: int32 [sequences], taken into
+ *   0 .. path_len.  A path entry below 0, or whose row is past the capacity, moves nothing.
+ *   new_lens: int32 [sequences], apart from lens: min(lens[s] + accepted[s], capacity).
+ */
+int marian_hip_cache_keep(const marian_hip_kv_cache* cache, const int32_t* lens, const int32_t* path, int64_t path_len,
+                          const int32_t* accepted, int32_t* new_lens, void* stream);
 
 #ifdef __cplusplus
 }

@@ -82,7 +82,32 @@ SIGNATURES = {
     "marian_hip_attention_rows": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f, _vp, _vp]),
     "marian_hip_attention_cached": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
                                          _f, _vp, _vp, _vp, _vp]),
+    "marian_hip_rotary_turns": (_i, [_vp, _vp, _i64, _c.c_double, _i, _c.c_double, _i64, _c.c_double, _c.c_double]),
+    "marian_hip_rotary": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _vp, _i, _vp, _vp]),
+    "marian_hip_cache_append": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i64, _vp, _vp, _vp]),
+    "marian_hip_cache_read": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _vp]),
+    "marian_hip_cache_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "marian_hip_cache_attention_workspace_init": (_i, [_vp, _sz, _vp]),
+    "marian_hip_cache_attention": (_i, [_vp, _vp, _vp, _vp, _i64, _i, _f, _vp, _vp, _vp, _sz, _vp]),
+    "marian_hip_cache_keep": (_i, [_vp, _vp, _vp, _i64, _vp, _vp, _vp]),
 }
+
+
+class KvCache(_c.Structure):
+    """marian_hip_kv_cache"""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("sequences", _i64), ("heads", _i64), ("capacity", _i64),
+                ("dk", _i64), ("format", _i)]
+
+
+class Drafts(_c.Structure):
+    """marian_hip_drafts"""
+    _fields_ = [("lens", _vp), ("counts", _vp), ("parents", _vp), ("n", _i64)]
+
+
+class Rotation(_c.Structure):
+    """marian_hip_rotation"""
+    _fields_ = [("turns", _vp), ("dims", _i64), ("magnitude", _c.c_double), ("interleaved", _i)]
+
 
 # include/marian_hip_int8_tuning.h (tuning build only)
 TUNING_SIGNATURES = {

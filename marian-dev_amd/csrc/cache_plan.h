@@ -1,0 +1,47 @@
+// How marian_hip_cache_attention deals its rows and positions to workgroups (host code, no HIP).
+#pragma once
+
+#include <stdint.h>
+
+#include <algorithm>
+
+namespace marian_hip {
+
+constexpr int kCacheBlock = 128;        // positions that a workgroup's four waves take in one turn
+constexpr int kCacheWorkgroups = 1024;  // what the positions of few rows are split for: four to a CU
+
+struct CacheAttentionPlan {
+  int dp;              // values of a row as the kernel holds it: dk rounded up to 64, 128 or 256
+  int qt;              // sixteens of query rows to a workgroup
+  int64_t row_tiles;   // workgroups that share an entry's positions
+  int64_t target;      // parts that the positions of all sequences together are split into
+  int64_t items;       // the most parts there can be, a sequence having at least one
+  int64_t slots;       // the most parts of sequences that have more than one: these leave partial results
+  int64_t grid;
+  int64_t row_floats;  // of a partial result: dp values and the logarithm of the sum of its weights
+};
+
+// A part is a whole number of blocks of positions, as many as all sequences have divided by target: then the parts of the
+// sequences that have several are less than 2 * target, whatever the lengths.
+inline CacheAttentionPlan cache_attention_plan(int64_t sequences, int64_t heads, int64_t q_heads, int64_t n, int64_t dk) {
+  CacheAttentionPlan p{};
+  p.dp = dk <= 64 ? 64 : dk <= 128 ? 128 : 256;
+  const int64_t rows = n * (q_heads / heads);
+  p.qt = rows <= 16 || p.dp == 256 ? 1 : 2;   // (what the registers hold)
+  p.row_tiles = (rows + 16 * p.qt - 1) / (16 * p.qt);
+  p.target = std::max<int64_t>(1, kCacheWorkgroups / (heads * p.row_tiles));
+  p.items = p.target == 1 ? sequences : p.target + sequences;
+  p.slots = p.target == 1 ? 0 : 2 * p.target;
+  p.grid = (p.items * heads + 7) / 8 * 8 * p.row_tiles;
+  p.row_floats = p.dp + 1;
+  return p;
+}
+
+// The workspace: a counter for each row tile of a sequence with several parts (at most slots * heads * row_tiles, 2 * kCacheWorkgroups of
+// them), in the same place for all sizes, then the partial results.
+constexpr int64_t kCacheCounterBytes = 2 * kCacheWorkgroups * 4;
+inline int64_t cache_attention_bytes(const CacheAttentionPlan& p, int64_t heads) {
+  return p.slots == 0 ? 0 : kCacheCounterBytes + p.slots * heads * p.row_tiles * 16 * p.qt * p.row_floats * 4;
+}
+
+}  // namespace marian_hip

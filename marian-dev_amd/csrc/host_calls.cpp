@@ -14,6 +14,7 @@
 // build inside _lib.forced_kernel()).
 //
 // The interpreter lock is released around every ABI call, as ctypes does.
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -46,7 +47,8 @@ namespace {
   F(int16_scratch_bytes) F(int8_affine_f32_normed) F(int8_proj_attention_normed) F(int8_proj_attention_ancestors)                                                                                 \
   F(layer_norm) F(embed) F(attention_cached) F(attention_rows) F(attention_ancestors) F(ancestors_advance)                 \
   F(select_state) F(nbest) F(nbest_words) F(nbest_beams) F(nbest_beams_workspace_bytes) F(nbest_beams_workspace_init)   \
-  F(logsoftmax_nbest_beams)
+  F(logsoftmax_nbest_beams) F(rotary) F(cache_append) F(cache_read) F(cache_attention) F(cache_attention_workspace_bytes) \
+  F(cache_attention_workspace_init) F(cache_keep)
 
 struct Library {
 #define F(name) decltype(&marian_hip_##name) name;
@@ -150,6 +152,7 @@ struct PerStream {
   at::Tensor workspace;              // abs-max partials, one-pass exchange
   std::mutex turn;                   // held while a call makes its launches over the workspace
   std::vector<at::Tensor> nbest;     // the last one the largest
+  std::vector<at::Tensor> cache;     // of the attention over a quantized cache, the same
   at::Tensor scratch;                // of the calls, not lent at the moment
 };
 std::map<std::pair<int, hipStream_t>, PerStream> per_stream;   // (looked up with the interpreter lock held)
@@ -1233,6 +1236,254 @@ PyObject* py_logsoftmax_nbest_beams(PyObject*, PyObject* const* args, Py_ssize_t
   MH_END
 }
 
+// ---- keys and values in 8 bits -------------------------------------------------------------------
+// MARIAN_HIP_FLOAT32 .. of a tensor's type; -1: another
+inline int activation_type(const at::Tensor& t) {
+  switch(t.scalar_type()) {
+    case at::kFloat: return MARIAN_HIP_FLOAT32;
+    case at::kHalf: return MARIAN_HIP_FLOAT16;
+    case at::kBFloat16: return MARIAN_HIP_BFLOAT16;
+    default: return -1;
+  }
+}
+
+// A tensor [sequences, heads, n, dk] of one of the activation types on device d (any: that of t), read or written by its
+// strides, which with its address are whole multiples of sixteen bytes.
+struct Rows {
+  const at::Tensor* t = nullptr;
+  int64_t strides[3];
+  int type;
+};
+bool rows_of(const at::Tensor* t, const c10::Device* d, Rows& r) {
+  if(!t || !t->is_cuda() || t->dim() != 4 || (d && t->device() != *d)) return false;
+  r.type = activation_type(*t);
+  if(r.type < 0 || (t->size(3) > 1 && t->stride(3) != 1) || reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 != 0) return false;
+  const int64_t whole = r.type == MARIAN_HIP_FLOAT32 ? 4 : 8;
+  for(int i = 0; i < 3; ++i) {
+    r.strides[i] = t->stride(i);
+    if(t->size(i) > 1 && (r.strides[i] < 0 || r.strides[i] % whole != 0)) return false;
+  }
+  r.t = t;
+  return true;
+}
+// A tensor like r's that lies in memory as r's does: head by head, or the heads of a position side by side.
+at::Tensor rows_like(const Rows& r, int64_t (&st)[3]) {
+  const at::Tensor& t = *r.t;
+  const int64_t heads = t.size(1), n = t.size(2), dk = t.size(3);
+  if(t.is_contiguous()) {
+    st[0] = heads * n * dk;
+    st[1] = n * dk;
+    st[2] = dk;
+    return empty(t.sizes(), t.scalar_type(), t.device());
+  }
+  st[0] = heads * n * dk;
+  st[1] = dk;
+  st[2] = heads * dk;
+  const int64_t stride[4] = {st[0], st[1], st[2], 1};
+  return at::Tensor(at::detail::empty_strided_cuda(t.sizes(), stride, t.scalar_type(), t.device()));
+}
+
+// (k, v, kScale, vScale), dense, on one device
+struct KvCache {
+  marian_hip_kv_cache c;
+  c10::Device device{c10::kCUDA, 0};
+};
+bool cache_of(PyObject* o, KvCache& x) {
+  if(!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+  const at::Tensor* t[4];
+  for(int i = 0; i < 4; ++i) {
+    t[i] = tensor(PyTuple_GET_ITEM(o, i));
+    if(!t[i] || !t[i]->is_cuda() || !t[i]->is_contiguous() || t[i]->device() != t[0]->device()) return false;
+  }
+  if(t[0]->dim() != 4 || t[0]->sizes() != t[1]->sizes() || t[0]->scalar_type() != t[1]->scalar_type() || t[2]->sizes() != t[3]->sizes() ||
+     t[2]->sizes() != t[0]->sizes().slice(0, 3) || t[2]->scalar_type() != at::kFloat || t[3]->scalar_type() != at::kFloat)
+    return false;
+  if(t[0]->scalar_type() == at::kChar) x.c.format = MARIAN_HIP_CACHE_INT8;
+  else if(t[0]->scalar_type() == at::kFloat8_e4m3fn) x.c.format = MARIAN_HIP_CACHE_E4M3;
+  else return false;
+  x.c.k = t[0]->data_ptr();
+  x.c.v = t[1]->data_ptr();
+  x.c.k_scale = fptr_mut(*t[2]);
+  x.c.v_scale = fptr_mut(*t[3]);
+  x.c.sequences = t[0]->size(0);
+  x.c.heads = t[0]->size(1);
+  x.c.capacity = t[0]->size(2);
+  x.c.dk = t[0]->size(3);
+  x.device = t[0]->device();
+  return true;
+}
+
+// int32 [sequences], or with n >= 0 [sequences, n], dense on device d; or None, if that may be
+bool whole_numbers(PyObject* o, bool may_be_none, int64_t sequences, int64_t n, c10::Device d, const int32_t** p) {
+  *p = nullptr;
+  if(none(o)) return may_be_none;
+  const at::Tensor* t = tensor(o);
+  if(!t || t->scalar_type() != at::kInt || t->device() != d || !t->is_contiguous() || t->dim() != (n >= 0 ? 2 : 1) || t->size(0) != sequences ||
+     (n >= 0 && t->size(1) != n))
+    return false;
+  *p = static_cast<const int32_t*>(t->const_data_ptr());
+  return true;
+}
+bool drafts_of(PyObject* lens, PyObject* parents, PyObject* counts, const KvCache& c, int64_t n, marian_hip_drafts& x) {
+  x.n = n;
+  return whole_numbers(lens, false, c.c.sequences, -1, c.device, &x.lens) && whole_numbers(counts, true, c.c.sequences, -1, c.device, &x.counts) &&
+         whole_numbers(parents, true, c.c.sequences, n, c.device, &x.parents);
+}
+
+// (turns, magnitude, interleaved) or None: x.turns is null
+bool rotation_of(PyObject* o, c10::Device d, marian_hip_rotation& x) {
+  x = marian_hip_rotation{};
+  if(none(o)) return true;
+  if(!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 3) return false;
+  const at::Tensor* t = tensor(PyTuple_GET_ITEM(o, 0));
+  if(!t || t->scalar_type() != at::kLong || t->device() != d || !t->is_contiguous() || t->dim() != 1) return false;
+  x.turns = static_cast<const uint64_t*>(t->const_data_ptr());
+  x.dims = 2 * t->size(0);
+  x.magnitude = number(PyTuple_GET_ITEM(o, 1));
+  x.interleaved = truth(PyTuple_GET_ITEM(o, 2));
+  return true;
+}
+
+// rotary(x, positions, rotation, out or None) -> out
+PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  MH_TRY MH_ARGS(4, "rotary");
+  Rows x, o;
+  if(!rows_of(tensor(args[0]), nullptr, x)) Py_RETURN_NONE;
+  const c10::Device d = x.t->device();
+  const int64_t sequences = x.t->size(0), n = x.t->size(2);
+  marian_hip_rotation r;
+  const int32_t* at;
+  const bool each = !whole_numbers(args[1], false, sequences, -1, d, &at);
+  if((each && !whole_numbers(args[1], false, sequences, n, d, &at)) || none(args[2]) || !rotation_of(args[2], d, r)) Py_RETURN_NONE;
+  at::Tensor out;
+  if(none(args[3])) {
+    out = rows_like(x, o.strides);
+  } else {
+    if(!rows_of(tensor(args[3]), &d, o) || o.type != x.type || o.t->sizes() != x.t->sizes()) Py_RETURN_NONE;
+    out = *o.t;
+  }
+  const hipStream_t st = stream_of(d);
+  call("rotaryPositions", [&] {
+    return L.rotary(x.t->const_data_ptr(), x.strides, out.data_ptr(), o.strides, x.type, sequences, x.t->size(1), n, x.t->size(3), at, each, &r, st);
+  });
+  return wrap(std::move(out));
+  MH_END
+}
+
+// cache_append(cache, k, v, lens, parents, counts, rotation, q, q_out) -> q_out; q_out None: a new tensor
+PyObject* py_cache_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  MH_TRY MH_ARGS(9, "cache_append");
+  KvCache c;
+  Rows k, v, q, o;
+  marian_hip_drafts x;
+  marian_hip_rotation r;
+  if(!cache_of(args[0], c) || !rows_of(tensor(args[1]), &c.device, k) || !rows_of(tensor(args[2]), &c.device, v) || k.type != v.type ||
+     k.t->sizes() != v.t->sizes() || k.t->size(0) != c.c.sequences || k.t->size(1) != c.c.heads || k.t->size(3) != c.c.dk ||
+     !drafts_of(args[3], args[4], args[5], c, k.t->size(2), x) || !rotation_of(args[6], c.device, r))
+    Py_RETURN_NONE;
+  at::Tensor out;
+  if(!none(args[7])) {
+    if(!rows_of(tensor(args[7]), &c.device, q) || q.type != k.type || q.t->size(0) != c.c.sequences || q.t->size(2) != x.n ||
+       q.t->size(3) != c.c.dk)
+      Py_RETURN_NONE;
+    if(none(args[8])) {
+      out = rows_like(q, o.strides);
+    } else {
+      if(!rows_of(tensor(args[8]), &c.device, o) || o.type != q.type || o.t->sizes() != q.t->sizes()) Py_RETURN_NONE;
+      out = *o.t;
+    }
+  } else if(!none(args[8])) {
+    Py_RETURN_NONE;
+  }
+  const hipStream_t st = stream_of(c.device);
+  call("appendToCache", [&] {
+    return L.cache_append(&c.c, &x, k.t->const_data_ptr(), k.strides, v.t->const_data_ptr(), v.strides, k.type, r.turns ? &r : nullptr,
+                          q.t ? q.t->const_data_ptr() : nullptr, q.strides, q.t ? q.t->size(1) : 0, q.t ? out.data_ptr() : nullptr, o.strides, st);
+  });
+  if(!q.t) return PyBool_FromLong(1);   // (None: arguments that are not in normal form)
+  return wrap(std::move(out));
+  MH_END
+}
+
+// cache_read(cache, first, n, type) -> (k, v) [sequences, heads, n, dk]; type: a tensor's of that type, any size
+PyObject* py_cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  MH_TRY MH_ARGS(4, "cache_read");
+  KvCache c;
+  const int32_t* first;
+  if(!cache_of(args[0], c) || !whole_numbers(args[1], false, c.c.sequences, -1, c.device, &first) || !THPDtype_Check(args[3])) Py_RETURN_NONE;
+  const int64_t n = whole(args[2]);
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(args[3])->scalar_type;
+  if(n < 0 || (type != at::kFloat && type != at::kHalf && type != at::kBFloat16)) Py_RETURN_NONE;
+  const int64_t size[4] = {c.c.sequences, c.c.heads, n, c.c.dk};
+  at::Tensor k = empty(size, type, c.device), v = empty(size, type, c.device);
+  const hipStream_t st = stream_of(c.device);
+  call("readCache", [&] { return L.cache_read(&c.c, first, n, k.data_ptr(), v.data_ptr(), activation_type(k), st); });
+  Ref a(wrap(std::move(k))), b(wrap(std::move(v)));
+  return PyTuple_Pack(2, a.p, b.p);
+  MH_END
+}
+
+// The workspace of an attention over a quantized cache: a stream's own, for good, or of a call that is recorded its own, cleared
+// by the graph ahead of it (the graph may be replayed on another stream, and beside another graph).
+at::Tensor cache_workspace(int64_t need, c10::Device d, hipStream_t st) {
+  const bool once = marian_hip::recorded(st);
+  if(!once) {
+    std::vector<at::Tensor>& held = per_stream[{d.index(), st}].cache;
+    if(!held.empty() && held.back().numel() >= need) return held.back();
+  }
+  at::Tensor made = empty({need}, at::kByte, d);
+  call("AttentionOverCache", [&] { return L.cache_attention_workspace_init(made.data_ptr(), (size_t)need, st); });
+  if(!once) per_stream[{d.index(), st}].cache.push_back(made);
+  return made;
+}
+
+// cache_attention(q, cache, lens, parents, counts, scale, out or None) -> out
+PyObject* py_cache_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  MH_TRY MH_ARGS(7, "cache_attention");
+  KvCache c;
+  Rows q, o;
+  marian_hip_drafts x;
+  if(!cache_of(args[1], c) || !rows_of(tensor(args[0]), &c.device, q) || q.t->size(0) != c.c.sequences || q.t->size(3) != c.c.dk ||
+     !drafts_of(args[2], args[3], args[4], c, q.t->size(2), x))
+    Py_RETURN_NONE;
+  const double scale = none(args[5]) ? 1.0 / std::pow((double)c.c.dk, 0.5) : number(args[5]);
+  at::Tensor out;
+  if(none(args[6])) {
+    out = rows_like(q, o.strides);
+  } else {
+    if(!rows_of(tensor(args[6]), &c.device, o) || o.type != q.type || o.t->sizes() != q.t->sizes()) Py_RETURN_NONE;
+    out = *o.t;
+  }
+  const hipStream_t st = stream_of(c.device);
+  const int64_t q_heads = q.t->size(1);
+  const int64_t need = (int64_t)L.cache_attention_workspace_bytes(c.c.sequences, c.c.heads, q_heads, x.n, c.c.dk);
+  at::Tensor ws;
+  if(need > 0) ws = cache_workspace(need, c.device, st);
+  call("AttentionOverCache", [&] {
+    return L.cache_attention(&c.c, &x, q.t->const_data_ptr(), q.strides, q_heads, q.type, (float)scale, out.data_ptr(), o.strides,
+                             ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0, st);
+  });
+  return wrap(std::move(out));
+  MH_END
+}
+
+// cache_keep(cache, lens, path, accepted) -> new lens
+PyObject* py_cache_keep(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  MH_TRY MH_ARGS(4, "cache_keep");
+  KvCache c;
+  const at::Tensor* path = tensor(args[2]);
+  const int32_t *lens, *along, *accepted;
+  if(!cache_of(args[0], c) || !path || path->dim() != 2 || !whole_numbers(args[1], false, c.c.sequences, -1, c.device, &lens) ||
+     !whole_numbers(args[2], false, c.c.sequences, path->size(1), c.device, &along) ||
+     !whole_numbers(args[3], false, c.c.sequences, -1, c.device, &accepted))
+    Py_RETURN_NONE;
+  at::Tensor out = empty({c.c.sequences}, at::kInt, c.device);
+  const hipStream_t st = stream_of(c.device);
+  call("keepDrafts", [&] { return L.cache_keep(&c.c, lens, along, path->size(1), accepted, static_cast<int32_t*>(out.data_ptr()), st); });
+  return wrap(std::move(out));
+  MH_END
+}
+
 // ---- module -------------------------------------------------------------------------------------
 // workspace(device index) -> the workspace of that device's current stream
 PyObject* py_workspace(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -1293,6 +1544,7 @@ PyMethodDef methods[] = {
     MH_METHOD(affine_f32_grouped), MH_METHOD(affine_f32_normed), MH_METHOD(proj_attention_normed), MH_METHOD(proj_attention_ancestors), MH_METHOD(prepare_a), MH_METHOD(prepare_b), MH_METHOD(prepare_stored), MH_METHOD(layer_norm),
     MH_METHOD(embed), MH_METHOD(select_state), MH_METHOD(attention), MH_METHOD(attention_rows), MH_METHOD(split_heads), MH_METHOD(join_heads), MH_METHOD(proj_attention), MH_METHOD(attention_ancestors), MH_METHOD(decoder_layers),
     MH_METHOD(ancestors_advance), MH_METHOD(nbest), MH_METHOD(nbest_words), MH_METHOD(nbest_beams), MH_METHOD(logsoftmax_nbest_beams),
+    MH_METHOD(rotary), MH_METHOD(cache_append), MH_METHOD(cache_read), MH_METHOD(cache_attention), MH_METHOD(cache_keep),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_calls", "host path of the operators", -1, methods, nullptr, nullptr, nullptr, nullptr};
