@@ -28,6 +28,7 @@
 #pragma once
 
 #include "cache_codes.h"
+#include "cache_plan.h"
 
 namespace marian_hip {
 
@@ -56,71 +57,69 @@ struct CachePart {
   int s, len, count, used, from, to, parts, part, slot;
 };
 
+// Inclusive sum over the lanes of a wave: within rows of sixteen lanes, then over the rows, without LDS.
+__device__ __forceinline__ unsigned lanes_sum(unsigned x) {
+  int v = (int)x;
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return (unsigned)v;
+}
+
 // Finds part `item`; false where there are fewer.  All waves do the same, lanes being sequences.
-template <int BLOCK>
 __device__ __forceinline__ bool cache_part(const CacheAttentionArgs& a, int item, int lane, CachePart& w) {
-  auto lengths = [&](int s, int& len, int& count) {
-    len = clamp_int(a.lens[s], 0, a.cap);
-    count = a.counts ? clamp_int(a.counts[s], 0, a.n) : a.n;
+  auto blocks_of = [&](int s) -> unsigned {   // of positions that sequence s has in reach
+    if(s >= a.S) return 0;
+    const int len = clamp_int(a.lens[s], 0, a.cap), count = a.counts ? clamp_int(a.counts[s], 0, a.n) : a.n;
+    return count > 0 ? (unsigned)(min(len + count, a.cap) + kCacheBlock - 1) / kCacheBlock : 0;
   };
   w.parts = 1;
   w.part = 0;
   w.slot = 0;
-  int blocks = 1 << 30;   // of a part
+  unsigned each = 1u << 20;   // blocks of a part
   w.s = item;
   if(a.target > 1) {
-    unsigned total = 0;
-    for(int base = 0; base < a.S; base += 64) {
-      const int s = base + lane;
-      int len = 0, count = 0;
-      if(s < a.S) lengths(s, len, count);
-      if(count > 0) total += (unsigned)(min(len + count, a.cap) + BLOCK - 1) / BLOCK;
-    }
+    constexpr int kHeld = 4;   // up to 256 sequences are asked for once, all at a time
+    unsigned held[kHeld], total = 0;
 #pragma unroll
-    for(int o = 32; o > 0; o >>= 1) total += (unsigned)__shfl_xor((int)total, o, 64);
-    blocks = max(1, (int)((total + a.target - 1) / a.target));
-    int before = 0, slots = 0;   // parts, and parts of sequences with several, of the sequences so far
+    for(int i = 0; i < kHeld; ++i) held[i] = blocks_of(64 * i + lane);
+#pragma unroll
+    for(int i = 0; i < kHeld; ++i) total += held[i];
+    for(int base = 64 * kHeld; base < a.S; base += 64) total += blocks_of(base + lane);
+    total = (unsigned)__builtin_amdgcn_readlane((int)lanes_sum(total), 63);
+    each = max(1u, (total + a.target - 1) / a.target);
+    // parts in the lower bits, those of sequences with several in the upper twelve (less than 2 * target)
+    unsigned before = 0;
     bool found = false;
-    for(int base = 0; base < a.S && !found; base += 64) {
-      const int s = base + lane;
-      int len = 0, count = 0;
-      if(s < a.S) lengths(s, len, count);
-      const int mine = count > 0 ? (min(len + count, a.cap) + BLOCK - 1) / BLOCK : 0;
-      const int parts = s < a.S ? max(1, (mine + blocks - 1) / blocks) : 0;
-      int sum = parts, several = parts > 1 ? parts : 0;   // inclusive sums
-#pragma unroll
-      for(int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(sum, o, 64), y = __shfl_up(several, o, 64);
-        if(lane >= o) {
-          sum += x;
-          several += y;
-        }
-      }
-      const unsigned long long at = __ballot(before + sum > item);
+    auto look = [&](int base, unsigned mine) __attribute__((always_inline)) {
+      const unsigned parts = base + lane < a.S ? max(1u, (mine + each - 1) / each) : 0;
+      const unsigned sum = before + lanes_sum(parts > 1 ? parts | parts << 20 : parts);
+      const unsigned long long at = __ballot((int)(sum & 0xfffff) > item);
       if(at) {
         const int l = __ffsll((long long)at) - 1;
+        const unsigned upto = (unsigned)__builtin_amdgcn_readlane((int)sum, l);
         w.s = base + l;
-        w.parts = __shfl(parts, l, 64);
-        w.part = item - (before + __shfl(sum, l, 64) - w.parts);
-        w.slot = slots + __shfl(several, l, 64) - w.parts;
+        w.parts = __builtin_amdgcn_readlane((int)parts, l);
+        w.part = item - ((int)(upto & 0xfffff) - w.parts);
+        w.slot = w.parts > 1 ? (int)(upto >> 20) - w.parts : 0;
         found = true;
       }
-      before += __shfl(sum, 63, 64);
-      slots += __shfl(several, 63, 64);
-    }
+      before = (unsigned)__builtin_amdgcn_readlane((int)sum, 63);
+    };
+#pragma unroll
+    for(int i = 0; i < kHeld; ++i)
+      if(!found && 64 * i < a.S) look(64 * i, held[i]);
+    for(int base = 64 * kHeld; base < a.S && !found; base += 64) look(base, blocks_of(base + lane));
     if(!found) return false;
   }
-  w.s = __builtin_amdgcn_readfirstlane(w.s);
-  w.parts = __builtin_amdgcn_readfirstlane(w.parts);
-  w.part = __builtin_amdgcn_readfirstlane(w.part);
-  w.slot = __builtin_amdgcn_readfirstlane(w.slot);
-  lengths(w.s, w.len, w.count);
-  w.len = __builtin_amdgcn_readfirstlane(w.len);
-  w.count = __builtin_amdgcn_readfirstlane(w.count);
+  w.len = clamp_int(a.lens[w.s], 0, a.cap);
+  w.count = a.counts ? clamp_int(a.counts[w.s], 0, a.n) : a.n;
   w.used = w.count > 0 ? min(w.len + w.count, a.cap) : 0;
-  if(a.target == 1) blocks = (w.used + BLOCK - 1) / BLOCK;
-  w.from = w.part * blocks * BLOCK;
-  w.to = min(w.from + blocks * BLOCK, w.used);
+  w.from = a.target > 1 ? w.part * (int)each * kCacheBlock : 0;
+  w.to = a.target > 1 ? min(w.from + (int)each * kCacheBlock, w.used) : w.used;
   return true;
 }
 
@@ -132,64 +131,65 @@ struct CacheAttention {
   static constexpr int kDims = DP / 16;                   // of a value's row to a lane
   static constexpr int kWords = kDims / 4;
 
-  struct Tile {   // 32 positions as they are loaded
-    cache_u4 k[2][kPieces];
-    unsigned v[8][kWords];
-    cache_f4 ks[2], vs[2];
+  // 32 positions as they are loaded: what is needed for the scores, and what is needed behind them.
+  struct Keys {
+    cache_u4 code[2][kPieces];
+    cache_f4 scale[2];
+  };
+  struct Values {
+    unsigned code[8][kWords];
+    cache_f4 scale[2];
   };
 
-  // ENDS: positions from `last` on are past the end.
+  // Positions at .. at + 31 of an entry; ENDS: those behind `last` are `last`.  Lanes past a row's end (dk < DP) take its start: the
+  // queries are zero there, and the values are not stored.
   template <bool ENDS>
-  static __device__ __forceinline__ void load(Tile& t, const unsigned char* k, const unsigned char* v, const float* ks, const float* vs,
-                                              int at, int last, int dk, int lane) {
+  static __device__ __forceinline__ void load(Keys& t, const unsigned char* k, const float* scale, int at, int last, int dk, int lane) {
     const int c = lane & 15, g = lane >> 4;
-    if(!ENDS) {
-      k += (size_t)(unsigned)at * dk;
-      v += (size_t)(unsigned)at * dk;
-      ks += at;
-      vs += at;
-    }
 #pragma unroll
     for(int b = 0; b < 2; ++b) {
-      const int key = 16 * b + c;
-      const unsigned row = (unsigned)((ENDS ? min(at + key, last) : key) * dk);
+      const unsigned row = ENDS ? (unsigned)min(at + 16 * b + c, last) * dk : (unsigned)(at + c) * dk;
+      const unsigned char* p = ENDS ? k : k + (size_t)(16 * b * dk);
 #pragma unroll
-      for(int p = 0; p < kPieces; ++p) {
-        const unsigned d = 64 * p + 16 * g;
-        t.k[b][p] = cache_u4{0, 0, 0, 0};
-        if(d < (unsigned)dk) t.k[b][p] = *reinterpret_cast<const cache_u4*>(k + row + d);
-      }
-      if(ENDS) {
-#pragma unroll
-        for(int e = 0; e < 4; ++e) {
-          const int i = min(at + 16 * b + 4 * g + e, last);
-          t.ks[b][e] = ks[i];
-          t.vs[b][e] = vs[i];
-        }
-      } else {
-        t.ks[b] = *reinterpret_cast<const cache_f4_any*>(ks + 16 * b + 4 * g);
-        t.vs[b] = *reinterpret_cast<const cache_f4_any*>(vs + 16 * b + 4 * g);
+      for(int i = 0; i < kPieces; ++i) {
+        const unsigned d = 64 * i + 16 * g;
+        t.code[b][i] = *reinterpret_cast<const cache_u4*>(p + (row + (d < (unsigned)dk ? d : 0)));
       }
     }
+    load_scales<ENDS>(t.scale, scale, at, last, g);
+  }
+  template <bool ENDS>
+  static __device__ __forceinline__ void load(Values& t, const unsigned char* v, const float* scale, int at, int last, int dk, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    const unsigned d = (unsigned)(kDims * c) < (unsigned)dk ? kDims * c : 0;
 #pragma unroll
     for(int e = 0; e < 8; ++e) {
-      const int key = 16 * (e / 4) + 4 * g + e % 4;
-      const unsigned row = (unsigned)((ENDS ? min(at + key, last) : key) * dk), d = kDims * c;
+      const int key = 16 * (e / 4) + e % 4;
+      const unsigned row = ENDS ? (unsigned)min(at + 4 * g + key, last) * dk : (unsigned)(at + 4 * g) * dk;
+      const unsigned char* p = (ENDS ? v : v + (size_t)(key * dk)) + (row + d);
+      if constexpr(kWords == 1) {
+        t.code[e][0] = *reinterpret_cast<const unsigned*>(p);
+      } else if constexpr(kWords == 2) {
+        const cache_u2 x = *reinterpret_cast<const cache_u2*>(p);
+        t.code[e][0] = x[0];
+        t.code[e][1] = x[1];
+      } else {
+        const cache_u4 x = *reinterpret_cast<const cache_u4*>(p);
 #pragma unroll
-      for(int w = 0; w < kWords; ++w) t.v[e][w] = 0;
-      if(d < (unsigned)dk) {
-        const unsigned char* p = v + row + d;
-        if constexpr(kWords == 1) {
-          t.v[e][0] = *reinterpret_cast<const unsigned*>(p);
-        } else if constexpr(kWords == 2) {
-          const cache_u2 x = *reinterpret_cast<const cache_u2*>(p);
-          t.v[e][0] = x[0];
-          t.v[e][1] = x[1];
-        } else {
-          const cache_u4 x = *reinterpret_cast<const cache_u4*>(p);
+        for(int w = 0; w < 4; ++w) t.code[e][w] = x[w];
+      }
+    }
+    load_scales<ENDS>(t.scale, scale, at, last, g);
+  }
+  template <bool ENDS>
+  static __device__ __forceinline__ void load_scales(cache_f4 (&to)[2], const float* scale, int at, int last, int g) {
 #pragma unroll
-          for(int w = 0; w < 4; ++w) t.v[e][w] = x[w];
-        }
+    for(int b = 0; b < 2; ++b) {
+      if(ENDS) {
+#pragma unroll
+        for(int e = 0; e < 4; ++e) to[b][e] = scale[(unsigned)min(at + 16 * b + 4 * g + e, last)];
+      } else {
+        to[b] = *reinterpret_cast<const cache_f4_any*>(scale + 16 * b + (unsigned)(at + 4 * g));
       }
     }
   }
@@ -216,7 +216,7 @@ __device__ __forceinline__ float over_lanes_sum(float x) {
 constexpr float kNone = -__builtin_huge_valf();
 
 template <typename T, CacheFormat F, int DP, int QT>
-__global__ __launch_bounds__(256, (DP == 64 ? 2 : 1)) void cache_attention_kernel(CacheAttentionArgs a) {
+__global__ __launch_bounds__(256, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT : 2)) void cache_attention_kernel(CacheAttentionArgs a) {
   using A = CacheAttention<T, F, DP, QT>;
   constexpr int kTerms = A::kTerms, kSteps = A::kSteps, kDims = A::kDims;
   constexpr int kHalf = DP < 128 ? DP : 128;   // dimensions that are joined at a time
@@ -230,7 +230,7 @@ __global__ __launch_bounds__(256, (DP == 64 ? 2 : 1)) void cache_attention_kerne
   if(entry >= a.items * a.Hk) return;
   const int head = entry % a.Hk;
   CachePart w;
-  if(!cache_part<128>(a, entry / a.Hk, lane, w)) return;
+  if(!cache_part(a, entry / a.Hk, lane, w)) return;
   const int rows = w.count * a.G, row0 = tile * 16 * QT;   // rows of the sequence that are there
   T* const out = static_cast<T*>(a.out) + w.s * a.o_s;
   auto row_out = [&](int r) { return out + (long long)(head * a.G + r % a.G) * a.o_h + (long long)(r / a.G) * a.o_n; };
@@ -246,6 +246,28 @@ __global__ __launch_bounds__(256, (DP == 64 ? 2 : 1)) void cache_attention_kerne
     }
   }
   if(row0 >= rows) return;
+
+  // ---- positions
+  const int last_token = min(rows - 1, row0 + 16 * QT - 1) / a.G;
+  const int end = min(w.to, w.len + last_token + 1);                              // of what any row sees
+  const int open = min(end, w.len + (a.parents ? 0 : row0 / a.G + 1));            // of what all rows see
+  const long long first = ((long long)w.s * a.Hk + head) * a.cap;
+  const unsigned char *k = a.k + first * a.dk, *v = a.v + first * a.dk;
+  const float *ks = a.ks + first, *vs = a.vs + first;
+  auto fetch_keys = [&](typename A::Keys& x, int at) __attribute__((always_inline)) {
+    if(at + 32 <= end) A::template load<false>(x, k, ks, at, 0, a.dk, lane);
+    else if(at < end) A::template load<true>(x, k, ks, at, end - 1, a.dk, lane);
+  };
+  auto fetch_values = [&](typename A::Values& x, int at) __attribute__((always_inline)) {
+    if(at + 32 <= end) A::template load<false>(x, v, vs, at, 0, a.dk, lane);
+    else if(at < end) A::template load<true>(x, v, vs, at, end - 1, a.dk, lane);
+  };
+  // (the first positions are asked for ahead of the queries, the next keys as soon as the last ones are used up, and so the values)
+  const int begin = w.from + 32 * wave;
+  typename A::Keys key;
+  typename A::Values value;
+  fetch_keys(key, begin);
+  fetch_values(value, begin);
 
   // ---- queries
   unsigned long long seen = 0;
@@ -280,7 +302,7 @@ __global__ __launch_bounds__(256, (DP == 64 ? 2 : 1)) void cache_attention_kerne
     most = max(most, (unsigned)__shfl_xor((int)most, 32, 64));
     const int up = clamp_int(127 + 14 + 127 - (int)(most >> 23), 2, 252);   // exponent that brings it to 2^14
     const float factor = __builtin_bit_cast(float, (unsigned)up << 23), back = __builtin_bit_cast(float, (unsigned)(254 - up) << 23);
-    row_scale[t] = most >= 0x7f800000u ? __builtin_nanf("") : back * (a.scale_log2 / kCodeUnit<F>);
+    row_scale[t] = most >= 0x7f800000u ? __builtin_nanf("") : fmaxf(back * (a.scale_log2 / kCodeUnit<F>), 0x1p-126f);   // (never zero)
 #pragma unroll
     for(int i = 0; i < kSteps; ++i) {
       float y[8];
@@ -295,13 +317,6 @@ __global__ __launch_bounds__(256, (DP == 64 ? 2 : 1)) void cache_attention_kerne
     }
   }
 
-  // ---- positions
-  const int last_token = min(rows - 1, row0 + 16 * QT - 1) / a.G;
-  const int end = min(w.to, w.len + last_token + 1);                              // of what any row sees
-  const int open = min(end, w.len + (a.parents ? 0 : row0 / a.G + 1));            // of what all rows see
-  const long long first = ((long long)w.s * a.Hk + head) * a.cap;
-  const unsigned char *k = a.k + first * a.dk, *v = a.v + first * a.dk;
-  const float *ks = a.ks + first, *vs = a.vs + first;
   cache_f4 o[QT][kDims];
   float top[QT], sum[QT], unit[QT];   // carried maximum (base 2), the lane's part of the sum, carried scale
 #pragma unroll
@@ -313,8 +328,7 @@ __global__ __launch_bounds__(256, (DP == 64 ? 2 : 1)) void cache_attention_kerne
     for(int j = 0; j < kDims; ++j) o[t][j] = cache_f4{0, 0, 0, 0};
   }
 
-  auto take = [&](const typename A::Tile& x, int at, auto masked) __attribute__((always_inline)) {
-    constexpr bool MASKED = decltype(masked)::value;
+  for(int at = begin; at < end; at += kCacheBlock) {
     // scores
     cache_f4 s[QT][2];
 #pragma unroll
@@ -323,45 +337,56 @@ __global__ __launch_bounds__(256, (DP == 64 ? 2 : 1)) void cache_attention_kerne
     for(int b = 0; b < 2; ++b)
 #pragma unroll
       for(int i = 0; i < kSteps; ++i) {
-        const cache_u4 piece = x.k[b][i / 2];
-        const cache_h8 key = i % 2 ? half8_of<F>(piece[2], piece[3]) : half8_of<F>(piece[0], piece[1]);
+        const cache_u4 piece = key.code[b][i / 2];
+        const cache_h8 operand = i % 2 ? half8_of<F>(piece[2], piece[3]) : half8_of<F>(piece[0], piece[1]);
 #pragma unroll
         for(int t = 0; t < QT; ++t)
 #pragma unroll
-          for(int m = kTerms - 1; m >= 0; --m) s[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q[t][m][i], s[t][b], 0, 0, 0);
+          for(int m = kTerms - 1; m >= 0; --m) s[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand, q[t][m][i], s[t][b], 0, 0, 0);
       }
-    float widest = 0.0f;
-    if constexpr(!MASKED) {
 #pragma unroll
-      for(int e = 0; e < 8; ++e) widest = fmaxf(widest, x.vs[e / 4][e % 4]);
+    for(int t = 0; t < QT; ++t)
+#pragma unroll
+      for(int e = 0; e < 8; ++e) s[t][e / 4][e % 4] *= key.scale[e / 4][e % 4];
+    fetch_keys(key, at + kCacheBlock);
+    // Positions that a row does not see score minus infinity (a weight of zero) and have a scale of zero.
+    const bool masked = at + 32 > open;
+    unsigned hidden[QT];   // bit e: key e
+    float widest = 0.0f;
+#pragma unroll
+    for(int t = 0; t < QT; ++t) hidden[t] = 0;
+    if(masked) {
+#pragma unroll
+      for(int t = 0; t < QT; ++t)
+#pragma unroll
+        for(int e = 0; e < 8; ++e) {
+          const int p = at + 16 * (e / 4) + 4 * g + e % 4, j = p - w.len;
+          const bool see = p < end && (j < 0 || (a.parents ? (sees[t] >> (j & 63) & 1) != 0 : j <= token[t]));
+          hidden[t] |= see ? 0u : 1u << e;
+          s[t][e / 4][e % 4] = see ? s[t][e / 4][e % 4] : kNone;
+        }
+    } else {
+#pragma unroll
+      for(int e = 0; e < 8; ++e) widest = fmaxf(widest, value.scale[e / 4][e % 4]);
     }
     float high[QT], wide[QT];
-    unsigned hidden[QT];   // bit e: key e is not seen
     bool grown = false;
 #pragma unroll
     for(int t = 0; t < QT; ++t) {
       high[t] = kNone;
-      wide[t] = widest;
-      hidden[t] = 0;
 #pragma unroll
-      for(int e = 0; e < 8; ++e) {
-        const float y = s[t][e / 4][e % 4] * x.ks[e / 4][e % 4];
-        s[t][e / 4][e % 4] = y;
-        if constexpr(MASKED) {
-          const int p = at + 16 * (e / 4) + 4 * g + e % 4, j = p - w.len;
-          const bool see = p < end && (j < 0 || (a.parents ? (sees[t] >> (j & 63) & 1) != 0 : j <= token[t]));
-          hidden[t] |= see ? 0u : 1u << e;
-          if(see) {
-            high[t] = fmaxf(high[t], y);
-            wide[t] = fmaxf(wide[t], x.vs[e / 4][e % 4]);
-          }
-        } else {
-          high[t] = fmaxf(high[t], y);
-        }
-      }
+      for(int e = 0; e < 8; ++e) high[t] = fmaxf(high[t], s[t][e / 4][e % 4]);
       high[t] *= row_scale[t];
-      grown |= high[t] > top[t] + kMaximumSlack || wide[t] > unit[t] * kScaleSlack;
+      wide[t] = widest;
     }
+    if(masked) {
+#pragma unroll
+      for(int t = 0; t < QT; ++t)
+#pragma unroll
+        for(int e = 0; e < 8; ++e) wide[t] = fmaxf(wide[t], hidden[t] >> e & 1 ? 0.0f : value.scale[e / 4][e % 4]);
+    }
+#pragma unroll
+    for(int t = 0; t < QT; ++t) grown |= high[t] > top[t] + kMaximumSlack || wide[t] > unit[t] * kScaleSlack;
     if(__any(grown)) {
 #pragma unroll
       for(int t = 0; t < QT; ++t) {
@@ -376,18 +401,26 @@ __global__ __launch_bounds__(256, (DP == 64 ? 2 : 1)) void cache_attention_kerne
       }
     }
     // weights
-    cache_h8 p[QT][kTerms];
+    float r[QT][8];   // scales over the carried one
 #pragma unroll
     for(int t = 0; t < QT; ++t) {
       const float per = kWeightUnit / unit[t];
 #pragma unroll
+      for(int e = 0; e < 8; ++e) r[t][e] = value.scale[e / 4][e % 4] * per;
+    }
+    if(masked) {
+#pragma unroll
+      for(int t = 0; t < QT; ++t)
+#pragma unroll
+        for(int e = 0; e < 8; ++e) r[t][e] = hidden[t] >> e & 1 ? 0.0f : r[t][e];
+    }
+    cache_h8 p[QT][kTerms];
+#pragma unroll
+    for(int t = 0; t < QT; ++t) {
+      const float from = top[t] == kNone ? 0.0f : -top[t];   // (nothing seen so far: minus infinity stays that)
+#pragma unroll
       for(int e = 0; e < 8; ++e) {
-        float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], row_scale[t], -top[t]));
-        float z = y * (x.vs[e / 4][e % 4] * per);
-        if constexpr(MASKED) {
-          y = hidden[t] >> e & 1 ? 0.0f : y;
-          z = hidden[t] >> e & 1 ? 0.0f : z;
-        }
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], row_scale[t], from)), z = y * r[t][e];
         sum[t] += y;
         p[t][0][e] = (_Float16)z;
         if constexpr(kTerms == 2) p[t][1][e] = (_Float16)(z - (float)p[t][0][e]);
@@ -398,7 +431,7 @@ __global__ __launch_bounds__(256, (DP == 64 ? 2 : 1)) void cache_attention_kerne
 #pragma unroll
     for(int e = 0; e < 8; ++e)
 #pragma unroll
-      for(int i = 0; i < A::kWords; ++i) vh[e][i] = held<F>(x.v[e][i]);
+      for(int i = 0; i < A::kWords; ++i) vh[e][i] = held<F>(value.code[e][i]);
 #pragma unroll
     for(int i = 0; i < A::kWords; ++i) {
       const cache_h8 d[4] = {A::template value_operand<0>(vh, i), A::template value_operand<1>(vh, i), A::template value_operand<2>(vh, i),
@@ -411,19 +444,7 @@ __global__ __launch_bounds__(256, (DP == 64 ? 2 : 1)) void cache_attention_kerne
           for(int m = kTerms - 1; m >= 0; --m)
             o[t][4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d[j], p[t][m], o[t][4 * i + j], 0, 0, 0);
     }
-  };
-  auto fetch = [&](typename A::Tile& x, int at) __attribute__((always_inline)) {
-    if(at + 32 <= end) A::template load<false>(x, k, v, ks, vs, at, 0, a.dk, lane);
-    else if(at < end) A::template load<true>(x, k, v, ks, vs, at, end - 1, a.dk, lane);
-  };
-  const int begin = w.from + 32 * wave;
-  typename A::Tile now, next;
-  fetch(now, begin);
-  for(int at = begin; at < end; at += 128) {
-    fetch(next, at + 128);
-    if(at + 32 <= open) take(now, at, std::false_type());
-    else take(now, at, std::true_type());
-    now = next;
+    fetch_values(value, at + kCacheBlock);
   }
 
   // ---- the four waves' results
