@@ -1,0 +1,10 @@
+// Attention over a quantized cache, float16 activations.
+#include "cache_attention_launch.h"
+
+namespace marian_hip {
+
+int launch_cache_attention_float16(const CacheAttentionArgs& a, const CacheAttentionPlan& p, int format, hipStream_t st) {
+  return launch_cache_attention<_Float16>(a, p, format, st);
+}
+
+}  // namespace marian_hip

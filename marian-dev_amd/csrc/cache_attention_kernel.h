@@ -27,30 +27,14 @@
 // last position in reach, whose codes are finite whatever they hold.
 #pragma once
 
+#include "cache_attention.h"
 #include "cache_codes.h"
-#include "cache_plan.h"
 
 namespace marian_hip {
-
-struct CacheAttentionArgs {
-  const void* q;
-  long long q_s, q_h, q_n;   // in values
-  void* out;
-  long long o_s, o_h, o_n;
-  const unsigned char *k, *v;
-  const float *ks, *vs;
-  const int *lens, *counts, *parents;
-  float* part;          // partial results, row_floats to a row: the rows' values, then their logarithms
-  unsigned* counters;   // parts that have arrived, zero between calls
-  int S, Hk, G, n, cap, dk, row_tiles, target, items;
-  float scale_log2;     // scale / ln 2
-};
 
 constexpr float kWeightUnit = 512.0f;     // 2^9, see above
 constexpr float kMaximumSlack = 4.0f;     // weights may be 2^4 above the carried maximum's ...
 constexpr float kScaleSlack = 4.0f;       // ... and scales four times the carried one before the sums are scaled down
-
-__device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 
 // The part of a workgroup: sequence, positions from..to (of the `used` in reach), and its place among the parts.
 struct CachePart {
@@ -85,7 +69,7 @@ __device__ __forceinline__ bool cache_part(const CacheAttentionArgs& a, int item
     constexpr int kHeld = 4;   // up to 256 sequences are asked for once, all at a time
     unsigned held[kHeld], total = 0;
 #pragma unroll
-    for(int i = 0; i < kHeld; ++i) held[i] = blocks_of(64 * i + lane);
+    for(int i = 0; i < kHeld; ++i) held[i] = 64 * i < a.S ? blocks_of(64 * i + lane) : 0;
 #pragma unroll
     for(int i = 0; i < kHeld; ++i) total += held[i];
     for(int base = 64 * kHeld; base < a.S; base += 64) total += blocks_of(base + lane);
@@ -123,7 +107,7 @@ __device__ __forceinline__ bool cache_part(const CacheAttentionArgs& a, int item
   return true;
 }
 
-template <typename T, CacheFormat F, int DP, int QT>
+template <typename T, CacheFormat F, int DP>
 struct CacheAttention {
   static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;   // float16 to a query value or weight
   static constexpr int kSteps = DP / 32;                  // of a product over a row
@@ -167,17 +151,7 @@ struct CacheAttention {
       const int key = 16 * (e / 4) + e % 4;
       const unsigned row = ENDS ? (unsigned)min(at + 4 * g + key, last) * dk : (unsigned)(at + 4 * g) * dk;
       const unsigned char* p = (ENDS ? v : v + (size_t)(key * dk)) + (row + d);
-      if constexpr(kWords == 1) {
-        t.code[e][0] = *reinterpret_cast<const unsigned*>(p);
-      } else if constexpr(kWords == 2) {
-        const cache_u2 x = *reinterpret_cast<const cache_u2*>(p);
-        t.code[e][0] = x[0];
-        t.code[e][1] = x[1];
-      } else {
-        const cache_u4 x = *reinterpret_cast<const cache_u4*>(p);
-#pragma unroll
-        for(int w = 0; w < 4; ++w) t.code[e][w] = x[w];
-      }
+      load_codes(t.code[e], p);
     }
     load_scales<ENDS>(t.scale, scale, at, last, g);
   }
@@ -191,6 +165,20 @@ struct CacheAttention {
       } else {
         to[b] = *reinterpret_cast<const cache_f4_any*>(scale + 16 * b + (unsigned)(at + 4 * g));
       }
+    }
+  }
+
+  static __device__ __forceinline__ void load_codes(unsigned (&to)[kWords], const unsigned char* p) {
+    if constexpr(kWords == 1) {
+      to[0] = *reinterpret_cast<const unsigned*>(p);
+    } else if constexpr(kWords == 2) {
+      const cache_u2 x = *reinterpret_cast<const cache_u2*>(p);
+      to[0] = x[0];
+      to[1] = x[1];
+    } else {
+      const cache_u4 x = *reinterpret_cast<const cache_u4*>(p);
+#pragma unroll
+      for(int w = 0; w < 4; ++w) to[w] = x[w];
     }
   }
 
@@ -215,106 +203,288 @@ __device__ __forceinline__ float over_lanes_sum(float x) {
 
 constexpr float kNone = -__builtin_huge_valf();
 
-template <typename T, CacheFormat F, int DP, int QT>
-__global__ __launch_bounds__(256, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT : 2)) void cache_attention_kernel(CacheAttentionArgs a) {
-  using A = CacheAttention<T, F, DP, QT>;
-  constexpr int kTerms = A::kTerms, kSteps = A::kSteps, kDims = A::kDims;
-  constexpr int kHalf = DP < 128 ? DP : 128;   // dimensions that are joined at a time
-  __shared__ float joined[4][16][kHalf + 4];
-  __shared__ float row_max[4][16 * QT], row_sum[4][16 * QT];
-  __shared__ int is_last;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = lane & 15, g = lane >> 4;
-  // Workgroups with the same positions follow each other on one XCD (a workgroup to each of the eight in turn).
-  const int place = blockIdx.x >> 3, tile = place % a.row_tiles, entry = place / a.row_tiles * 8 + (blockIdx.x & 7);
-  if(entry >= a.items * a.Hk) return;
-  const int head = entry % a.Hk;
+// What a workgroup works on: rows row0 .. of an entry (up to ROWS of them), and its part of the positions.
+struct CacheTile {
   CachePart w;
-  if(!cache_part(a, entry / a.Hk, lane, w)) return;
-  const int rows = w.count * a.G, row0 = tile * 16 * QT;   // rows of the sequence that are there
-  T* const out = static_cast<T*>(a.out) + w.s * a.o_s;
-  auto row_out = [&](int r) { return out + (long long)(head * a.G + r % a.G) * a.o_h + (long long)(r / a.G) * a.o_n; };
-  const int d_mine = (tid & 15) * kDims;   // of the row tid / 16 that the thread writes
-  if(w.part == 0) {
+  int head, tile, rows, row0;   // rows: of the sequence that are there
+  int end, open;                // of what any row sees, of what all rows see
+  const unsigned char *k, *v;   // of the entry
+  const float *ks, *vs;
+};
+
+template <typename T>
+__device__ __forceinline__ T* cache_row_out(const CacheAttentionArgs& a, const CacheTile& x, int r) {
+  return static_cast<T*>(a.out) + x.w.s * a.o_s + (long long)(x.head * a.G + r % a.G) * a.o_h + (long long)(r / a.G) * a.o_n;
+}
+
+// Finds a workgroup's tile and clears the rows of it that are not there; false where nothing is to be done.
+template <typename T, int DP, int ROWS, int WAVES>
+__device__ __forceinline__ bool cache_tile(const CacheAttentionArgs& a, int tid, CacheTile& x) {
+  constexpr int kDims = DP / 16;
+  // Workgroups with the same positions follow each other on one XCD (a workgroup to each of the eight in turn).
+  const int place = blockIdx.x >> 3, entry = place / a.row_tiles * 8 + (blockIdx.x & 7);
+  x.tile = place % a.row_tiles;
+  if(entry >= a.items * a.Hk) return false;
+  x.head = entry % a.Hk;
+  if(!cache_part(a, entry / a.Hk, tid & 63, x.w)) return false;
+  x.rows = x.w.count * a.G;
+  x.row0 = x.tile * ROWS;
+  if(x.w.part == 0 && x.row0 + ROWS > x.rows) {
+    const int d = (tid & 15) * kDims;
+    for(int r = x.row0 + (tid >> 4); r < min(x.row0 + ROWS, a.n * a.G); r += 4 * WAVES) {
+      const float zeros[kDims] = {};
+      if(r >= x.rows && d < a.dk) store_row<kDims, T>(cache_row_out<T>(a, x, r) + d, zeros);
+    }
+  }
+  if(x.row0 >= x.rows) return false;
+  const int last_token = min(x.rows - 1, x.row0 + ROWS - 1) / a.G;
+  x.end = min(x.w.to, x.w.len + last_token + 1);
+  x.open = min(x.end, x.w.len + (a.parents ? 0 : x.row0 / a.G + 1));
+  const long long first = ((long long)x.w.s * a.Hk + x.head) * a.cap;
+  x.k = a.k + first * a.dk;
+  x.v = a.v + first * a.dk;
+  x.ks = a.ks + first;
+  x.vs = a.vs + first;
+  return true;
+}
+
+// What a row sees: in a chain positions before limit, in a tree the settled ones and the drafted ones of bits sees, before end.
+struct CacheSight {
+  int limit;
+  unsigned long long sees;
+};
+__device__ __forceinline__ CacheSight cache_sight(const CacheAttentionArgs& a, const CacheTile& x, int row, unsigned long long seen) {
+  const int token = row / a.G;
+  CacheSight y{min(x.end, x.w.len + token + 1), 0};
+  if(a.parents) {
+    const unsigned lo = __shfl((unsigned)seen, token, 64), hi = __shfl((unsigned)(seen >> 32), token, 64);
+    y.sees = (unsigned long long)hi << 32 | lo;
+  }
+  return y;
+}
+
+// The lane's part of query row `row` as an operand, four lanes (16 apart) to a row; returns the factor of a score, to logarithms of base 2.
+template <typename T, CacheFormat F, int DP>
+__device__ __forceinline__ float cache_query(const CacheAttentionArgs& a, const CacheTile& x, int row, int g,
+                                             cache_h8 (&q)[CacheAttention<T, F, DP>::kTerms][DP / 32]) {
+  constexpr int kTerms = CacheAttention<T, F, DP>::kTerms, kSteps = DP / 32;
+  const T* p = static_cast<const T*>(a.q) + x.w.s * a.q_s + (long long)(x.head * a.G + row % a.G) * a.q_h + (long long)(row / a.G) * a.q_n;
+  float y[kSteps][8];
+  unsigned most = 0;   // bits of the row's largest magnitude (NaN above all)
+#pragma unroll
+  for(int i = 0; i < kSteps; ++i) {
+    const int d = 64 * (i / 2) + 16 * g + 8 * (i % 2);
+#pragma unroll
+    for(int e = 0; e < 8; ++e) y[i][e] = 0.0f;
+    if(d < a.dk) load_row<8>(p + d, y[i]);
+#pragma unroll
+    for(int e = 0; e < 8; ++e) most = max(most, __builtin_bit_cast(unsigned, y[i][e]) & 0x7fffffffu);
+  }
+  most = max(most, (unsigned)__shfl_xor((int)most, 16, 64));
+  most = max(most, (unsigned)__shfl_xor((int)most, 32, 64));
+  const int up = clamp_int(127 + 14 + 127 - (int)(most >> 23), 2, 252);   // exponent that brings it to 2^14
+  const float factor = __builtin_bit_cast(float, (unsigned)up << 23), back = __builtin_bit_cast(float, (unsigned)(254 - up) << 23);
+#pragma unroll
+  for(int i = 0; i < kSteps; ++i) {
+#pragma unroll
+    for(int e = 0; e < 8; ++e) {
+      const float z = y[i][e] * factor;
+      q[0][i][e] = (_Float16)z;
+      if constexpr(kTerms == 2) q[1][i][e] = (_Float16)(z - (float)q[0][i][e]);
+    }
+  }
+  return most >= 0x7f800000u ? __builtin_nanf("") : fmaxf(back * (a.scale_log2 / kCodeUnit<F>), 0x1p-126f);   // (never zero)
+}
+
+// What the waves of a workgroup join their results through.
+template <int DP, int QT, int WAVES>
+struct CacheJoin {
+  static constexpr int kHalf = DP < 128 ? DP : 128;   // dimensions that are joined at a time
+  float joined[WAVES][16][kHalf + 4];
+  float row_max[WAVES][16 * QT], row_sum[WAVES][16 * QT];
+  int is_last;
+};
+
+// The waves' results of the tile, joined and written; of a sequence in several parts by the workgroup that arrives last.  Lane (c, g) holds
+// values 4 * kDims * g .. of row c of each sixteen, unnormalized, the carried maximum and scale and its part of the sum.
+template <typename T, CacheFormat F, int DP, int QT, int WAVES>
+__device__ __forceinline__ void cache_finish(const CacheAttentionArgs& a, const CacheTile& x, const cache_f4 (&o)[QT][DP / 16], const float (&top)[QT],
+                                             float (&sum)[QT], const float (&unit)[QT], CacheJoin<DP, QT, WAVES>& sh) {
+  constexpr int kDims = DP / 16, kHalf = CacheJoin<DP, QT, WAVES>::kHalf;
+  const int tid = threadIdx.x, lane = tid & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+#pragma unroll
+  for(int t = 0; t < QT; ++t) {
+    sum[t] = over_lanes_sum(sum[t]);
+    if(WAVES > 1 && g == 0) {
+      sh.row_max[wave][16 * t + c] = top[t];
+      sh.row_sum[wave][16 * t + c] = sum[t];
+    }
+  }
+  const bool whole = x.w.parts == 1;
+  const long long place_of_tile = ((long long)x.w.slot * a.Hk + x.head) * a.row_tiles + x.tile, part_stride = (long long)a.Hk * a.row_tiles;
+  constexpr int kTileFloats = 16 * QT * (DP + 1);
+  float* const part = whole ? nullptr : a.part + (place_of_tile + x.w.part * part_stride) * kTileFloats;
+  auto emit = [&](int r, int d, const auto& y) __attribute__((always_inline)) {   // values d .. of row r of the tile
+    constexpr int kCount = sizeof(y) / sizeof(float);
+    if(x.row0 + r >= x.rows || d >= a.dk) return;
+    if(whole) {
+      store_row<kCount, T>(cache_row_out<T>(a, x, x.row0 + r) + d, y);
+    } else {
+      unsigned long long* to = reinterpret_cast<unsigned long long*>(part + r * DP + d);
+#pragma unroll
+      for(int j = 0; j < kCount; j += 2)
+        __hip_atomic_store(to + j / 2, (unsigned long long)__builtin_bit_cast(unsigned, y[j + 1]) << 32 | __builtin_bit_cast(unsigned, y[j]),
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  };
+  auto emit_log = [&](int r, float m, float total) __attribute__((always_inline)) {   // of the sum of the row's weights
+    if(!whole && x.row0 + r < x.rows)
+      __hip_atomic_store(part + 16 * QT * DP + r, total == 0.0f ? kNone : m + __builtin_amdgcn_logf(total), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  constexpr float kUnit = 1.0f / (kWeightUnit * kCodeUnit<F>);
+  if constexpr(WAVES == 1) {
 #pragma unroll
     for(int t = 0; t < QT; ++t) {
-      const int r = row0 + 16 * t + (tid >> 4);
-      if(r >= rows && r < a.n * a.G && d_mine < a.dk) {
-        const float zeros[kDims] = {};
-        store_row<kDims, T>(row_out(r) + d_mine, zeros);
+      const float factor = (sum[t] == 0.0f ? 0.0f : 1.0f / sum[t]) * (unit[t] * kUnit);
+#pragma unroll
+      for(int e = 0; e < 4; ++e) {
+        float y[kDims];
+#pragma unroll
+        for(int j = 0; j < kDims; ++j) y[j] = o[t][j][e] * factor;
+        emit(16 * t + c, kDims * (4 * g + e), y);
+      }
+      if(g == 0) emit_log(16 * t + c, top[t], sum[t]);
+    }
+  } else {
+    __syncthreads();
+#pragma unroll
+    for(int t = 0; t < QT; ++t) {
+      float m = sh.row_max[0][16 * t + c];
+#pragma unroll
+      for(int i = 1; i < WAVES; ++i) m = fmaxf(m, sh.row_max[i][16 * t + c]);
+      const float mine = top[t] == kNone ? 0.0f : __builtin_amdgcn_exp2f(top[t] - m) * (unit[t] * kUnit);
+#pragma unroll
+      for(int h = 0; h < DP / kHalf; ++h) {
+        if(h || t) __syncthreads();
+        if(DP == kHalf || (g >> 1) == h) {
+#pragma unroll
+          for(int e = 0; e < 4; ++e)
+#pragma unroll
+            for(int j = 0; j < kDims; j += 4)
+              *reinterpret_cast<cache_f4*>(&sh.joined[wave][c][4 * kDims * g + kDims * e + j - h * kHalf]) =
+                  cache_f4{o[t][j][e] * mine, o[t][j + 1][e] * mine, o[t][j + 2][e] * mine, o[t][j + 3][e] * mine};
+        }
+        __syncthreads();
+        constexpr int kEach = kHalf / 16;
+        const int d = (tid & 15) * kEach;
+#pragma unroll
+        for(int r = tid >> 4; r < 16; r += 4 * WAVES) {   // a row to sixteen threads
+          float top_r = sh.row_max[0][16 * t + r], total = 0.0f, y[kEach];
+#pragma unroll
+          for(int i = 1; i < WAVES; ++i) top_r = fmaxf(top_r, sh.row_max[i][16 * t + r]);
+#pragma unroll
+          for(int i = 0; i < WAVES; ++i) {
+            const float from = sh.row_max[i][16 * t + r];   // (of a wave that saw nothing the sum is 0, or NaN)
+            total += sh.row_sum[i][16 * t + r] * (from == kNone ? 1.0f : __builtin_amdgcn_exp2f(from - top_r));
+          }
+          const float per = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+          for(int j = 0; j < kEach; ++j) {
+            y[j] = sh.joined[0][r][d + j];
+#pragma unroll
+            for(int i = 1; i < WAVES; ++i) y[j] += sh.joined[i][r][d + j];
+            y[j] *= per;
+          }
+          emit(16 * t + r, h * kHalf + d, y);
+          if(h == 0 && (tid & 15) == 0) emit_log(16 * t + r, top_r, total);
+        }
       }
     }
   }
-  if(row0 >= rows) return;
+  if(whole) return;
 
-  // ---- positions
-  const int last_token = min(rows - 1, row0 + 16 * QT - 1) / a.G;
-  const int end = min(w.to, w.len + last_token + 1);                              // of what any row sees
-  const int open = min(end, w.len + (a.parents ? 0 : row0 / a.G + 1));            // of what all rows see
-  const long long first = ((long long)w.s * a.Hk + head) * a.cap;
-  const unsigned char *k = a.k + first * a.dk, *v = a.v + first * a.dk;
-  const float *ks = a.ks + first, *vs = a.vs + first;
-  auto fetch_keys = [&](typename A::Keys& x, int at) __attribute__((always_inline)) {
-    if(at + 32 <= end) A::template load<false>(x, k, ks, at, 0, a.dk, lane);
-    else if(at < end) A::template load<true>(x, k, ks, at, end - 1, a.dk, lane);
+  // ---- the parts of a sequence: the workgroup that arrives last joins them, in their order.
+  // (Stores and loads of agent scope go past the caches of an XCD; every wave's stores are acknowledged before the count
+  // goes up, so whoever reads the last count finds them all.)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if(tid == 0) {
+    unsigned* const counter = a.counters + place_of_tile;
+    const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(x.w.parts - 1);
+    if(last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // (for the next call)
+    sh.is_last = last;
+  }
+  __syncthreads();
+  if(!sh.is_last) return;
+  const float* const all = a.part + place_of_tile * kTileFloats;
+  const long long stride = part_stride * kTileFloats;
+  const int d_mine = (tid & 15) * kDims;   // of a row to sixteen threads
+  if(d_mine >= a.dk) return;
+#pragma unroll 1
+  for(int r = tid >> 4; r < min(16 * QT, x.rows - x.row0); r += 4 * WAVES) {
+    const float* logs = all + 16 * QT * DP + r;
+    const float* from = all + r * DP + d_mine;
+    float m = kNone;
+#pragma unroll 4
+    for(int i = 0; i < x.w.parts; ++i) m = fmaxf(m, __hip_atomic_load(logs + i * stride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    float total = 0.0f, y[kDims] = {};
+#pragma unroll 4
+    for(int i = 0; i < x.w.parts; ++i) {
+      const float l = __hip_atomic_load(logs + i * stride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const float weight = l == kNone ? 0.0f : __builtin_amdgcn_exp2f(l - m);
+      total += weight;
+#pragma unroll
+      for(int j = 0; j < kDims; j += 2) {
+        const unsigned long long x = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(from + i * stride + j), __ATOMIC_RELAXED,
+                                                       __HIP_MEMORY_SCOPE_AGENT);
+        y[j] = __builtin_fmaf(weight, __builtin_bit_cast(float, (unsigned)x), y[j]);
+        y[j + 1] = __builtin_fmaf(weight, __builtin_bit_cast(float, (unsigned)(x >> 32)), y[j + 1]);
+      }
+    }
+    const float per = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for(int j = 0; j < kDims; ++j) y[j] *= per;
+    store_row<kDims, T>(cache_row_out<T>(a, x, x.row0 + r) + d_mine, y);
+  }
+}
+
+// ---- sixteen rows and more to a wave
+template <typename T, CacheFormat F, int DP, int QT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT : 2)) void cache_attention_kernel(CacheAttentionArgs a) {
+  using A = CacheAttention<T, F, DP>;
+  constexpr int kTerms = A::kTerms, kSteps = A::kSteps, kDims = A::kDims;
+  constexpr int kTurn = 32 * WAVES;   // positions that the waves take in one turn
+  __shared__ CacheJoin<DP, QT, WAVES> sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  CacheTile x;
+  if(!cache_tile<T, DP, 16 * QT, WAVES>(a, tid, x)) return;
+  const int end = x.end;
+  auto fetch_keys = [&](typename A::Keys& y, int at) __attribute__((always_inline)) {
+    if(at + 32 <= end) A::template load<false>(y, x.k, x.ks, at, 0, a.dk, lane);
+    else if(at < end) A::template load<true>(y, x.k, x.ks, at, end - 1, a.dk, lane);
   };
-  auto fetch_values = [&](typename A::Values& x, int at) __attribute__((always_inline)) {
-    if(at + 32 <= end) A::template load<false>(x, v, vs, at, 0, a.dk, lane);
-    else if(at < end) A::template load<true>(x, v, vs, at, end - 1, a.dk, lane);
+  auto fetch_values = [&](typename A::Values& y, int at) __attribute__((always_inline)) {
+    if(at + 32 <= end) A::template load<false>(y, x.v, x.vs, at, 0, a.dk, lane);
+    else if(at < end) A::template load<true>(y, x.v, x.vs, at, end - 1, a.dk, lane);
   };
   // (the first positions are asked for ahead of the queries, the next keys as soon as the last ones are used up, and so the values)
-  const int begin = w.from + 32 * wave;
+  const int begin = x.w.from + 32 * wave;
   typename A::Keys key;
   typename A::Values value;
   fetch_keys(key, begin);
   fetch_values(value, begin);
-
-  // ---- queries
   unsigned long long seen = 0;
-  if(a.parents) seen = lineage(a.parents + (long long)w.s * a.n, a.n, lane);
+  if(a.parents) seen = lineage(a.parents + (long long)x.w.s * a.n, a.n, lane);
   cache_h8 q[QT][kTerms][kSteps];
-  float row_scale[QT];          // of a score, to logarithms of base 2
-  int token[QT];
-  unsigned long long sees[QT];   // drafted tokens
+  float row_scale[QT];
+  CacheSight sight[QT];
 #pragma unroll
   for(int t = 0; t < QT; ++t) {
-    const int r = row0 + 16 * t + c, rr = min(r, rows - 1);
-    token[t] = rr / a.G;
-    if(a.parents) {
-      const unsigned lo = __shfl((unsigned)seen, token[t], 64), hi = __shfl((unsigned)(seen >> 32), token[t], 64);
-      sees[t] = (unsigned long long)hi << 32 | lo;
-    } else {
-      sees[t] = 0;
-    }
-    const T* row = static_cast<const T*>(a.q) + w.s * a.q_s + (long long)(head * a.G + rr % a.G) * a.q_h + (long long)token[t] * a.q_n;
-    float x[kSteps][8];
-    unsigned most = 0;   // bits of the row's largest magnitude (NaN above all)
-#pragma unroll
-    for(int i = 0; i < kSteps; ++i) {
-      const int d = 64 * (i / 2) + 16 * g + 8 * (i % 2);
-#pragma unroll
-      for(int e = 0; e < 8; ++e) x[i][e] = 0.0f;
-      if(d < a.dk) load_row<8>(row + d, x[i]);
-#pragma unroll
-      for(int e = 0; e < 8; ++e) most = max(most, __builtin_bit_cast(unsigned, x[i][e]) & 0x7fffffffu);
-    }
-    most = max(most, (unsigned)__shfl_xor((int)most, 16, 64));
-    most = max(most, (unsigned)__shfl_xor((int)most, 32, 64));
-    const int up = clamp_int(127 + 14 + 127 - (int)(most >> 23), 2, 252);   // exponent that brings it to 2^14
-    const float factor = __builtin_bit_cast(float, (unsigned)up << 23), back = __builtin_bit_cast(float, (unsigned)(254 - up) << 23);
-    row_scale[t] = most >= 0x7f800000u ? __builtin_nanf("") : fmaxf(back * (a.scale_log2 / kCodeUnit<F>), 0x1p-126f);   // (never zero)
-#pragma unroll
-    for(int i = 0; i < kSteps; ++i) {
-      float y[8];
-#pragma unroll
-      for(int e = 0; e < 8; ++e) y[e] = x[i][e] * factor;
-#pragma unroll
-      for(int e = 0; e < 8; ++e) q[t][0][i][e] = (_Float16)y[e];
-      if constexpr(kTerms == 2) {
-#pragma unroll
-        for(int e = 0; e < 8; ++e) q[t][1][i][e] = (_Float16)(y[e] - (float)q[t][0][i][e]);
-      }
-    }
+    const int row = min(x.row0 + 16 * t + c, x.rows - 1);
+    sight[t] = cache_sight(a, x, row, seen);
+    row_scale[t] = cache_query<T, F, DP>(a, x, row, g, q[t]);
   }
 
   cache_f4 o[QT][kDims];
@@ -328,7 +498,7 @@ __global__ __launch_bounds__(256, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT : 2)) 
     for(int j = 0; j < kDims; ++j) o[t][j] = cache_f4{0, 0, 0, 0};
   }
 
-  for(int at = begin; at < end; at += kCacheBlock) {
+  for(int at = begin; at < end; at += kTurn) {
     // scores
     cache_f4 s[QT][2];
 #pragma unroll
@@ -348,23 +518,31 @@ __global__ __launch_bounds__(256, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT : 2)) 
     for(int t = 0; t < QT; ++t)
 #pragma unroll
       for(int e = 0; e < 8; ++e) s[t][e / 4][e % 4] *= key.scale[e / 4][e % 4];
-    fetch_keys(key, at + kCacheBlock);
+    fetch_keys(key, at + kTurn);
     // Positions that a row does not see score minus infinity (a weight of zero) and have a scale of zero.
-    const bool masked = at + 32 > open;
-    unsigned hidden[QT];   // bit e: key e
+    const bool masked = at + 32 > x.open;
+    unsigned seen_here[QT];   // bit e: key e
     float widest = 0.0f;
 #pragma unroll
-    for(int t = 0; t < QT; ++t) hidden[t] = 0;
+    for(int t = 0; t < QT; ++t) seen_here[t] = 0xff;
     if(masked) {
 #pragma unroll
-      for(int t = 0; t < QT; ++t)
+      for(int t = 0; t < QT; ++t) {
+        unsigned bits = 0;
 #pragma unroll
-        for(int e = 0; e < 8; ++e) {
-          const int p = at + 16 * (e / 4) + 4 * g + e % 4, j = p - w.len;
-          const bool see = p < end && (j < 0 || (a.parents ? (sees[t] >> (j & 63) & 1) != 0 : j <= token[t]));
-          hidden[t] |= see ? 0u : 1u << e;
-          s[t][e / 4][e % 4] = see ? s[t][e / 4][e % 4] : kNone;
+        for(int b = 0; b < 2; ++b) {
+          const int from = at + 16 * b + 4 * g;
+          unsigned four = (1u << clamp_int((a.parents ? end : sight[t].limit) - from, 0, 4)) - 1;
+          if(a.parents) {   // settled positions, then the drafted ones from bit 0 on
+            const int j = from - x.w.len, settled = clamp_int(-j, 0, 4);
+            four &= j < 0 ? ((unsigned)sight[t].sees << settled | ((1u << settled) - 1)) : (unsigned)(sight[t].sees >> min(j, 63));
+          }
+          bits |= four << (4 * b);
         }
+        seen_here[t] = bits;
+#pragma unroll
+        for(int e = 0; e < 8; ++e) s[t][e / 4][e % 4] = bits >> e & 1 ? s[t][e / 4][e % 4] : kNone;
+      }
     } else {
 #pragma unroll
       for(int e = 0; e < 8; ++e) widest = fmaxf(widest, value.scale[e / 4][e % 4]);
@@ -383,7 +561,7 @@ __global__ __launch_bounds__(256, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT : 2)) 
 #pragma unroll
       for(int t = 0; t < QT; ++t)
 #pragma unroll
-        for(int e = 0; e < 8; ++e) wide[t] = fmaxf(wide[t], hidden[t] >> e & 1 ? 0.0f : value.scale[e / 4][e % 4]);
+        for(int e = 0; e < 8; ++e) wide[t] = fmaxf(wide[t], seen_here[t] >> e & 1 ? value.scale[e / 4][e % 4] : 0.0f);
     }
 #pragma unroll
     for(int t = 0; t < QT; ++t) grown |= high[t] > top[t] + kMaximumSlack || wide[t] > unit[t] * kScaleSlack;
@@ -412,7 +590,7 @@ __global__ __launch_bounds__(256, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT : 2)) 
 #pragma unroll
       for(int t = 0; t < QT; ++t)
 #pragma unroll
-        for(int e = 0; e < 8; ++e) r[t][e] = hidden[t] >> e & 1 ? 0.0f : r[t][e];
+        for(int e = 0; e < 8; ++e) r[t][e] = seen_here[t] >> e & 1 ? r[t][e] : 0.0f;
     }
     cache_h8 p[QT][kTerms];
 #pragma unroll
@@ -444,120 +622,260 @@ __global__ __launch_bounds__(256, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT : 2)) 
           for(int m = kTerms - 1; m >= 0; --m)
             o[t][4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d[j], p[t][m], o[t][4 * i + j], 0, 0, 0);
     }
-    fetch_values(value, at + kCacheBlock);
+    fetch_values(value, at + kTurn);
   }
 
-  // ---- the four waves' results
+  cache_finish<T, F, DP, QT, WAVES>(a, x, o, top, sum, unit, sh);
+}
+
+// ---- up to eight rows to a wave
+// Scores of a few rows would leave most columns of the form above empty, and weights cost more instructions than codes do.  Here
+// 64 positions are taken at a time, S = Q K^T with the rows repeated over the sixteen of an operand, so that every lane has, of
+// one of the four products' sixteen keys each, scores of up to four rows - of one key (ROWS up to 4) or two (8) - and each
+// score is in one lane only.  A key's scales are a value to a lane, whole lines of memory.  The weights go
+// through LDS, a row of 64 a query, to where they are an operand: lane (c, g) takes eight of row c, those of positions
+// 4 e + g of 32, so that four rows of values that follow each other in memory are loaded at a time.
+template <typename T, CacheFormat F, int DP, int ROWS>
+struct CacheFew {
+  using A = CacheAttention<T, F, DP>;
+  static constexpr int kRegs = ROWS < 4 ? ROWS : 4;    // rows whose scores a lane has
+  static constexpr int kKeys = ROWS <= 4 ? 1 : 2;      // keys whose scores a lane has
+  static constexpr int kStride = 72;                   // weights of a row in LDS, and eight more
+  typedef _Float16 Weights[A::kTerms][ROWS][kStride];
+
+  struct Keys {
+    cache_u4 code[4][A::kPieces];
+    float scale[kKeys];
+  };
+  struct Values {
+    unsigned code[2][8][A::kWords];
+    float scale[kKeys];
+  };
+  // The position, of 64, whose scores lane (c, g) has.
+  static __device__ __forceinline__ int key_of(int i, int lane) { return kKeys == 1 ? lane : 32 * i + 16 * (lane >> 5) + (lane & 15); }
+
+  template <bool ENDS>
+  static __device__ __forceinline__ void load(Keys& t, const unsigned char* k, const float* scale, int at, int last, int dk, int lane) {
+    const int c = lane & 15, g = lane >> 4;
 #pragma unroll
-  for(int t = 0; t < QT; ++t) {
-    sum[t] = over_lanes_sum(sum[t]);
-    if(g == 0) {
-      row_max[wave][16 * t + c] = top[t];
-      row_sum[wave][16 * t + c] = sum[t];
-    }
-  }
-  __syncthreads();
-  const bool whole = w.parts == 1;
-  const long long place_of_tile = ((long long)w.slot * a.Hk + head) * a.row_tiles + tile, part_stride = (long long)a.Hk * a.row_tiles;
-  constexpr int kTileFloats = 16 * QT * (DP + 1);
-  float* const part = whole ? nullptr : a.part + (place_of_tile + w.part * part_stride) * kTileFloats;
+    for(int b = 0; b < 4; ++b) {
+      const unsigned row = ENDS ? (unsigned)min(at + 16 * b + c, last) * dk : (unsigned)(at + c) * dk;
+      const unsigned char* p = ENDS ? k : k + (size_t)(16 * b * dk);
 #pragma unroll
-  for(int t = 0; t < QT; ++t) {
-    float m = row_max[0][16 * t + c];
-#pragma unroll
-    for(int i = 1; i < 4; ++i) m = fmaxf(m, row_max[i][16 * t + c]);
-    const float mine = top[t] == kNone ? 0.0f : __builtin_amdgcn_exp2f(top[t] - m) * (unit[t] / (kWeightUnit * kCodeUnit<F>));
-    const int r = tid >> 4;   // the row whose values the thread adds up
-    float m_r = row_max[0][16 * t + r];
-#pragma unroll
-    for(int i = 1; i < 4; ++i) m_r = fmaxf(m_r, row_max[i][16 * t + r]);
-    float total = 0.0f;
-#pragma unroll
-    for(int i = 0; i < 4; ++i)
-      total += row_max[i][16 * t + r] == kNone ? row_sum[i][16 * t + r] : row_sum[i][16 * t + r] * __builtin_amdgcn_exp2f(row_max[i][16 * t + r] - m_r);
-    const float per = total == 0.0f ? 0.0f : 1.0f / total;
-    const bool there = row0 + 16 * t + r < rows;
-#pragma unroll
-    for(int h = 0; h < DP / kHalf; ++h) {
-      if(h || t) __syncthreads();
-      if(DP == kHalf || (g >> 1) == h) {
-#pragma unroll
-        for(int e = 0; e < 4; ++e)
-#pragma unroll
-          for(int j = 0; j < kDims; j += 4) {
-            const int d = 4 * kDims * g + kDims * e + j - h * kHalf;
-            *reinterpret_cast<cache_f4*>(&joined[wave][c][d]) =
-                cache_f4{o[t][j][e] * mine, o[t][j + 1][e] * mine, o[t][j + 2][e] * mine, o[t][j + 3][e] * mine};
-          }
+      for(int i = 0; i < A::kPieces; ++i) {
+        const unsigned d = 64 * i + 16 * g;
+        t.code[b][i] = *reinterpret_cast<const cache_u4*>(p + (row + (d < (unsigned)dk ? d : 0)));
       }
-      __syncthreads();
-      constexpr int kEach = kHalf / 16;
-      const int d = (tid & 15) * kEach;
-      float y[kEach];
+    }
 #pragma unroll
-      for(int j = 0; j < kEach; ++j)
-        y[j] = ((joined[0][r][d + j] + joined[1][r][d + j]) + (joined[2][r][d + j] + joined[3][r][d + j])) * per;
-      if(there && d + h * kHalf < a.dk) {
-        if(whole) {
-          store_row<kEach, T>(row_out(row0 + 16 * t + r) + d + h * kHalf, y);
+    for(int i = 0; i < kKeys; ++i) t.scale[i] = scale[(unsigned)(ENDS ? min(at + key_of(i, lane), last) : at + key_of(i, lane))];
+  }
+  template <bool ENDS>
+  static __device__ __forceinline__ void load(Values& t, const unsigned char* v, const float* scale, int at, int last, int dk, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    const unsigned d = (unsigned)(A::kDims * c) < (unsigned)dk ? A::kDims * c : 0;
+#pragma unroll
+    for(int h = 0; h < 2; ++h)
+#pragma unroll
+      for(int e = 0; e < 8; ++e) {
+        const int key = 32 * h + 4 * e;
+        const unsigned row = ENDS ? (unsigned)min(at + g + key, last) * dk : (unsigned)(at + g) * dk;
+        A::load_codes(t.code[h][e], (ENDS ? v : v + (size_t)(key * dk)) + (row + d));
+      }
+#pragma unroll
+    for(int i = 0; i < kKeys; ++i) t.scale[i] = scale[(unsigned)(ENDS ? min(at + key_of(i, lane), last) : at + key_of(i, lane))];
+  }
+};
+
+template <typename T, CacheFormat F, int DP, int ROWS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) void cache_attention_few_kernel(CacheAttentionArgs a) {
+  using A = CacheAttention<T, F, DP>;
+  using B = CacheFew<T, F, DP, ROWS>;
+  constexpr int kTerms = A::kTerms, kSteps = A::kSteps, kDims = A::kDims, kRegs = B::kRegs, kKeys = B::kKeys;
+  constexpr int kTurn = 64 * WAVES;   // positions that the waves take in one turn
+  __shared__ union {
+    CacheJoin<DP, 1, WAVES> join;
+    typename B::Weights weights[WAVES];
+  } sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  CacheTile x;
+  if(!cache_tile<T, DP, ROWS, WAVES>(a, tid, x)) return;
+  const int end = x.end;
+  auto fetch_keys = [&](typename B::Keys& y, int at) __attribute__((always_inline)) {
+    if(at + 64 <= end) B::template load<false>(y, x.k, x.ks, at, 0, a.dk, lane);
+    else if(at < end) B::template load<true>(y, x.k, x.ks, at, end - 1, a.dk, lane);
+  };
+  auto fetch_values = [&](typename B::Values& y, int at) __attribute__((always_inline)) {
+    if(at + 64 <= end) B::template load<false>(y, x.v, x.vs, at, 0, a.dk, lane);
+    else if(at < end) B::template load<true>(y, x.v, x.vs, at, end - 1, a.dk, lane);
+  };
+  const int begin = x.w.from + 64 * wave;
+  typename B::Keys key;
+  typename B::Values value;
+  fetch_keys(key, begin);
+  fetch_values(value, begin);
+  unsigned long long seen = 0;
+  if(a.parents) seen = lineage(a.parents + (long long)x.w.s * a.n, a.n, lane);
+  cache_h8 q[kTerms][kSteps];
+  const float query_scale = cache_query<T, F, DP>(a, x, min(x.row0 + c % ROWS, x.rows - 1), g, q);
+  const int mine0 = ROWS == 8 ? 4 * (g & 1) : 0;   // the first of the rows whose scores the lane has
+  float row_scale[kRegs];
+  CacheSight sight[kRegs];
+#pragma unroll
+  for(int t = 0; t < kRegs; ++t) {
+    row_scale[t] = __shfl(query_scale, mine0 + t, 64);
+    sight[t] = cache_sight(a, x, min(x.row0 + mine0 + t, x.rows - 1), seen);
+  }
+  cache_f4 o[1][kDims];
+#pragma unroll
+  for(int j = 0; j < kDims; ++j) o[0][j] = cache_f4{0, 0, 0, 0};
+  float top[kRegs], sum[kRegs], unit[kRegs], per[kRegs];
+#pragma unroll
+  for(int t = 0; t < kRegs; ++t) {
+    top[t] = kNone;
+    sum[t] = 0.0f;
+    unit[t] = 1e-30f;
+    per[t] = kWeightUnit / unit[t];
+  }
+  // of row c, what the lanes that have its scores hold
+  auto of_row = [&](const float(&y)[kRegs]) __attribute__((always_inline)) {
+    const int from = ROWS == 8 ? (c >> 2 & 1) * 16 : 0;
+    float z = ROWS == 8 ? __shfl(y[0], from, 64) : y[0];
+#pragma unroll
+    for(int t = 1; t < kRegs; ++t) {
+      const float next = ROWS == 8 ? __shfl(y[t], from, 64) : y[t];
+      z = (c & 3) == t ? next : z;
+    }
+    return z;
+  };
+  auto over_rows_lanes = [&](float y, auto join) __attribute__((always_inline)) {   // over the lanes that have scores of the same rows
+#pragma unroll
+    for(int i = 1; i < 64; i <<= 1)
+      if(ROWS != 8 || i != 16) y = join(y, __shfl_xor(y, i, 64));
+    return y;
+  };
+  auto larger = [](float y, float z) { return fmaxf(y, z); };
+  auto added = [](float y, float z) { return y + z; };
+
+  for(int at = begin; at < end; at += kTurn) {
+    // scores
+    float s[kKeys][kRegs];
+    {
+      cache_f4 p[4];
+#pragma unroll
+      for(int b = 0; b < 4; ++b) {
+        p[b] = cache_f4{0, 0, 0, 0};
+#pragma unroll
+        for(int i = 0; i < kSteps; ++i) {
+          const cache_u4 piece = key.code[b][i / 2];
+          const cache_h8 operand = i % 2 ? half8_of<F>(piece[2], piece[3]) : half8_of<F>(piece[0], piece[1]);
+#pragma unroll
+          for(int m = kTerms - 1; m >= 0; --m) p[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[m][i], operand, p[b], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for(int t = 0; t < kRegs; ++t) {
+        if(kKeys == 1) {
+          s[0][t] = g & 2 ? (g & 1 ? p[3][t] : p[2][t]) : (g & 1 ? p[1][t] : p[0][t]);
         } else {
-          unsigned long long* to = reinterpret_cast<unsigned long long*>(part + (16 * t + r) * DP + d + h * kHalf);
-#pragma unroll
-          for(int j = 0; j < kEach; j += 2)
-            __hip_atomic_store(to + j / 2, (unsigned long long)__builtin_bit_cast(unsigned, y[j + 1]) << 32 | __builtin_bit_cast(unsigned, y[j]),
-                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          s[0][t] = g & 2 ? p[1][t] : p[0][t];
+          s[kKeys - 1][t] = g & 2 ? p[3][t] : p[2][t];
         }
       }
     }
-    if(!whole && there && (tid & 15) == 0)
-      __hip_atomic_store(part + 16 * QT * DP + 16 * t + r, total == 0.0f ? kNone : m_r + __builtin_amdgcn_logf(total), __ATOMIC_RELAXED,
-                         __HIP_MEMORY_SCOPE_AGENT);
-  }
-  if(whole) return;
-
-  // ---- the parts of a sequence: the workgroup that arrives last joins them, in their order.
-  // (Stores and loads of agent scope go past the caches of an XCD; every wave's stores are acknowledged before the count
-  // goes up, so whoever reads the last count finds them all.)
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if(tid == 0) {
-    unsigned* const counter = a.counters + place_of_tile;
-    const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(w.parts - 1);
-    if(last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // (for the next call)
-    is_last = last;
-  }
-  __syncthreads();
-  if(!is_last) return;
-  const float* const all = a.part + place_of_tile * kTileFloats;
-  const long long stride = part_stride * kTileFloats;
-#pragma unroll 1
-  for(int t = 0; t < QT; ++t) {
-    const int r = tid >> 4;
-    if(row0 + 16 * t + r >= rows || d_mine >= a.dk) continue;
-    const float* logs = all + 16 * QT * DP + 16 * t + r;
-    const float* from = all + (16 * t + r) * DP + d_mine;
-    float m = kNone;
-#pragma unroll 4
-    for(int i = 0; i < w.parts; ++i) m = fmaxf(m, __hip_atomic_load(logs + i * stride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    float total = 0.0f, y[kDims] = {};
-#pragma unroll 4
-    for(int i = 0; i < w.parts; ++i) {
-      const float l = __hip_atomic_load(logs + i * stride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const float weight = l == kNone ? 0.0f : __builtin_amdgcn_exp2f(l - m);
-      total += weight;
 #pragma unroll
-      for(int j = 0; j < kDims; j += 2) {
-        const unsigned long long x = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(from + i * stride + j), __ATOMIC_RELAXED,
-                                                       __HIP_MEMORY_SCOPE_AGENT);
-        y[j] = __builtin_fmaf(weight, __builtin_bit_cast(float, (unsigned)x), y[j]);
-        y[j + 1] = __builtin_fmaf(weight, __builtin_bit_cast(float, (unsigned)(x >> 32)), y[j + 1]);
+    for(int i = 0; i < kKeys; ++i)
+#pragma unroll
+      for(int t = 0; t < kRegs; ++t) s[i][t] *= key.scale[i];
+    fetch_keys(key, at + kTurn);
+    // Positions that a row does not see score minus infinity (a weight of zero) and have a scale of zero.
+    float scale[kKeys][kRegs];
+#pragma unroll
+    for(int i = 0; i < kKeys; ++i)
+#pragma unroll
+      for(int t = 0; t < kRegs; ++t) scale[i][t] = value.scale[i];
+    if(at + 64 > x.open) {
+#pragma unroll
+      for(int i = 0; i < kKeys; ++i) {
+        const int p = at + B::key_of(i, lane), j = p - x.w.len;
+#pragma unroll
+        for(int t = 0; t < kRegs; ++t) {
+          const bool see = a.parents ? p < end && (j < 0 || (sight[t].sees >> (j & 63) & 1) != 0) : p < sight[t].limit;
+          s[i][t] = see ? s[i][t] : kNone;
+          scale[i][t] = see ? scale[i][t] : 0.0f;
+        }
       }
     }
-    const float per = total == 0.0f ? 0.0f : 1.0f / total;
+    float high[kRegs], wide[kRegs];
+    bool grown = false;
 #pragma unroll
-    for(int j = 0; j < kDims; ++j) y[j] *= per;
-    store_row<kDims, T>(row_out(row0 + 16 * t + r) + d_mine, y);
+    for(int t = 0; t < kRegs; ++t) {
+      high[t] = (kKeys == 1 ? s[0][t] : fmaxf(s[0][t], s[kKeys - 1][t])) * row_scale[t];
+      wide[t] = kKeys == 1 ? scale[0][t] : fmaxf(scale[0][t], scale[kKeys - 1][t]);
+      grown |= high[t] > top[t] + kMaximumSlack || wide[t] > unit[t] * kScaleSlack;
+    }
+    if(__any(grown)) {
+      float both[kRegs];
+#pragma unroll
+      for(int t = 0; t < kRegs; ++t) {
+        // (a NaN is left out by both maxima, its row by its sum)
+        const float m = fmaxf(top[t], over_rows_lanes(high[t], larger)), u = fmaxf(unit[t], over_rows_lanes(wide[t], larger));
+        const float down = m == top[t] ? 1.0f : __builtin_amdgcn_exp2f(top[t] - m);
+        both[t] = u == unit[t] ? down : down * (unit[t] / u);
+        sum[t] *= down;
+        top[t] = m;
+        unit[t] = u;
+        per[t] = kWeightUnit / u;
+      }
+      const float factor = of_row(both);
+#pragma unroll
+      for(int j = 0; j < kDims; ++j) o[0][j] *= factor;
+    }
+    // weights
+#pragma unroll
+    for(int i = 0; i < kKeys; ++i) {
+      const int p = B::key_of(i, lane), slot = (p & 32) + 8 * (p & 3) + (p >> 2 & 7);
+#pragma unroll
+      for(int t = 0; t < kRegs; ++t) {
+        const float from = top[t] == kNone ? 0.0f : -top[t];   // (nothing seen so far: minus infinity stays that)
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][t], row_scale[t], from)), z = y * (scale[i][t] * per[t]);
+        sum[t] += y;
+        const _Float16 hi = (_Float16)z;
+        sh.weights[wave][0][mine0 + t][slot] = hi;
+        if constexpr(kTerms == 2) sh.weights[wave][kTerms - 1][mine0 + t][slot] = (_Float16)(z - (float)hi);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();   // (a wave's accesses to LDS are done in their order)
+    // weighted values
+#pragma unroll
+    for(int h = 0; h < 2; ++h) {
+      cache_h8 p[kTerms];
+#pragma unroll
+      for(int m = 0; m < kTerms; ++m) p[m] = *reinterpret_cast<const cache_h8*>(&sh.weights[wave][m][c % ROWS][32 * h + 8 * g]);
+      unsigned vh[8][A::kWords];
+#pragma unroll
+      for(int e = 0; e < 8; ++e)
+#pragma unroll
+        for(int i = 0; i < A::kWords; ++i) vh[e][i] = held<F>(value.code[h][e][i]);
+#pragma unroll
+      for(int i = 0; i < A::kWords; ++i) {
+        const cache_h8 d[4] = {A::template value_operand<0>(vh, i), A::template value_operand<1>(vh, i), A::template value_operand<2>(vh, i),
+                               A::template value_operand<3>(vh, i)};
+#pragma unroll
+        for(int j = 0; j < 4; ++j)
+#pragma unroll
+          for(int m = kTerms - 1; m >= 0; --m) o[0][4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d[j], p[m], o[0][4 * i + j], 0, 0, 0);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    fetch_values(value, at + kTurn);
   }
+#pragma unroll
+  for(int t = 0; t < kRegs; ++t) sum[t] = over_rows_lanes(sum[t], added);
+  float row_top[1] = {of_row(top)}, row_sum[1] = {of_row(sum) * 0.25f}, row_unit[1] = {of_row(unit)};   // (four lanes of a row add up in the end)
+  if(WAVES > 1) __syncthreads();   // (the weights' memory is taken for the results)
+  cache_finish<T, F, DP, 1, WAVES>(a, x, o, row_top, row_sum, row_unit, sh.join);
 }
 
 }  // namespace marian_hip

@@ -19,6 +19,8 @@ typedef _Float16 cache_h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 cache_b2 __attribute__((ext_vector_type(2)));
 typedef short cache_s2 __attribute__((ext_vector_type(2)));
 
+__device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
+
 struct bf16_t {   // sixteen bits of a bfloat16
   uint16_t bits;
 };

@@ -8,7 +8,7 @@
 
 #include "../../include/marian_hip_int8.h"
 #include "abi_common.h"
-#include "cache_attention_kernel.h"
+#include "cache_attention.h"
 #include "cache_codes.h"
 #include "cache_plan.h"
 
@@ -607,19 +607,9 @@ int marian_hip_cache_attention(const marian_hip_kv_cache* cache, const marian_hi
   a.items = (int)p.items;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  return for_type(type, [&](auto t) -> int {
-    using T = decltype(t);
-    return for_format(cache->format, [&](auto f) -> int {
-      constexpr CacheFormat F = decltype(f)::value;
-      const dim3 grid((unsigned)p.grid), block(256);
-      if(p.dp == 64 && p.qt == 1) MH_LAUNCH((cache_attention_kernel<T, F, 64, 1>), grid, block, 0, st, a);
-      else if(p.dp == 64) MH_LAUNCH((cache_attention_kernel<T, F, 64, 2>), grid, block, 0, st, a);
-      else if(p.dp == 128 && p.qt == 1) MH_LAUNCH((cache_attention_kernel<T, F, 128, 1>), grid, block, 0, st, a);
-      else if(p.dp == 128) MH_LAUNCH((cache_attention_kernel<T, F, 128, 2>), grid, block, 0, st, a);
-      else MH_LAUNCH((cache_attention_kernel<T, F, 256, 1>), grid, block, 0, st, a);
-      return MARIAN_HIP_OK;
-    });
-  });
+  if(type == MARIAN_HIP_FLOAT32) return launch_cache_attention_float32(a, p, cache->format, st);
+  if(type == MARIAN_HIP_FLOAT16) return launch_cache_attention_float16(a, p, cache->format, st);
+  return launch_cache_attention_bfloat16(a, p, cache->format, st);
 }
 
 int marian_hip_cache_keep(const marian_hip_kv_cache* cache, const int32_t* lens, const int32_t* path, int64_t path_len,

@@ -7,12 +7,14 @@
 
 namespace marian_hip {
 
-constexpr int kCacheBlock = 128;        // positions that a workgroup's four waves take in one turn
-constexpr int kCacheWorkgroups = 1024;  // what the positions of few rows are split for: four to a CU
+constexpr int kCacheBlock = 128;    // positions that parts are counted in: four waves take as many in one turn
+constexpr int kCacheWaves = 4096;   // what the positions of few rows are split for: four to a SIMD
 
 struct CacheAttentionPlan {
   int dp;              // values of a row as the kernel holds it: dk rounded up to 64, 128 or 256
   int qt;              // sixteens of query rows to a workgroup
+  int few;             // the rows of an entry, up to 1, 2, 4 or 8 of them (0: more, or values too long for that form)
+  int waves;           // of a workgroup, which share its positions
   int64_t row_tiles;   // workgroups that share an entry's positions
   int64_t target;      // parts that the positions of all sequences together are split into
   int64_t items;       // the most parts there can be, a sequence having at least one
@@ -27,9 +29,12 @@ inline CacheAttentionPlan cache_attention_plan(int64_t sequences, int64_t heads,
   CacheAttentionPlan p{};
   p.dp = dk <= 64 ? 64 : dk <= 128 ? 128 : 256;
   const int64_t rows = n * (q_heads / heads);
+  p.few = rows > 8 || p.dp == 256 ? 0 : rows > 4 ? 8 : rows > 2 ? 4 : (int)rows;
   p.qt = rows <= 16 || p.dp == 256 ? 1 : 2;   // (what the registers hold)
   p.row_tiles = (rows + 16 * p.qt - 1) / (16 * p.qt);
-  p.target = std::max<int64_t>(1, kCacheWorkgroups / (heads * p.row_tiles));
+  const int64_t entries = sequences * heads * p.row_tiles;
+  p.waves = entries >= 4096 ? 1 : entries >= 2048 ? 2 : 4;
+  p.target = std::max<int64_t>(1, kCacheWaves / p.waves / (heads * p.row_tiles));
   p.items = p.target == 1 ? sequences : p.target + sequences;
   p.slots = p.target == 1 ? 0 : 2 * p.target;
   p.grid = (p.items * heads + 7) / 8 * 8 * p.row_tiles;
@@ -37,9 +42,9 @@ inline CacheAttentionPlan cache_attention_plan(int64_t sequences, int64_t heads,
   return p;
 }
 
-// The workspace: a counter for each row tile of a sequence with several parts (at most slots * heads * row_tiles, 2 * kCacheWorkgroups of
+// The workspace: a counter for each row tile of a sequence with several parts (at most slots * heads * row_tiles, 2 * kCacheWaves of
 // them), in the same place for all sizes, then the partial results.
-constexpr int64_t kCacheCounterBytes = 2 * kCacheWorkgroups * 4;
+constexpr int64_t kCacheCounterBytes = 2 * kCacheWaves * 4;
 inline int64_t cache_attention_bytes(const CacheAttentionPlan& p, int64_t heads) {
   return p.slots == 0 ? 0 : kCacheCounterBytes + p.slots * heads * p.row_tiles * 16 * p.qt * p.row_floats * 4;
 }
