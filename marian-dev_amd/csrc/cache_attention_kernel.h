@@ -27,6 +27,8 @@
 // last position in reach, whose codes are finite whatever they hold.
 #pragma once
 
+#include <type_traits>
+
 #include "cache_attention.h"
 #include "cache_codes.h"
 
@@ -74,12 +76,13 @@ __device__ __forceinline__ bool cache_part(const CacheAttentionArgs& a, int item
     for(int i = 0; i < kHeld; ++i) total += held[i];
     for(int base = 64 * kHeld; base < a.S; base += 64) total += blocks_of(base + lane);
     total = (unsigned)__builtin_amdgcn_readlane((int)lanes_sum(total), 63);
-    each = max(1u, (total + a.target - 1) / a.target);
+    each = max((unsigned)a.least, (total + a.target - 1) / a.target);
+    auto size_of = [&](unsigned mine) { return max(each, (mine + kCacheMostParts - 1) / kCacheMostParts); };
     // parts in the lower bits, those of sequences with several in the upper twelve (less than 2 * target)
     unsigned before = 0;
     bool found = false;
     auto look = [&](int base, unsigned mine) __attribute__((always_inline)) {
-      const unsigned parts = base + lane < a.S ? max(1u, (mine + each - 1) / each) : 0;
+      const unsigned size = size_of(mine), parts = base + lane < a.S ? max(1u, (mine + size - 1) / size) : 0;
       const unsigned sum = before + lanes_sum(parts > 1 ? parts | parts << 20 : parts);
       const unsigned long long at = __ballot((int)(sum & 0xfffff) > item);
       if(at) {
@@ -102,8 +105,10 @@ __device__ __forceinline__ bool cache_part(const CacheAttentionArgs& a, int item
   w.len = clamp_int(a.lens[w.s], 0, a.cap);
   w.count = a.counts ? clamp_int(a.counts[w.s], 0, a.n) : a.n;
   w.used = w.count > 0 ? min(w.len + w.count, a.cap) : 0;
-  w.from = a.target > 1 ? w.part * (int)each * kCacheBlock : 0;
-  w.to = a.target > 1 ? min(w.from + (int)each * kCacheBlock, w.used) : w.used;
+  const unsigned mine = (unsigned)(w.used + kCacheBlock - 1) / kCacheBlock;
+  const int size = (int)max(each, (mine + kCacheMostParts - 1) / kCacheMostParts) * kCacheBlock;
+  w.from = a.target > 1 ? w.part * size : 0;
+  w.to = a.target > 1 ? min(w.from + size, w.used) : w.used;
   return true;
 }
 
@@ -191,15 +196,46 @@ struct CacheAttention {
   }
 };
 
-// The maximum over the four lanes of a query row.
-__device__ __forceinline__ float over_lanes_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16, 64));
-  return fmaxf(x, __shfl_xor(x, 32, 64));
+// Values of lanes that differ in one bit of their number, joined: bits 4 and 5 by an exchange of whole rows of sixteen lanes (in
+// assembly, with the wait states around it: the compiler's builtin gives one of the two registers only).
+template <typename Join>
+__device__ __forceinline__ float over_bit4(float x, Join join) {
+  float y = x;
+  asm("s_nop 3\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 3" : "+v"(x), "+v"(y));
+  return join(x, y);
 }
-__device__ __forceinline__ float over_lanes_sum(float x) {
-  x += __shfl_xor(x, 16, 64);
-  return x + __shfl_xor(x, 32, 64);
+template <typename Join>
+__device__ __forceinline__ float over_bit5(float x, Join join) {
+  float y = x;
+  asm("s_nop 3\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 3" : "+v"(x), "+v"(y));
+  return join(x, y);
 }
+// Over the sixteen lanes of a row, by rotations.
+template <typename Join>
+__device__ __forceinline__ float over_row(float x, Join join) {
+  auto turned = [](float y, auto by) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, y), 0x120 + decltype(by)::value, 0xf, 0xf, false));
+  };
+  x = join(x, turned(x, std::integral_constant<int, 8>()));
+  x = join(x, turned(x, std::integral_constant<int, 4>()));
+  x = join(x, turned(x, std::integral_constant<int, 2>()));
+  return join(x, turned(x, std::integral_constant<int, 1>()));
+}
+struct Larger {
+  __device__ __forceinline__ float operator()(float x, float y) const { return fmaxf(x, y); }
+};
+struct Added {
+  __device__ __forceinline__ float operator()(float x, float y) const { return x + y; }
+};
+struct LargerBits {   // (of magnitudes: NaN is above all)
+  __device__ __forceinline__ float operator()(float x, float y) const {
+    return __builtin_bit_cast(float, max(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y)));
+  }
+};
+// The maximum, and the sum, over the four lanes of a query row.
+__device__ __forceinline__ float over_lanes_max(float x) { return over_bit5(over_bit4(x, Larger()), Larger()); }
+__device__ __forceinline__ float over_lanes_sum(float x) { return over_bit5(over_bit4(x, Added()), Added()); }
+__device__ __forceinline__ float lane_value(float x, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane)); }
 
 constexpr float kNone = -__builtin_huge_valf();
 
@@ -214,7 +250,9 @@ struct CacheTile {
 
 template <typename T>
 __device__ __forceinline__ T* cache_row_out(const CacheAttentionArgs& a, const CacheTile& x, int r) {
-  return static_cast<T*>(a.out) + x.w.s * a.o_s + (long long)(x.head * a.G + r % a.G) * a.o_h + (long long)(r / a.G) * a.o_n;
+  unsigned of_group;
+  const unsigned token = a.by_group.of((unsigned)r, of_group);
+  return static_cast<T*>(a.out) + x.w.s * a.o_s + (long long)(x.head * a.G + (int)of_group) * a.o_h + (long long)token * a.o_n;
 }
 
 // Finds a workgroup's tile and clears the rows of it that are not there; false where nothing is to be done.
@@ -222,11 +260,13 @@ template <typename T, int DP, int ROWS, int WAVES>
 __device__ __forceinline__ bool cache_tile(const CacheAttentionArgs& a, int tid, CacheTile& x) {
   constexpr int kDims = DP / 16;
   // Workgroups with the same positions follow each other on one XCD (a workgroup to each of the eight in turn).
-  const int place = blockIdx.x >> 3, entry = place / a.row_tiles * 8 + (blockIdx.x & 7);
-  x.tile = place % a.row_tiles;
+  unsigned tile, head;
+  const int entry = (int)a.by_tiles.of(blockIdx.x >> 3, tile) * 8 + (blockIdx.x & 7);
   if(entry >= a.items * a.Hk) return false;
-  x.head = entry % a.Hk;
-  if(!cache_part(a, entry / a.Hk, tid & 63, x.w)) return false;
+  const int item = (int)a.by_heads.of((unsigned)entry, head);
+  x.tile = (int)tile;
+  x.head = (int)head;
+  if(!cache_part(a, item, tid & 63, x.w)) return false;
   x.rows = x.w.count * a.G;
   x.row0 = x.tile * ROWS;
   if(x.w.part == 0 && x.row0 + ROWS > x.rows) {
@@ -237,9 +277,9 @@ __device__ __forceinline__ bool cache_tile(const CacheAttentionArgs& a, int tid,
     }
   }
   if(x.row0 >= x.rows) return false;
-  const int last_token = min(x.rows - 1, x.row0 + ROWS - 1) / a.G;
+  const int last_token = (int)a.by_group.of((unsigned)min(x.rows - 1, x.row0 + ROWS - 1));
   x.end = min(x.w.to, x.w.len + last_token + 1);
-  x.open = min(x.end, x.w.len + (a.parents ? 0 : x.row0 / a.G + 1));
+  x.open = min(x.end, x.w.len + (a.parents ? 0 : (int)a.by_group.of((unsigned)x.row0) + 1));
   const long long first = ((long long)x.w.s * a.Hk + x.head) * a.cap;
   x.k = a.k + first * a.dk;
   x.v = a.v + first * a.dk;
@@ -254,7 +294,7 @@ struct CacheSight {
   unsigned long long sees;
 };
 __device__ __forceinline__ CacheSight cache_sight(const CacheAttentionArgs& a, const CacheTile& x, int row, unsigned long long seen) {
-  const int token = row / a.G;
+  const int token = (int)a.by_group.of((unsigned)row);
   CacheSight y{min(x.end, x.w.len + token + 1), 0};
   if(a.parents) {
     const unsigned lo = __shfl((unsigned)seen, token, 64), hi = __shfl((unsigned)(seen >> 32), token, 64);
@@ -268,7 +308,9 @@ template <typename T, CacheFormat F, int DP>
 __device__ __forceinline__ float cache_query(const CacheAttentionArgs& a, const CacheTile& x, int row, int g,
                                              cache_h8 (&q)[CacheAttention<T, F, DP>::kTerms][DP / 32]) {
   constexpr int kTerms = CacheAttention<T, F, DP>::kTerms, kSteps = DP / 32;
-  const T* p = static_cast<const T*>(a.q) + x.w.s * a.q_s + (long long)(x.head * a.G + row % a.G) * a.q_h + (long long)(row / a.G) * a.q_n;
+  unsigned of_group;
+  const unsigned token = a.by_group.of((unsigned)row, of_group);
+  const T* p = static_cast<const T*>(a.q) + x.w.s * a.q_s + (long long)(x.head * a.G + (int)of_group) * a.q_h + (long long)token * a.q_n;
   float y[kSteps][8];
   unsigned most = 0;   // bits of the row's largest magnitude (NaN above all)
 #pragma unroll
@@ -280,8 +322,7 @@ __device__ __forceinline__ float cache_query(const CacheAttentionArgs& a, const 
 #pragma unroll
     for(int e = 0; e < 8; ++e) most = max(most, __builtin_bit_cast(unsigned, y[i][e]) & 0x7fffffffu);
   }
-  most = max(most, (unsigned)__shfl_xor((int)most, 16, 64));
-  most = max(most, (unsigned)__shfl_xor((int)most, 32, 64));
+  most = __builtin_bit_cast(unsigned, over_bit5(over_bit4(__builtin_bit_cast(float, most), LargerBits()), LargerBits()));
   const int up = clamp_int(127 + 14 + 127 - (int)(most >> 23), 2, 252);   // exponent that brings it to 2^14
   const float factor = __builtin_bit_cast(float, (unsigned)up << 23), back = __builtin_bit_cast(float, (unsigned)(254 - up) << 23);
 #pragma unroll
@@ -417,36 +458,85 @@ __device__ __forceinline__ void cache_finish(const CacheAttentionArgs& a, const 
   }
   __syncthreads();
   if(!sh.is_last) return;
+  // Sixteen threads to a row; where there are fewer rows than sixteens, several of them share a row's parts.  A batch of parts is
+  // asked for at a time: the loads come from the memory side, about a microsecond away.
   const float* const all = a.part + place_of_tile * kTileFloats;
   const long long stride = part_stride * kTileFloats;
-  const int d_mine = (tid & 15) * kDims;   // of a row to sixteen threads
-  if(d_mine >= a.dk) return;
+  constexpr int kGroups = 4 * WAVES, kBatch = DP == 256 ? 4 : 8;
+  const int here = min(16 * QT, x.rows - x.row0), group = tid >> 4, d_mine = (tid & 15) * kDims;
+  int share = 1;
+  while(share * here * 2 <= kGroups) share *= 2;
 #pragma unroll 1
-  for(int r = tid >> 4; r < min(16 * QT, x.rows - x.row0); r += 4 * WAVES) {
+  for(int r = group / share; r < here; r += kGroups / share) {   // (one turn where parts are shared)
     const float* logs = all + 16 * QT * DP + r;
-    const float* from = all + r * DP + d_mine;
-    float m = kNone;
-#pragma unroll 4
-    for(int i = 0; i < x.w.parts; ++i) m = fmaxf(m, __hip_atomic_load(logs + i * stride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    float total = 0.0f, y[kDims] = {};
-#pragma unroll 4
-    for(int i = 0; i < x.w.parts; ++i) {
-      const float l = __hip_atomic_load(logs + i * stride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const float weight = l == kNone ? 0.0f : __builtin_amdgcn_exp2f(l - m);
-      total += weight;
+    const float* from = all + r * DP + (d_mine < a.dk ? d_mine : 0);
+    float m = kNone, total = 0.0f, y[kDims] = {};
+#pragma unroll 1
+    for(int i = group % share; i < x.w.parts; i += kBatch * share) {
+      float l[kBatch];
+      unsigned long long z[kBatch][kDims / 2];
 #pragma unroll
-      for(int j = 0; j < kDims; j += 2) {
-        const unsigned long long x = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(from + i * stride + j), __ATOMIC_RELAXED,
-                                                       __HIP_MEMORY_SCOPE_AGENT);
-        y[j] = __builtin_fmaf(weight, __builtin_bit_cast(float, (unsigned)x), y[j]);
-        y[j + 1] = __builtin_fmaf(weight, __builtin_bit_cast(float, (unsigned)(x >> 32)), y[j + 1]);
+      for(int b = 0; b < kBatch; ++b) {
+        l[b] = kNone;
+#pragma unroll
+        for(int j = 0; j < kDims / 2; ++j) z[b][j] = 0;
+        if(i + b * share < x.w.parts) {
+          const long long at = (i + b * share) * stride;
+          l[b] = __hip_atomic_load(logs + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+          for(int j = 0; j < kDims / 2; ++j)
+            z[b][j] = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(from + at) + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+      }
+      float next = m;
+#pragma unroll
+      for(int b = 0; b < kBatch; ++b) next = fmaxf(next, l[b]);
+      const float down = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      total *= down;
+#pragma unroll
+      for(int j = 0; j < kDims; ++j) y[j] *= down;
+#pragma unroll
+      for(int b = 0; b < kBatch; ++b) {
+        const float weight = l[b] == kNone ? 0.0f : __builtin_amdgcn_exp2f(l[b] - m);
+        total += weight;
+#pragma unroll
+        for(int j = 0; j < kDims; ++j) y[j] = __builtin_fmaf(weight, __builtin_bit_cast(float, (unsigned)(z[b][j / 2] >> (32 * (j % 2)))), y[j]);
       }
     }
-    const float per = total == 0.0f ? 0.0f : 1.0f / total;
+    if(share > 1) {   // (r is the only row of all threads: sixteens beyond the rows have left)
+      float* const rest = &sh.joined[0][0][0] + group * (16 * kDims) + (tid & 15) * kDims;
 #pragma unroll
-    for(int j = 0; j < kDims; ++j) y[j] *= per;
-    store_row<kDims, T>(cache_row_out<T>(a, x, x.row0 + r) + d_mine, y);
+      for(int j = 0; j < kDims; ++j) rest[j] = y[j];
+      if((tid & 15) == 0) {
+        (&sh.row_max[0][0])[group] = m;
+        (&sh.row_sum[0][0])[group] = total;
+      }
+    }
+    if(share == 1 && d_mine < a.dk) {
+      const float per = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+      for(int j = 0; j < kDims; ++j) y[j] *= per;
+      store_row<kDims, T>(cache_row_out<T>(a, x, x.row0 + r) + d_mine, y);
+    }
   }
+  if(share == 1) return;
+  __syncthreads();
+  const int r = group / share;
+  if(group % share != 0 || r >= here || d_mine >= a.dk) return;
+  float m = kNone, total = 0.0f, y[kDims] = {};
+  for(int i = 0; i < share; ++i) m = fmaxf(m, (&sh.row_max[0][0])[group + i]);
+  for(int i = 0; i < share; ++i) {
+    const float from = (&sh.row_max[0][0])[group + i], weight = from == kNone ? 1.0f : __builtin_amdgcn_exp2f(from - m);   // (of none: 0, or NaN)
+    const float* const rest = &sh.joined[0][0][0] + (group + i) * (16 * kDims) + (tid & 15) * kDims;
+    total += (&sh.row_sum[0][0])[group + i] * weight;
+#pragma unroll
+    for(int j = 0; j < kDims; ++j) y[j] = __builtin_fmaf(rest[j], weight, y[j]);
+  }
+  const float per = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+  for(int j = 0; j < kDims; ++j) y[j] *= per;
+  store_row<kDims, T>(cache_row_out<T>(a, x, x.row0 + r) + d_mine, y);
 }
 
 // ---- sixteen rows and more to a wave
@@ -473,8 +563,10 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
   const int begin = x.w.from + 32 * wave;
   typename A::Keys key;
   typename A::Values value;
-  fetch_keys(key, begin);
-  fetch_values(value, begin);
+  if(begin < end) {
+    A::template load<true>(key, x.k, x.ks, begin, end - 1, a.dk, lane);
+    A::template load<true>(value, x.v, x.vs, begin, end - 1, a.dk, lane);
+  }
   unsigned long long seen = 0;
   if(a.parents) seen = lineage(a.parents + (long long)x.w.s * a.n, a.n, lane);
   cache_h8 q[QT][kTerms][kSteps];
@@ -713,8 +805,10 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
   const int begin = x.w.from + 64 * wave;
   typename B::Keys key;
   typename B::Values value;
-  fetch_keys(key, begin);
-  fetch_values(value, begin);
+  if(begin < end) {
+    B::template load<true>(key, x.k, x.ks, begin, end - 1, a.dk, lane);
+    B::template load<true>(value, x.v, x.vs, begin, end - 1, a.dk, lane);
+  }
   unsigned long long seen = 0;
   if(a.parents) seen = lineage(a.parents + (long long)x.w.s * a.n, a.n, lane);
   cache_h8 q[kTerms][kSteps];
@@ -724,7 +818,8 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
   CacheSight sight[kRegs];
 #pragma unroll
   for(int t = 0; t < kRegs; ++t) {
-    row_scale[t] = __shfl(query_scale, mine0 + t, 64);
+    row_scale[t] = lane_value(query_scale, t);
+    if constexpr(ROWS == 8) row_scale[t] = g & 1 ? lane_value(query_scale, t + 4) : row_scale[t];
     sight[t] = cache_sight(a, x, min(x.row0 + mine0 + t, x.rows - 1), seen);
   }
   cache_f4 o[1][kDims];
@@ -740,23 +835,19 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
   }
   // of row c, what the lanes that have its scores hold
   auto of_row = [&](const float(&y)[kRegs]) __attribute__((always_inline)) {
-    const int from = ROWS == 8 ? (c >> 2 & 1) * 16 : 0;
-    float z = ROWS == 8 ? __shfl(y[0], from, 64) : y[0];
+    float z = 0.0f;
 #pragma unroll
-    for(int t = 1; t < kRegs; ++t) {
-      const float next = ROWS == 8 ? __shfl(y[t], from, 64) : y[t];
-      z = (c & 3) == t ? next : z;
+    for(int r = 0; r < ROWS; ++r) {
+      const float it = lane_value(y[r % 4], r < 4 ? 0 : 16);
+      z = r == 0 || c % ROWS == r ? it : z;
     }
     return z;
   };
   auto over_rows_lanes = [&](float y, auto join) __attribute__((always_inline)) {   // over the lanes that have scores of the same rows
-#pragma unroll
-    for(int i = 1; i < 64; i <<= 1)
-      if(ROWS != 8 || i != 16) y = join(y, __shfl_xor(y, i, 64));
+    y = over_bit5(over_row(y, join), join);
+    if constexpr(ROWS != 8) y = over_bit4(y, join);
     return y;
   };
-  auto larger = [](float y, float z) { return fmaxf(y, z); };
-  auto added = [](float y, float z) { return y + z; };
 
   for(int at = begin; at < end; at += kTurn) {
     // scores
@@ -820,7 +911,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
 #pragma unroll
       for(int t = 0; t < kRegs; ++t) {
         // (a NaN is left out by both maxima, its row by its sum)
-        const float m = fmaxf(top[t], over_rows_lanes(high[t], larger)), u = fmaxf(unit[t], over_rows_lanes(wide[t], larger));
+        const float m = fmaxf(top[t], over_rows_lanes(high[t], Larger())), u = fmaxf(unit[t], over_rows_lanes(wide[t], Larger()));
         const float down = m == top[t] ? 1.0f : __builtin_amdgcn_exp2f(top[t] - m);
         both[t] = u == unit[t] ? down : down * (unit[t] / u);
         sum[t] *= down;
@@ -872,7 +963,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
     fetch_values(value, at + kTurn);
   }
 #pragma unroll
-  for(int t = 0; t < kRegs; ++t) sum[t] = over_rows_lanes(sum[t], added);
+  for(int t = 0; t < kRegs; ++t) sum[t] = over_rows_lanes(sum[t], Added());
   float row_top[1] = {of_row(top)}, row_sum[1] = {of_row(sum) * 0.25f}, row_unit[1] = {of_row(unit)};   // (four lanes of a row add up in the end)
   if(WAVES > 1) __syncthreads();   // (the weights' memory is taken for the results)
   cache_finish<T, F, DP, 1, WAVES>(a, x, o, row_top, row_sum, row_unit, sh.join);

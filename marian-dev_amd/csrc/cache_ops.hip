@@ -604,7 +604,11 @@ int marian_hip_cache_attention(const marian_hip_kv_cache* cache, const marian_hi
   a.dk = (int)dk;
   a.row_tiles = (int)p.row_tiles;
   a.target = (int)p.target;
+  a.least = p.least;
   a.items = (int)p.items;
+  a.by_tiles = CacheDivisor((unsigned)p.row_tiles);
+  a.by_heads = CacheDivisor((unsigned)heads);
+  a.by_group = CacheDivisor((unsigned)a.G);
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if(type == MARIAN_HIP_FLOAT32) return launch_cache_attention_float32(a, p, cache->format, st);

@@ -8,7 +8,8 @@
 namespace marian_hip {
 
 constexpr int kCacheBlock = 128;    // positions that parts are counted in: four waves take as many in one turn
-constexpr int kCacheWaves = 4096;   // what the positions of few rows are split for: four to a SIMD
+constexpr unsigned kCacheMostParts = 48;   // of a sequence: joining them takes as long as what they save
+constexpr int kCacheMost = 8192;    // counters of a workspace: two for each of the workgroups that positions are split for
 
 struct CacheAttentionPlan {
   int dp;              // values of a row as the kernel holds it: dk rounded up to 64, 128 or 256
@@ -16,6 +17,7 @@ struct CacheAttentionPlan {
   int few;             // the rows of an entry, up to 1, 2, 4 or 8 of them (0: more, or values too long for that form)
   int waves;           // of a workgroup, which share its positions
   int64_t row_tiles;   // workgroups that share an entry's positions
+  int least;           // blocks of a part
   int64_t target;      // parts that the positions of all sequences together are split into
   int64_t items;       // the most parts there can be, a sequence having at least one
   int64_t slots;       // the most parts of sequences that have more than one: these leave partial results
@@ -34,7 +36,12 @@ inline CacheAttentionPlan cache_attention_plan(int64_t sequences, int64_t heads,
   p.row_tiles = (rows + 16 * p.qt - 1) / (16 * p.qt);
   const int64_t entries = sequences * heads * p.row_tiles;
   p.waves = entries >= 4096 ? 1 : entries >= 2048 ? 2 : 4;
-  p.target = std::max<int64_t>(1, kCacheWaves / p.waves / (heads * p.row_tiles));
+  // Workgroups that run at a time, by the registers of their form, and parts for twice as many (a sequence's last part is half as
+  // long as the others on average).
+  const int to_a_simd = p.few ? (p.dp == 128 ? 2 : p.few <= 2 ? 4 : 3) : p.dp == 64 ? 5 - p.qt : p.dp == 128 ? 4 - p.qt : 2;
+  const int64_t at_a_time = 1024 * to_a_simd / p.waves;
+  p.target = std::max<int64_t>(1, at_a_time / (heads * p.row_tiles) - sequences / 2);
+  p.least = entries >= at_a_time || !p.few ? 4 : 2;
   p.items = p.target == 1 ? sequences : p.target + sequences;
   p.slots = p.target == 1 ? 0 : 2 * p.target;
   p.grid = (p.items * heads + 7) / 8 * 8 * p.row_tiles;
@@ -42,9 +49,9 @@ inline CacheAttentionPlan cache_attention_plan(int64_t sequences, int64_t heads,
   return p;
 }
 
-// The workspace: a counter for each row tile of a sequence with several parts (at most slots * heads * row_tiles, 2 * kCacheWaves of
+// The workspace: a counter for each row tile of a sequence with several parts (at most slots * heads * row_tiles, kCacheMost of
 // them), in the same place for all sizes, then the partial results.
-constexpr int64_t kCacheCounterBytes = 2 * kCacheWaves * 4;
+constexpr int64_t kCacheCounterBytes = kCacheMost * 4;
 inline int64_t cache_attention_bytes(const CacheAttentionPlan& p, int64_t heads) {
   return p.slots == 0 ? 0 : kCacheCounterBytes + p.slots * heads * p.row_tiles * 16 * p.qt * p.row_floats * 4;
 }
