@@ -102,8 +102,9 @@ __device__ __forceinline__ bool cache_part(const CacheAttentionArgs& a, int item
     for(int base = 64 * kHeld; base < a.S && !found; base += 64) look(base, blocks_of(base + lane));
     if(!found) return false;
   }
-  w.len = clamp_int(a.lens[w.s], 0, a.cap);
-  w.count = a.counts ? clamp_int(a.counts[w.s], 0, a.n) : a.n;
+  w.s = __builtin_amdgcn_readfirstlane(w.s);
+  w.len = __builtin_amdgcn_readfirstlane(clamp_int(a.lens[w.s], 0, a.cap));
+  w.count = a.counts ? __builtin_amdgcn_readfirstlane(clamp_int(a.counts[w.s], 0, a.n)) : a.n;
   w.used = w.count > 0 ? min(w.len + w.count, a.cap) : 0;
   const unsigned mine = (unsigned)(w.used + kCacheBlock - 1) / kCacheBlock;
   const int size = (int)max(each, (mine + kCacheMostParts - 1) / kCacheMostParts) * kCacheBlock;
@@ -120,81 +121,63 @@ struct CacheAttention {
   static constexpr int kDims = DP / 16;                   // of a value's row to a lane
   static constexpr int kWords = kDims / 4;
 
-  // 32 positions as they are loaded: what is needed for the scores, and what is needed behind them.
+  // 32 positions as they are loaded.
   struct Keys {
     cache_u4 code[2][kPieces];
-    cache_f4 scale[2];
   };
   struct Values {
     unsigned code[8][kWords];
-    cache_f4 scale[2];
   };
+};
 
-  // Positions at .. at + 31 of an entry; ENDS: those behind `last` are `last`.  Lanes past a row's end (dk < DP) take its start: the
-  // queries are zero there, and the values are not stored.
-  template <bool ENDS>
-  static __device__ __forceinline__ void load(Keys& t, const unsigned char* k, const float* scale, int at, int last, int dk, int lane) {
-    const int c = lane & 15, g = lane >> 4;
-#pragma unroll
-    for(int b = 0; b < 2; ++b) {
-      const unsigned row = ENDS ? (unsigned)min(at + 16 * b + c, last) * dk : (unsigned)(at + c) * dk;
-      const unsigned char* p = ENDS ? k : k + (size_t)(16 * b * dk);
-#pragma unroll
-      for(int i = 0; i < kPieces; ++i) {
-        const unsigned d = 64 * i + 16 * g;
-        t.code[b][i] = *reinterpret_cast<const cache_u4*>(p + (row + (d < (unsigned)dk ? d : 0)));
-      }
-    }
-    load_scales<ENDS>(t.scale, scale, at, last, g);
+// The codes, or the scales, of an entry's positions up to an end, as a buffer: what lies behind it reads as zeros, so that loads need neither
+// branches nor bounds of their own.  (A branch around loads whose registers live on makes the compiler wait for them behind it.)
+// All offsets go through the lane's, against which the buffer's size is held; a load lies in one row, whole or not at all inside.
+struct CacheBuffer {
+  __amdgpu_buffer_rsrc_t rsrc;
+  __device__ __forceinline__ CacheBuffer(const void* p, unsigned bytes)
+      : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000)) {}   // (32-bit data, no swizzle)
+  __device__ __forceinline__ float number(int i) const {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, (unsigned)i * 4u, 0, 0));
   }
-  template <bool ENDS>
-  static __device__ __forceinline__ void load(Values& t, const unsigned char* v, const float* scale, int at, int last, int dk, int lane) {
-    const int c = lane & 15, g = lane >> 4;
-    const unsigned d = (unsigned)(kDims * c) < (unsigned)dk ? kDims * c : 0;
-#pragma unroll
-    for(int e = 0; e < 8; ++e) {
-      const int key = 16 * (e / 4) + e % 4;
-      const unsigned row = ENDS ? (unsigned)min(at + 4 * g + key, last) * dk : (unsigned)(at + 4 * g) * dk;
-      const unsigned char* p = (ENDS ? v : v + (size_t)(key * dk)) + (row + d);
-      load_codes(t.code[e], p);
-    }
-    load_scales<ENDS>(t.scale, scale, at, last, g);
-  }
-  template <bool ENDS>
-  static __device__ __forceinline__ void load_scales(cache_f4 (&to)[2], const float* scale, int at, int last, int g) {
-#pragma unroll
-    for(int b = 0; b < 2; ++b) {
-      if(ENDS) {
-#pragma unroll
-        for(int e = 0; e < 4; ++e) to[b][e] = scale[(unsigned)min(at + 16 * b + 4 * g + e, last)];
-      } else {
-        to[b] = *reinterpret_cast<const cache_f4_any*>(scale + 16 * b + (unsigned)(at + 4 * g));
-      }
-    }
-  }
-
-  static __device__ __forceinline__ void load_codes(unsigned (&to)[kWords], const unsigned char* p) {
-    if constexpr(kWords == 1) {
-      to[0] = *reinterpret_cast<const unsigned*>(p);
-    } else if constexpr(kWords == 2) {
-      const cache_u2 x = *reinterpret_cast<const cache_u2*>(p);
+  __device__ __forceinline__ cache_u4 piece(unsigned at) const { return __builtin_bit_cast(cache_u4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0)); }
+  template <int WORDS>
+  __device__ __forceinline__ void words(unsigned (&to)[WORDS], unsigned at) const {
+    if constexpr(WORDS == 1) {
+      to[0] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, at, 0, 0);
+    } else if constexpr(WORDS == 2) {
+      const cache_u2 x = __builtin_bit_cast(cache_u2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, at, 0, 0));
       to[0] = x[0];
       to[1] = x[1];
     } else {
-      const cache_u4 x = *reinterpret_cast<const cache_u4*>(p);
+      const cache_u4 x = piece(at);
 #pragma unroll
       for(int w = 0; w < 4; ++w) to[w] = x[w];
     }
   }
-
-  // Dimension B of word W of the lane's values, eight keys.
-  template <int B>
-  static __device__ __forceinline__ cache_h8 value_operand(const unsigned (&v)[8][kWords], int w) {
-    const cache_h2 h[4] = {half2_of<F, B, B>(v[0][w], v[1][w]), half2_of<F, B, B>(v[2][w], v[3][w]),
-                           half2_of<F, B, B>(v[4][w], v[5][w]), half2_of<F, B, B>(v[6][w], v[7][w])};
-    return cache_h8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
-  }
 };
+
+// Sixteen codes at a time of rows row, row + 16, ..: lane (c, g) those of row + c from 64 i + 16 g on.  Lanes past a row's end (dk < DP) take
+// its start: the queries are zero there, and of values they are not stored.
+template <int BLOCKS, int PIECES>
+__device__ __forceinline__ void load_keys(cache_u4 (&to)[BLOCKS][PIECES], const CacheBuffer& k, int row, int dk, int lane) {
+  const unsigned at = (unsigned)(row + (lane & 15)) * dk;
+#pragma unroll
+  for(int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for(int i = 0; i < PIECES; ++i) {
+      const unsigned d = 64 * i + 16 * (lane >> 4);
+      to[b][i] = k.piece(at + (unsigned)(16 * b) * dk + (d < (unsigned)dk ? d : 0));
+    }
+}
+
+// Dimension B of word w of a lane's values, eight keys.
+template <CacheFormat F, int B, int WORDS>
+__device__ __forceinline__ cache_h8 value_operand_of(const unsigned (&v)[8][WORDS], int w) {
+  const cache_h2 h[4] = {half2_of<F, B, B>(v[0][w], v[1][w]), half2_of<F, B, B>(v[2][w], v[3][w]), half2_of<F, B, B>(v[4][w], v[5][w]),
+                         half2_of<F, B, B>(v[6][w], v[7][w])};
+  return cache_h8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
+}
 
 // Values of lanes that differ in one bit of their number, joined: bits 4 and 5 by an exchange of whole rows of sixteen lanes (in
 // assembly, with the wait states around it: the compiler's builtin gives one of the two registers only).
@@ -312,15 +295,20 @@ __device__ __forceinline__ float cache_query(const CacheAttentionArgs& a, const 
   const unsigned token = a.by_group.of((unsigned)row, of_group);
   const T* p = static_cast<const T*>(a.q) + x.w.s * a.q_s + (long long)(x.head * a.G + (int)of_group) * a.q_h + (long long)token * a.q_n;
   float y[kSteps][8];
+#pragma unroll
+  for(int i = 0; i < kSteps; ++i) {   // (past the row's end its start is read, and dropped: a branch around each load would wait for it)
+    const int d = 64 * (i / 2) + 16 * g + 8 * (i % 2);
+    load_row<8>(p + (d < a.dk ? d : 0), y[i]);
+  }
   unsigned most = 0;   // bits of the row's largest magnitude (NaN above all)
 #pragma unroll
   for(int i = 0; i < kSteps; ++i) {
     const int d = 64 * (i / 2) + 16 * g + 8 * (i % 2);
 #pragma unroll
-    for(int e = 0; e < 8; ++e) y[i][e] = 0.0f;
-    if(d < a.dk) load_row<8>(p + d, y[i]);
-#pragma unroll
-    for(int e = 0; e < 8; ++e) most = max(most, __builtin_bit_cast(unsigned, y[i][e]) & 0x7fffffffu);
+    for(int e = 0; e < 8; ++e) {
+      y[i][e] = d < a.dk ? y[i][e] : 0.0f;
+      most = max(most, __builtin_bit_cast(unsigned, y[i][e]) & 0x7fffffffu);
+    }
   }
   most = __builtin_bit_cast(unsigned, over_bit5(over_bit4(__builtin_bit_cast(float, most), LargerBits()), LargerBits()));
   const int up = clamp_int(127 + 14 + 127 - (int)(most >> 23), 2, 252);   // exponent that brings it to 2^14
@@ -337,17 +325,160 @@ __device__ __forceinline__ float cache_query(const CacheAttentionArgs& a, const 
   return most >= 0x7f800000u ? __builtin_nanf("") : fmaxf(back * (a.scale_log2 / kCodeUnit<F>), 0x1p-126f);   // (never zero)
 }
 
+// Where a workgroup's rows go: to the output, or where a sequence has several parts to the workspace.
+template <typename T, int DP, int ROWS>
+struct CacheOut {
+  static constexpr int kTileFloats = ROWS * (DP + 1);
+  const CacheAttentionArgs& a;
+  const CacheTile& x;
+  const bool whole;
+  const long long place, stride;   // of the tile's first part, of a part to the next, in tiles
+  float* const part;
+  __device__ __forceinline__ CacheOut(const CacheAttentionArgs& a_, const CacheTile& x_)
+      : a(a_), x(x_), whole(x.w.parts == 1), place(((long long)x.w.slot * a.Hk + x.head) * a.row_tiles + x.tile),
+        stride((long long)a.Hk * a.row_tiles), part(a.part + (place + x.w.part * stride) * kTileFloats) {}
+  // Values d .. of row r of the tile.
+  template <int COUNT>
+  __device__ __forceinline__ void emit(int r, int d, const float (&y)[COUNT]) const {
+    if(x.row0 + r >= x.rows || d >= a.dk) return;
+    if(whole) {
+      store_row<COUNT, T>(cache_row_out<T>(a, x, x.row0 + r) + d, y);
+    } else {
+      unsigned long long* to = reinterpret_cast<unsigned long long*>(part + r * DP + d);
+#pragma unroll
+      for(int j = 0; j < COUNT; j += 2)
+        __hip_atomic_store(to + j / 2, (unsigned long long)__builtin_bit_cast(unsigned, y[j + 1]) << 32 | __builtin_bit_cast(unsigned, y[j]),
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  // The logarithm of the sum of row r's weights, 2^m times total.
+  __device__ __forceinline__ void emit_log(int r, float m, float total) const {
+    if(!whole && x.row0 + r < x.rows)
+      __hip_atomic_store(part + ROWS * DP + r, total == 0.0f ? kNone : m + __builtin_amdgcn_logf(total), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+};
+
+// What sixteens of threads that share a row's parts join them through.
+template <int DP, int WAVES>
+struct CacheParts {
+  float rest[4 * WAVES][DP];
+  float top[4 * WAVES], sum[4 * WAVES];
+  int is_last;
+};
+
+// The parts of a sequence: the workgroup that arrives last joins them, in their order.
+template <typename T, int DP, int ROWS, int WAVES>
+__device__ __forceinline__ void cache_join_parts(const CacheAttentionArgs& a, const CacheTile& x, const CacheOut<T, DP, ROWS>& out,
+                                                 CacheParts<DP, WAVES>& sh) {
+  using Out = CacheOut<T, DP, ROWS>;
+  constexpr int kDims = DP / 16;
+  const int tid = threadIdx.x;
+  // (Stores and loads of agent scope go past the caches of an XCD; every wave's stores are acknowledged before the count
+  // goes up, so whoever reads the last count finds them all.)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if(tid == 0) {
+    unsigned* const counter = a.counters + out.place;
+    const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(x.w.parts - 1);
+    if(last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // (for the next call)
+    sh.is_last = last;
+  }
+  __syncthreads();
+  if(!sh.is_last) return;
+  // Sixteen threads to a row; where there are fewer rows than sixteens, several of them share a row's parts.  A batch of parts is
+  // asked for at a time: the loads come from the memory side, about a microsecond away.
+  const float* const all = a.part + out.place * Out::kTileFloats;
+  const long long stride = out.stride * Out::kTileFloats;
+  constexpr int kGroups = 4 * WAVES, kBatch = DP == 256 ? 4 : 8;
+  const int here = min(ROWS, x.rows - x.row0), group = tid >> 4, d_mine = (tid & 15) * kDims;
+  int share = 1;
+  while(share * here * 2 <= kGroups) share *= 2;
+#pragma unroll 1
+  for(int r = group / share; r < here; r += kGroups / share) {   // (one turn where parts are shared)
+    const float* logs = all + ROWS * DP + r;
+    const float* from = all + r * DP + (d_mine < a.dk ? d_mine : 0);
+    float m = kNone, total = 0.0f, y[kDims] = {};
+#pragma unroll 1
+    for(int i = group % share; i < x.w.parts; i += kBatch * share) {
+      float l[kBatch];
+      unsigned long long z[kBatch][kDims / 2];
+#pragma unroll
+      for(int b = 0; b < kBatch; ++b) {
+        l[b] = kNone;
+#pragma unroll
+        for(int j = 0; j < kDims / 2; ++j) z[b][j] = 0;
+        if(i + b * share < x.w.parts) {
+          const long long at = (i + b * share) * stride;
+          l[b] = __hip_atomic_load(logs + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+          for(int j = 0; j < kDims / 2; ++j)
+            z[b][j] = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(from + at) + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+      }
+      float next = m;
+#pragma unroll
+      for(int b = 0; b < kBatch; ++b) next = fmaxf(next, l[b]);
+      const float down = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      total *= down;
+#pragma unroll
+      for(int j = 0; j < kDims; ++j) y[j] *= down;
+#pragma unroll
+      for(int b = 0; b < kBatch; ++b) {
+        const float weight = l[b] == kNone ? 0.0f : __builtin_amdgcn_exp2f(l[b] - m);
+        total += weight;
+#pragma unroll
+        for(int j = 0; j < kDims; ++j) y[j] = __builtin_fmaf(weight, __builtin_bit_cast(float, (unsigned)(z[b][j / 2] >> (32 * (j % 2)))), y[j]);
+      }
+    }
+    if(share > 1) {   // (r is the only row of all threads: sixteens beyond the rows have left)
+      float* const rest = &sh.rest[group][(tid & 15) * kDims];
+#pragma unroll
+      for(int j = 0; j < kDims; ++j) rest[j] = y[j];
+      if((tid & 15) == 0) {
+        sh.top[group] = m;
+        sh.sum[group] = total;
+      }
+    }
+    if(share == 1 && d_mine < a.dk) {
+      const float per = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+      for(int j = 0; j < kDims; ++j) y[j] *= per;
+      store_row<kDims, T>(cache_row_out<T>(a, x, x.row0 + r) + d_mine, y);
+    }
+  }
+  if(share == 1) return;
+  __syncthreads();
+  const int r = group / share;
+  if(group % share != 0 || r >= here || d_mine >= a.dk) return;
+  float m = kNone, total = 0.0f, y[kDims] = {};
+  for(int i = 0; i < share; ++i) m = fmaxf(m, sh.top[group + i]);
+  for(int i = 0; i < share; ++i) {
+    const float from = sh.top[group + i], weight = from == kNone ? 1.0f : __builtin_amdgcn_exp2f(from - m);   // (of none: 0, or NaN)
+    const float* const rest = &sh.rest[group + i][(tid & 15) * kDims];
+    total += sh.sum[group + i] * weight;
+#pragma unroll
+    for(int j = 0; j < kDims; ++j) y[j] = __builtin_fmaf(rest[j], weight, y[j]);
+  }
+  const float per = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+  for(int j = 0; j < kDims; ++j) y[j] *= per;
+  store_row<kDims, T>(cache_row_out<T>(a, x, x.row0 + r) + d_mine, y);
+}
+
 // What the waves of a workgroup join their results through.
 template <int DP, int QT, int WAVES>
 struct CacheJoin {
   static constexpr int kHalf = DP < 128 ? DP : 128;   // dimensions that are joined at a time
-  float joined[WAVES][16][kHalf + 4];
+  union {
+    float joined[WAVES][16][kHalf + 4];
+    CacheParts<DP, WAVES> parts;
+  };
   float row_max[WAVES][16 * QT], row_sum[WAVES][16 * QT];
-  int is_last;
 };
 
-// The waves' results of the tile, joined and written; of a sequence in several parts by the workgroup that arrives last.  Lane (c, g) holds
-// values 4 * kDims * g .. of row c of each sixteen, unnormalized, the carried maximum and scale and its part of the sum.
+// The results of waves that share rows, joined and written.  Lane (c, g) holds values 4 * kDims * g .. of row c of each sixteen,
+// unnormalized, the carried maximum and scale and its part of the sum.
 template <typename T, CacheFormat F, int DP, int QT, int WAVES>
 __device__ __forceinline__ void cache_finish(const CacheAttentionArgs& a, const CacheTile& x, const cache_f4 (&o)[QT][DP / 16], const float (&top)[QT],
                                              float (&sum)[QT], const float (&unit)[QT], CacheJoin<DP, QT, WAVES>& sh) {
@@ -362,27 +493,7 @@ __device__ __forceinline__ void cache_finish(const CacheAttentionArgs& a, const 
       sh.row_sum[wave][16 * t + c] = sum[t];
     }
   }
-  const bool whole = x.w.parts == 1;
-  const long long place_of_tile = ((long long)x.w.slot * a.Hk + x.head) * a.row_tiles + x.tile, part_stride = (long long)a.Hk * a.row_tiles;
-  constexpr int kTileFloats = 16 * QT * (DP + 1);
-  float* const part = whole ? nullptr : a.part + (place_of_tile + x.w.part * part_stride) * kTileFloats;
-  auto emit = [&](int r, int d, const auto& y) __attribute__((always_inline)) {   // values d .. of row r of the tile
-    constexpr int kCount = sizeof(y) / sizeof(float);
-    if(x.row0 + r >= x.rows || d >= a.dk) return;
-    if(whole) {
-      store_row<kCount, T>(cache_row_out<T>(a, x, x.row0 + r) + d, y);
-    } else {
-      unsigned long long* to = reinterpret_cast<unsigned long long*>(part + r * DP + d);
-#pragma unroll
-      for(int j = 0; j < kCount; j += 2)
-        __hip_atomic_store(to + j / 2, (unsigned long long)__builtin_bit_cast(unsigned, y[j + 1]) << 32 | __builtin_bit_cast(unsigned, y[j]),
-                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-  };
-  auto emit_log = [&](int r, float m, float total) __attribute__((always_inline)) {   // of the sum of the row's weights
-    if(!whole && x.row0 + r < x.rows)
-      __hip_atomic_store(part + 16 * QT * DP + r, total == 0.0f ? kNone : m + __builtin_amdgcn_logf(total), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  };
+  const CacheOut<T, DP, 16 * QT> out(a, x);
   constexpr float kUnit = 1.0f / (kWeightUnit * kCodeUnit<F>);
   if constexpr(WAVES == 1) {
 #pragma unroll
@@ -393,9 +504,9 @@ __device__ __forceinline__ void cache_finish(const CacheAttentionArgs& a, const 
         float y[kDims];
 #pragma unroll
         for(int j = 0; j < kDims; ++j) y[j] = o[t][j][e] * factor;
-        emit(16 * t + c, kDims * (4 * g + e), y);
+        out.emit(16 * t + c, kDims * (4 * g + e), y);
       }
-      if(g == 0) emit_log(16 * t + c, top[t], sum[t]);
+      if(g == 0) out.emit_log(16 * t + c, top[t], sum[t]);
     }
   } else {
     __syncthreads();
@@ -437,106 +548,13 @@ __device__ __forceinline__ void cache_finish(const CacheAttentionArgs& a, const 
             for(int i = 1; i < WAVES; ++i) y[j] += sh.joined[i][r][d + j];
             y[j] *= per;
           }
-          emit(16 * t + r, h * kHalf + d, y);
-          if(h == 0 && (tid & 15) == 0) emit_log(16 * t + r, top_r, total);
+          out.emit(16 * t + r, h * kHalf + d, y);
+          if(h == 0 && (tid & 15) == 0) out.emit_log(16 * t + r, top_r, total);
         }
       }
     }
   }
-  if(whole) return;
-
-  // ---- the parts of a sequence: the workgroup that arrives last joins them, in their order.
-  // (Stores and loads of agent scope go past the caches of an XCD; every wave's stores are acknowledged before the count
-  // goes up, so whoever reads the last count finds them all.)
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if(tid == 0) {
-    unsigned* const counter = a.counters + place_of_tile;
-    const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(x.w.parts - 1);
-    if(last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // (for the next call)
-    sh.is_last = last;
-  }
-  __syncthreads();
-  if(!sh.is_last) return;
-  // Sixteen threads to a row; where there are fewer rows than sixteens, several of them share a row's parts.  A batch of parts is
-  // asked for at a time: the loads come from the memory side, about a microsecond away.
-  const float* const all = a.part + place_of_tile * kTileFloats;
-  const long long stride = part_stride * kTileFloats;
-  constexpr int kGroups = 4 * WAVES, kBatch = DP == 256 ? 4 : 8;
-  const int here = min(16 * QT, x.rows - x.row0), group = tid >> 4, d_mine = (tid & 15) * kDims;
-  int share = 1;
-  while(share * here * 2 <= kGroups) share *= 2;
-#pragma unroll 1
-  for(int r = group / share; r < here; r += kGroups / share) {   // (one turn where parts are shared)
-    const float* logs = all + 16 * QT * DP + r;
-    const float* from = all + r * DP + (d_mine < a.dk ? d_mine : 0);
-    float m = kNone, total = 0.0f, y[kDims] = {};
-#pragma unroll 1
-    for(int i = group % share; i < x.w.parts; i += kBatch * share) {
-      float l[kBatch];
-      unsigned long long z[kBatch][kDims / 2];
-#pragma unroll
-      for(int b = 0; b < kBatch; ++b) {
-        l[b] = kNone;
-#pragma unroll
-        for(int j = 0; j < kDims / 2; ++j) z[b][j] = 0;
-        if(i + b * share < x.w.parts) {
-          const long long at = (i + b * share) * stride;
-          l[b] = __hip_atomic_load(logs + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-          for(int j = 0; j < kDims / 2; ++j)
-            z[b][j] = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(from + at) + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-      }
-      float next = m;
-#pragma unroll
-      for(int b = 0; b < kBatch; ++b) next = fmaxf(next, l[b]);
-      const float down = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - next);
-      m = next;
-      total *= down;
-#pragma unroll
-      for(int j = 0; j < kDims; ++j) y[j] *= down;
-#pragma unroll
-      for(int b = 0; b < kBatch; ++b) {
-        const float weight = l[b] == kNone ? 0.0f : __builtin_amdgcn_exp2f(l[b] - m);
-        total += weight;
-#pragma unroll
-        for(int j = 0; j < kDims; ++j) y[j] = __builtin_fmaf(weight, __builtin_bit_cast(float, (unsigned)(z[b][j / 2] >> (32 * (j % 2)))), y[j]);
-      }
-    }
-    if(share > 1) {   // (r is the only row of all threads: sixteens beyond the rows have left)
-      float* const rest = &sh.joined[0][0][0] + group * (16 * kDims) + (tid & 15) * kDims;
-#pragma unroll
-      for(int j = 0; j < kDims; ++j) rest[j] = y[j];
-      if((tid & 15) == 0) {
-        (&sh.row_max[0][0])[group] = m;
-        (&sh.row_sum[0][0])[group] = total;
-      }
-    }
-    if(share == 1 && d_mine < a.dk) {
-      const float per = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-      for(int j = 0; j < kDims; ++j) y[j] *= per;
-      store_row<kDims, T>(cache_row_out<T>(a, x, x.row0 + r) + d_mine, y);
-    }
-  }
-  if(share == 1) return;
-  __syncthreads();
-  const int r = group / share;
-  if(group % share != 0 || r >= here || d_mine >= a.dk) return;
-  float m = kNone, total = 0.0f, y[kDims] = {};
-  for(int i = 0; i < share; ++i) m = fmaxf(m, (&sh.row_max[0][0])[group + i]);
-  for(int i = 0; i < share; ++i) {
-    const float from = (&sh.row_max[0][0])[group + i], weight = from == kNone ? 1.0f : __builtin_amdgcn_exp2f(from - m);   // (of none: 0, or NaN)
-    const float* const rest = &sh.joined[0][0][0] + (group + i) * (16 * kDims) + (tid & 15) * kDims;
-    total += (&sh.row_sum[0][0])[group + i] * weight;
-#pragma unroll
-    for(int j = 0; j < kDims; ++j) y[j] = __builtin_fmaf(rest[j], weight, y[j]);
-  }
-  const float per = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-  for(int j = 0; j < kDims; ++j) y[j] *= per;
-  store_row<kDims, T>(cache_row_out<T>(a, x, x.row0 + r) + d_mine, y);
+  if(!out.whole) cache_join_parts<T, DP, 16 * QT, WAVES>(a, x, out, sh.parts);
 }
 
 // ---- sixteen rows and more to a wave
@@ -545,28 +563,35 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
   using A = CacheAttention<T, F, DP>;
   constexpr int kTerms = A::kTerms, kSteps = A::kSteps, kDims = A::kDims;
   constexpr int kTurn = 32 * WAVES;   // positions that the waves take in one turn
-  __shared__ CacheJoin<DP, QT, WAVES> sh;
+  __shared__ struct {
+    CacheJoin<DP, QT, WAVES> join;
+    alignas(16) float scales[WAVES][64];
+  } sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   CacheTile x;
   if(!cache_tile<T, DP, 16 * QT, WAVES>(a, tid, x)) return;
   const int end = x.end;
+  const CacheBuffer k_codes(x.k, (unsigned)end * a.dk), v_codes(x.v, (unsigned)end * a.dk);
+  // (a position's scales are loaded to one lane, and go through LDS to those that have its scores)
+  const CacheBuffer k_scales(x.ks, 4u * end), v_scales(x.vs, 4u * end);
+  float scale_k, scale_v;
   auto fetch_keys = [&](typename A::Keys& y, int at) __attribute__((always_inline)) {
-    if(at + 32 <= end) A::template load<false>(y, x.k, x.ks, at, 0, a.dk, lane);
-    else if(at < end) A::template load<true>(y, x.k, x.ks, at, end - 1, a.dk, lane);
+    load_keys(y.code, k_codes, at, a.dk, lane);
+    scale_k = k_scales.number(at + (lane & 31));
   };
   auto fetch_values = [&](typename A::Values& y, int at) __attribute__((always_inline)) {
-    if(at + 32 <= end) A::template load<false>(y, x.v, x.vs, at, 0, a.dk, lane);
-    else if(at < end) A::template load<true>(y, x.v, x.vs, at, end - 1, a.dk, lane);
+    const unsigned d = (unsigned)(kDims * c) < (unsigned)a.dk ? kDims * c : 0, row = (unsigned)(at + 4 * g) * a.dk + d;
+#pragma unroll
+    for(int e = 0; e < 8; ++e) v_codes.words(y.code[e], row + (unsigned)(16 * (e / 4) + e % 4) * a.dk);
+    scale_v = v_scales.number(at + (lane & 31));
   };
   // (the first positions are asked for ahead of the queries, the next keys as soon as the last ones are used up, and so the values)
   const int begin = x.w.from + 32 * wave;
   typename A::Keys key;
   typename A::Values value;
-  if(begin < end) {
-    A::template load<true>(key, x.k, x.ks, begin, end - 1, a.dk, lane);
-    A::template load<true>(value, x.v, x.vs, begin, end - 1, a.dk, lane);
-  }
+  fetch_keys(key, begin);
+  fetch_values(value, begin);
   unsigned long long seen = 0;
   if(a.parents) seen = lineage(a.parents + (long long)x.w.s * a.n, a.n, lane);
   cache_h8 q[QT][kTerms][kSteps];
@@ -591,6 +616,11 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
   }
 
   for(int at = begin; at < end; at += kTurn) {
+    if(lane < 32) {
+      sh.scales[wave][lane] = scale_k;
+      sh.scales[wave][32 + lane] = scale_v;
+    }
+    __builtin_amdgcn_wave_barrier();   // (a wave's accesses to LDS are done in their order)
     // scores
     cache_f4 s[QT][2];
 #pragma unroll
@@ -606,10 +636,17 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
 #pragma unroll
           for(int m = kTerms - 1; m >= 0; --m) s[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand, q[t][m][i], s[t][b], 0, 0, 0);
       }
+    cache_f4 ks[2], vs[2];
+#pragma unroll
+    for(int b = 0; b < 2; ++b) {
+      ks[b] = *reinterpret_cast<const cache_f4*>(&sh.scales[wave][16 * b + 4 * g]);
+      vs[b] = *reinterpret_cast<const cache_f4*>(&sh.scales[wave][32 + 16 * b + 4 * g]);
+    }
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for(int t = 0; t < QT; ++t)
 #pragma unroll
-      for(int e = 0; e < 8; ++e) s[t][e / 4][e % 4] *= key.scale[e / 4][e % 4];
+      for(int e = 0; e < 8; ++e) s[t][e / 4][e % 4] *= ks[e / 4][e % 4];
     fetch_keys(key, at + kTurn);
     // Positions that a row does not see score minus infinity (a weight of zero) and have a scale of zero.
     const bool masked = at + 32 > x.open;
@@ -637,7 +674,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
       }
     } else {
 #pragma unroll
-      for(int e = 0; e < 8; ++e) widest = fmaxf(widest, value.scale[e / 4][e % 4]);
+      for(int e = 0; e < 8; ++e) widest = fmaxf(widest, vs[e / 4][e % 4]);
     }
     float high[QT], wide[QT];
     bool grown = false;
@@ -653,7 +690,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
 #pragma unroll
       for(int t = 0; t < QT; ++t)
 #pragma unroll
-        for(int e = 0; e < 8; ++e) wide[t] = fmaxf(wide[t], seen_here[t] >> e & 1 ? value.scale[e / 4][e % 4] : 0.0f);
+        for(int e = 0; e < 8; ++e) wide[t] = fmaxf(wide[t], seen_here[t] >> e & 1 ? vs[e / 4][e % 4] : 0.0f);
     }
 #pragma unroll
     for(int t = 0; t < QT; ++t) grown |= high[t] > top[t] + kMaximumSlack || wide[t] > unit[t] * kScaleSlack;
@@ -676,7 +713,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
     for(int t = 0; t < QT; ++t) {
       const float per = kWeightUnit / unit[t];
 #pragma unroll
-      for(int e = 0; e < 8; ++e) r[t][e] = value.scale[e / 4][e % 4] * per;
+      for(int e = 0; e < 8; ++e) r[t][e] = vs[e / 4][e % 4] * per;
     }
     if(masked) {
 #pragma unroll
@@ -704,8 +741,8 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
       for(int i = 0; i < A::kWords; ++i) vh[e][i] = held<F>(value.code[e][i]);
 #pragma unroll
     for(int i = 0; i < A::kWords; ++i) {
-      const cache_h8 d[4] = {A::template value_operand<0>(vh, i), A::template value_operand<1>(vh, i), A::template value_operand<2>(vh, i),
-                             A::template value_operand<3>(vh, i)};
+      const cache_h8 d[4] = {value_operand_of<F, 0>(vh, i), value_operand_of<F, 1>(vh, i), value_operand_of<F, 2>(vh, i),
+                             value_operand_of<F, 3>(vh, i)};
 #pragma unroll
       for(int j = 0; j < 4; ++j)
 #pragma unroll
@@ -717,7 +754,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
     fetch_values(value, at + kTurn);
   }
 
-  cache_finish<T, F, DP, QT, WAVES>(a, x, o, top, sum, unit, sh);
+  cache_finish<T, F, DP, QT, WAVES>(a, x, o, top, sum, unit, sh.join);
 }
 
 // ---- up to eight rows to a wave
@@ -745,38 +782,6 @@ struct CacheFew {
   };
   // The position, of 64, whose scores lane (c, g) has.
   static __device__ __forceinline__ int key_of(int i, int lane) { return kKeys == 1 ? lane : 32 * i + 16 * (lane >> 5) + (lane & 15); }
-
-  template <bool ENDS>
-  static __device__ __forceinline__ void load(Keys& t, const unsigned char* k, const float* scale, int at, int last, int dk, int lane) {
-    const int c = lane & 15, g = lane >> 4;
-#pragma unroll
-    for(int b = 0; b < 4; ++b) {
-      const unsigned row = ENDS ? (unsigned)min(at + 16 * b + c, last) * dk : (unsigned)(at + c) * dk;
-      const unsigned char* p = ENDS ? k : k + (size_t)(16 * b * dk);
-#pragma unroll
-      for(int i = 0; i < A::kPieces; ++i) {
-        const unsigned d = 64 * i + 16 * g;
-        t.code[b][i] = *reinterpret_cast<const cache_u4*>(p + (row + (d < (unsigned)dk ? d : 0)));
-      }
-    }
-#pragma unroll
-    for(int i = 0; i < kKeys; ++i) t.scale[i] = scale[(unsigned)(ENDS ? min(at + key_of(i, lane), last) : at + key_of(i, lane))];
-  }
-  template <bool ENDS>
-  static __device__ __forceinline__ void load(Values& t, const unsigned char* v, const float* scale, int at, int last, int dk, int lane) {
-    const int c = lane & 15, g = lane >> 4;
-    const unsigned d = (unsigned)(A::kDims * c) < (unsigned)dk ? A::kDims * c : 0;
-#pragma unroll
-    for(int h = 0; h < 2; ++h)
-#pragma unroll
-      for(int e = 0; e < 8; ++e) {
-        const int key = 32 * h + 4 * e;
-        const unsigned row = ENDS ? (unsigned)min(at + g + key, last) * dk : (unsigned)(at + g) * dk;
-        A::load_codes(t.code[h][e], (ENDS ? v : v + (size_t)(key * dk)) + (row + d));
-      }
-#pragma unroll
-    for(int i = 0; i < kKeys; ++i) t.scale[i] = scale[(unsigned)(ENDS ? min(at + key_of(i, lane), last) : at + key_of(i, lane))];
-  }
 };
 
 template <typename T, CacheFormat F, int DP, int ROWS, int WAVES>
@@ -794,21 +799,24 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
   CacheTile x;
   if(!cache_tile<T, DP, ROWS, WAVES>(a, tid, x)) return;
   const int end = x.end;
+  const CacheBuffer k_codes(x.k, (unsigned)end * a.dk), v_codes(x.v, (unsigned)end * a.dk), k_scales(x.ks, 4u * end), v_scales(x.vs, 4u * end);
   auto fetch_keys = [&](typename B::Keys& y, int at) __attribute__((always_inline)) {
-    if(at + 64 <= end) B::template load<false>(y, x.k, x.ks, at, 0, a.dk, lane);
-    else if(at < end) B::template load<true>(y, x.k, x.ks, at, end - 1, a.dk, lane);
+    load_keys(y.code, k_codes, at, a.dk, lane);
+#pragma unroll
+    for(int i = 0; i < kKeys; ++i) y.scale[i] = k_scales.number(at + B::key_of(i, lane));
   };
   auto fetch_values = [&](typename B::Values& y, int at) __attribute__((always_inline)) {
-    if(at + 64 <= end) B::template load<false>(y, x.v, x.vs, at, 0, a.dk, lane);
-    else if(at < end) B::template load<true>(y, x.v, x.vs, at, end - 1, a.dk, lane);
+    const unsigned d = (unsigned)(kDims * c) < (unsigned)a.dk ? kDims * c : 0, row = (unsigned)(at + g) * a.dk + d;
+#pragma unroll
+    for(int e = 0; e < 16; ++e) v_codes.words(y.code[e / 8][e % 8], row + (unsigned)(4 * e) * a.dk);
+#pragma unroll
+    for(int i = 0; i < kKeys; ++i) y.scale[i] = v_scales.number(at + B::key_of(i, lane));
   };
   const int begin = x.w.from + 64 * wave;
   typename B::Keys key;
   typename B::Values value;
-  if(begin < end) {
-    B::template load<true>(key, x.k, x.ks, begin, end - 1, a.dk, lane);
-    B::template load<true>(value, x.v, x.vs, begin, end - 1, a.dk, lane);
-  }
+  fetch_keys(key, begin);
+  fetch_values(value, begin);
   unsigned long long seen = 0;
   if(a.parents) seen = lineage(a.parents + (long long)x.w.s * a.n, a.n, lane);
   cache_h8 q[kTerms][kSteps];
@@ -951,8 +959,8 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
         for(int i = 0; i < A::kWords; ++i) vh[e][i] = held<F>(value.code[h][e][i]);
 #pragma unroll
       for(int i = 0; i < A::kWords; ++i) {
-        const cache_h8 d[4] = {A::template value_operand<0>(vh, i), A::template value_operand<1>(vh, i), A::template value_operand<2>(vh, i),
-                               A::template value_operand<3>(vh, i)};
+        const cache_h8 d[4] = {value_operand_of<F, 0>(vh, i), value_operand_of<F, 1>(vh, i), value_operand_of<F, 2>(vh, i),
+                               value_operand_of<F, 3>(vh, i)};
 #pragma unroll
         for(int j = 0; j < 4; ++j)
 #pragma unroll
@@ -967,6 +975,258 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
   float row_top[1] = {of_row(top)}, row_sum[1] = {of_row(sum) * 0.25f}, row_unit[1] = {of_row(unit)};   // (four lanes of a row add up in the end)
   if(WAVES > 1) __syncthreads();   // (the weights' memory is taken for the results)
   cache_finish<T, F, DP, 1, WAVES>(a, x, o, row_top, row_sum, row_unit, sh.join);
+}
+
+// ---- many rows to an entry
+// 16 * QT rows to a wave, whose waves share 64 positions at a time: these are loaded once, turned into float16 and laid into LDS as the
+// operands that every wave then reads, piece after piece of 64 lanes.  Wave w turns the keys of block w of sixteen, and of
+// half w / 2 of the positions half the dimensions of the values; the next codes are on their way meanwhile.  The products are those
+// of the first form, but for the dimensions, lane (c, g) having 64 i + 16 g + 4 e + j.
+template <typename T, CacheFormat F, int DP, int QT>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void cache_attention_many_kernel(CacheAttentionArgs a) {
+  using A = CacheAttention<T, F, DP>;
+  constexpr int kTerms = A::kTerms, kSteps = A::kSteps, kDims = A::kDims, kPieces = A::kPieces;
+  constexpr int kTile = 64, kRows = 16 * QT * 4;
+  constexpr int kMine = kDims / 2;                      // dimensions' operands that a wave makes ...
+  constexpr int kMineWords = kMine < 4 ? 1 : kMine / 4;   // ... of so many words of a row
+  __shared__ union {
+    struct {
+      cache_h8 k[4 * kSteps][64], v[2 * kDims][64];
+      cache_f4 ks[kTile / 4], vs[kTile / 4];
+    } tile;
+    CacheParts<DP, 4> parts;
+  } sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  CacheTile x;
+  if(!cache_tile<T, DP, kRows, 4>(a, tid, x)) return;
+
+  // ---- what the wave loads
+  const int half = wave >> 1, side = wave & 1;
+  cache_u4 k_code[1][kPieces];
+  unsigned v_code[8][kMineWords];
+  float scale;   // of a position's key, or, in waves 1 and 3, value
+  const CacheBuffer k_codes(x.k, (unsigned)x.end * a.dk), v_codes(x.v, (unsigned)x.end * a.dk), scales(side ? x.vs : x.ks, 4u * x.end);
+  auto fetch = [&](int at) __attribute__((always_inline)) {
+    load_keys(k_code, k_codes, at + 16 * wave, a.dk, lane);
+    const unsigned row = (unsigned)(at + 32 * half + 4 * g) * a.dk;
+#pragma unroll
+    for(int i = 0; i < kMineWords; ++i) {
+      const unsigned d = 64 * (DP == 64 ? 0 : side * kMineWords + i) + 4 * c, from = row + (d < (unsigned)a.dk ? d : 0);
+#pragma unroll
+      for(int e = 0; e < 8; ++e) {
+        unsigned word[1];
+        v_codes.words(word, from + (unsigned)(16 * (e / 4) + e % 4) * a.dk);
+        v_code[e][i] = word[0];
+      }
+    }
+    scale = scales.number(at + lane);
+  };
+  auto lay = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for(int i = 0; i < kPieces; ++i) {
+      sh.tile.k[wave * kSteps + 2 * i][lane] = half8_of<F>(k_code[0][i][0], k_code[0][i][1]);
+      sh.tile.k[wave * kSteps + 2 * i + 1][lane] = half8_of<F>(k_code[0][i][2], k_code[0][i][3]);
+    }
+    unsigned vh[8][kMineWords];
+#pragma unroll
+    for(int e = 0; e < 8; ++e)
+#pragma unroll
+      for(int i = 0; i < kMineWords; ++i) vh[e][i] = held<F>(v_code[e][i]);
+    cache_h8(*to)[64] = &sh.tile.v[half * kDims + side * kMine];
+    if constexpr(DP == 64) {   // two of the four dimensions of the only word
+      to[0][lane] = side ? value_operand_of<F, 2>(vh, 0) : value_operand_of<F, 0>(vh, 0);
+      to[1][lane] = side ? value_operand_of<F, 3>(vh, 0) : value_operand_of<F, 1>(vh, 0);
+    } else {
+#pragma unroll
+      for(int i = 0; i < kMineWords; ++i) {
+        to[4 * i][lane] = value_operand_of<F, 0>(vh, i);
+        to[4 * i + 1][lane] = value_operand_of<F, 1>(vh, i);
+        to[4 * i + 2][lane] = value_operand_of<F, 2>(vh, i);
+        to[4 * i + 3][lane] = value_operand_of<F, 3>(vh, i);
+      }
+    }
+    if(tid < 128) (tid < 64 ? reinterpret_cast<float*>(sh.tile.ks) : reinterpret_cast<float*>(sh.tile.vs))[lane] = scale;
+  };
+  fetch(x.w.from);
+
+  // ---- the wave's rows
+  unsigned long long seen = 0;
+  if(a.parents) seen = lineage(a.parents + (long long)x.w.s * a.n, a.n, lane);
+  const int row0 = x.row0 + 16 * QT * wave;
+  cache_h8 q[QT][kTerms][kSteps];
+  float row_scale[QT];
+  CacheSight sight[QT];
+#pragma unroll
+  for(int t = 0; t < QT; ++t) {
+    const int row = min(row0 + 16 * t + c, x.rows - 1);
+    sight[t] = cache_sight(a, x, row, seen);
+    row_scale[t] = cache_query<T, F, DP>(a, x, row, g, q[t]);
+  }
+  // of what any of them see (trees: as the workgroup's)
+  const int end = row0 >= x.rows ? 0 : a.parents ? x.end : min(x.end, x.w.len + (int)a.by_group.of((unsigned)min(x.rows - 1, row0 + 16 * QT - 1)) + 1);
+  cache_f4 o[QT][kDims];
+  float top[QT], sum[QT], unit[QT], per[QT];
+#pragma unroll
+  for(int t = 0; t < QT; ++t) {
+    top[t] = kNone;
+    sum[t] = 0.0f;
+    unit[t] = 1e-30f;   // (scales below it are as good as zero)
+    per[t] = kWeightUnit / unit[t];
+#pragma unroll
+    for(int j = 0; j < kDims; ++j) o[t][j] = cache_f4{0, 0, 0, 0};
+  }
+
+  // Positions at .. at + 31, half h of the block.  MASKED: not all of them are seen by all rows.  Up to the first such block the carried
+  // scale is the same for all rows.
+  auto take = [&](int at, int h, auto masked) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked)::value;
+    cache_f4 s[QT][2], vs[2];
+#pragma unroll
+    for(int b = 0; b < 2; ++b)
+#pragma unroll
+      for(int t = 0; t < QT; ++t) s[t][b] = cache_f4{0, 0, 0, 0};
+    {
+      cache_h8 operand[2][kSteps];
+#pragma unroll
+      for(int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for(int b = 0; b < 2; ++b) operand[b][i] = sh.tile.k[(2 * h + b) * kSteps + i][lane];
+#pragma unroll
+      for(int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for(int m = kTerms - 1; m >= 0; --m)
+#pragma unroll
+          for(int b = 0; b < 2; ++b)
+#pragma unroll
+            for(int t = 0; t < QT; ++t) s[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand[b][i], q[t][m][i], s[t][b], 0, 0, 0);
+    }
+    // (the first values are on their way while the weights are made)
+    constexpr int kAhead = 4;
+    cache_h8 ahead[kAhead];
+#pragma unroll
+    for(int j = 0; j < kAhead; ++j) ahead[j] = sh.tile.v[h * kDims + j][lane];
+#pragma unroll
+    for(int b = 0; b < 2; ++b) {
+      const cache_f4 ks = sh.tile.ks[4 * (2 * h + b) + g];
+      vs[b] = sh.tile.vs[4 * (2 * h + b) + g];
+#pragma unroll
+      for(int t = 0; t < QT; ++t)
+#pragma unroll
+        for(int e = 0; e < 4; ++e) s[t][b][e] *= ks[e];
+    }
+    unsigned seen_here[QT];   // bit 4 b + e
+    float widest = 0.0f;
+    if constexpr(MASKED) {
+#pragma unroll
+      for(int t = 0; t < QT; ++t) {
+        seen_here[t] = 0;
+#pragma unroll
+        for(int b = 0; b < 2; ++b) {
+          const int from = at + 16 * b + 4 * g;
+          unsigned four = (1u << clamp_int((a.parents ? end : sight[t].limit) - from, 0, 4)) - 1;
+          if(a.parents) {   // settled positions, then the drafted ones from bit 0 on
+            const int j = from - x.w.len, settled = clamp_int(-j, 0, 4);
+            four &= j < 0 ? ((unsigned)sight[t].sees << settled | ((1u << settled) - 1)) : (unsigned)(sight[t].sees >> min(j, 63));
+          }
+          seen_here[t] |= four << (4 * b);
+#pragma unroll
+          for(int e = 0; e < 4; ++e) s[t][b][e] = four >> e & 1 ? s[t][b][e] : kNone;
+        }
+      }
+    } else {
+#pragma unroll
+      for(int e = 0; e < 8; ++e) widest = fmaxf(widest, vs[e / 4][e % 4]);
+    }
+    float high[QT], wide[QT];
+    bool grown = false;
+#pragma unroll
+    for(int t = 0; t < QT; ++t) {
+      high[t] = kNone;
+      wide[t] = widest;
+#pragma unroll
+      for(int e = 0; e < 8; ++e) {
+        high[t] = fmaxf(high[t], s[t][e / 4][e % 4]);
+        if constexpr(MASKED) wide[t] = fmaxf(wide[t], seen_here[t] >> e & 1 ? vs[e / 4][e % 4] : 0.0f);
+      }
+      high[t] *= row_scale[t];
+      grown |= high[t] > top[t] + kMaximumSlack || wide[t] > unit[t] * kScaleSlack;
+    }
+    if(__any(grown)) {
+#pragma unroll
+      for(int t = 0; t < QT; ++t) {
+        const float m = fmaxf(top[t], over_lanes_max(high[t])), u = fmaxf(unit[t], over_lanes_max(wide[t]));
+        const float down = m == top[t] ? 1.0f : __builtin_amdgcn_exp2f(top[t] - m);
+        const float both = u == unit[t] ? down : down * (unit[t] / u);
+        sum[t] *= down;
+#pragma unroll
+        for(int j = 0; j < kDims; ++j) o[t][j] *= both;
+        top[t] = m;
+        unit[t] = u;
+        per[t] = kWeightUnit / u;
+      }
+    }
+    cache_h8 p[QT][kTerms];
+#pragma unroll
+    for(int t = 0; t < QT; ++t) {
+      const float from = MASKED && top[t] == kNone ? 0.0f : -top[t];   // (nothing seen so far: minus infinity stays that)
+#pragma unroll
+      for(int e = 0; e < 8; ++e) {
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], row_scale[t], from));
+        float r = vs[e / 4][e % 4] * per[MASKED ? t : 0];
+        if constexpr(MASKED) r = seen_here[t] >> e & 1 ? r : 0.0f;
+        const float z = y * r;
+        sum[t] += y;
+        p[t][0][e] = (_Float16)z;
+        if constexpr(kTerms == 2) p[t][kTerms - 1][e] = (_Float16)(z - (float)p[t][0][e]);
+      }
+    }
+#pragma unroll
+    for(int j = 0; j < kDims; ++j) {
+      const cache_h8 operand = ahead[j % kAhead];
+      if(j + kAhead < kDims) ahead[j % kAhead] = sh.tile.v[h * kDims + j + kAhead][lane];
+#pragma unroll
+      for(int t = 0; t < QT; ++t)
+#pragma unroll
+        for(int m = kTerms - 1; m >= 0; --m) o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand, p[t][m], o[t][j], 0, 0, 0);
+    }
+  };
+  auto turn = [&](int at) __attribute__((always_inline)) {   // the positions in hand into LDS, the next ones asked for
+    __syncthreads();   // (nobody reads the last ones any more)
+    lay();
+    __syncthreads();
+    fetch(at + kTile);
+  };
+  int at = x.w.from;
+  for(; at + kTile <= x.open; at += kTile) {
+    turn(at);
+#pragma unroll 1
+    for(int h = 0; h < 2; ++h) take(at + 32 * h, h, std::false_type());
+  }
+  for(; at < x.end; at += kTile) {
+    turn(at);
+#pragma unroll 1
+    for(int h = 0; h < 2; ++h)
+      if(at + 32 * h < end) take(at + 32 * h, h, std::true_type());
+  }
+
+  const CacheOut<T, DP, kRows> out(a, x);
+  constexpr float kUnit = 1.0f / (kWeightUnit * kCodeUnit<F>);
+#pragma unroll
+  for(int t = 0; t < QT; ++t) {
+    const int r = 16 * (QT * wave + t) + c;
+    sum[t] = over_lanes_sum(sum[t]);
+    const float factor = (sum[t] == 0.0f ? 0.0f : 1.0f / sum[t]) * (unit[t] * kUnit);
+#pragma unroll
+    for(int e = 0; e < 4; ++e)
+#pragma unroll
+      for(int i = 0; i < kDims / 4; ++i) {
+        const float y[4] = {o[t][4 * i][e] * factor, o[t][4 * i + 1][e] * factor, o[t][4 * i + 2][e] * factor, o[t][4 * i + 3][e] * factor};
+        out.emit(r, 64 * i + 16 * g + 4 * e, y);
+      }
+    if(g == 0) out.emit_log(r, top[t], sum[t]);
+  }
+  if(!out.whole) cache_join_parts<T, DP, kRows, 4>(a, x, out, sh.parts);
 }
 
 }  // namespace marian_hip

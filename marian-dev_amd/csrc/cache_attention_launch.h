@@ -31,7 +31,19 @@ int launch_cache_attention(const CacheAttentionArgs& a, const CacheAttentionPlan
 }
 
 template <typename T, CacheFormat F>
+int launch_cache_attention_many(const CacheAttentionArgs& a, const CacheAttentionPlan& p, hipStream_t st) {
+  const dim3 grid((unsigned)p.grid), block(256);
+  if(p.dp == 64 && p.qt == 1) MH_LAUNCH((cache_attention_many_kernel<T, F, 64, 1>), grid, block, 0, st, a);
+  else if(p.dp == 64) MH_LAUNCH((cache_attention_many_kernel<T, F, 64, 2>), grid, block, 0, st, a);
+  else if(p.dp == 128 && p.qt == 1) MH_LAUNCH((cache_attention_many_kernel<T, F, 128, 1>), grid, block, 0, st, a);
+  else if(p.dp == 128) MH_LAUNCH((cache_attention_many_kernel<T, F, 128, 2>), grid, block, 0, st, a);
+  else MH_LAUNCH((cache_attention_many_kernel<T, F, 256, 1>), grid, block, 0, st, a);
+  return MARIAN_HIP_OK;
+}
+
+template <typename T, CacheFormat F>
 int launch_cache_attention(const CacheAttentionArgs& a, const CacheAttentionPlan& p, hipStream_t st) {
+  if(p.many) return launch_cache_attention_many<T, F>(a, p, st);
   if(p.waves == 4) return launch_cache_attention<T, F, 4>(a, p, st);
   if(p.waves == 2) return launch_cache_attention<T, F, 2>(a, p, st);
   return launch_cache_attention<T, F, 1>(a, p, st);

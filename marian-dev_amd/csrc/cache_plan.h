@@ -15,7 +15,9 @@ struct CacheAttentionPlan {
   int dp;              // values of a row as the kernel holds it: dk rounded up to 64, 128 or 256
   int qt;              // sixteens of query rows to a workgroup
   int few;             // the rows of an entry, up to 1, 2, 4 or 8 of them (0: more, or values too long for that form)
+  int many;            // rows of a workgroup of four waves that share positions laid out in LDS (0: fewer rows)
   int waves;           // of a workgroup, which share its positions
+  int tile_rows;       // of a workgroup
   int64_t row_tiles;   // workgroups that share an entry's positions
   int least;           // blocks of a part
   int64_t target;      // parts that the positions of all sequences together are split into
@@ -27,18 +29,21 @@ struct CacheAttentionPlan {
 
 // A part is a whole number of blocks of positions, as many as all sequences have divided by target: then the parts of the
 // sequences that have several are less than 2 * target, whatever the lengths.
-inline CacheAttentionPlan cache_attention_plan(int64_t sequences, int64_t heads, int64_t q_heads, int64_t n, int64_t dk) {
+inline CacheAttentionPlan cache_attention_plan(int64_t sequences, int64_t heads, int64_t q_heads, int64_t n, int64_t dk, bool float32) {
   CacheAttentionPlan p{};
   p.dp = dk <= 64 ? 64 : dk <= 128 ? 128 : 256;
   const int64_t rows = n * (q_heads / heads);
   p.few = rows > 8 || p.dp == 256 ? 0 : rows > 4 ? 8 : rows > 2 ? 4 : (int)rows;
   p.qt = rows <= 16 || p.dp == 256 ? 1 : 2;   // (what the registers hold)
-  p.row_tiles = (rows + 16 * p.qt - 1) / (16 * p.qt);
+  if(rows > 32 && p.dp == 128 && float32) p.qt = 1;
+  p.many = rows > 32 ? 64 * p.qt : 0;
+  p.tile_rows = p.many ? p.many : 16 * p.qt;
+  p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const int64_t entries = sequences * heads * p.row_tiles;
-  p.waves = entries >= 4096 ? 1 : entries >= 2048 ? 2 : 4;
+  p.waves = p.many ? 4 : entries >= 4096 ? 1 : entries >= 2048 ? 2 : 4;
   // Workgroups that run at a time, by the registers of their form, and parts for twice as many (a sequence's last part is half as
   // long as the others on average).
-  const int to_a_simd = p.few ? (p.dp == 128 ? 2 : p.few <= 2 ? 4 : 3) : p.dp == 64 ? 5 - p.qt : p.dp == 128 ? 4 - p.qt : 2;
+  const int to_a_simd = p.many ? (p.dp == 256 ? 1 : 2) : p.few ? (p.dp == 128 ? 2 : p.few <= 2 ? 4 : 3) : p.dp == 64 ? 5 - p.qt : p.dp == 128 ? 4 - p.qt : 2;
   const int64_t at_a_time = 1024 * to_a_simd / p.waves;
   p.target = std::max<int64_t>(1, at_a_time / (heads * p.row_tiles) - sequences / 2);
   p.least = entries >= at_a_time || !p.few ? 4 : 2;
@@ -53,7 +58,7 @@ inline CacheAttentionPlan cache_attention_plan(int64_t sequences, int64_t heads,
 // them), in the same place for all sizes, then the partial results.
 constexpr int64_t kCacheCounterBytes = kCacheMost * 4;
 inline int64_t cache_attention_bytes(const CacheAttentionPlan& p, int64_t heads) {
-  return p.slots == 0 ? 0 : kCacheCounterBytes + p.slots * heads * p.row_tiles * 16 * p.qt * p.row_floats * 4;
+  return p.slots == 0 ? 0 : kCacheCounterBytes + p.slots * heads * p.row_tiles * p.tile_rows * p.row_floats * 4;
 }
 
 }  // namespace marian_hip
