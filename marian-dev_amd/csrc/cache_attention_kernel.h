@@ -141,6 +141,20 @@ struct CacheBuffer {
     return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, (unsigned)i * 4u, 0, 0));
   }
   __device__ __forceinline__ cache_u4 piece(unsigned at) const { return __builtin_bit_cast(cache_u4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0)); }
+  // Past the caches of an XCD, as loads and stores of agent scope go.
+  static constexpr int kThrough = 16;   // sc1
+  __device__ __forceinline__ float number_through(unsigned at) const {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, at, 0, kThrough));
+  }
+  __device__ __forceinline__ cache_f4 piece_through(unsigned at) const {
+    return __builtin_bit_cast(cache_f4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, kThrough));
+  }
+  __device__ __forceinline__ void store_through(cache_f4 y, unsigned at) const {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(cache_u4, y), rsrc, at, 0, kThrough);
+  }
+  __device__ __forceinline__ void store_through(float y, unsigned at) const {
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, y), rsrc, at, 0, kThrough);
+  }
   template <int WORDS>
   __device__ __forceinline__ void words(unsigned (&to)[WORDS], unsigned at) const {
     if constexpr(WORDS == 1) {
@@ -358,6 +372,21 @@ struct CacheOut {
   }
 };
 
+// Counts a workgroup of `parts` that share a counter in, and whether it is the last.  What it has stored for the others is of agent scope, past
+// the caches of an XCD: every wave's stores are acknowledged before the count goes up, so whoever reads the last count finds them
+// all, with loads of that scope.
+__device__ __forceinline__ bool cache_arrived_last(unsigned* counter, int parts, int& is_last) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if(threadIdx.x == 0) {
+    const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(parts - 1);
+    if(last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // (for the next call)
+    is_last = last;
+  }
+  __syncthreads();
+  return is_last;
+}
+
 // What sixteens of threads that share a row's parts join them through.
 template <int DP, int WAVES>
 struct CacheParts {
@@ -373,18 +402,7 @@ __device__ __forceinline__ void cache_join_parts(const CacheAttentionArgs& a, co
   using Out = CacheOut<T, DP, ROWS>;
   constexpr int kDims = DP / 16;
   const int tid = threadIdx.x;
-  // (Stores and loads of agent scope go past the caches of an XCD; every wave's stores are acknowledged before the count
-  // goes up, so whoever reads the last count finds them all.)
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if(tid == 0) {
-    unsigned* const counter = a.counters + out.place;
-    const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(x.w.parts - 1);
-    if(last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // (for the next call)
-    sh.is_last = last;
-  }
-  __syncthreads();
-  if(!sh.is_last) return;
+  if(!cache_arrived_last(a.counters + out.place, x.w.parts, sh.is_last)) return;
   // Sixteen threads to a row; where there are fewer rows than sixteens, several of them share a row's parts.  A batch of parts is
   // asked for at a time: the loads come from the memory side, about a microsecond away.
   const float* const all = a.part + out.place * Out::kTileFloats;
@@ -1210,23 +1228,85 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void cache_attention_many_k
       if(at + 32 * h < end) take(at + 32 * h, h, std::true_type());
   }
 
-  const CacheOut<T, DP, kRows> out(a, x);
+  // A sequence in several parts: a part's values go to the workspace as the registers have them, whole lines at a time, a lane's where the
+  // same lane of the workgroup that arrives last finds them, the logarithms of the rows' sums behind them.
   constexpr float kUnit = 1.0f / (kWeightUnit * kCodeUnit<F>);
+  float factor[QT], log[QT];
 #pragma unroll
   for(int t = 0; t < QT; ++t) {
-    const int r = 16 * (QT * wave + t) + c;
     sum[t] = over_lanes_sum(sum[t]);
-    const float factor = (sum[t] == 0.0f ? 0.0f : 1.0f / sum[t]) * (unit[t] * kUnit);
+    factor[t] = (sum[t] == 0.0f ? 0.0f : 1.0f / sum[t]) * (unit[t] * kUnit);
+    log[t] = sum[t] == 0.0f ? kNone : top[t] + __builtin_amdgcn_logf(sum[t]);
+#pragma unroll
+    for(int j = 0; j < kDims; ++j) o[t][j] *= factor[t];
+  }
+  if(x.w.parts > 1) {
+    constexpr int kTileFloats = kRows * (DP + 1);
+    const long long place = ((long long)x.w.slot * a.Hk + x.head) * a.row_tiles + x.tile, stride = (long long)a.Hk * a.row_tiles * kTileFloats;
+    float* const first = a.part + place * kTileFloats;
+    const unsigned mine = wave * (16 * QT * DP) + 4 * lane, my_log = kRows * DP + wave * 16 * QT + c;
+    {
+      const CacheBuffer to(first + x.w.part * stride, 4u * kTileFloats);
+#pragma unroll
+      for(int t = 0; t < QT; ++t) {
+#pragma unroll
+        for(int j = 0; j < kDims; ++j) to.store_through(o[t][j], 4u * (mine + 256u * (t * kDims + j)));
+        if(g == 0) to.store_through(log[t], 4u * (my_log + 16u * t));
+      }
+    }
+    if(!cache_arrived_last(a.counters + place, x.w.parts, sh.parts.is_last)) return;
+    float most[QT], total[QT];
+#pragma unroll
+    for(int t = 0; t < QT; ++t) {
+      most[t] = kNone;
+      total[t] = 0.0f;
+#pragma unroll
+      for(int j = 0; j < kDims; ++j) o[t][j] = cache_f4{0, 0, 0, 0};
+    }
+#pragma unroll 1
+    for(int i = 0; i < x.w.parts; ++i) {
+      const CacheBuffer from(first + i * stride, 4u * kTileFloats);
+      cache_f4 y[QT][kDims];
+      float l[QT];
+#pragma unroll
+      for(int t = 0; t < QT; ++t) {
+        l[t] = from.number_through(4u * (my_log + 16u * t));
+#pragma unroll
+        for(int j = 0; j < kDims; ++j) y[t][j] = from.piece_through(4u * (mine + 256u * (t * kDims + j)));
+      }
+#pragma unroll
+      for(int t = 0; t < QT; ++t) {
+        const float m = fmaxf(most[t], l[t]), down = most[t] == kNone ? 0.0f : __builtin_amdgcn_exp2f(most[t] - m);
+        const float weight = l[t] == kNone ? 0.0f : __builtin_amdgcn_exp2f(l[t] - m);
+        most[t] = m;
+        total[t] = total[t] * down + weight;
+#pragma unroll
+        for(int j = 0; j < kDims; ++j)
+#pragma unroll
+          for(int e = 0; e < 4; ++e) o[t][j][e] = __builtin_fmaf(weight, y[t][j][e], o[t][j][e] * down);
+      }
+    }
+#pragma unroll
+    for(int t = 0; t < QT; ++t) {
+      const float all = total[t] == 0.0f ? 0.0f : 1.0f / total[t];
+#pragma unroll
+      for(int j = 0; j < kDims; ++j) o[t][j] *= all;
+    }
+  }
+#pragma unroll
+  for(int t = 0; t < QT; ++t) {
+    const int r = row0 + 16 * t + c;
+    if(r >= x.rows) continue;
+    T* const out = cache_row_out<T>(a, x, r);
 #pragma unroll
     for(int e = 0; e < 4; ++e)
 #pragma unroll
       for(int i = 0; i < kDims / 4; ++i) {
-        const float y[4] = {o[t][4 * i][e] * factor, o[t][4 * i + 1][e] * factor, o[t][4 * i + 2][e] * factor, o[t][4 * i + 3][e] * factor};
-        out.emit(r, 64 * i + 16 * g + 4 * e, y);
+        const int d = 64 * i + 16 * g + 4 * e;
+        const float y[4] = {o[t][4 * i][e], o[t][4 * i + 1][e], o[t][4 * i + 2][e], o[t][4 * i + 3][e]};
+        if(d < a.dk) store_row<4, T>(out + d, y);
       }
-    if(g == 0) out.emit_log(r, top[t], sum[t]);
   }
-  if(!out.whole) cache_join_parts<T, DP, kRows, 4>(a, x, out, sh.parts);
 }
 
 }  // namespace marian_hip
