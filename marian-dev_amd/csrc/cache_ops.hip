@@ -126,56 +126,67 @@ __global__ __launch_bounds__(256) void append_kernel(const T* k, const T* v, con
   const int lane = tid % LANES, all = 2 * a.heads + a.q_heads, row = blockIdx.x * kRows + tid / LANES;
   const int d = 8 * lane;
   const bool there = row < all && d < a.dk;
-  const int what = row < a.heads ? 0 : row < 2 * a.heads ? 1 : 2, h = row - what * a.heads;
-  const T* x = nullptr;
-  long long step = 0;
-  if(there) {
-    const Strides& st = what == 0 ? a.kx : what == 1 ? a.vx : a.qx;
-    x = (what == 0 ? k : what == 1 ? v : q) + s * st.s + h * st.h + first * st.n;
-    step = st.n;
+  const int what = row < a.heads ? 0 : row < 2 * a.heads ? 1 : 2, h = there ? row - what * a.heads : 0;
+  const Strides& st = what == 0 ? a.kx : what == 1 ? a.vx : a.qx;
+  const T* const x = (!there || what == 0 ? k : what == 1 ? v : q) + s * (there ? st.s : a.kx.s) + h * st.h + (there ? d : 0);
+  const long long step = there ? st.n : a.kx.n;
+  // Halves: where the values that the lane's two fours are turned with lie (a four beyond the turned ones: itself).
+  int other[2];
+#pragma unroll
+  for(int quad = 0; quad < 2; ++quad) {
+    const int e = 4 * quad;
+    other[quad] = e + (d + e < half ? half : d + e < a.dims ? -half : 0);
+    if(!there || a.interleaved || what == 1) other[quad] = e;
   }
-#pragma unroll 1
-  for(int t = 0; t < tokens; ++t) {
+  // All tokens are asked for at once.
+  float y[kAppendTokens][8], z[kAppendTokens][2][4];
+#pragma unroll
+  for(int t = 0; t < kAppendTokens; ++t) {
+    const T* const in = x + min(first + t, a.n - 1) * step;
+    load_row<8>(in, y[t]);
+#pragma unroll
+    for(int quad = 0; quad < 2; ++quad) load_row<4>(in + other[quad], z[t][quad]);
+  }
+#pragma unroll
+  for(int t = 0; t < kAppendTokens; ++t) {
     const int token = first + t, slot = len + token;
-    float y[8] = {};
     const bool kept = token < count && (what == 2 || slot < a.cap);
-    if(there && kept) {
-      const T* in = x + t * step;
-      load_row<8>(in + d, y);
-      if(what != 1 && d < a.dims) {
+    if(what != 1) {
 #pragma unroll
-        for(int quad = 0; quad < 2; ++quad) {
-          const int b = d + 4 * quad;
-          if(b >= a.dims) break;
-          float* z = y + 4 * quad;
-          if(a.interleaved) {
+      for(int quad = 0; quad < 2; ++quad) {
+        const int e = 4 * quad;
+        if(d + e >= a.dims) continue;
+        if(a.interleaved) {
 #pragma unroll
-            for(int p = 0; p < 2; ++p) {
-              const double2 w = turn[t][b / 2 + p];
-              const double va = z[2 * p], vb = z[2 * p + 1];
-              z[2 * p] = (float)__builtin_fma(va, w.x, -(vb * w.y));
-              z[2 * p + 1] = (float)__builtin_fma(va, w.y, vb * w.x);
-            }
-          } else {
-            float other[4];
-            load_row<4>(in + (b < half ? b + half : b - half), other);
+          for(int p = 0; p < 2; ++p) {
+            const double2 w = turn[t][(d + e) / 2 + p];
+            const double va = y[t][e + 2 * p], vb = y[t][e + 2 * p + 1];
+            y[t][e + 2 * p] = (float)__builtin_fma(va, w.x, -(vb * w.y));
+            y[t][e + 2 * p + 1] = (float)__builtin_fma(va, w.y, vb * w.x);
+          }
+        } else {
+          const bool upper = d + e >= half;   // (its sine counts the other way)
 #pragma unroll
-            for(int p = 0; p < 4; ++p) {
-              const double2 w = turn[t][(b < half ? b : b - half) + p];
-              const double mine = z[p], its = other[p];
-              z[p] = b < half ? (float)__builtin_fma(mine, w.x, -(its * w.y)) : (float)__builtin_fma(its, w.y, mine * w.x);
-            }
+          for(int p = 0; p < 4; ++p) {
+            const double2 w = turn[t][d + e - (upper ? half : 0) + p];
+            const double mine = y[t][e + p], its = z[t][quad][p];
+            y[t][e + p] = (float)__builtin_fma(mine, w.x, its * (upper ? w.y : -w.y));
           }
         }
       }
     }
     if(what == 2) {
-      if(there) store_row<8, T>(q_out + s * a.qo.s + h * a.qo.h + (long long)token * a.qo.n + d, y);
+      if(there && token < a.n) {
+        float out[8];
+#pragma unroll
+        for(int e = 0; e < 8; ++e) out[e] = kept ? y[t][e] : 0.0f;
+        store_row<8, T>(q_out + s * a.qo.s + h * a.qo.h + (long long)token * a.qo.n + d, out);
+      }
       continue;
     }
     unsigned most = 0;   // bits of the largest magnitude, NaN above all
 #pragma unroll
-    for(int e = 0; e < 8; ++e) most = max(most, __builtin_bit_cast(unsigned, y[e]) & 0x7fffffffu);
+    for(int e = 0; e < 8; ++e) most = max(most, __builtin_bit_cast(unsigned, there ? y[t][e] : 0.0f) & 0x7fffffffu);
 #pragma unroll
     for(int o = 1; o < LANES; o <<= 1) most = max(most, (unsigned)__shfl_xor((int)most, o, 64));
     if(!there || !kept) continue;
@@ -184,7 +195,7 @@ __global__ __launch_bounds__(256) void append_kernel(const T* k, const T* v, con
     if(most != 0 && most < 0x7f800000u) {
       const float fast = code_factor<F>(m);
 #pragma unroll
-      for(int e = 0; e < 8; ++e) code[e / 4] |= code_of<F>(y[e], fast, m) << (8 * (e % 4));
+      for(int e = 0; e < 8; ++e) code[e / 4] |= code_of<F>(y[t][e], fast, m) << (8 * (e % 4));
     }
     const long long at = ((long long)s * a.heads + h) * a.cap + slot;
     *reinterpret_cast<cache_u2*>((what == 0 ? a.k : a.v) + at * a.dk + d) = cache_u2{code[0], code[1]};

@@ -35,7 +35,7 @@ inline CacheAttentionPlan cache_attention_plan(int64_t sequences, int64_t heads,
   const int64_t rows = n * (q_heads / heads);
   p.few = rows > 8 || p.dp == 256 ? 0 : rows > 4 ? 8 : rows > 2 ? 4 : (int)rows;
   p.qt = rows <= 16 || p.dp == 256 ? 1 : 2;   // (what the registers hold)
-  if(rows > 32 && p.dp == 128 && float32) p.qt = 1;
+  if(rows > 32 && (rows <= 64 || sequences * heads * ((rows + 127) / 128) < 128 || (p.dp == 128 && float32))) p.qt = 1;
   p.many = rows > 32 ? 64 * p.qt : 0;
   p.tile_rows = p.many ? p.many : 16 * p.qt;
   p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
@@ -43,7 +43,7 @@ inline CacheAttentionPlan cache_attention_plan(int64_t sequences, int64_t heads,
   p.waves = p.many ? 4 : entries >= 4096 ? 1 : entries >= 2048 ? 2 : 4;
   // Workgroups that run at a time, by the registers of their form, and parts for twice as many (a sequence's last part is half as
   // long as the others on average).
-  const int to_a_simd = p.many ? (p.dp == 256 ? 1 : 2) : p.few ? (p.dp == 128 ? 2 : p.few <= 2 ? 4 : 3) : p.dp == 64 ? 5 - p.qt : p.dp == 128 ? 4 - p.qt : 2;
+  const int to_a_simd = p.many ? (p.dp == 256 ? 1 : p.qt == 1 ? 3 : 2) : p.few ? (p.dp == 128 ? 2 : p.few <= 2 ? 4 : 3) : p.dp == 64 ? 5 - p.qt : p.dp == 128 ? 4 - p.qt : 2;
   const int64_t at_a_time = 1024 * to_a_simd / p.waves;
   p.target = std::max<int64_t>(1, at_a_time / (heads * p.row_tiles) - sequences / 2);
   p.least = entries >= at_a_time || !p.few ? 4 : 2;
