@@ -1211,7 +1211,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void cache_attention_many_k
   };
   auto turn = [&](int at) __attribute__((always_inline)) {   // the positions in hand into LDS, the next ones asked for
     __syncthreads();   // (nobody reads the last ones any more)
+    __builtin_amdgcn_s_setprio(2);
     lay();
+    __builtin_amdgcn_s_setprio(0);
     __syncthreads();
     fetch(at + kTile);
   };

@@ -551,9 +551,8 @@ int marian_hip_cache_read(const marian_hip_kv_cache* cache, const int32_t* first
 
 size_t marian_hip_cache_attention_workspace_bytes(int64_t sequences, int64_t heads, int64_t q_heads, int64_t n, int64_t dk) {
   if(sequences < 1 || heads < 1 || q_heads < heads || q_heads % heads != 0 || n < 1 || !row_size(dk)) return 0;
-  int64_t bytes = 0;   // (enough for activations of any type)
-  for(const bool float32 : {false, true}) bytes = std::max(bytes, cache_attention_bytes(cache_attention_plan(sequences, heads, q_heads, n, dk, float32), heads));
-  return (size_t)bytes;
+  if(sequences > 0xffff || q_heads > (int64_t)kMaxHeads * heads || n > 1 << 20) return 0;
+  return (size_t)cache_attention_bytes(cache_attention_plan(sequences, heads, q_heads, n, dk), heads);
 }
 
 int marian_hip_cache_attention_workspace_init(void* workspace, size_t workspace_bytes, void* stream) {
@@ -580,7 +579,7 @@ int marian_hip_cache_attention(const marian_hip_kv_cache* cache, const marian_hi
   Span qs, os;
   MH_CHECK(check_rows(q, q_strides, type, sequences, q_heads, n, dk, &qs));
   MH_CHECK(check_rows(out, out_strides, type, sequences, q_heads, n, dk, &os));
-  const CacheAttentionPlan p = cache_attention_plan(sequences, heads, q_heads, n, dk, type == MARIAN_HIP_FLOAT32);
+  const CacheAttentionPlan p = cache_attention_plan(sequences, heads, q_heads, n, dk);
   if(p.grid > 0x7fffffff || p.items * heads > 0x7fffffff) return MARIAN_HIP_ERR_RANGE;
   const int64_t need = cache_attention_bytes(p, heads), rows = cache_rows(cache);
   if(need > 0 && !workspace) return MARIAN_HIP_ERR_NULL;

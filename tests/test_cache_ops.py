@@ -196,7 +196,7 @@ int main() {
   long long s, h, hq, n, dk;
   while(std::scanf("%lld %lld %lld %lld %lld", &s, &h, &hq, &n, &dk) == 5) {
     const auto p = marian_hip::cache_attention_plan(s, h, hq, n, dk);
-    std::printf("%d %d %d %lld %lld %lld %lld %lld %lld\n", p.dp, p.qt, p.least, (long long)p.row_tiles, (long long)p.target, (long long)p.items,
+    std::printf("%d %d %d %lld %lld %lld %lld %lld %lld\n", p.dp, p.tile_rows, p.least, (long long)p.row_tiles, (long long)p.target, (long long)p.items,
                 (long long)p.slots, (long long)p.grid, (long long)marian_hip::cache_attention_bytes(p, h));
   }
 }
@@ -217,15 +217,15 @@ def test_parts_stay_within_grid_and_workspace(tmp_path):
     out = subprocess.run([str(exe)], input="\n".join(" ".join(map(str, c)) for c in cases), capture_output=True, text=True, check=True).stdout
     lib = load("_lib").lib()
     for (s, h, hq, n, dk), line in zip(cases, out.splitlines()):
-        dp, qt, least, tiles, target, items, slots, grid, size = map(int, line.split())
+        dp, tile, least, tiles, target, items, slots, grid, size = map(int, line.split())
         rows = n * (hq // h)
-        assert dp >= dk and 16 * qt * tiles >= rows > 16 * qt * (tiles - 1) and grid >= items * h * tiles
+        assert dp >= dk and tile * tiles >= rows > tile * (tiles - 1) and grid >= items * h * tiles
         assert lib.marian_hip_cache_attention_workspace_bytes(s, h, hq, n, dk) == size
         if target == 1:
             assert items == s and slots == 0 and size == 0
             continue
         counters = slots * h * tiles
-        assert 4 * counters <= 32768 and size == 32768 + counters * 16 * qt * (dp + 1) * 4
+        assert 4 * counters <= 32768 and size == 32768 + counters * tile * (dp + 1) * 4
         for longest in (0, 1, 127, 128, 129, 5000, 1 << 20):
             blocks = [(rng.randint(0, longest) + 127) // 128 for _ in range(s)]
             blocks[rng.randrange(s)] = (longest + 127) // 128
