@@ -290,7 +290,9 @@ int marian_hip_fill(void* begin, int64_t count, int elem_bytes, uint64_t pattern
  *
  * Activations are float32, float16 or bfloat16 ("type"), [sequences, heads, n, dk] with the values between two
  * sequences, heads and positions given (three strides, in values, whole multiples of 16 bytes), so that rows of an
- * affine call are read as they are.  16-byte aligned; dk a multiple of 16 from 16 to 256.
+ * affine call are read as they are.  16-byte aligned; dk a multiple of 16 from 16 to 256.  Rows that are read may share
+ * memory (a stride of 0), rows that are written may not (MARIAN_HIP_ERR_ALIAS: a stride reaches over all that lies
+ * within one of its steps, in any order of the dimensions).  n up to 2^20 (marian_hip_cache_append: 262140).
  */
 #define MARIAN_HIP_FLOAT32 0
 #define MARIAN_HIP_FLOAT16 1
@@ -304,6 +306,7 @@ int marian_hip_fill(void* begin, int64_t count, int elem_bytes, uint64_t pattern
  * A code is the exact quotient value * 127 / largest (448) rounded to the nearest, ties to even.  A row of zeros
  * has scale 0.  A row that holds an infinity or NaN has zeros for codes and a NaN scale: everything that reads it
  * is NaN, and nothing that does not read it.
+ * Codes that come from elsewhere are taken by their bits: int8 -128 is -128, and e4m3's NaN (0x7f, 0xff) is 480 (-480).
  *   heads <= 4096, sequences <= 65535, capacity * dk < 2^31; k and v 16-byte, scales 4-byte aligned.
  */
 #define MARIAN_HIP_CACHE_INT8 0

@@ -89,7 +89,9 @@ def _whole_numbers(t, shape, device, what):
     _abort_if(not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64) or t.device != device, "{}: whole numbers (int32) on {}",
               what, device)
     _abort_if(tuple(t.shape) != tuple(shape), "{}: shape {}, not {}", what, tuple(shape), tuple(t.shape))
-    return t.to(torch.int32).contiguous()
+    if t.dtype == torch.int64:   # (what 32 bits do not hold stays beyond any length)
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
+    return t.contiguous()
 
 
 def _cache(cache, what):
@@ -130,7 +132,7 @@ def _out(out, like, what):
 
 def rotaryPositions(x, positions, rotary, out=None):
     """x [sequences, heads, n, dk] with the first values of every row turned by its position: positions [sequences] -
-    row i of a sequence at positions[s] + i - or [sequences, n].  out: x itself, or a tensor apart from it; None: a new
+    row i of a sequence at positions[s] + i - or [sequences, n], 32 bits of them.  out: x itself, or a tensor apart from it; None: a new
     one that lies in memory as x does."""
     res = _host.rotary(x, positions, rotary, out)
     if res is not None:

@@ -4,7 +4,10 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <array>
 #include <cmath>
+#include <utility>
 
 #include "../../include/marian_hip_int8.h"
 #include "abi_common.h"
@@ -22,8 +25,8 @@ struct Strides {   // in values
 
 // ---------------------------------------------------------------- rotary positions
 // A pair's angle in half turns, -1 .. 1: position times turns mod 2^64 is the fraction of a turn exactly.
-__device__ __forceinline__ float half_turns(int position, unsigned long long turns) {
-  const long long f = (long long)(turns * (unsigned long long)(long long)position);
+__device__ __forceinline__ float half_turns(long long position, unsigned long long turns) {
+  const long long f = (long long)(turns * (unsigned long long)position);
   return __builtin_fmaf((float)(unsigned)f, 0x1p-63f, (float)(int)(f >> 32) * 0x1p-31f);
 }
 
@@ -38,7 +41,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const T* x, Strides xs, T* 
   const int u = id % units, hg = id / units % groups, i = id / units / groups, s = blockIdx.y;
   if(i >= n) return;
   const bool turned = 8 * u < dims;
-  const int at = each ? positions[(long long)s * n + i] : positions[s] + i;
+  const long long at = each ? positions[(long long)s * n + i] : (long long)positions[s] + i;
   const int d0 = turned && !interleaved ? 4 * u : 8 * u, d1 = turned && !interleaved ? dims / 2 + 4 * u : 8 * u + 4;
   x += s * xs.s + i * xs.n;
   out += s * os.s + i * os.n;
@@ -314,7 +317,14 @@ int for_format(int format, F f) {
 inline int width_of(int type) { return type == MARIAN_HIP_FLOAT32 ? 4 : 2; }
 inline bool aligned(const void* p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline bool row_size(int64_t dk) { return dk >= 16 && dk <= 256 && dk % 16 == 0; }
+constexpr int64_t kMostThreads = 0xffffffff;   // of a launch, in one dimension
 constexpr int64_t kMaxTokens = 1 << 20, kMaxHeads = 4096, kMaxSequences = 65535;
+
+#define MH_CHECK(expr)                             \
+  do {                                             \
+    const int check_status_ = (expr);              \
+    if(check_status_ != MARIAN_HIP_OK) return check_status_; \
+  } while(0)
 
 int check_type(int type) { return type >= MARIAN_HIP_FLOAT32 && type <= MARIAN_HIP_BFLOAT16 ? MARIAN_HIP_OK : MARIAN_HIP_ERR_SHAPE; }
 
@@ -363,17 +373,24 @@ int check_rows(const void* p, const int64_t* st, int type, int64_t sequences, in
   *span = Span{p, last * width_of(type)};
   return MARIAN_HIP_OK;
 }
+// ... that is written: its rows share no memory, each dimension's step reaching over all that lies within one of its steps.
+int check_written(const void* p, const int64_t* st, int type, int64_t sequences, int64_t heads, int64_t n, int64_t dk, Span* span) {
+  MH_CHECK(check_rows(p, st, type, sequences, heads, n, dk, span));
+  std::array<std::pair<int64_t, int64_t>, 3> dim{{{sequences > 1 ? st[0] : 0, sequences}, {heads > 1 ? st[1] : 0, heads}, {n > 1 ? st[2] : 0, n}}};
+  std::sort(dim.begin(), dim.end());
+  int64_t within = dk;
+  for(const auto& [step, size] : dim) {
+    if(size <= 1) continue;
+    if(step < within) return MARIAN_HIP_ERR_ALIAS;
+    within += (size - 1) * step;
+  }
+  return MARIAN_HIP_OK;
+}
 inline Strides strides(const int64_t* st) { return Strides{st[0], st[1], st[2]}; }
 inline bool same_rows(const void* a, const int64_t* x, const void* b, const int64_t* y, int64_t sequences, int64_t heads, int64_t n) {
   return a == b && (sequences <= 1 || x[0] == y[0]) && (heads <= 1 || x[1] == y[1]) && (n <= 1 || x[2] == y[2]);
 }
 inline int64_t cache_rows(const marian_hip_kv_cache* c) { return c->sequences * c->heads * c->capacity; }
-
-#define MH_CHECK(expr)                             \
-  do {                                             \
-    const int check_status_ = (expr);              \
-    if(check_status_ != MARIAN_HIP_OK) return check_status_; \
-  } while(0)
 
 __global__ __launch_bounds__(256) void clear_kernel(unsigned* p, unsigned n) {
   const unsigned i = blockIdx.x * 256u + threadIdx.x;
@@ -423,7 +440,7 @@ int marian_hip_rotary(const void* x, const int64_t* x_strides, void* out, const 
   MH_CHECK(check_rotation(rotation, dk));
   Span in, to;
   MH_CHECK(check_rows(x, x_strides, type, sequences, heads, n, dk, &in));
-  MH_CHECK(check_rows(out, out_strides, type, sequences, heads, n, dk, &to));
+  MH_CHECK(check_written(out, out_strides, type, sequences, heads, n, dk, &to));
   if(!aligned(positions, 4)) return MARIAN_HIP_ERR_ALIGN;
   if(!same_rows(x, x_strides, out, out_strides, sequences, heads, n)) MH_CHECK(apart({to}, {in}));
   MH_CHECK(apart({to}, {{positions, 4 * (each ? sequences * n : sequences)}, {rotation->turns, 4 * rotation->dims}}));
@@ -464,7 +481,7 @@ int marian_hip_cache_append(const marian_hip_kv_cache* cache, const marian_hip_d
   MH_CHECK(check_rows(v, v_strides, type, sequences, cache->heads, n, dk, &vs));
   if(q) {
     MH_CHECK(check_rows(q, q_strides, type, sequences, q_heads, n, dk, &qs));
-    MH_CHECK(check_rows(q_out, q_out_strides, type, sequences, q_heads, n, dk, &qo));
+    MH_CHECK(check_written(q_out, q_out_strides, type, sequences, q_heads, n, dk, &qo));
   }
   const int64_t rows = cache_rows(cache);
   const Span codes[2] = {{cache->k, rows * dk}, {cache->v, rows * dk}}, scales[2] = {{cache->k_scale, rows * 4}, {cache->v_scale, rows * 4}};
@@ -528,6 +545,8 @@ int marian_hip_cache_read(const marian_hip_kv_cache* cache, const int32_t* first
   const int64_t entries = cache->sequences * cache->heads, dk = cache->dk;
   if(n > 0x7fffff00 / dk) return MARIAN_HIP_ERR_RANGE;
   if(entries == 0 || n == 0) return MARIAN_HIP_OK;
+  const int64_t blocks = (n * dk * width_of(type) / 16 + 256 * kReadTurns - 1) / (256 * kReadTurns);
+  if(blocks * entries > kMostThreads / 256) return MARIAN_HIP_ERR_RANGE;
   MH_CHECK(check_cache_memory(cache));
   if(!first || !k_out || !v_out) return MARIAN_HIP_ERR_NULL;
   if(!aligned(first, 4) || !aligned(k_out, 16) || !aligned(v_out, 16)) return MARIAN_HIP_ERR_ALIGN;
@@ -535,8 +554,6 @@ int marian_hip_cache_read(const marian_hip_kv_cache* cache, const int32_t* first
   MH_CHECK(apart({{k_out, bytes}}, {{v_out, bytes}}));
   MH_CHECK(apart({{k_out, bytes}, {v_out, bytes}}, {{cache->k, rows * dk}, {cache->v, rows * dk}, {cache->k_scale, rows * 4},
                                                     {cache->v_scale, rows * 4}, {first, 4 * cache->sequences}}));
-  const int64_t blocks = (n * dk * width_of(type) / 16 + 256 * kReadTurns - 1) / (256 * kReadTurns);
-  if(blocks * entries > 0x7fffffff) return MARIAN_HIP_ERR_RANGE;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   return for_type(type, [&](auto t) -> int {
     using T = decltype(t);
@@ -574,13 +591,13 @@ int marian_hip_cache_attention(const marian_hip_kv_cache* cache, const marian_hi
   if(q_heads < heads || q_heads % heads != 0 || !(scale > 0.0f) || !std::isfinite(scale)) return MARIAN_HIP_ERR_SHAPE;
   if(q_heads / heads > kMaxHeads || n * (q_heads / heads) > 1 << 26) return MARIAN_HIP_ERR_RANGE;
   if(sequences == 0 || n == 0) return MARIAN_HIP_OK;
+  const CacheAttentionPlan p = cache_attention_plan(sequences, heads, q_heads, n, dk);
+  if(p.grid > kMostThreads / (64 * p.waves)) return MARIAN_HIP_ERR_RANGE;
   MH_CHECK(check_cache_memory(cache));
   MH_CHECK(check_drafts_memory(drafts));
   Span qs, os;
   MH_CHECK(check_rows(q, q_strides, type, sequences, q_heads, n, dk, &qs));
-  MH_CHECK(check_rows(out, out_strides, type, sequences, q_heads, n, dk, &os));
-  const CacheAttentionPlan p = cache_attention_plan(sequences, heads, q_heads, n, dk);
-  if(p.grid > 0x7fffffff || p.items * heads > 0x7fffffff) return MARIAN_HIP_ERR_RANGE;
+  MH_CHECK(check_written(out, out_strides, type, sequences, q_heads, n, dk, &os));
   const int64_t need = cache_attention_bytes(p, heads), rows = cache_rows(cache);
   if(need > 0 && !workspace) return MARIAN_HIP_ERR_NULL;
   if((int64_t)workspace_bytes < need) return MARIAN_HIP_ERR_WORKSPACE;
@@ -632,6 +649,7 @@ int marian_hip_cache_keep(const marian_hip_kv_cache* cache, const int32_t* lens,
   MH_CHECK(check_cache(cache));
   if(path_len < 0 || path_len > MARIAN_HIP_TREE_MAX) return MARIAN_HIP_ERR_SHAPE;
   const int64_t sequences = cache->sequences, rows = cache_rows(cache), dk = cache->dk;
+  if(sequences * cache->heads > kMostThreads / 256) return MARIAN_HIP_ERR_RANGE;
   if(sequences == 0) return MARIAN_HIP_OK;
   MH_CHECK(check_cache_memory(cache));
   if(!lens || !accepted || !new_lens || (path_len > 0 && !path)) return MARIAN_HIP_ERR_NULL;

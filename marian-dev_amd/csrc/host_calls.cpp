@@ -21,6 +21,8 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/ops/as_strided_native.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 
@@ -152,7 +154,7 @@ struct PerStream {
   at::Tensor workspace;              // abs-max partials, one-pass exchange
   std::mutex turn;                   // held while a call makes its launches over the workspace
   std::vector<at::Tensor> nbest;     // the last one the largest
-  std::vector<at::Tensor> cache;     // of the attention over a quantized cache, the same
+  at::Tensor cache;                  // of the attention over a quantized cache (recorded calls have their own)
   at::Tensor scratch;                // of the calls, not lent at the moment
 };
 std::map<std::pair<int, hipStream_t>, PerStream> per_stream;   // (looked up with the interpreter lock held)
@@ -1247,6 +1249,18 @@ inline int activation_type(const at::Tensor& t) {
   }
 }
 
+// The thread's device until the end of a call (a default stream's launches go to the current one), where there are several.
+class On {
+ public:
+  explicit On(c10::Device d) {
+    static const bool several = c10::hip::device_count() > 1;
+    if(several) guard_.reset_device(d);
+  }
+
+ private:
+  c10::OptionalDeviceGuard guard_;
+};
+
 // A tensor [sequences, heads, n, dk] of one of the activation types on device d (any: that of t), read or written by its
 // strides, which with its address are whole multiples of sixteen bytes.
 struct Rows {
@@ -1362,6 +1376,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if(!rows_of(tensor(args[3]), &d, o) || o.type != x.type || o.t->sizes() != x.t->sizes()) Py_RETURN_NONE;
     out = *o.t;
   }
+  const On on(d);
   const hipStream_t st = stream_of(d);
   call("rotaryPositions", [&] {
     return L.rotary(x.t->const_data_ptr(), x.strides, out.data_ptr(), o.strides, x.type, sequences, x.t->size(1), n, x.t->size(3), at, each, &r, st);
@@ -1395,6 +1410,7 @@ PyObject* py_cache_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   } else if(!none(args[8])) {
     Py_RETURN_NONE;
   }
+  const On on(c.device);
   const hipStream_t st = stream_of(c.device);
   call("appendToCache", [&] {
     return L.cache_append(&c.c, &x, k.t->const_data_ptr(), k.strides, v.t->const_data_ptr(), v.strides, k.type, r.turns ? &r : nullptr,
@@ -1416,6 +1432,7 @@ PyObject* py_cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if(n < 0 || (type != at::kFloat && type != at::kHalf && type != at::kBFloat16)) Py_RETURN_NONE;
   const int64_t size[4] = {c.c.sequences, c.c.heads, n, c.c.dk};
   at::Tensor k = empty(size, type, c.device), v = empty(size, type, c.device);
+  const On on(c.device);
   const hipStream_t st = stream_of(c.device);
   call("readCache", [&] { return L.cache_read(&c.c, first, n, k.data_ptr(), v.data_ptr(), activation_type(k), st); });
   Ref a(wrap(std::move(k))), b(wrap(std::move(v)));
@@ -1423,17 +1440,23 @@ PyObject* py_cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   MH_END
 }
 
-// The workspace of an attention over a quantized cache: a stream's own, for good, or of a call that is recorded its own, cleared
-// by the graph ahead of it (the graph may be replayed on another stream, and beside another graph).
+// The workspace of an attention over a quantized cache: a stream's own, kept until a call needs a larger one (then with room to spare, and
+// the old one goes back to the stream that it was used on), or of a call that is recorded its own, cleared by the graph ahead of it
+// (the graph may be replayed on another stream, and beside another graph).
 at::Tensor cache_workspace(int64_t need, c10::Device d, hipStream_t st) {
   const bool once = marian_hip::recorded(st);
+  int64_t size = need;
   if(!once) {
-    std::vector<at::Tensor>& held = per_stream[{d.index(), st}].cache;
-    if(!held.empty() && held.back().numel() >= need) return held.back();
+    const at::Tensor& held = per_stream[{d.index(), st}].cache;
+    if(held.defined() && held.numel() >= need) return held;
+    for(size = 1 << 20; size < need;) size *= 2;
   }
-  at::Tensor made = empty({need}, at::kByte, d);
-  call("AttentionOverCache", [&] { return L.cache_attention_workspace_init(made.data_ptr(), (size_t)need, st); });
-  if(!once) per_stream[{d.index(), st}].cache.push_back(made);
+  at::Tensor made = empty({size}, at::kByte, d);
+  call("AttentionOverCache", [&] { return L.cache_attention_workspace_init(made.data_ptr(), (size_t)size, st); });
+  if(!once) {
+    at::Tensor& held = per_stream[{d.index(), st}].cache;
+    if(!held.defined() || held.numel() < size) held = made;   // (another thread may have been here meanwhile)
+  }
   return made;
 }
 
@@ -1454,6 +1477,7 @@ PyObject* py_cache_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     if(!rows_of(tensor(args[6]), &c.device, o) || o.type != q.type || o.t->sizes() != q.t->sizes()) Py_RETURN_NONE;
     out = *o.t;
   }
+  const On on(c.device);
   const hipStream_t st = stream_of(c.device);
   const int64_t q_heads = q.t->size(1);
   const int64_t need = (int64_t)L.cache_attention_workspace_bytes(c.c.sequences, c.c.heads, q_heads, x.n, c.c.dk);
@@ -1478,6 +1502,7 @@ PyObject* py_cache_keep(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
      !whole_numbers(args[3], false, c.c.sequences, -1, c.device, &accepted))
     Py_RETURN_NONE;
   at::Tensor out = empty({c.c.sequences}, at::kInt, c.device);
+  const On on(c.device);
   const hipStream_t st = stream_of(c.device);
   call("keepDrafts", [&] { return L.cache_keep(&c.c, lens, along, path->size(1), accepted, static_cast<int32_t*>(out.data_ptr()), st); });
   return wrap(std::move(out));

@@ -238,3 +238,35 @@ def test_the_operators_are_exported_under_their_names():
     kv = importlib.import_module(PKG + ".cache")
     for name in ("KeyValueCache", "Rotary", "newCache", "makeRotary", "rotaryPositions", "appendToCache", "readCache", "AttentionOverCache", "keepDrafts"):
         assert callable(getattr(kv, name))
+
+
+# ---- rows that are written ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("strides,status", [
+    ((HQ * N * DK, N * DK, DK), "OK"), ((HQ * N * DK, DK, HQ * DK), "OK"), ((DK, S * DK, S * HQ * DK), "OK"), ((2 * HQ * N * DK, N * DK, DK), "OK"),
+    ((0, N * DK, DK), "ALIAS"), ((HQ * N * DK, 0, DK), "ALIAS"), ((HQ * N * DK, N * DK, 0), "ALIAS"), ((HQ * N * DK, N * DK, DK - 16), "ALIAS"),
+    ((HQ * N * DK, (N - 1) * DK, DK), "ALIAS"), ((HQ * N * DK - 16, N * DK, DK), "ALIAS")])
+def test_rows_that_are_written_share_no_memory(strides, status):
+    """(a call that is fine so far is stopped by an argument that is looked at later)"""
+    L, st = load("_lib"), (ctypes.c_int64 * 3)(*strides)
+    want = getattr(L, "ERR_" + status) if status != "OK" else None
+    c, d, r = structs()
+    at = PLACES
+    far = {**at, "lens": at["lens"] + 2}
+    calls = [lambda: L.lib().marian_hip_rotary(at["xq"], dense(HQ), at["qo"], st, 0, S, HQ, N, DK, far["lens"], 0, ctypes.byref(r), None),
+             lambda: L.lib().marian_hip_rotary(at["qo"], st, at["qo"], st, 0, S, HQ, N, DK, far["lens"], 0, ctypes.byref(r), None),
+             lambda: L.lib().marian_hip_cache_append(ctypes.byref(c), ctypes.byref(d), at["k"], dense(H), at["xv"], dense(H), 0, None, at["xq"], dense(HQ),
+                                                     HQ, at["qo"], st, None),
+             lambda: L.lib().marian_hip_cache_attention(ctypes.byref(c), ctypes.byref(d), at["xq"], dense(HQ), HQ, 0, 0.125, at["qo"], st, at["ws"] + 2,
+                                                        1 << 40, None)]
+    for call, later in zip(calls, (L.ERR_ALIGN, L.ERR_ALIGN, L.ERR_ALIAS, L.ERR_ALIGN)):
+        assert call() == (later if want is None else want)
+
+
+def test_launches_past_the_devices_range_are_refused():
+    L = load("_lib")
+    many = {"sequences": 65535, "heads": 4096, "capacity": 1, "dk": 16}
+    assert attention(q_heads=4096, n=1, **many) == L.ERR_RANGE
+    assert keep(**many) == L.ERR_RANGE
+    assert read(n=1 << 10, **many) == L.ERR_RANGE
+    size = L.lib().marian_hip_cache_attention_workspace_bytes
+    assert size(1 << 40, 8, 8, 1, 64) == 0 and size(1, 1, 1 << 40, 1, 64) == 0 and size(1, 1, 1, 1 << 62, 64) == 0 and size(1, 8, 8, 1, 64) > 0

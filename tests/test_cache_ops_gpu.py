@@ -602,3 +602,94 @@ def test_two_threads_with_a_stream_each():
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+# ---- calls at the edges -----------------------------------------------------------------------------------------
+def test_rows_that_share_memory():
+    """Expanded keys, values and queries are read as they are; expanded outputs, in place or not, are refused"""
+    kv, error, r = load("cache"), load("_lib").MarianHipError, maker(3)
+    S, H, G, n, dk = 3, 2, 4, 5, 64
+    rotary = kv.makeRotary(dk)
+    lens = ints([0, 3, 9])
+    one = r(1, 1, n, dk)
+    k, q = one.expand(S, H, n, dk), one.expand(S, H * G, n, dk)
+    a, b = kv.newCache(S, H, 20, dk), kv.newCache(S, H, 20, dk)
+    turned = kv.appendToCache(a, k, k, lens, rotary=rotary, q=q)
+    again = kv.appendToCache(b, k.contiguous(), k.contiguous(), lens, rotary=rotary, q=q.contiguous())
+    assert same(turned, again) and all(same(x, y) for x, y in zip(a, b))
+    assert same(kv.AttentionOverCache(q, a, lens), kv.AttentionOverCache(q.contiguous(), a, lens))
+    assert same(kv.rotaryPositions(q, lens, rotary), kv.rotaryPositions(q.contiguous(), lens, rotary))
+    before = [t.clone() for t in a]
+    for call in (lambda: kv.rotaryPositions(q, lens, rotary, out=q), lambda: kv.appendToCache(a, k.contiguous(), k.contiguous(), lens, rotary=rotary, q=q, qOut=q),
+                 lambda: kv.AttentionOverCache(turned, a, lens, out=r(S, 1, n, dk).expand(S, H * G, n, dk))):
+        with pytest.raises(error):
+            call()
+    assert all(same(x, y) for x, y in zip(a, before))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_in_place(interleaved):
+    kv, r = load("cache"), maker(4)
+    S, H, n, dk = 2, 3, 9, 80
+    rotary = kv.makeRotary(48, interleaved=interleaved)
+    lens = ints([5, 1000])
+    for lay in (lambda: r(S, H, n, dk), lambda: side_by_side(r, S, H, n, dk, BF16)):
+        x = lay()
+        want = kv.rotaryPositions(x, lens, rotary)
+        cache, other = kv.newCache(S, H, 1100, dk), kv.newCache(S, H, 1100, dk)
+        k = x.clone()
+        q = kv.appendToCache(cache, k, k, lens, rotary=rotary, q=x)
+        y = x.clone()
+        assert kv.rotaryPositions(y, lens, rotary, out=y) is not None and same(y, want)
+        y = x.clone()
+        kv.appendToCache(other, k, k, lens, rotary=rotary, q=y, qOut=y)
+        assert same(y, q) and all(same(a, b) for a, b in zip(cache, other))
+
+
+def test_positions_at_the_ends_of_32_bits():
+    """Row i stands at positions[s] + i also where that passes 2^31 - 1; lengths of 64 bits are beyond any capacity"""
+    kv, r = load("cache"), maker(5)
+    x = r(2, 1, 4, 64)
+    rotary = kv.makeRotary(64)
+    first = [2 ** 31 - 2, -2 ** 31]
+    got = kv.rotaryPositions(x, ints(first), rotary).cpu()
+    turns = [int(t) % 2 ** 64 for t in rotary.turns.cpu()]
+    for s in range(2):
+        for i in range(4):
+            for p in range(32):
+                angle = 2 * math.pi * ((first[s] + i) * turns[p] % 2 ** 64) / 2 ** 64
+                a, b = float(x[s, 0, i, p]), float(x[s, 0, i, p + 32])
+                size = abs(a) + abs(b)
+                # an angle in float32, up to a half turn: 2^-24 of it; sine and cosine within 2 steps; two products and a sum
+                bound = size * (math.pi * 2 ** -23 + 6 * 2 ** -24)
+                assert abs(float(got[s, 0, i, p]) - (a * math.cos(angle) - b * math.sin(angle))) <= bound
+                assert abs(float(got[s, 0, i, p + 32]) - (a * math.sin(angle) + b * math.cos(angle))) <= bound
+    cache = filled(r, 2, 1, 10, 64, "int8")
+    far = torch.tensor([2 ** 32 + 3, -2 ** 32], device="cuda")
+    near = ints([10, 0])
+    q = r(2, 1, 1, 64)
+    assert same(kv.AttentionOverCache(q, cache, far), kv.AttentionOverCache(q, cache, near))
+    assert kv.keepDrafts(cache, far, ints([[0], [0]]), ints([1, 1])).tolist() == [10, 1]
+
+
+def test_lengths_that_grow_on_one_stream_and_codes_from_elsewhere():
+    """Calls of all sizes after each other, the workspace growing on the way and serving the smaller ones again; e4m3's NaN codes
+    and int8's -128 are taken by their bits, alike by attention and reading"""
+    kv, r = load("cache"), maker(6)
+    for dtype in (F32, BF16):
+        for n, H, cap in ((1, 8, 3000), (40, 2, 5000), (1, 8, 3000), (130, 1, 900), (64, 8, 700), (1, 1, 9000)):
+            cache = filled(r, 2, H, cap, 64, "int8")
+            q, lens = r(2, 2 * H, n, 64).to(dtype), ints([cap - n, cap // 3])
+            check(kv.AttentionOverCache(q, cache, lens), *expected(q, cache, lens))
+    for format, bits, value in (("e4m3", 0x7f, 480.0), ("e4m3", 0xff, -480.0), ("int8", 0x80, -128.0)):
+        cache = kv.newCache(1, 1, 4, 64, format)
+        for t in cache[:2]:
+            t.view(torch.uint8).fill_(bits)
+        for t in cache[2:]:
+            t.fill_(0.5)
+        assert all((x == value / 2).all() for x in kv.readCache(cache, ints([0]), 4))
+        # (the sum is divided by through its reciprocal, and weights are exponentials: not exact even here, but within the oracle's
+        # bound, which counts both)
+        q, codes, scales = torch.ones(1, 1, 1, 64), torch.full((1, 1, 4, 64), value, dtype=torch.float64), torch.full((1, 1, 4), 0.5)
+        got = kv.AttentionOverCache(q.cuda(), cache, ints([3]))
+        check(got, *oracle.attention(q, codes, codes, scales, scales, torch.tensor([3]), None, None, 0.125))
