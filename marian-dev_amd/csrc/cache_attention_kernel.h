@@ -55,6 +55,11 @@ __device__ __forceinline__ unsigned lanes_sum(unsigned x) {
   return (unsigned)v;
 }
 
+// Blocks of a part of a sequence of `blocks`.
+__device__ __forceinline__ unsigned cache_part_size(unsigned blocks, unsigned each) {
+  return max(blocks <= kCacheWhole ? max(each, kCacheWhole) : each, (blocks + kCacheMostParts - 1) / kCacheMostParts);
+}
+
 // Finds part `item`; false where there are fewer.  All waves do the same, lanes being sequences.
 __device__ __forceinline__ bool cache_part(const CacheAttentionArgs& a, int item, int lane, CachePart& w) {
   auto blocks_of = [&](int s) -> unsigned {   // of positions that sequence s has in reach
@@ -77,12 +82,11 @@ __device__ __forceinline__ bool cache_part(const CacheAttentionArgs& a, int item
     for(int base = 64 * kHeld; base < a.S; base += 64) total += blocks_of(base + lane);
     total = (unsigned)__builtin_amdgcn_readlane((int)lanes_sum(total), 63);
     each = max((unsigned)a.least, (total + a.target - 1) / a.target);
-    auto size_of = [&](unsigned mine) { return max(each, (mine + kCacheMostParts - 1) / kCacheMostParts); };
     // parts in the lower bits, those of sequences with several in the upper twelve (less than 2 * target)
     unsigned before = 0;
     bool found = false;
     auto look = [&](int base, unsigned mine) __attribute__((always_inline)) {
-      const unsigned size = size_of(mine), parts = base + lane < a.S ? max(1u, (mine + size - 1) / size) : 0;
+      const unsigned size = cache_part_size(mine, each), parts = base + lane < a.S ? max(1u, (mine + size - 1) / size) : 0;
       const unsigned sum = before + lanes_sum(parts > 1 ? parts | parts << 20 : parts);
       const unsigned long long at = __ballot((int)(sum & 0xfffff) > item);
       if(at) {
@@ -107,10 +111,18 @@ __device__ __forceinline__ bool cache_part(const CacheAttentionArgs& a, int item
   w.count = a.counts ? __builtin_amdgcn_readfirstlane(clamp_int(a.counts[w.s], 0, a.n)) : a.n;
   w.used = w.count > 0 ? min(w.len + w.count, a.cap) : 0;
   const unsigned mine = (unsigned)(w.used + kCacheBlock - 1) / kCacheBlock;
-  const int size = (int)max(each, (mine + kCacheMostParts - 1) / kCacheMostParts) * kCacheBlock;
+  const int size = (int)cache_part_size(mine, each) * kCacheBlock;
   w.from = a.target > 1 ? w.part * size : 0;
   w.to = a.target > 1 ? min(w.from + size, w.used) : w.used;
   return true;
+}
+
+// A product as a number of its own.  Where it becomes a float16 and the rest of it a second one, both have to start from the
+// same float32: the compiler would turn the product into float16 in one instruction, with one rounding, for what it subtracts, and in two for
+// what it keeps, and the two float16 differ where the first rounding comes to lie half way (a weight in 16000, by 2^-11 of it).
+__device__ __forceinline__ float settled(float z) {
+  asm("" : "+v"(z));
+  return z;
 }
 
 template <typename T, CacheFormat F, int DP>
@@ -331,7 +343,7 @@ __device__ __forceinline__ float cache_query(const CacheAttentionArgs& a, const 
   for(int i = 0; i < kSteps; ++i) {
 #pragma unroll
     for(int e = 0; e < 8; ++e) {
-      const float z = y[i][e] * factor;
+      const float z = y[i][e] * factor;   // (exact)
       q[0][i][e] = (_Float16)z;
       if constexpr(kTerms == 2) q[1][i][e] = (_Float16)(z - (float)q[0][i][e]);
     }
@@ -745,7 +757,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
       const float from = top[t] == kNone ? 0.0f : -top[t];   // (nothing seen so far: minus infinity stays that)
 #pragma unroll
       for(int e = 0; e < 8; ++e) {
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], row_scale[t], from)), z = y * r[t][e];
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], row_scale[t], from)), z = kTerms == 2 ? settled(y * r[t][e]) : y * r[t][e];
         sum[t] += y;
         p[t][0][e] = (_Float16)z;
         if constexpr(kTerms == 2) p[t][1][e] = (_Float16)(z - (float)p[t][0][e]);
@@ -956,7 +968,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
 #pragma unroll
       for(int t = 0; t < kRegs; ++t) {
         const float from = top[t] == kNone ? 0.0f : -top[t];   // (nothing seen so far: minus infinity stays that)
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][t], row_scale[t], from)), z = y * (scale[i][t] * per[t]);
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][t], row_scale[t], from)), whole = y * (scale[i][t] * per[t]), z = kTerms == 2 ? settled(whole) : whole;
         sum[t] += y;
         const _Float16 hi = (_Float16)z;
         sh.weights[wave][0][mine0 + t][slot] = hi;
@@ -1187,13 +1199,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void cache_attention_many_k
     cache_h8 p[QT][kTerms];
 #pragma unroll
     for(int t = 0; t < QT; ++t) {
-      const float from = MASKED && top[t] == kNone ? 0.0f : -top[t];   // (nothing seen so far: minus infinity stays that)
+      const float from = top[t] == kNone ? 0.0f : -top[t];   // (nothing seen so far: minus infinity stays that)
 #pragma unroll
       for(int e = 0; e < 8; ++e) {
         const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], row_scale[t], from));
         float r = vs[e / 4][e % 4] * per[MASKED ? t : 0];
         if constexpr(MASKED) r = seen_here[t] >> e & 1 ? r : 0.0f;
-        const float z = y * r;
+        const float z = kTerms == 2 ? settled(y * r) : y * r;
         sum[t] += y;
         p[t][0][e] = (_Float16)z;
         if constexpr(kTerms == 2) p[t][kTerms - 1][e] = (_Float16)(z - (float)p[t][0][e]);

@@ -11,7 +11,6 @@ namespace marian_hip {
 enum class CacheFormat { int8 = 0, e4m3 = 1 };
 
 typedef float cache_f4 __attribute__((ext_vector_type(4)));
-typedef float cache_f4_any __attribute__((ext_vector_type(4), aligned(4)));   // (only its elements are aligned)
 typedef unsigned cache_u2 __attribute__((ext_vector_type(2)));
 typedef unsigned cache_u4 __attribute__((ext_vector_type(4)));
 typedef _Float16 cache_h2 __attribute__((ext_vector_type(2)));

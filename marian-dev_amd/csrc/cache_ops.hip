@@ -569,7 +569,10 @@ int marian_hip_cache_read(const marian_hip_kv_cache* cache, const int32_t* first
 size_t marian_hip_cache_attention_workspace_bytes(int64_t sequences, int64_t heads, int64_t q_heads, int64_t n, int64_t dk) {
   if(sequences < 1 || heads < 1 || q_heads < heads || q_heads % heads != 0 || n < 1 || !row_size(dk)) return 0;
   if(sequences > 0xffff || q_heads > (int64_t)kMaxHeads * heads || n > 1 << 20) return 0;
-  return (size_t)cache_attention_bytes(cache_attention_plan(sequences, heads, q_heads, n, dk), heads);
+  int64_t bytes = 0;   // (enough for any capacity)
+  for(const int64_t capacity : {(int64_t)1, (int64_t)1 << 31})
+    bytes = std::max(bytes, cache_attention_bytes(cache_attention_plan(sequences, heads, q_heads, capacity, n, dk), heads));
+  return (size_t)bytes;
 }
 
 int marian_hip_cache_attention_workspace_init(void* workspace, size_t workspace_bytes, void* stream) {
@@ -591,7 +594,7 @@ int marian_hip_cache_attention(const marian_hip_kv_cache* cache, const marian_hi
   if(q_heads < heads || q_heads % heads != 0 || !(scale > 0.0f) || !std::isfinite(scale)) return MARIAN_HIP_ERR_SHAPE;
   if(q_heads / heads > kMaxHeads || n * (q_heads / heads) > 1 << 26) return MARIAN_HIP_ERR_RANGE;
   if(sequences == 0 || n == 0) return MARIAN_HIP_OK;
-  const CacheAttentionPlan p = cache_attention_plan(sequences, heads, q_heads, n, dk);
+  const CacheAttentionPlan p = cache_attention_plan(sequences, heads, q_heads, cache->capacity, n, dk);
   if(p.grid > kMostThreads / (64 * p.waves)) return MARIAN_HIP_ERR_RANGE;
   MH_CHECK(check_cache_memory(cache));
   MH_CHECK(check_drafts_memory(drafts));

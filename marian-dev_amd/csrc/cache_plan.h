@@ -8,6 +8,7 @@
 namespace marian_hip {
 
 constexpr int kCacheBlock = 128;    // positions that parts are counted in: four waves take as many in one turn
+constexpr unsigned kCacheWhole = 4;        // blocks that are not worth splitting
 constexpr unsigned kCacheMostParts = 48;   // of a sequence: joining them takes as long as what they save
 constexpr int kCacheMost = 8192;    // counters of a workspace: two for each of the workgroups that positions are split for
 
@@ -29,11 +30,11 @@ struct CacheAttentionPlan {
 
 // A part is a whole number of blocks of positions, as many as all sequences have divided by target: then the parts of the
 // sequences that have several are less than 2 * target, whatever the lengths.
-inline CacheAttentionPlan cache_attention_plan(int64_t sequences, int64_t heads, int64_t q_heads, int64_t n, int64_t dk) {
+inline CacheAttentionPlan cache_attention_plan(int64_t sequences, int64_t heads, int64_t q_heads, int64_t capacity, int64_t n, int64_t dk) {
   CacheAttentionPlan p{};
   p.dp = dk <= 64 ? 64 : dk <= 128 ? 128 : 256;
   const int64_t rows = n * (q_heads / heads);
-  p.few = rows > 8 || p.dp == 256 ? 0 : rows > 4 ? 8 : rows > 2 ? 4 : (int)rows;
+  p.few = rows > 8 || p.dp == 256 || sequences * heads * capacity < 400000 ? 0 : rows > 4 ? 8 : rows > 2 ? 4 : (int)rows;
   p.qt = rows <= 16 || p.dp == 256 ? 1 : 2;   // (what the registers hold)
   // More than 32 rows: a workgroup of 128 takes 11 to 15 % less time a row than one of 64, unless the last of several is half empty
   // (300 rows of 16 sequences, 16 heads, 4000 positions of 128 values: 239 us in 64s, 254 us in 128s; 440 rows: 329 and 312)
@@ -50,7 +51,7 @@ inline CacheAttentionPlan cache_attention_plan(int64_t sequences, int64_t heads,
   const int to_a_simd = p.many ? (p.dp == 256 ? 1 : p.qt == 1 ? 3 : 2) : p.few ? (p.dp == 128 ? 2 : p.few <= 2 ? 4 : 3) : p.dp == 64 ? 5 - p.qt : p.dp == 128 ? 4 - p.qt : 2;
   const int64_t at_a_time = 1024 * to_a_simd / p.waves;
   p.target = std::max<int64_t>(1, at_a_time / (heads * p.row_tiles) - sequences / 2);
-  p.least = entries >= at_a_time || !p.few ? 4 : 2;
+  p.least = !p.many && entries <= 32 ? 2 : 4;
   p.items = p.target == 1 ? sequences : p.target + sequences;
   p.slots = p.target == 1 ? 0 : 2 * p.target;
   p.grid = (p.items * heads + 7) / 8 * 8 * p.row_tiles;

@@ -693,3 +693,19 @@ def test_lengths_that_grow_on_one_stream_and_codes_from_elsewhere():
         q, codes, scales = torch.ones(1, 1, 1, 64), torch.full((1, 1, 4, 64), value, dtype=torch.float64), torch.full((1, 1, 4), 0.5)
         got = kv.AttentionOverCache(q.cuda(), cache, ints([3]))
         check(got, *oracle.attention(q, codes, codes, scales, scales, torch.tensor([3]), None, None, 0.125))
+
+
+@pytest.mark.parametrize("S,H,G,cap", [(32, 32, 8, 64), (32, 32, 8, 400), (32, 32, 1, 64), (16, 16, 24, 64), (8, 16, 40, 64), (4, 8, 150, 64)])
+def test_every_weight_of_float32(S, H, G, cap):
+    """Values that are a row of the identity each show the weights one by one: all within what their scores may be off (some 2^-13 here),
+    none short of its second float16 (2^-11 of it)"""
+    kv, r = load("cache"), maker(G + cap)
+    cache = kv.newCache(S, H, cap, 64)
+    k, v = r(S, H, 64, 64), torch.eye(64, device="cuda") * torch.exp(0.3 * r(S, H, 64, 1))   # (scales of their own)
+    kv.appendToCache(cache, k, v, ints([0] * S))
+    q = r(S, H * G, 1, 64)
+    lens = ints([63] * S)
+    small = kv.KeyValueCache(*(t[:, :, :64] for t in cache))
+    want, tol = expected(q, small, lens)
+    assert (tol[want > 1e-3] < want[want > 1e-3] * 2.0 ** -12).all()
+    check(kv.AttentionOverCache(q, cache, lens), want, tol)
