@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <array>
 #include <cmath>
+#include <type_traits>
 #include <utility>
 
 #include "../../include/marian_hip_int8.h"
@@ -100,17 +101,16 @@ struct AppendArgs {
 };
 
 // A row - a head's key, value or query of one token - to LANES lanes, eight values each; a workgroup takes 256 / LANES
-// rows at a time of up to kAppendTokens tokens, whose sines and cosines its threads make first (in 64 bits: keys are
+// rows at a time of up to TOKENS tokens, whose sines and cosines its threads make first (in 64 bits: keys are
 // rounded once to float32 and then quantized, so that a key next to a border of a code falls on its own side).
-constexpr int kAppendTokens = 4;
-template <typename T, CacheFormat F, int LANES>
+template <typename T, CacheFormat F, int LANES, int TOKENS>
 __global__ __launch_bounds__(256) void append_kernel(const T* k, const T* v, const T* q, T* q_out, AppendArgs a) {
   constexpr int kRows = 256 / LANES;
-  __shared__ double2 turn[kAppendTokens][LANES * 4];
+  __shared__ double2 turn[TOKENS][LANES * 4];
   __shared__ int stands[64];   // tokens of a tree: how many they descend from
-  const int tid = threadIdx.x, s = blockIdx.z, first = blockIdx.y * kAppendTokens;
+  const int tid = threadIdx.x, s = blockIdx.z, first = blockIdx.y * TOKENS;
   const int len = clamp_int(a.lens[s], 0, a.cap), count = a.counts ? clamp_int(a.counts[s], 0, a.n) : a.n;
-  const int tokens = min(kAppendTokens, a.n - first), half = a.dims / 2;
+  const int tokens = min(TOKENS, a.n - first), half = a.dims / 2;
   if(a.dims) {
     if(a.parents) {
       if(tid < 64) stands[tid] = __popcll(lineage(a.parents + (long long)s * a.n, a.n, tid)) - 1;
@@ -142,17 +142,18 @@ __global__ __launch_bounds__(256) void append_kernel(const T* k, const T* v, con
     if(!there || a.interleaved || what == 1) other[quad] = e;
   }
   // All tokens are asked for at once.
-  float y[kAppendTokens][8], z[kAppendTokens][2][4];
+  float y[TOKENS][8], z[TOKENS][2][4];
 #pragma unroll
-  for(int t = 0; t < kAppendTokens; ++t) {
+  for(int t = 0; t < TOKENS; ++t) {
     const T* const in = x + min(first + t, a.n - 1) * step;
     load_row<8>(in, y[t]);
 #pragma unroll
     for(int quad = 0; quad < 2; ++quad) load_row<4>(in + other[quad], z[t][quad]);
   }
 #pragma unroll
-  for(int t = 0; t < kAppendTokens; ++t) {
+  for(int t = 0; t < TOKENS; ++t) {
     const int token = first + t, slot = len + token;
+    if(t && token >= a.n) break;
     const bool kept = token < count && (what == 2 || slot < a.cap);
     if(what != 1) {
 #pragma unroll
@@ -520,19 +521,30 @@ int marian_hip_cache_append(const marian_hip_kv_cache* cache, const marian_hip_d
   a.cap = (int)cache->capacity;
   a.dk = (int)dk;
   const int64_t all = 2 * a.heads + a.q_heads;
-  const int64_t tokens = (n + kAppendTokens - 1) / kAppendTokens;
+  // Four tokens to a workgroup, all asked for at once, where a workgroup each would be more than 32 to a CU: 512 tokens of 16 sequences, 48 rows
+  // of 128 values a token, 44.8 us against 52.1 (a prompt's angles and the wait for memory count); below that a workgroup to each: 64
+  // tokens 10.5 us against 12.0, 3 of 64 sequences 4.5 against 6.9.
+  const int lanes = dk <= 64 ? 8 : dk <= 128 ? 16 : 32;
+  const int64_t row_groups = (all * lanes + 255) / 256;
+  const int each = row_groups * n * sequences > 8192 ? 4 : 1;
+  const int64_t tokens = (n + each - 1) / each;
   if(tokens > 65535) return MARIAN_HIP_ERR_RANGE;
   return for_type(type, [&](auto t) -> int {
     using T = decltype(t);
     return for_format(cache->format, [&](auto f) -> int {
       constexpr CacheFormat F = decltype(f)::value;
-      auto grid = [&](int lanes) { return dim3((unsigned)((all * lanes + 255) / 256), (unsigned)tokens, (unsigned)sequences); };
       const T *kp = static_cast<const T*>(k), *vp = static_cast<const T*>(v), *qp = static_cast<const T*>(q);
       T* qop = static_cast<T*>(q_out);
-      if(dk <= 64) MH_LAUNCH((append_kernel<T, F, 8>), grid(8), dim3(256), 0, st, kp, vp, qp, qop, a);
-      else if(dk <= 128) MH_LAUNCH((append_kernel<T, F, 16>), grid(16), dim3(256), 0, st, kp, vp, qp, qop, a);
-      else MH_LAUNCH((append_kernel<T, F, 32>), grid(32), dim3(256), 0, st, kp, vp, qp, qop, a);
-      return MARIAN_HIP_OK;
+      const dim3 grid((unsigned)row_groups, (unsigned)tokens, (unsigned)sequences);
+      auto launch = [&](auto given) -> int {
+        constexpr int LANES = decltype(given)::value;
+        if(each == 1) MH_LAUNCH((append_kernel<T, F, LANES, 1>), grid, dim3(256), 0, st, kp, vp, qp, qop, a);
+        else MH_LAUNCH((append_kernel<T, F, LANES, 4>), grid, dim3(256), 0, st, kp, vp, qp, qop, a);
+        return MARIAN_HIP_OK;
+      };
+      if(lanes == 8) return launch(std::integral_constant<int, 8>());
+      if(lanes == 16) return launch(std::integral_constant<int, 16>());
+      return launch(std::integral_constant<int, 32>());
     });
   });
 }

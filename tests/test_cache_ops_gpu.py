@@ -709,3 +709,20 @@ def test_every_weight_of_float32(S, H, G, cap):
     want, tol = expected(q, small, lens)
     assert (tol[want > 1e-3] < want[want > 1e-3] * 2.0 ** -12).all()
     check(kv.AttentionOverCache(q, cache, lens), want, tol)
+
+
+@pytest.mark.parametrize("S,H,G,n,dk", [(3, 2, 2, 1500, 64), (1, 8, 4, 1001, 128), (40, 4, 1, 67, 256), (70, 16, 1, 63, 64)])
+def test_append_of_many_tokens(S, H, G, n, dk):
+    """Alike whether a workgroup takes four tokens or one: all at once, and in pieces"""
+    kv, r = load("cache"), maker(n)
+    rotary = kv.makeRotary(dk, base=50000.0)
+    whole, pieces = kv.newCache(S, H, n + 9, dk, "e4m3"), kv.newCache(S, H, n + 9, dk, "e4m3")
+    k, v, q = side_by_side(r, S, H, n, dk, BF16), side_by_side(r, S, H, n, dk, BF16), side_by_side(r, S, H * G, n, dk, BF16)
+    lens = [s % 7 for s in range(S)]
+    counts = [n - (s * 5) % 11 for s in range(S)]
+    turned = kv.appendToCache(whole, k, v, ints(lens), None, ints(counts), rotary, q)
+    for i in range(0, n, 16):
+        m = min(16, n - i)
+        part = kv.appendToCache(pieces, k[:, :, i:i + m], v[:, :, i:i + m], ints([x + i for x in lens]), None, ints([c - i for c in counts]), rotary, q[:, :, i:i + m])
+        assert same(part, turned[:, :, i:i + m])
+    assert all(same(a, b) for a, b in zip(whole, pieces))
