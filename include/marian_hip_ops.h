@@ -412,11 +412,11 @@ int marian_hip_cache_read(const marian_hip_kv_cache* cache, const int32_t* first
  * and all before it past the capacity) gives zeros, and so do rows at or past counts[s].  out shares no memory with q
  * or the cache.  scale: finite, above zero.
  * Products and sums are float32.  Of float16 and bfloat16 queries, weights enter the product with the values in
- * 11 bits, of float32 ones in 22, relative to the largest weight times scale of value of a tile; the sum of the weights is exact.
+ * 11 bits, of float32 ones in 22, each of its own size down to 2^-24 of the largest; the sum is of the weights in float32.
  * A sequence's positions are split over workgroups where there are few of them, by the lengths of all
  * sequences: the last bits of a result depend on the batch it is in, and not on the order of anything.
- *   workspace: at least marian_hip_cache_attention_workspace_bytes(...) bytes, 256-byte aligned (0 bytes: may be
- *   null), which marian_hip_cache_attention_workspace_init clears once after allocating (a kernel: it may be
+ *   workspace: at least marian_hip_cache_attention_workspace_bytes(...) bytes (enough for any capacity and type; 0 too where
+ *   sizes are out of range), 256-byte aligned (0 bytes: may be null), which marian_hip_cache_attention_workspace_init clears once after allocating (a kernel: it may be
  *   recorded).  One workspace serves one stream, like that of marian_hip_nbest_beams.
  */
 size_t marian_hip_cache_attention_workspace_bytes(int64_t sequences, int64_t heads, int64_t q_heads, int64_t n, int64_t dk);

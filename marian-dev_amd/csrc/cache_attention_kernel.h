@@ -8,23 +8,30 @@
 //
 // What has to move is dk bytes and a scale of each position's key and value, 2 * (dk + 4) bytes; the products are
 // 4 * dk operations a row and position.  Up to some sixty rows an entry the bytes are the bound, beyond it the matrix
-// instructions.
+// instructions.  (The card copies 5.1 TB/s and multiplies large float16 matrices at 1.3 PFLOP/s.)
 //
-// Layout: a wave takes 32 positions at a time and 16 * QT rows, all in registers.
-//   S^T = K Q^T (16x16x32): lane (c = lane % 16, g = lane / 16) loads sixteen codes at a time of key c - whole 64-byte
-//   pieces of a row between four lanes - and uses them as two operands; which codes a step of the product takes is the same
-//   for Q, so no code moves between lanes.  The result has row c's scores of keys 4 g .. 4 g + 3, for two blocks of 16 keys.
-//   O^T = V^T P^T: those eight weights of a lane are its operand as they are, if V's operand has the keys in that
-//   order: lane (c, g) loads DP / 16 codes at c * DP / 16 of each of these eight keys - a row of keys between
-//   sixteen lanes - and picks a dimension's eight codes out of its registers, two at a time, while they become float16.
-//   So neither keys, values nor weights go through LDS.
+// Three forms, all with S^T = K Q^T or its transpose and O^T = V^T P^T on 16x16x32 float16 products, a row's maximum, sum and
+// values in float32 registers, and the next positions' loads under way during the products of the last:
+//   cache_attention_kernel: 9 to 32 rows an entry, rows of more than 128 values, and fewer rows over short contexts.  A wave takes 32 positions at
+//   a time and 16 * QT rows, all in registers.
+//     S^T: lane (c = lane % 16, g = lane / 16) loads sixteen codes at a time of key c - whole 64-byte pieces of a row between four lanes
+//     - and uses them as two operands; which codes a step of the product takes is the same for Q, so no code moves between lanes.
+//     The result has row c's scores of keys 4 g .. 4 g + 3, for two blocks of 16 keys.
+//     O^T: those eight weights of a lane are its operand as they are, if V's operand has the keys in that order: lane (c, g) loads DP / 16
+//     codes at c * DP / 16 of each of these eight keys - a row of keys between sixteen lanes - and picks a dimension's eight
+//     codes out of its registers, two at a time, while they become float16.
+//     So neither keys, values nor weights go through LDS; only the scales do.
+//     16 sequences, 4 drafted tokens, 32 heads on 8, 4000 positions of 128 values at most: 32.1 us, 2.8 TB/s.
+//   cache_attention_few_kernel: up to 8 rows over long contexts, cache_attention_many_kernel: more than 32 rows; see there.
 // Codes are exact in float16.  Q is scaled row by row by a power of two up to 2^14 .. 2^15 and enters in one float16
 // (float16 and bfloat16: exact but for values 2^-29 below the row's largest) or two (float32: 22 bits).  A weight is
 // p_rj times the value's scale over a running scale S_r (as the maximum runs), times 2^9: in one float16 or two, rounded
 // to nearest, of what is at most 2^15 and, with normal numbers, down to 2^-14: 11 (22) bits of weights up to 2^-24 below the
-// largest.  Their sum is of the weights in float32.
-// Positions that a row does not see, and rows past the end that pad a block, weigh a selected zero; loads past the end go to the
-// last position in reach, whose codes are finite whatever they hold.
+// largest.  Their sum is of the weights in float32.  (float16 outputs are rounded to 11 bits themselves: the weights' rounding adds
+// 40 % to the error of the result at most, and a second float16 would double the instructions of the larger product.)
+// The sums are scaled down only where a maximum or scale outgrows the carried one by 2^4 (4): most turns skip it.
+// Positions that a row does not see, and rows past the end that pad a block, weigh a selected zero; loads go through buffers that end where
+// the part does, and give zeros behind it.
 #pragma once
 
 #include <type_traits>
@@ -588,6 +595,8 @@ __device__ __forceinline__ void cache_finish(const CacheAttentionArgs& a, const 
 }
 
 // ---- sixteen rows and more to a wave
+// Between two barriers of LDS there is nothing to wait for but memory; the loads of the next 32 positions are out while these are worked on.
+// The workgroup's waves take turns of 32 positions of the same rows and join in LDS in the end, so a short context is one turn.
 template <typename T, CacheFormat F, int DP, int QT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT : 2)) void cache_attention_kernel(CacheAttentionArgs a) {
   using A = CacheAttention<T, F, DP>;
@@ -794,6 +803,9 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
 // score is in one lane only.  A key's scales are a value to a lane, whole lines of memory.  The weights go
 // through LDS, a row of 64 a query, to where they are an operand: lane (c, g) takes eight of row c, those of positions
 // 4 e + g of 32, so that four rows of values that follow each other in memory are loaded at a time.
+// Memory bounds it: 16 sequences, 32 heads on 8, up to 32768 positions of 128 values in e4m3 157 us, 5.5 TB/s (the form above 163), 64 of up to
+// 4096 in int8 73.5 us, 5.0 TB/s (84.7); 128 sequences, 16 heads, up to 512 of 64 values, float32, 22.4 us, 4.2 TB/s (24.7).
+// Its start costs more, so short contexts are left to the form above.
 template <typename T, CacheFormat F, int DP, int ROWS>
 struct CacheFew {
   using A = CacheAttention<T, F, DP>;
@@ -1011,7 +1023,12 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
 // 16 * QT rows to a wave, whose waves share 64 positions at a time: these are loaded once, turned into float16 and laid into LDS as the
 // operands that every wave then reads, piece after piece of 64 lanes.  Wave w turns the keys of block w of sixteen, and of
 // half w / 2 of the positions half the dimensions of the values; the next codes are on their way meanwhile.  The products are those
-// of the first form, but for the dimensions, lane (c, g) having 64 i + 16 g + 4 e + j.
+// of the first form, but for the dimensions, lane (c, g) having 64 i + 16 g + 4 e + j.  While a wave lays positions out it goes ahead of those in
+// products (the others wait for it): 81.3 us against 84.8 (the trees below).  A second buffer in LDS, with one barrier a turn, gained nothing.
+// The matrix instructions and the exponentials between them bound it: 4 sequences, 1024 tokens, 32 heads on 8, 4096 positions of 128 values,
+// bfloat16, 327 us, 857 TFLOP/s; 8 trees of 64 tokens, 32 heads on 4, up to 8192 positions 81 us, 590 TFLOP/s (57 us at
+// the rate of the first; the rest goes to parts of unequal length, and to results on their way through memory to the workgroup that joins them).  The first form: 8 sequences of 16 tokens, 32 heads on 8, 8192 positions
+// 47.3 us, this one 45.2; 64 sequences of 50 rows, 16 heads, 36.7 and 26.3.
 template <typename T, CacheFormat F, int DP, int QT>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void cache_attention_many_kernel(CacheAttentionArgs a) {
   using A = CacheAttention<T, F, DP>;

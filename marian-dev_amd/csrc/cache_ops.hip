@@ -33,6 +33,8 @@ __device__ __forceinline__ float half_turns(long long position, unsigned long lo
 
 // A thread turns one unit - four pairs, or eight values behind the turned ones - of up to HEADS heads of a position: the
 // angles are the same for all of them.  Units of a row are side by side, then heads, then positions.
+// out = x turned, in float32 with the angle's fraction of a turn exact: the error does not grow with the position.  Memory bounds it: 4 sequences of 4093
+// positions, 32 heads of 128 values, bfloat16, 54 us, 5.0 TB/s (a copy: 5.1); a single token's 2.3 us are a launch's.
 template <typename T, int HEADS>
 __global__ __launch_bounds__(256) void rotary_kernel(const T* x, Strides xs, T* out, Strides os, const int* __restrict__ positions, int each,
                                                      const unsigned long long* __restrict__ turns, int dims, float magnitude, int interleaved,
@@ -103,6 +105,11 @@ struct AppendArgs {
 // A row - a head's key, value or query of one token - to LANES lanes, eight values each; a workgroup takes 256 / LANES
 // rows at a time of up to TOKENS tokens, whose sines and cosines its threads make first (in 64 bits: keys are
 // rounded once to float32 and then quantized, so that a key next to a border of a code falls on its own side).
+//   scale = largest magnitude of the row / 127 (448), code = value / scale rounded to the nearest, ties to even.
+// A row's lanes are side by side, its largest value a few exchanges away; a value and the one it is turned with are both loaded, the second
+// from a cache, in place of an exchange.  3 sequences of 2731 tokens, 32 + 8 + 8 heads of 128 values, float16 to e4m3: 52 us,
+// 3.5 TB/s, where a copy of these bytes takes 36: the rest is the 64-bit turns (48 us with them in 32 bits, which would move codes at
+// borders) and the quotients.  128 sequences' single tokens, 48 heads of 64 values, float32: 4.0 us one after the other, most of it a launch's.
 template <typename T, CacheFormat F, int LANES, int TOKENS>
 __global__ __launch_bounds__(256) void append_kernel(const T* k, const T* v, const T* q, T* q_out, AppendArgs a) {
   constexpr int kRows = 256 / LANES;
@@ -209,7 +216,8 @@ __global__ __launch_bounds__(256) void append_kernel(const T* k, const T* v, con
 
 // ---------------------------------------------------------------- reading back
 // A thread takes sixteen bytes of output at a time - four float32, eight of the shorter types -, kReadTurns of them
-// a workgroup's stride apart, of keys and values alike.
+// a workgroup's stride apart, of keys and values alike: all loads are out before the first is used.  Memory bounds it: 8 sequences, 8 heads,
+// 4001 positions of 128 values, e4m3 to bfloat16, 35.6 us, 5.5 TB/s; 33 positions of 6 sequences 2.9 us.
 constexpr int kReadTurns = 4;
 template <typename T, CacheFormat F>
 __global__ __launch_bounds__(256) void cache_read_kernel(const unsigned char* __restrict__ k, const unsigned char* __restrict__ v,
@@ -266,7 +274,8 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const unsigned char* __
 }
 
 // ---------------------------------------------------------------- accepted drafts
-// A workgroup to the keys or the values of an entry: everything is read before anything is written.
+// A workgroup to the keys or the values of an entry: everything is read before anything is written, so a path may go anywhere, twice to
+// the same row too.  64 sequences, 16 heads, 64 rows of 128 codes: 6.1 us, 5.5 TB/s; 16 rows of one sequence 2.9 us, a launch's.
 __global__ __launch_bounds__(256) void cache_keep_kernel(unsigned char* k, unsigned char* v, float* ks, float* vs, const int* __restrict__ lens,
                                                          const int* __restrict__ path, int path_len, const int* __restrict__ accepted,
                                                          int* __restrict__ new_lens, int heads, int cap, int dk) {
