@@ -21,7 +21,7 @@
 //     codes at c * DP / 16 of each of these eight keys - a row of keys between sixteen lanes - and picks a dimension's eight
 //     codes out of its registers, two at a time, while they become float16.
 //     So neither keys, values nor weights go through LDS; only the scales do.
-//     16 sequences, 4 drafted tokens, 32 heads on 8, 4000 positions of 128 values at most: 32.1 us, 2.8 TB/s.
+//     16 sequences, 4 drafted tokens, 32 heads on 8, 4000 positions of 128 values at most: 29.9 us, 3.0 TB/s.
 //   cache_attention_few_kernel: up to 8 rows over long contexts, cache_attention_many_kernel: more than 32 rows; see there.
 // Codes are exact in float16.  Q is scaled row by row by a power of two up to 2^14 .. 2^15 and enters in one float16
 // (float16 and bfloat16: exact but for values 2^-29 below the row's largest) or two (float32: 22 bits).  A weight is
@@ -361,7 +361,7 @@ __device__ __forceinline__ float cache_query(const CacheAttentionArgs& a, const 
 // Where a workgroup's rows go: to the output, or where a sequence has several parts to the workspace.
 template <typename T, int DP, int ROWS>
 struct CacheOut {
-  static constexpr int kTileFloats = ROWS * (DP + 1);
+  static constexpr int kTileFloats = ROWS * DP + (ROWS + 3) / 4 * 4;   // (whole pieces of 16 bytes)
   const CacheAttentionArgs& a;
   const CacheTile& x;
   const bool whole;
@@ -423,35 +423,32 @@ __device__ __forceinline__ void cache_join_parts(const CacheAttentionArgs& a, co
   const int tid = threadIdx.x;
   if(!cache_arrived_last(a.counters + out.place, x.w.parts, sh.is_last)) return;
   // Sixteen threads to a row; where there are fewer rows than sixteens, several of them share a row's parts.  A batch of parts is
-  // asked for at a time: the loads come from the memory side, about a microsecond away.
-  const float* const all = a.part + out.place * Out::kTileFloats;
-  const long long stride = out.stride * Out::kTileFloats;
-  constexpr int kGroups = 4 * WAVES, kBatch = DP == 256 ? 4 : 8;
+  // asked for at a time, through a buffer that ends behind the last one: the loads come from the memory side, about a microsecond away, and
+  // a branch around each would wait for it (2 sequences, 2 heads, 16 rows of 256 values, up to 56618 positions
+  // in 48 parts: 51 us, 75 with branches).
+  const unsigned stride = (unsigned)(out.stride * Out::kTileFloats), all_parts = x.w.parts;
+  const CacheBuffer from(a.part + out.place * Out::kTileFloats, 4u * stride * all_parts);
+  constexpr int kGroups = 4 * WAVES, kBatch = 8;
   const int here = min(ROWS, x.rows - x.row0), group = tid >> 4, d_mine = (tid & 15) * kDims;
   int share = 1;
   while(share * here * 2 <= kGroups) share *= 2;
 #pragma unroll 1
   for(int r = group / share; r < here; r += kGroups / share) {   // (one turn where parts are shared)
-    const float* logs = all + ROWS * DP + r;
-    const float* from = all + r * DP + (d_mine < a.dk ? d_mine : 0);
+    const unsigned mine = 4u * (r * DP + (d_mine < a.dk ? d_mine : 0)), my_log = 4u * (ROWS * DP + r);
     float m = kNone, total = 0.0f, y[kDims] = {};
 #pragma unroll 1
     for(int i = group % share; i < x.w.parts; i += kBatch * share) {
       float l[kBatch];
-      unsigned long long z[kBatch][kDims / 2];
+      cache_f4 z[kBatch][kDims / 4];
 #pragma unroll
       for(int b = 0; b < kBatch; ++b) {
-        l[b] = kNone;
+        const unsigned at = 4u * stride * (unsigned)(i + b * share);
+        l[b] = from.number_through(at + my_log);
 #pragma unroll
-        for(int j = 0; j < kDims / 2; ++j) z[b][j] = 0;
-        if(i + b * share < x.w.parts) {
-          const long long at = (i + b * share) * stride;
-          l[b] = __hip_atomic_load(logs + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-          for(int j = 0; j < kDims / 2; ++j)
-            z[b][j] = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(from + at) + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
+        for(int j = 0; j < kDims / 4; ++j) z[b][j] = from.piece_through(at + mine + 16u * j);
       }
+#pragma unroll
+      for(int b = 0; b < kBatch; ++b) l[b] = i + b * share < x.w.parts ? l[b] : kNone;
       float next = m;
 #pragma unroll
       for(int b = 0; b < kBatch; ++b) next = fmaxf(next, l[b]);
@@ -465,7 +462,7 @@ __device__ __forceinline__ void cache_join_parts(const CacheAttentionArgs& a, co
         const float weight = l[b] == kNone ? 0.0f : __builtin_amdgcn_exp2f(l[b] - m);
         total += weight;
 #pragma unroll
-        for(int j = 0; j < kDims; ++j) y[j] = __builtin_fmaf(weight, __builtin_bit_cast(float, (unsigned)(z[b][j / 2] >> (32 * (j % 2)))), y[j]);
+        for(int j = 0; j < kDims; ++j) y[j] = __builtin_fmaf(weight, z[b][j / 4][j % 4], y[j]);
       }
     }
     if(share > 1) {   // (r is the only row of all threads: sixteens beyond the rows have left)
