@@ -9,10 +9,14 @@ laid out in whole rows of 16-byte pieces are copied first.  lens, counts, parent
 is converted) and read there: a step needs no synchronisation, and may be recorded into a graph.  There is no CPU fallback.
 
 One step of a decoder with drafted tokens:
-    q = appendToCache(cache, k, v, lens, parents, rotary=rotary, q=q)      # for every layer
-    o = AttentionOverCache(q, cache, lens, parents)
-    ..
-    lens = keepDrafts(cache, lens, path, accepted)                         # for every layer, when the drafts are judged
+    for layer, cache in zip(layers, caches):
+        q, k, v = layer.project(x)
+        q = appendToCache(cache, k, v, lens, parents, rotary=rotary, q=q)
+        x = layer.finish(AttentionOverCache(q, cache, lens, parents))
+    path, accepted = judge(x)
+    for cache in caches:   # (each of them from the lengths that its drafts were written behind)
+        newLens = keepDrafts(cache, lens, path, accepted)
+    lens = newLens
 For one token, or a prompt, parents is None and lens + n the next step's.  The caches of the surviving hypotheses of
 a beam are gathered like any decoder state: ops.selectState on the tensors' float32 views.
 """
@@ -210,7 +214,7 @@ def AttentionOverCache(q, cache, lens, parents=None, counts=None, scale=None, ou
 
 def keepDrafts(cache, lens, path, accepted):
     """The accepted drafted tokens become settled: for j < accepted[s], token path[s, j] (path [sequences, up to 64]) moves to
-    row lens[s] + j.  Returns the new lens."""
+    row lens[s] + j.  Returns the new lens; lens itself stays, for the other layers' caches."""
     res = _host.cache_keep(cache, lens, path, accepted)
     if res is not None:
         return res
