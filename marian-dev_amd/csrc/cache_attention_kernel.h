@@ -414,6 +414,11 @@ struct CacheParts {
   int is_last;
 };
 
+// A part's weight is at most 1, times this: the sum of their weighted values is no larger than the largest of them, which may be next to the
+// largest float32.  (A power of two, which the reciprocal of the weights' sum takes away again: no bit of a result depends on it.)
+constexpr float kPartUnit = 1.0f / 64;
+static_assert(kPartUnit * kCacheMostParts <= 1.0f, "the parts' weights add up to one at the most");
+
 // The parts of a sequence: the workgroup that arrives last joins them, in their order.
 template <typename T, int DP, int ROWS, int WAVES>
 __device__ __forceinline__ void cache_join_parts(const CacheAttentionArgs& a, const CacheTile& x, const CacheOut<T, DP, ROWS>& out,
@@ -459,7 +464,7 @@ __device__ __forceinline__ void cache_join_parts(const CacheAttentionArgs& a, co
       for(int j = 0; j < kDims; ++j) y[j] *= down;
 #pragma unroll
       for(int b = 0; b < kBatch; ++b) {
-        const float weight = l[b] == kNone ? 0.0f : __builtin_amdgcn_exp2f(l[b] - m);
+        const float weight = l[b] == kNone ? 0.0f : __builtin_amdgcn_exp2f(l[b] - m) * kPartUnit;
         total += weight;
 #pragma unroll
         for(int j = 0; j < kDims; ++j) y[j] = __builtin_fmaf(weight, z[b][j / 4][j % 4], y[j]);
@@ -543,13 +548,18 @@ __device__ __forceinline__ void cache_finish(const CacheAttentionArgs& a, const 
       if(g == 0) out.emit_log(16 * t + c, top[t], sum[t]);
     }
   } else {
+    // A row's weights of N positions add up to 2^kMaximumSlack N at the most, and their values to that many times the largest, which may be next
+    // to the largest float32: they are summed over a power of two above it, twice as large for the roundings.  (It changes no bit of a result.)
+    const int up = 5 + 32 - __builtin_clz((unsigned)max(x.end - x.w.from, 1));
+    const float over = __builtin_bit_cast(float, (unsigned)(127 - up) << 23), back = __builtin_bit_cast(float, (unsigned)(127 + up) << 23);
+    static_assert(kMaximumSlack <= 4.0f, "up counts it");
     __syncthreads();
 #pragma unroll
     for(int t = 0; t < QT; ++t) {
       float m = sh.row_max[0][16 * t + c];
 #pragma unroll
       for(int i = 1; i < WAVES; ++i) m = fmaxf(m, sh.row_max[i][16 * t + c]);
-      const float mine = top[t] == kNone ? 0.0f : __builtin_amdgcn_exp2f(top[t] - m) * (unit[t] * kUnit);
+      const float mine = top[t] == kNone ? 0.0f : __builtin_amdgcn_exp2f(top[t] - m) * (unit[t] * kUnit) * over;
 #pragma unroll
       for(int h = 0; h < DP / kHalf; ++h) {
         if(h || t) __syncthreads();
@@ -574,7 +584,7 @@ __device__ __forceinline__ void cache_finish(const CacheAttentionArgs& a, const 
             const float from = sh.row_max[i][16 * t + r];   // (of a wave that saw nothing the sum is 0, or NaN)
             total += sh.row_sum[i][16 * t + r] * (from == kNone ? 1.0f : __builtin_amdgcn_exp2f(from - top_r));
           }
-          const float per = total == 0.0f ? 0.0f : 1.0f / total;
+          const float per = total == 0.0f ? 0.0f : 1.0f / total * back;
 #pragma unroll
           for(int j = 0; j < kEach; ++j) {
             y[j] = sh.joined[0][r][d + j];
@@ -1305,7 +1315,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void cache_attention_many_k
 #pragma unroll
       for(int t = 0; t < QT; ++t) {
         const float m = fmaxf(most[t], l[t]), down = most[t] == kNone ? 0.0f : __builtin_amdgcn_exp2f(most[t] - m);
-        const float weight = l[t] == kNone ? 0.0f : __builtin_amdgcn_exp2f(l[t] - m);
+        const float weight = l[t] == kNone ? 0.0f : __builtin_amdgcn_exp2f(l[t] - m) * kPartUnit;
         most[t] = m;
         total[t] = total[t] * down + weight;
 #pragma unroll
