@@ -307,6 +307,7 @@ int marian_hip_fill(void* begin, int64_t count, int elem_bytes, uint64_t pattern
  * has scale 0.  A row that holds an infinity or NaN has zeros for codes and a NaN scale: everything that reads it
  * is NaN, and nothing that does not read it.
  * Codes that come from elsewhere are taken by their bits: int8 -128 is -128, and e4m3's NaN (0x7f, 0xff) is 480 (-480).
+ * Scales that come from elsewhere may be below zero.
  *   heads <= 4096, sequences <= 65535, capacity * dk < 2^31; k and v 16-byte, scales 4-byte aligned.
  */
 #define MARIAN_HIP_CACHE_INT8 0

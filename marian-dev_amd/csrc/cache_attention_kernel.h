@@ -25,10 +25,11 @@
 //   cache_attention_few_kernel: up to 8 rows over long contexts, cache_attention_many_kernel: more than 32 rows; see there.
 // Codes are exact in float16.  Q is scaled row by row by a power of two up to 2^14 .. 2^15 and enters in one float16
 // (float16 and bfloat16: exact but for values 2^-29 below the row's largest) or two (float32: 22 bits).  A weight is
-// p_rj times the value's scale over a running scale S_r (as the maximum runs), times 2^9: in one float16 or two, rounded
-// to nearest, of what is at most 2^15 and, with normal numbers, down to 2^-14: 11 (22) bits of weights up to 2^-24 below the
-// largest.  Their sum is of the weights in float32.  (float16 outputs are rounded to 11 bits themselves: the weights' rounding adds
-// 40 % to the error of the result at most, and a second float16 would double the instructions of the larger product.)
+// p_rj times the value's scale over a running scale S_r (as the maximum runs; of magnitudes, since a scale may be below zero), times
+// 2^9: in one float16 or two, rounded to nearest, of what is at most 2^15 and, with normal numbers, down to 2^-14: 11 (22) bits
+// of weights up to 2^-24 below the largest.  Their sum is of the weights in float32.  (float16 outputs are rounded to 11 bits
+// themselves: the weights' rounding adds 40 % to the error of the result at most, and a second float16 would double the
+// instructions of the larger product.)
 // The sums are scaled down only where a maximum or scale outgrows the carried one by 2^4 (4): most turns skip it.
 // Positions that a row does not see, and rows past the end that pad a block, weigh a selected zero; loads go through buffers that end where
 // the part does, and give zeros behind it.
@@ -720,7 +721,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
       }
     } else {
 #pragma unroll
-      for(int e = 0; e < 8; ++e) widest = fmaxf(widest, vs[e / 4][e % 4]);
+      for(int e = 0; e < 8; ++e) widest = fmaxf(widest, __builtin_fabsf(vs[e / 4][e % 4]));
     }
     float high[QT], wide[QT];
     bool grown = false;
@@ -736,7 +737,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
 #pragma unroll
       for(int t = 0; t < QT; ++t)
 #pragma unroll
-        for(int e = 0; e < 8; ++e) wide[t] = fmaxf(wide[t], seen_here[t] >> e & 1 ? vs[e / 4][e % 4] : 0.0f);
+        for(int e = 0; e < 8; ++e) wide[t] = fmaxf(wide[t], seen_here[t] >> e & 1 ? __builtin_fabsf(vs[e / 4][e % 4]) : 0.0f);
     }
 #pragma unroll
     for(int t = 0; t < QT; ++t) grown |= high[t] > top[t] + kMaximumSlack || wide[t] > unit[t] * kScaleSlack;
@@ -960,7 +961,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
 #pragma unroll
     for(int t = 0; t < kRegs; ++t) {
       high[t] = (kKeys == 1 ? s[0][t] : fmaxf(s[0][t], s[kKeys - 1][t])) * row_scale[t];
-      wide[t] = kKeys == 1 ? scale[0][t] : fmaxf(scale[0][t], scale[kKeys - 1][t]);
+      wide[t] = kKeys == 1 ? __builtin_fabsf(scale[0][t]) : fmaxf(__builtin_fabsf(scale[0][t]), __builtin_fabsf(scale[kKeys - 1][t]));
       grown |= high[t] > top[t] + kMaximumSlack || wide[t] > unit[t] * kScaleSlack;
     }
     if(__any(grown)) {
@@ -1190,7 +1191,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void cache_attention_many_k
       }
     } else {
 #pragma unroll
-      for(int e = 0; e < 8; ++e) widest = fmaxf(widest, vs[e / 4][e % 4]);
+      for(int e = 0; e < 8; ++e) widest = fmaxf(widest, __builtin_fabsf(vs[e / 4][e % 4]));
     }
     float high[QT], wide[QT];
     bool grown = false;
@@ -1201,7 +1202,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void cache_attention_many_k
 #pragma unroll
       for(int e = 0; e < 8; ++e) {
         high[t] = fmaxf(high[t], s[t][e / 4][e % 4]);
-        if constexpr(MASKED) wide[t] = fmaxf(wide[t], seen_here[t] >> e & 1 ? vs[e / 4][e % 4] : 0.0f);
+        if constexpr(MASKED) wide[t] = fmaxf(wide[t], seen_here[t] >> e & 1 ? __builtin_fabsf(vs[e / 4][e % 4]) : 0.0f);
       }
       high[t] *= row_scale[t];
       grown |= high[t] > top[t] + kMaximumSlack || wide[t] > unit[t] * kScaleSlack;

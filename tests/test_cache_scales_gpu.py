@@ -35,3 +35,21 @@ def test_values_next_to_the_largest(S, H, G, n, dk, cap, format, dtype):
     got = kv.AttentionOverCache(q, cache, lens)
     assert bool(torch.isfinite(got).all())
     check(got, *forms.attention(q, cache, lens))
+
+
+@pytest.mark.parametrize("format", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("S,H,G,n,dk,cap", SHAPES)
+def test_scales_below_zero(S, H, G, n, dk, cap, format, dtype):
+    """A value is code * scale whatever the scale's sign, to attention as to reading back"""
+    kv = load("cache")
+    cache, q, lens = batch(S, H, G, n, dk, cap, format, dtype)
+    for flips in (lambda: torch.ones(S, H, cap, device="cuda") * -1, lambda: torch.sign(torch.arange(cap, device="cuda") % 7 - 3.5).expand(S, H, cap)):
+        cache.vScale.mul_(flips())
+        cache.kScale.mul_(flips())
+        check(kv.AttentionOverCache(q, cache, lens), *forms.attention(q, cache, lens))
+        k, v = kv.readCache(cache, lens, n)
+        at = lens.long()[:, None, None, None] + torch.arange(n, device="cuda")[None, None, :, None]
+        for got, codes, scales in ((k, cache.k, cache.kScale), (v, cache.v, cache.vScale)):
+            at4 = at.expand(S, H, n, dk)
+            assert same(got, codes.float().gather(2, at4) * scales.gather(2, at4[..., 0])[..., None])
