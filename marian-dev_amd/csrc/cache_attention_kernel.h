@@ -506,10 +506,11 @@ __device__ __forceinline__ void cache_join_parts(const CacheAttentionArgs& a, co
   store_row<kDims, T>(cache_row_out<T>(a, x, x.row0 + r) + d_mine, y);
 }
 
-// What the waves of a workgroup join their results through.
+// What the waves of a workgroup join their results through.  (Rows are written in pieces of 16 bytes.)
 template <int DP, int QT, int WAVES>
-struct CacheJoin {
+struct alignas(16) CacheJoin {
   static constexpr int kHalf = DP < 128 ? DP : 128;   // dimensions that are joined at a time
+  static_assert((kHalf + 4) % 4 == 0, "whole pieces to a row");
   union {
     float joined[WAVES][16][kHalf + 4];
     CacheParts<DP, WAVES> parts;
@@ -832,6 +833,14 @@ struct CacheFew {
   };
   // The position, of 64, whose scores lane (c, g) has.
   static __device__ __forceinline__ int key_of(int i, int lane) { return kKeys == 1 ? lane : 32 * i + 16 * (lane >> 5) + (lane & 15); }
+  static_assert(kStride % 8 == 0, "weights are read in pieces of 16 bytes");
+};
+
+// Weights until the last turn, then what the waves join through.
+template <typename T, CacheFormat F, int DP, int ROWS, int WAVES>
+union CacheFewShared {
+  CacheJoin<DP, 1, WAVES> join;
+  alignas(16) typename CacheFew<T, F, DP, ROWS>::Weights weights[WAVES];
 };
 
 template <typename T, CacheFormat F, int DP, int ROWS, int WAVES>
@@ -840,10 +849,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
   using B = CacheFew<T, F, DP, ROWS>;
   constexpr int kTerms = A::kTerms, kSteps = A::kSteps, kDims = A::kDims, kRegs = B::kRegs, kKeys = B::kKeys;
   constexpr int kTurn = 64 * WAVES;   // positions that the waves take in one turn
-  __shared__ union {
-    CacheJoin<DP, 1, WAVES> join;
-    typename B::Weights weights[WAVES];
-  } sh;
+  __shared__ CacheFewShared<T, F, DP, ROWS, WAVES> sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   CacheTile x;
