@@ -149,12 +149,12 @@ inline void call(const char* where, F f, const char** which = nullptr, std::mute
   }
 }
 
-// ---- what stays with a stream: workspaces, for good (a graph may have recorded one), and scratch ---------
+// ---- what stays with a stream: workspaces, for good (a graph may have recorded one) but for `cache`, and scratch ---------
 struct PerStream {
   at::Tensor workspace;              // abs-max partials, one-pass exchange
   std::mutex turn;                   // held while a call makes its launches over the workspace
   std::vector<at::Tensor> nbest;     // the last one the largest
-  at::Tensor cache;                  // of the attention over a quantized cache (recorded calls have their own)
+  at::Tensor cache;                  // of the attention over a quantized cache (recorded calls have their own), until release_scratch
   at::Tensor scratch;                // of the calls, not lent at the moment
 };
 std::map<std::pair<int, hipStream_t>, PerStream> per_stream;   // (looked up with the interpreter lock held)
@@ -1441,7 +1441,7 @@ PyObject* py_cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // The workspace of an attention over a quantized cache: a stream's own, kept until a call needs a larger one (then with room to spare, and
-// the old one goes back to the stream that it was used on), or of a call that is recorded its own, cleared by the graph ahead of it
+// the old one goes back to the stream that it was used on) or until release_scratch, or of a call that is recorded its own, cleared by the graph ahead of it
 // (the graph may be replayed on another stream, and beside another graph).
 at::Tensor cache_workspace(int64_t need, c10::Device d, hipStream_t st) {
   const bool once = marian_hip::recorded(st);
@@ -1518,10 +1518,11 @@ PyObject* py_workspace(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   MH_END
 }
 
-// release_scratch(): the scratch of all streams goes back to torch's allocator
+// release_scratch(): the scratch of all streams goes back to torch's allocator, and so do the workspaces of the attention over a quantized
+// cache (no graph has recorded one, a call under way holds its own)
 PyObject* py_release_scratch(PyObject*, PyObject* const*, Py_ssize_t nargs) {
   MH_TRY MH_ARGS(0, "release_scratch");
-  for(auto& p : per_stream) p.second.scratch = at::Tensor();
+  for(auto& p : per_stream) p.second.scratch = p.second.cache = at::Tensor();
   scratch_kept = 0;
   Py_RETURN_NONE;
   MH_END

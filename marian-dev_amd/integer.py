@@ -162,7 +162,9 @@ class Backend:
     @staticmethod
     def releaseScratch():
         """Gives the memory that small calls keep between them (one piece of up to 1 MB a stream, of up to
-        16 streams) back to torch's allocator, from where torch.cuda.empty_cache() gives it to the device."""
+        16 streams) and the workspaces of AttentionOverCache (one a stream, of the power of two that its
+        calls needed, 1 to 128 MB) back to torch's allocator, from where torch.cuda.empty_cache() gives it
+        to the device."""
         _host.release_scratch()
 
     def setGemmType(self, type_):
