@@ -6,7 +6,8 @@ No counterpart in the reference, whose decoder state is float32 (src/models/tran
 positions are added to the embeddings (:110-117).  Activations are torch tensors on the GPU, float32, float16 or
 bfloat16, [sequences, heads, n, dk] as SplitHeads gives them (dk a multiple of 16, up to 256); tensors that are not
 laid out in whole rows of 16-byte pieces are copied first.  lens, counts, parents, paths are int32 on the GPU (int64
-is converted) and read there: a step needs no synchronisation, and may be recorded into a graph.  There is no CPU fallback.
+is converted) and read there: a step needs no synchronisation, and may be recorded into a graph.  New outputs are dense and lie
+in memory as their input does: the heads of a position side by side, or head by head.  There is no CPU fallback.
 
 One step of a decoder with drafted tokens:
     for layer, cache in zip(layers, caches):
@@ -86,7 +87,9 @@ def _rows(x, what, like=None):
     whole = 16 // x.element_size()
     if x.data_ptr() % 16 == 0 and x.stride(3) == 1 and all(x.stride(i) % whole == 0 for i in range(3) if x.shape[i] > 1):
         return x
-    return x.contiguous() if not x.is_contiguous() else x.clone()
+    if x.stride(1) < x.stride(2):   # (the heads of a position side by side, as they were)
+        return x.transpose(1, 2).clone(memory_format=torch.contiguous_format).transpose(1, 2)
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def _whole_numbers(t, shape, device, what):

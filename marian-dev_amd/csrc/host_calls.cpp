@@ -1280,19 +1280,16 @@ bool rows_of(const at::Tensor* t, const c10::Device* d, Rows& r) {
   r.t = t;
   return true;
 }
-// A tensor like r's that lies in memory as r's does: head by head, or the heads of a position side by side.
+// A tensor like r's, dense, that lies in memory as r's does: the heads of a position side by side where r's are closer than its positions, or else
+// head by head.
 at::Tensor rows_like(const Rows& r, int64_t (&st)[3]) {
   const at::Tensor& t = *r.t;
   const int64_t heads = t.size(1), n = t.size(2), dk = t.size(3);
-  if(t.is_contiguous()) {
-    st[0] = heads * n * dk;
-    st[1] = n * dk;
-    st[2] = dk;
-    return empty(t.sizes(), t.scalar_type(), t.device());
-  }
+  const bool together = heads > 1 && n > 1 && t.stride(1) < t.stride(2);
   st[0] = heads * n * dk;
-  st[1] = dk;
-  st[2] = heads * dk;
+  st[1] = together ? dk : n * dk;
+  st[2] = together ? heads * dk : dk;
+  if(!together) return empty(t.sizes(), t.scalar_type(), t.device());
   const int64_t stride[4] = {st[0], st[1], st[2], 1};
   return at::Tensor(at::detail::empty_strided_cuda(t.sizes(), stride, t.scalar_type(), t.device()));
 }
