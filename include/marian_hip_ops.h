@@ -415,7 +415,8 @@ int marian_hip_cache_read(const marian_hip_kv_cache* cache, const int32_t* first
  * Products and sums are float32.  Of float16 and bfloat16 queries, weights enter the product with the values in
  * 11 bits, of float32 ones in 22, each of its own size down to 2^-24 of the largest; the sum is of the weights in float32.
  * A sequence's positions are split over workgroups where there are few of them, by the lengths of all
- * sequences: the last bits of a result depend on the batch it is in, and not on the order of anything.
+ * sequences, and the cache's sizes, its capacity among them, say which form of the kernel takes them: the last bits of a result depend on the
+ * batch and on the cache it is in, and not on the order of anything.
  *   workspace: at least marian_hip_cache_attention_workspace_bytes(...) bytes (enough for any capacity and type; 0 too where
  *   sizes are out of range), 256-byte aligned (0 bytes: may be null), which marian_hip_cache_attention_workspace_init clears once after allocating (a kernel: it may be
  *   recorded).  One workspace serves one stream, like that of marian_hip_nbest_beams.
