@@ -53,3 +53,32 @@ def test_scales_below_zero(S, H, G, n, dk, cap, format, dtype):
         for got, codes, scales in ((k, cache.k, cache.kScale), (v, cache.v, cache.vScale)):
             at4 = at.expand(S, H, n, dk)
             assert same(got, codes.float().gather(2, at4) * scales.gather(2, at4[..., 0])[..., None])
+
+
+@pytest.mark.parametrize("format", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e-26, 1e-30, 1e-33, 1e-37])
+@pytest.mark.parametrize("S,H,G,n,dk,cap", SHAPES)
+def test_values_next_to_the_smallest(S, H, G, n, dk, cap, size, format, dtype):
+    """Weights are rounded as those of scales of 1e-30, where all scales are below that: half a step of the smallest float16 at a unit of
+    2^9, 16 times at the most above the largest weight, of a code: 2^-25 / 2^9 * 16 = 2^-30 of it.  (The bound has it for the widest scale.)
+    float32 itself has steps of 2^-149 at its end, taken once by each of the sums, at most 48 parts and four waves and one position after
+    the other, over the power of two that waves are joined by."""
+    kv = load("cache")
+    cache, q, lens = batch(S, H, G, n, dk, cap, format, dtype)
+    cache.vScale.mul_(size)
+    want, tol = forms.attention(q, cache, lens)
+    far = 2.0 ** -30 * 1e-30 * cap * oracle.TOP[format] + 2.0 ** -149 * 64.0 * 2.0 ** (6 + cap.bit_length())
+    check(kv.AttentionOverCache(q, cache, lens), want, tol + far)
+
+
+@pytest.mark.parametrize("format", ["int8", "e4m3"])
+@pytest.mark.parametrize("S,H,G,n,dk,cap", SHAPES)
+def test_keys_of_all_sizes(S, H, G, n, dk, cap, format):
+    """Keys up to 2^110 by queries as small, and the other way around: scores of a few units"""
+    kv = load("cache")
+    for k_size, q_size in ((2.0 ** 104, 2.0 ** -105), (2.0 ** -80, 2.0 ** 80)):
+        cache, q, lens = batch(S, H, G, n, dk, cap, format, torch.float32)
+        cache.kScale.copy_(k_size * 2.0 ** -7 * (1 + torch.arange(cap, device="cuda") % 3))
+        q = q * q_size
+        check(kv.AttentionOverCache(q, cache, lens), *forms.attention(q, cache, lens))
