@@ -360,8 +360,9 @@ typedef struct marian_hip_rotation {
  *   MARIAN_HIP_ROTARY_LINEAR: all divided by factor;
  *   MARIAN_HIP_ROTARY_BASE: base * factor^(dims / (dims - 2)) in place of base;
  *   MARIAN_HIP_ROTARY_BANDS: pairs that turn less than `slow` times in `original` positions are divided by factor, those
- *   that turn more than `fast` times stay, between them a linear mixture (Peng et al., "YaRN", 2023); magnitude
- *   0.1 ln(factor) + 1.
+ *   that turn more than `fast` times stay, between them a mixture that is linear in the number of turns, as the formula of Peng et al., "YaRN",
+ *   2023, has it; magnitude 0.1 ln(factor) + 1.  (Some models' own code mixes linearly in the pair's index between the two bounds instead, with other
+ *   frequencies in between; for those, and any other scaling, `turns` is filled by the caller: round(frequency / 2 pi * 2^64).)
  * host_turns: dims / 2 values in HOST memory; host_magnitude: one.  No HIP call is made.
  * base > 1, factor >= 1; BASE: dims >= 4; BANDS: original >= 1, 0 <= slow < fast.
  */

@@ -65,8 +65,9 @@ def newCache(sequences, heads, capacity, dk, format="int8", device="cuda"):
 def makeRotary(dims, base=10000.0, interleaved=False, scaling=None, factor=1.0, original=None, slow=1.0, fast=32.0, device="cuda"):
     """The turns of `dims` values of a head: pair p by base^(-2 p / dims) radians a position.  scaling, for contexts
     `factor` times as long as the model was made for: "linear" (all slower), "base" (a larger base), "bands" (pairs of
-    fewer than `slow` turns in `original` positions slower, of more than `fast` as they are, a mixture in between, and a
-    magnitude of 0.1 ln(factor) + 1)."""
+    fewer than `slow` turns in `original` positions slower, of more than `fast` as they are, a mixture linear in the turns in
+    between, and a magnitude of 0.1 ln(factor) + 1).  Models that mix otherwise, linearly in the pair's index for one, are a Rotary of their own:
+    turns int64 round(frequency / 2 pi * 2^64), a magnitude, and the order of the pairs."""
     _abort_if(scaling not in SCALINGS, "makeRotary: unknown scaling {}", scaling)
     _abort_if(dims < 8 or dims % 8 != 0, "makeRotary: a multiple of 8 values, got {}", dims)
     turns, magnitude = torch.empty(dims // 2, dtype=torch.int64), ctypes.c_double()
