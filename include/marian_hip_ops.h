@@ -413,8 +413,8 @@ int marian_hip_cache_read(const marian_hip_kv_cache* cache, const int32_t* first
  * Positions that a token does not see are not read into its result, whatever they hold.  A token that sees nothing (it
  * and all before it past the capacity) gives zeros, and so do rows at or past counts[s].  out shares no memory with q
  * or the cache.  scale: finite, above zero.
- * Products and sums are float32.  Of float16 and bfloat16 queries, weights enter the product with the values in
- * 11 bits, of float32 ones in 22, each of its own size down to 2^-24 of the largest; the sum is of the weights in float32.
+ * Products and sums are float32.  Weights enter the product with the values in 22 bits, of bfloat16 queries with more than 32 rows an entry (n *
+ * q_heads / heads) in 11, each of its own size down to 2^-24 of the largest; the sum is of the weights in float32.
  * Scales of values below 1e-30 are weighed in steps that do not get smaller with them: off by up to 2^-30 * 1e-30 of a position's code.
  * Keys whose largest magnitude is above 2^110 may take a score out of float32, and the result is NaN then.
  * A sequence's positions are split over workgroups where there are few of them, by the lengths of all

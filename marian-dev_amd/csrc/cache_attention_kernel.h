@@ -26,10 +26,13 @@
 // Codes are exact in float16.  Q is scaled row by row by a power of two up to 2^14 .. 2^15 and enters in one float16
 // (float16 and bfloat16: exact but for values 2^-29 below the row's largest) or two (float32: 22 bits).  A weight is
 // p_rj times the value's scale over a running scale S_r (as the maximum runs; of magnitudes, since a scale may be below zero), times
-// 2^9: in one float16 or two, rounded to nearest, of what is at most 2^15 and, with normal numbers, down to 2^-14: 11 (22) bits
-// of weights up to 2^-24 below the largest.  Their sum is of the weights in float32.  (float16 outputs are rounded to 11 bits
-// themselves: the weights' rounding adds 40 % to the error of the result at most, and a second float16 would double the
-// instructions of the larger product.)
+// 2^9: in two float16, rounded to nearest, of what is at most 2^15 and, with normal numbers, down to 2^-14: 22 bits of weights up to
+// 2^-24 below the largest.  Their sum is of the weights in float32.  The second float16 costs another product with the values: next to nothing up
+// to 32 rows, where memory is waited for (bfloat16; 16 sequences, 32 heads on 8, up to 32768 positions 139.1 us without it, 138.2 with it; 4 drafted
+// tokens of them, up to 32000 147.8 and 149.0; at the most 128 sequences' 4 tokens, 32 heads on 16, up to 512 of 64 values 26.6 and 27.8).  With more
+// rows it does cost: bfloat16 leaves it out there and has 11 bits - 8 trees of 64 tokens 82 us, 100 with it, prompts of 1024 tokens 326
+// and 419 -, for its results are rounded to 8 bits, an error of 1.654e-3 of their norm, which such weights make 1.667e-3.  float16's are
+// rounded to 11 bits themselves, 2.08e-4, and would be off by 2.91e-4.
 // The sums are scaled down only where a maximum or scale outgrows the carried one by 2^4 (4): most turns skip it.
 // Positions that a row does not see, and rows past the end that pad a block, weigh a selected zero; loads go through buffers that end where
 // the part does, and give zeros behind it.
@@ -135,7 +138,9 @@ __device__ __forceinline__ float settled(float z) {
 
 template <typename T, CacheFormat F, int DP>
 struct CacheAttention {
-  static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;   // float16 to a query value or weight
+  static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;   // float16 to a query value ...
+  static constexpr int kWeightTerms = 2;                  // ... and to a weight, of up to 32 rows ...
+  static constexpr int kManyWeightTerms = __is_same(T, bf16_t) ? 1 : 2;   // ... and of more
   static constexpr int kSteps = DP / 32;                  // of a product over a row
   static constexpr int kPieces = DP / 64;                 // sixteen codes of a key to a lane
   static constexpr int kDims = DP / 16;                   // of a value's row to a lane
@@ -609,7 +614,7 @@ __device__ __forceinline__ void cache_finish(const CacheAttentionArgs& a, const 
 template <typename T, CacheFormat F, int DP, int QT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT : 2)) void cache_attention_kernel(CacheAttentionArgs a) {
   using A = CacheAttention<T, F, DP>;
-  constexpr int kTerms = A::kTerms, kSteps = A::kSteps, kDims = A::kDims;
+  constexpr int kTerms = A::kTerms, kWeightTerms = A::kWeightTerms, kSteps = A::kSteps, kDims = A::kDims;
   constexpr int kTurn = 32 * WAVES;   // positions that the waves take in one turn
   __shared__ struct {
     CacheJoin<DP, QT, WAVES> join;
@@ -769,16 +774,16 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
 #pragma unroll
         for(int e = 0; e < 8; ++e) r[t][e] = seen_here[t] >> e & 1 ? r[t][e] : 0.0f;
     }
-    cache_h8 p[QT][kTerms];
+    cache_h8 p[QT][kWeightTerms];
 #pragma unroll
     for(int t = 0; t < QT; ++t) {
       const float from = top[t] == kNone ? 0.0f : -top[t];   // (nothing seen so far: minus infinity stays that)
 #pragma unroll
       for(int e = 0; e < 8; ++e) {
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], row_scale[t], from)), z = kTerms == 2 ? settled(y * r[t][e]) : y * r[t][e];
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], row_scale[t], from)), z = settled(y * r[t][e]);
         sum[t] += y;
         p[t][0][e] = (_Float16)z;
-        if constexpr(kTerms == 2) p[t][1][e] = (_Float16)(z - (float)p[t][0][e]);
+        p[t][1][e] = (_Float16)(z - (float)p[t][0][e]);
       }
     }
     // weighted values
@@ -796,7 +801,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
 #pragma unroll
         for(int t = 0; t < QT; ++t)
 #pragma unroll
-          for(int m = kTerms - 1; m >= 0; --m)
+          for(int m = kWeightTerms - 1; m >= 0; --m)
             o[t][4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d[j], p[t][m], o[t][4 * i + j], 0, 0, 0);
     }
     fetch_values(value, at + kTurn);
@@ -821,7 +826,7 @@ struct CacheFew {
   static constexpr int kRegs = ROWS < 4 ? ROWS : 4;    // rows whose scores a lane has
   static constexpr int kKeys = ROWS <= 4 ? 1 : 2;      // keys whose scores a lane has
   static constexpr int kStride = 72;                   // weights of a row in LDS, and eight more
-  typedef _Float16 Weights[A::kTerms][ROWS][kStride];
+  typedef _Float16 Weights[A::kWeightTerms][ROWS][kStride];
 
   struct Keys {
     cache_u4 code[4][A::kPieces];
@@ -847,7 +852,7 @@ template <typename T, CacheFormat F, int DP, int ROWS, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) void cache_attention_few_kernel(CacheAttentionArgs a) {
   using A = CacheAttention<T, F, DP>;
   using B = CacheFew<T, F, DP, ROWS>;
-  constexpr int kTerms = A::kTerms, kSteps = A::kSteps, kDims = A::kDims, kRegs = B::kRegs, kKeys = B::kKeys;
+  constexpr int kTerms = A::kTerms, kWeightTerms = A::kWeightTerms, kSteps = A::kSteps, kDims = A::kDims, kRegs = B::kRegs, kKeys = B::kKeys;
   constexpr int kTurn = 64 * WAVES;   // positions that the waves take in one turn
   __shared__ CacheFewShared<T, F, DP, ROWS, WAVES> sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -994,20 +999,20 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
 #pragma unroll
       for(int t = 0; t < kRegs; ++t) {
         const float from = top[t] == kNone ? 0.0f : -top[t];   // (nothing seen so far: minus infinity stays that)
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][t], row_scale[t], from)), whole = y * (scale[i][t] * per[t]), z = kTerms == 2 ? settled(whole) : whole;
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][t], row_scale[t], from)), z = settled(y * (scale[i][t] * per[t]));
         sum[t] += y;
         const _Float16 hi = (_Float16)z;
         sh.weights[wave][0][mine0 + t][slot] = hi;
-        if constexpr(kTerms == 2) sh.weights[wave][kTerms - 1][mine0 + t][slot] = (_Float16)(z - (float)hi);
+        sh.weights[wave][1][mine0 + t][slot] = (_Float16)(z - (float)hi);
       }
     }
     __builtin_amdgcn_wave_barrier();   // (a wave's accesses to LDS are done in their order)
     // weighted values
 #pragma unroll
     for(int h = 0; h < 2; ++h) {
-      cache_h8 p[kTerms];
+      cache_h8 p[kWeightTerms];
 #pragma unroll
-      for(int m = 0; m < kTerms; ++m) p[m] = *reinterpret_cast<const cache_h8*>(&sh.weights[wave][m][c % ROWS][32 * h + 8 * g]);
+      for(int m = 0; m < kWeightTerms; ++m) p[m] = *reinterpret_cast<const cache_h8*>(&sh.weights[wave][m][c % ROWS][32 * h + 8 * g]);
       unsigned vh[8][A::kWords];
 #pragma unroll
       for(int e = 0; e < 8; ++e)
@@ -1020,7 +1025,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
 #pragma unroll
         for(int j = 0; j < 4; ++j)
 #pragma unroll
-          for(int m = kTerms - 1; m >= 0; --m) o[0][4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d[j], p[m], o[0][4 * i + j], 0, 0, 0);
+          for(int m = kWeightTerms - 1; m >= 0; --m) o[0][4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d[j], p[m], o[0][4 * i + j], 0, 0, 0);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -1046,7 +1051,7 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
 template <typename T, CacheFormat F, int DP, int QT>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void cache_attention_many_kernel(CacheAttentionArgs a) {
   using A = CacheAttention<T, F, DP>;
-  constexpr int kTerms = A::kTerms, kSteps = A::kSteps, kDims = A::kDims, kPieces = A::kPieces;
+  constexpr int kTerms = A::kTerms, kWeightTerms = A::kManyWeightTerms, kSteps = A::kSteps, kDims = A::kDims, kPieces = A::kPieces;
   constexpr int kTile = 64, kRows = 16 * QT * 4;
   constexpr int kMine = kDims / 2;                      // dimensions' operands that a wave makes ...
   constexpr int kMineWords = kMine < 4 ? 1 : kMine / 4;   // ... of so many words of a row
@@ -1227,7 +1232,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void cache_attention_many_k
         per[t] = kWeightUnit / u;
       }
     }
-    cache_h8 p[QT][kTerms];
+    cache_h8 p[QT][kWeightTerms];
 #pragma unroll
     for(int t = 0; t < QT; ++t) {
       const float from = top[t] == kNone ? 0.0f : -top[t];   // (nothing seen so far: minus infinity stays that)
@@ -1236,10 +1241,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void cache_attention_many_k
         const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], row_scale[t], from));
         float r = vs[e / 4][e % 4] * per[MASKED ? t : 0];
         if constexpr(MASKED) r = seen_here[t] >> e & 1 ? r : 0.0f;
-        const float z = kTerms == 2 ? settled(y * r) : y * r;
+        const float z = kWeightTerms == 2 ? settled(y * r) : y * r;
         sum[t] += y;
         p[t][0][e] = (_Float16)z;
-        if constexpr(kTerms == 2) p[t][kTerms - 1][e] = (_Float16)(z - (float)p[t][0][e]);
+        if constexpr(kWeightTerms == 2) p[t][kWeightTerms - 1][e] = (_Float16)(z - (float)p[t][0][e]);
       }
     }
 #pragma unroll
@@ -1249,7 +1254,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void cache_attention_many_k
 #pragma unroll
       for(int t = 0; t < QT; ++t)
 #pragma unroll
-        for(int m = kTerms - 1; m >= 0; --m) o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand, p[t][m], o[t][j], 0, 0, 0);
+        for(int m = kWeightTerms - 1; m >= 0; --m) o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand, p[t][m], o[t][j], 0, 0, 0);
     }
   };
   auto turn = [&](int at) __attribute__((always_inline)) {   // the positions in hand into LDS, the next ones asked for

@@ -132,13 +132,20 @@ def seen(parents, n, device):
     return reach > 0
 
 
-def attention(q, cache, lens, parents=None, counts=None, scale=None):
+def weight_rounding(dtype, rows):
+    """of a weight ahead of its product with a value: two float16 - the second one's half step, 2^-11 of what the first one leaves, which is
+    up to 2^-11 of the weight - or one, of bfloat16 with more than 32 rows an entry"""
+    return 2.0 ** -11 if dtype == torch.bfloat16 and rows > 32 else 2.0 ** -22
+
+
+def attention(q, cache, lens, parents=None, counts=None, scale=None, rounding=None):
     """As cache_oracle.attention, in products of whole batches on the tensors' own device: -> (result, how far a kernel's may be).
     What a row sees of a NaN makes it NaN; a NaN that it does not see is not in it."""
     S, HQ, n, dk = q.shape
     k, v, ks, vs = cache
     H, cap, dev = k.shape[1], k.shape[2], q.device
     G, scale = HQ // H, scale or dk ** -0.5
+    rounding = rounding or weight_rounding(q.dtype, G * n)
     out = torch.empty(q.shape, dtype=torch.float64, device=dev)
     tol = torch.empty_like(out)
     lens = lens.long().clamp(0, cap)
@@ -170,7 +177,6 @@ def attention(q, cache, lens, parents=None, counts=None, scale=None):
         products = (scale * (Q.abs() @ K.abs().transpose(2, 3))).masked_fill(hidden, 0.0).amax(-1)
         count = see.sum(-1).double()
         d = products * (dk + 8) * 2.0 ** -23 + e.abs().masked_fill(hidden, 0.0).amax(-1) * 2.0 ** -21 + 2.0 ** -21 + count * 2.0 ** -24
-        rounding = 2.0 ** -11 if q.dtype != torch.float32 else 2.0 ** -22
         steps = see.double() @ (V.abs() / torch.where(vsc > 0, vsc, torch.ones_like(vsc))[..., None])
         widest = vsc[:, :, None].expand(-1, -1, G * n, -1).masked_fill(hidden, 0.0).amax(-1)
         smallest = 2.0 ** -25 / 2.0 ** 9 * widest[..., None] * steps
