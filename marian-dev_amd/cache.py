@@ -140,8 +140,8 @@ def _out(out, like, what):
 
 def rotaryPositions(x, positions, rotary, out=None):
     """x [sequences, heads, n, dk] with the first values of every row turned by its position: positions [sequences] -
-    row i of a sequence at positions[s] + i - or [sequences, n], 32 bits of them.  out: x itself, or a tensor apart from it; None: a new
-    one that lies in memory as x does."""
+    row i of a sequence at positions[s] + i - or [sequences, n]; int64 that 32 bits do not hold are taken as the nearer end.
+    out: x itself, or a tensor apart from it; None: a new one that lies in memory as x does."""
     res = _host.rotary(x, positions, rotary, out)
     if res is not None:
         return res

@@ -21,7 +21,8 @@
 //     codes at c * DP / 16 of each of these eight keys - a row of keys between sixteen lanes - and picks a dimension's eight
 //     codes out of its registers, two at a time, while they become float16.
 //     So neither keys, values nor weights go through LDS; only the scales do.
-//     16 sequences, 4 drafted tokens, 32 heads on 8, 4000 positions of 128 values at most: 29.9 us, 3.0 TB/s.
+//     16 sequences, 4 drafted tokens, 32 heads on 8, up to 4000 positions of 128 values: 26.4 us, 3.5 TB/s; up to 32000 149 us, 5.1 TB/s.
+//     Memory bounds the long ones; a part of the short ones is four turns of a workgroup, and its start and the join show.
 //   cache_attention_few_kernel: up to 8 rows over long contexts, cache_attention_many_kernel: more than 32 rows; see there.
 // Codes are exact in float16.  Q is scaled row by row by a power of two up to 2^14 .. 2^15 and enters in one float16
 // (float16 and bfloat16: exact but for values 2^-29 below the row's largest) or two (float32: 22 bits).  A weight is
@@ -29,10 +30,10 @@
 // 2^9: in two float16, rounded to nearest, of what is at most 2^15 and, with normal numbers, down to 2^-14: 22 bits of weights up to
 // 2^-24 below the largest.  Their sum is of the weights in float32.  The second float16 costs another product with the values: next to nothing up
 // to 32 rows, where memory is waited for (bfloat16; 16 sequences, 32 heads on 8, up to 32768 positions 139.1 us without it, 138.2 with it; 4 drafted
-// tokens of them, up to 32000 147.8 and 149.0; at the most 128 sequences' 4 tokens, 32 heads on 16, up to 512 of 64 values 26.6 and 27.8).  With more
-// rows it does cost: bfloat16 leaves it out there and has 11 bits - 8 trees of 64 tokens 82 us, 100 with it, prompts of 1024 tokens 326
-// and 419 -, for its results are rounded to 8 bits, an error of 1.654e-3 of their norm, which such weights make 1.667e-3.  float16's are
-// rounded to 11 bits themselves, 2.08e-4, and would be off by 2.91e-4.
+// tokens of them, up to 32000 147.8 and 149.0; 128 sequences' 4 tokens, 32 heads on 16, up to 512 of 64 values 26.6 and 27.8; at the most, in a
+// sequence's own few parts, one head of 100000 24.5 and 26.4).  With more rows it does cost: bfloat16 leaves it out there and has 11 bits - 8 trees
+// of 64 tokens 82 us, 100 with it, prompts of 1024 tokens 326 and 419 -, for its results are rounded to 8 bits, an error of 1.654e-3 of their
+// norm, which such weights make 1.667e-3.  float16's are rounded to 11 bits themselves, 2.08e-4, and would be off by 2.91e-4.
 // The sums are scaled down only where a maximum or scale outgrows the carried one by 2^4 (4): most turns skip it.
 // Positions that a row does not see, and rows past the end that pad a block, weigh a selected zero; loads go through buffers that end where
 // the part does, and give zeros behind it.
@@ -817,8 +818,9 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 64 ? 5 - QT : DP == 128 ? 4 - QT
 // score is in one lane only.  A key's scales are a value to a lane, whole lines of memory.  The weights go
 // through LDS, a row of 64 a query, to where they are an operand: lane (c, g) takes eight of row c, those of positions
 // 4 e + g of 32, so that four rows of values that follow each other in memory are loaded at a time.
-// Memory bounds it: 16 sequences, 32 heads on 8, up to 32768 positions of 128 values in e4m3 157 us, 5.5 TB/s (the form above 163), 64 of up to
-// 4096 in int8 73.5 us, 5.0 TB/s (84.7); 128 sequences, 16 heads, up to 512 of 64 values, float32, 22.4 us, 4.2 TB/s (24.7).
+// Memory bounds it: 16 sequences, 32 heads on 8, up to 32768 positions of 128 values in e4m3 139 us, 5.5 TB/s (the form above 148), 64 of up to
+// 4096 in int8 74.3 us, 5.0 TB/s (83.8); 128 sequences, 16 heads, up to 512 of 64 values, float32, 20.3 us, 4.7 TB/s (22.0).  Not so one sequence
+// with few heads: its parts are few (kCacheMostParts), a head of 100000 positions takes 26.4 us, 1.0 TB/s.
 // Its start costs more, so short contexts are left to the form above.
 template <typename T, CacheFormat F, int DP, int ROWS>
 struct CacheFew {
@@ -1044,10 +1046,12 @@ __global__ __launch_bounds__(64 * WAVES, (DP == 128 ? 2 : ROWS <= 2 ? 4 : 3)) vo
 // half w / 2 of the positions half the dimensions of the values; the next codes are on their way meanwhile.  The products are those
 // of the first form, but for the dimensions, lane (c, g) having 64 i + 16 g + 4 e + j.  While a wave lays positions out it goes ahead of those in
 // products (the others wait for it): 81.3 us against 84.8 (the trees below).  A second buffer in LDS, with one barrier a turn, gained nothing.
-// The matrix instructions and the exponentials between them bound it: 4 sequences, 1024 tokens, 32 heads on 8, 4096 positions of 128 values,
-// bfloat16, 327 us, 857 TFLOP/s; 8 trees of 64 tokens, 32 heads on 4, up to 8192 positions 81 us, 590 TFLOP/s (57 us at
-// the rate of the first; the rest goes to parts of unequal length, and to results on their way through memory to the workgroup that joins them).  The first form: 8 sequences of 16 tokens, 32 heads on 8, 8192 positions
-// 47.3 us, this one 45.2; 64 sequences of 50 rows, 16 heads, 36.7 and 26.3.
+// 4 sequences, 1024 tokens behind 3072 positions, 32 heads on 8, 128 values, bfloat16: 328 us, 730 TFLOP/s of what the tokens see; 8 trees of 64
+// tokens, 32 heads on 4, behind 8192 positions 113 us, 610 TFLOP/s, up to 8192 82 us, 550 TFLOP/s: products and exponentials take turns in
+// the issue slots, and with lengths that differ parts do, too, and results go through memory to the workgroup that joins them.  The first form:
+// 8 sequences of 16 tokens, 32 heads on 8, up to 8192 positions 53.9 us, this one 42.8; 64 sequences of 50 rows, 16 heads, up to
+// 500 positions 53.0 and 37.2.  (Few entries of a few thousand positions leave most of the card idle, a part being 512 of them: 64 tokens of 8 heads
+// of 256 values, 4000 positions, 64 workgroups, 34 us, 62 TFLOP/s.)
 template <typename T, CacheFormat F, int DP, int QT>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void cache_attention_many_kernel(CacheAttentionArgs a) {
   using A = CacheAttention<T, F, DP>;

@@ -33,8 +33,10 @@ __device__ __forceinline__ float half_turns(long long position, unsigned long lo
 
 // A thread turns one unit - four pairs, or eight values behind the turned ones - of up to HEADS heads of a position: the
 // angles are the same for all of them.  Units of a row are side by side, then heads, then positions.
-// out = x turned, in float32 with the angle's fraction of a turn exact: the error does not grow with the position.  Memory bounds it: 4 sequences of 4093
-// positions, 32 heads of 128 values, bfloat16, 54 us, 5.0 TB/s (a copy: 5.1); a single token's 2.3 us are a launch's.
+// out = x turned, in float32 with the angle's fraction of a turn exact: the error does not grow with the position.  (The fraction is rounded to 24
+// bits ahead of sine and cosine: float32 results are off by 4.9e-8 of their norm, where angles in 64 bits leave 4.3e-8.)
+// Memory bounds it: 4 sequences of 4093 positions, 32 heads of 128 values, bfloat16, 54 us, 5.0 TB/s (a copy: 5.1); a single token's 2.3 us are a
+// launch's.
 template <typename T, int HEADS>
 __global__ __launch_bounds__(256) void rotary_kernel(const T* x, Strides xs, T* out, Strides os, const int* __restrict__ positions, int each,
                                                      const unsigned long long* __restrict__ turns, int dims, float magnitude, int interleaved,
@@ -107,9 +109,11 @@ struct AppendArgs {
 // rounded once to float32 and then quantized, so that a key next to a border of a code falls on its own side).
 //   scale = largest magnitude of the row / 127 (448), code = value / scale rounded to the nearest, ties to even.
 // A row's lanes are side by side, its largest value a few exchanges away; a value and the one it is turned with are both loaded, the second
-// from a cache, in place of an exchange.  3 sequences of 2731 tokens, 32 + 8 + 8 heads of 128 values, float16 to e4m3: 52 us,
-// 3.5 TB/s, where a copy of these bytes takes 36: the rest is the 64-bit turns (48 us with them in 32 bits, which would move codes at
-// borders) and the quotients.  128 sequences' single tokens, 48 heads of 64 values, float32: 4.0 us one after the other, most of it a launch's.
+// from a cache, in place of an exchange.  3 sequences of 2731 tokens, 32 + 8 + 8 heads of 128 values, float16 to e4m3: 50 us,
+// 3.7 TB/s.  Without a rotation they take 36, as a copy of these bytes does, so turning is what the rest goes to: angles made by each of the three
+// workgroups that share a token, ahead of its rows' loads, and turns in 64 bits, of queries like keys (in 32 bits, which would move codes of keys
+// at borders, 4 us less).  128 sequences' single tokens, 48 heads of 64 values, float32: 4.4 us, 3.8 without a rotation, one step after the
+// other, where a launch alone takes 2.3.
 template <typename T, CacheFormat F, int LANES, int TOKENS>
 __global__ __launch_bounds__(256) void append_kernel(const T* k, const T* v, const T* q, T* q_out, AppendArgs a) {
   constexpr int kRows = 256 / LANES;
@@ -275,7 +279,8 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const unsigned char* __
 
 // ---------------------------------------------------------------- accepted drafts
 // A workgroup to the keys or the values of an entry: everything is read before anything is written, so a path may go anywhere, twice to
-// the same row too.  64 sequences, 16 heads, 64 rows of 128 codes: 6.1 us, 5.5 TB/s; 16 rows of one sequence 2.9 us, a launch's.
+// the same row too.  A launch and the steps that follow each other (path, rows, stores) bound it: 16 to 32 rows of 128 codes in each of 64 sequences, 16
+// heads, 5.2 us, 2.4 TB/s; all 64 rows 7.0 us, 4.9 TB/s; 16 rows of one sequence 2.4 us.
 __global__ __launch_bounds__(256) void cache_keep_kernel(unsigned char* k, unsigned char* v, float* ks, float* vs, const int* __restrict__ lens,
                                                          const int* __restrict__ path, int path_len, const int* __restrict__ accepted,
                                                          int* __restrict__ new_lens, int heads, int cap, int dk) {
@@ -531,8 +536,8 @@ int marian_hip_cache_append(const marian_hip_kv_cache* cache, const marian_hip_d
   a.dk = (int)dk;
   const int64_t all = 2 * a.heads + a.q_heads;
   // Four tokens to a workgroup, all asked for at once, where a workgroup each would be more than 32 to a CU: 512 tokens of 16 sequences, 48 rows
-  // of 128 values a token, 44.8 us against 52.1 (a prompt's angles and the wait for memory count); below that a workgroup to each: 64
-  // tokens 10.5 us against 12.0, 3 of 64 sequences 4.5 against 6.9.
+  // of 128 values a token, bfloat16, 47.8 us against 59.0 (a prompt's angles and the wait for memory count; float32 74 both); below that a workgroup
+  // to each: 64 tokens 10.8 us against 11.9, 3 of 64 sequences 5.2 against 7.3.
   const int lanes = dk <= 64 ? 8 : dk <= 128 ? 16 : 32;
   const int64_t row_groups = (all * lanes + 255) / 256;
   const int each = row_groups * n * sequences > 8192 ? 4 : 1;
