@@ -203,7 +203,7 @@ def AttentionOverCache(q, cache, lens, parents=None, counts=None, scale=None, ou
     1 / sqrt(dk).  A token sees the lens[s] settled positions, itself and what it descends from: the tokens before it, or
     with parents [sequences, n] (n <= 64; -1: continues the settled ones) its branch of the tree.  Rows at or past counts[s]
     come out as zeros.  The last bits of a result depend on the batch's lengths and on the cache's sizes, capacity included; a cache with room for
-    400000 positions of all heads of all sequences is taken by a form for long contexts (a few us more for short ones).  The output lies in
+    400000 positions of all heads of all sequences is taken by a form for long contexts (some 2 us more for short ones).  The output lies in
     memory as q does."""
     res = _host.cache_attention(q, cache, lens, parents, counts, scale, out)
     if res is not None:
