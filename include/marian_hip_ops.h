@@ -440,6 +440,123 @@ int marian_hip_cache_attention(const marian_hip_kv_cache* cache, const marian_hi
 int marian_hip_cache_keep(const marian_hip_kv_cache* cache, const int32_t* lens, const int32_t* path, int64_t path_len,
                           const int32_t* accepted, int32_t* new_lens, void* stream);
 
+/*
+ * Verification of drafted tokens: which of the tokens that a cheaper model proposed the target keeps, and the token that
+ * follows them, such that the sequence is distributed as the target's own.  No counterpart in the reference.
+ *   tokens: int32 [sequences, n], n up to MARIAN_HIP_TREE_MAX, in the order they were given to the target: token 0 of a sequence is
+ *   settled (the one that the last step ended with), the others are drafted.
+ *   counts, parents: as in marian_hip_drafts; token 0 stands for itself, and a drafted token whose parent is none (below 0, or not before it)
+ *   is never reached.
+ *   target: [sequences, n, vocab] of `type`, row i the target's probabilities after token i; words of a row side by side, the
+ *   values between two sequences and two rows given (target_strides, any; aligned as the type is).
+ *   draft: null, or likewise [sequences, n - 1, vocab], row i what token i + 1 was drawn from; parents has to be null then.
+ *   random: float32 [sequences, n], each 0 <= u < 1 and independent of all else: random[s, 0] draws the next token, random[s, i] judges token i.
+ * With p the target's row after a token's parent, t the token and u its number:
+ *   draft given: t is kept if u * q(t) < p(t), q the draft's row; what follows the last kept token is drawn from max(p - q, 0) of its row
+ *   if a drafted token was refused there, else from p;
+ *   draft null (tokens that were not drawn, the drafter's best ones, in chains and trees): of the children of a kept token, in their
+ *   order, the first with u * (1 - sum of p of those refused before it) < p(t) is kept (a token that a sibling had already: none of p is left);
+ *   what follows is drawn from p without the tokens refused there.
+ * Drawing from weights w: the first word whose sum of weights up to itself exceeds u * sum of all, so ties go to the lowest word; where
+ * nothing is left (by rounding), from p itself; -1 where that is nothing, too.  Probabilities below zero and NaN count as zero, an infinite one leaves
+ * the word open.  All in 64 bits.
+ *   path: int32 [sequences, n], the kept tokens' numbers, 0 the first, then -1; accepted: int32 [sequences], how many (0 where counts is 0; next
+ *   is -1 then): what marian_hip_cache_keep takes.  next: int32 [sequences].  Outputs share no memory with anything else.
+ *   A token outside 0 .. vocab - 1 has probability zero.
+ *   workspace: at least marian_hip_verify_drafts_workspace_bytes(sequences, vocab) bytes, 256-byte aligned (0 bytes: may be null), cleared
+ *   once by marian_hip_cache_attention_workspace_init; one workspace serves one stream, and may be that of an attention.
+ * sequences <= 65535, vocab < 2^24.
+ */
+typedef struct marian_hip_drafted {
+  const int32_t* tokens;
+  const int32_t* counts;
+  const int32_t* parents;
+  const void* target;
+  const void* draft;
+  const float* random;
+  int64_t sequences, n, vocab;
+  int64_t target_strides[2], draft_strides[2];
+  int type;
+} marian_hip_drafted;
+size_t marian_hip_verify_drafts_workspace_bytes(int64_t sequences, int64_t vocab);
+int marian_hip_verify_drafts(const marian_hip_drafted* drafted, int32_t* path, int32_t* accepted, int32_t* next, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/*
+ * A cache in pages: memory for keys and values that sequences share, dealt out `page` positions at a time.  No counterpart in the reference.
+ *   k, v: [pages, heads, page, dk] of `type`, dense, 16-byte aligned; page a multiple of 8 up to 4096, dk as above, heads <= 4096,
+ *   pages * page < 2^30.
+ */
+typedef struct marian_hip_pages {
+  void* k;
+  void* v;
+  int64_t pages, heads, page, dk;
+  int type;
+} marian_hip_pages;
+
+/*
+ * Who has which pages, all on the device:
+ *   table: int32 [sequences, row]: the pages of a sequence in the order of its positions, -1 behind them;
+ *   held: int32 [sequences]: how many these are;
+ *   free: int32 [pages]: a stack of the pages that nobody has, its first free_count[0] entries.
+ * sequences <= 65535, row * sequences < 2^31.  A page belongs to one sequence; sequences that share one may read it only.
+ */
+typedef struct marian_hip_page_tables {
+  int32_t* table;
+  int32_t* held;
+  int32_t* free;
+  int32_t* free_count;
+  int64_t sequences, row, pages;
+} marian_hip_page_tables;
+
+/*
+ * Makes room for n new tokens a sequence (counts: null, or int32 [sequences], only so many of them) behind lens[s] positions: every
+ * sequence gets the pages that it lacks up to position lens[s] + counts[s], in the sequences' order from the top of the stack.  A sequence that the free
+ * pages do not reach for, or whose row of the table is too short, gets none; so does every later one that lacks some, in the first case.
+ *   slots: int32 [sequences, n]: where token i of sequence s lies, page number * page + place in it; -1 for tokens that are not
+ *   there or have no page (and so the sign of a sequence that got none).
+ * Lengths below 0 are taken as 0, counts into 0 .. n, held into 0 .. row, free_count into 0 .. pages.
+ * Replays of a recorded call go on from what the table holds then.
+ */
+int marian_hip_pages_reserve(const marian_hip_page_tables* tables, const int32_t* lens, const int32_t* counts, int64_t n, int64_t page,
+                             int32_t* slots, void* stream);
+
+/*
+ * Gives the pages behind lens[s] positions back, of every sequence (lens[s] = 0: all of them): what a refused draft or a finished
+ * sequence leaves.  Undoes a marian_hip_pages_reserve with the same lens, the order of the stack included.
+ */
+int marian_hip_pages_trim(const marian_hip_page_tables* tables, const int32_t* lens, int64_t page, void* stream);
+
+/*
+ * Writes keys and values of n tokens a sequence, [sequences, heads, n, dk] of the cache's type by strides (as for
+ * marian_hip_cache_append), to their slots: int32 [sequences, n]; a slot below 0 or past the last page writes nothing.  No two tokens of a call
+ * have the same slot.  n up to 2^20.
+ */
+int marian_hip_pages_write(const marian_hip_pages* cache, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                           int64_t sequences, int64_t n, const int32_t* slots, void* stream);
+
+/*
+ * Attention of n new tokens a sequence over the pages that they have been written to: q and out [sequences, q_heads, n, dk] of the cache's type
+ * by strides, q_heads a multiple of the cache's heads (query head h reads head h / (q_heads / heads)):
+ *   out = softmax(scale * q . key) value
+ * over the lens[s] positions before the new tokens, the token itself and the new ones before it.  table: int32 [sequences, row]; rows may share
+ * pages.  Positions of a page that is none (below 0, or at or past `pages`), and past the row, are not seen.  What a token does not see is
+ * not read into its result, infinities and NaN included.  A token that sees nothing, or whose scores are all minus infinity, gives zeros,
+ * and so do rows at or past counts[s] (counts: null, or int32 [sequences]).  out shares no memory with anything else.  scale: finite, above zero.
+ * Products and sums are float32; weights enter the product with the values in the cache's type (bfloat16: 8 bits, float16 11), their sum in float32.
+ * Values (bfloat16 and float32) below 2^-100 lose bits to the scale of the weights.
+ * The last bits of a result depend on the batch's lengths and the table's width, which say how positions are split over workgroups, and not on
+ * the order of anything.  Made for few rows a head of keys, n * q_heads / heads up to 64; more are taken 64 (or fewer, see the sources) at a time, each time
+ * reading keys and values again.
+ * lens outside 0 .. row * page are taken as the nearer end.  row * page < 2^30; n up to 2^20.
+ *   workspace: at least marian_hip_pages_attention_workspace_bytes(...) bytes, cleared once by marian_hip_cache_attention_workspace_init; as for
+ *   marian_hip_cache_attention, whose workspace serves this call too where it is large enough.
+ */
+size_t marian_hip_pages_attention_workspace_bytes(int64_t sequences, int64_t heads, int64_t q_heads, int64_t n, int64_t dk, int type);
+int marian_hip_pages_attention(const marian_hip_pages* cache, const int32_t* table, int64_t sequences, int64_t row, const int32_t* lens,
+                               const int32_t* counts, int64_t n, const void* q, const int64_t* q_strides, int64_t q_heads, float scale, void* out,
+                               const int64_t* out_strides, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -90,6 +90,13 @@ SIGNATURES = {
     "marian_hip_cache_attention_workspace_init": (_i, [_vp, _sz, _vp]),
     "marian_hip_cache_attention": (_i, [_vp, _vp, _vp, _vp, _i64, _i, _f, _vp, _vp, _vp, _sz, _vp]),
     "marian_hip_cache_keep": (_i, [_vp, _vp, _vp, _i64, _vp, _vp, _vp]),
+    "marian_hip_verify_drafts_workspace_bytes": (_sz, [_i64, _i64]),
+    "marian_hip_verify_drafts": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "marian_hip_pages_reserve": (_i, [_vp, _vp, _vp, _i64, _i64, _vp, _vp]),
+    "marian_hip_pages_trim": (_i, [_vp, _vp, _i64, _vp]),
+    "marian_hip_pages_write": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp]),
+    "marian_hip_pages_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i]),
+    "marian_hip_pages_attention": (_i, [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _f, _vp, _vp, _vp, _sz, _vp]),
 }
 
 
@@ -107,6 +114,22 @@ class Drafts(_c.Structure):
 class Rotation(_c.Structure):
     """marian_hip_rotation"""
     _fields_ = [("turns", _vp), ("dims", _i64), ("magnitude", _c.c_double), ("interleaved", _i)]
+
+
+class Drafted(_c.Structure):
+    """marian_hip_drafted"""
+    _fields_ = [("tokens", _vp), ("counts", _vp), ("parents", _vp), ("target", _vp), ("draft", _vp), ("random", _vp), ("sequences", _i64), ("n", _i64),
+                ("vocab", _i64), ("target_strides", _i64 * 2), ("draft_strides", _i64 * 2), ("type", _i)]
+
+
+class Pages(_c.Structure):
+    """marian_hip_pages"""
+    _fields_ = [("k", _vp), ("v", _vp), ("pages", _i64), ("heads", _i64), ("page", _i64), ("dk", _i64), ("type", _i)]
+
+
+class PageTables(_c.Structure):
+    """marian_hip_page_tables"""
+    _fields_ = [("table", _vp), ("held", _vp), ("free", _vp), ("free_count", _vp), ("sequences", _i64), ("row", _i64), ("pages", _i64)]
 
 
 # include/marian_hip_int8_tuning.h (tuning build only)

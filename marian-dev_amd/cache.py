@@ -1,6 +1,6 @@
 """Keys and values in 8 bits, on the HIP library (include/marian_hip_ops.h): rotary positions, a cache that is
-quantized as it is written, attention over it for single tokens, chains and trees of drafted ones, and the
-accepted drafts' move.
+quantized as it is written, attention over it for single tokens, chains and trees of drafted ones, the drafts'
+verification and the accepted ones' move.
 
 No counterpart in the reference, whose decoder state is float32 (src/models/transformer.h:683-700) and whose
 positions are added to the embeddings (:110-117).  Activations are torch tensors on the GPU, float32, float16 or
@@ -14,7 +14,7 @@ One step of a decoder with drafted tokens:
         q, k, v = layer.project(x)
         q = appendToCache(cache, k, v, lens, parents, rotary=rotary, q=q)
         x = layer.finish(AttentionOverCache(q, cache, lens, parents))
-    path, accepted = judge(x)
+    path, accepted, nextTokens = verifyDrafts(tokens, target(x), random, parents=parents)
     for cache in caches:   # (each of them from the lengths that its drafts were written behind)
         newLens = keepDrafts(cache, lens, path, accepted)
     lens = newLens
@@ -232,3 +232,42 @@ def keepDrafts(cache, lens, path, accepted):
     return _taken(_host.cache_keep(cache, _whole_numbers(lens, (sequences,), device, what + ": lens"),
                                    _whole_numbers(path, (sequences, path.shape[1]), device, what + ": path"),
                                    _whole_numbers(accepted, (sequences,), device, what + ": accepted")), what)
+
+
+def verifyDrafts(tokens, target, random, draft=None, parents=None, counts=None):
+    """Which of the tokens of a step are kept, and the token that follows them, so that the words are distributed as the target's own.
+    tokens int32 [sequences, n <= 64] as the target was given them: token 0 is settled (the last step's), the others are drafted, chains or
+    with parents [sequences, n] trees (as for AttentionOverCache); target [sequences, n, vocabulary], float32, float16 or bfloat16: row i the
+    target's probabilities behind token i; random float32 [sequences, n], numbers 0 <= u < 1 of their own: the first draws the next token, the others
+    judge theirs; draft [sequences, n - 1, vocabulary] (chains only), row i what token i + 1 was drawn from, or None: tokens that were not
+    drawn, the drafter's best.  counts [sequences]: only so many tokens are there.
+    draft given: a token is kept if u * draft(token) < target(token); what follows is drawn from max(target - draft, 0) where one was
+    refused.  None: of a kept token's children the first with u * (1 - target of those refused before it) < target(token) is kept; what follows
+    is drawn from the target without the refused ones.  Drawing: the first word up to which more than u of all weights lies.
+    Returns int32 path [sequences, n] (the kept tokens' numbers, 0 first, -1 behind them) and accepted [sequences], as keepDrafts takes them,
+    and the next tokens [sequences] (-1 where counts is 0)."""
+    res = _host.verify_drafts(tokens, target, random, draft, parents, counts)
+    if res is not None:
+        return res
+    what = "verifyDrafts"
+
+    def probabilities(t, n, name):
+        _abort_if(not isinstance(t, torch.Tensor) or t.dtype not in ACTIVATIONS or t.dim() != 3 or tuple(t.shape[:2]) != (sequences, n),
+                  "{}: {} float32, float16 or bfloat16 [{}, {}, vocabulary]", what, name, sequences, n)
+        return t if t.stride(2) == 1 and t.stride(0) >= 0 and t.stride(1) >= 0 else t.contiguous()
+    _abort_if(not isinstance(tokens, torch.Tensor) or tokens.dim() != 2 or not 1 <= tokens.shape[1] <= TREE_MAX, "{}: tokens [sequences, 1 .. {}]", what,
+              TREE_MAX)
+    sequences, n = tokens.shape
+    target = probabilities(target, n, "target")
+    _on_gpu(target)
+    device = target.device
+    if draft is not None:
+        _abort_if(parents is not None, "{}: a tree's tokens are not drawn from a distribution{}", what, "")
+        draft = probabilities(draft, n - 1, "draft")
+        _abort_if(draft.dtype != target.dtype or draft.device != device or draft.shape[2] != target.shape[2], "{}: draft {} {} beside target {} {}", what,
+                  tuple(draft.shape), draft.dtype, tuple(target.shape), target.dtype)
+    _abort_if(not isinstance(random, torch.Tensor) or random.dtype != torch.float32 or random.device != device or random.shape != tokens.shape,
+              "{}: random float32 {} on {}", what, tuple(tokens.shape), device)
+    return _taken(_host.verify_drafts(_whole_numbers(tokens, (sequences, n), device, what + ": tokens"), target, random.contiguous(), draft,
+                                      None if parents is None else _whole_numbers(parents, (sequences, n), device, what + ": parents"),
+                                      None if counts is None else _whole_numbers(counts, (sequences,), device, what + ": counts")), what)

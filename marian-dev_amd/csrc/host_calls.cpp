@@ -50,7 +50,8 @@ namespace {
   F(layer_norm) F(embed) F(attention_cached) F(attention_rows) F(attention_ancestors) F(ancestors_advance)                 \
   F(select_state) F(nbest) F(nbest_words) F(nbest_beams) F(nbest_beams_workspace_bytes) F(nbest_beams_workspace_init)   \
   F(logsoftmax_nbest_beams) F(rotary) F(cache_append) F(cache_read) F(cache_attention) F(cache_attention_workspace_bytes) \
-  F(cache_attention_workspace_init) F(cache_keep)
+  F(cache_attention_workspace_init) F(cache_keep) F(verify_drafts) F(verify_drafts_workspace_bytes) F(pages_reserve) F(pages_trim)      \
+  F(pages_write) F(pages_attention) F(pages_attention_workspace_bytes)
 
 struct Library {
 #define F(name) decltype(&marian_hip_##name) name;
@@ -1437,10 +1438,10 @@ PyObject* py_cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   MH_END
 }
 
-// The workspace of an attention over a quantized cache: a stream's own, kept until a call needs a larger one (then with room to spare, and
+// The workspace of an attention over a quantized cache or over pages, and of verified drafts: a stream's own, kept until a call needs a larger one (then with room to spare, and
 // the old one goes back to the stream that it was used on) or until release_scratch, or of a call that is recorded its own, cleared by the graph ahead of it
 // (the graph may be replayed on another stream, and beside another graph).
-at::Tensor cache_workspace(int64_t need, c10::Device d, hipStream_t st) {
+at::Tensor cache_workspace(int64_t need, c10::Device d, hipStream_t st, const char* where = "AttentionOverCache") {
   const bool once = marian_hip::recorded(st);
   int64_t size = need;
   if(!once) {
@@ -1449,7 +1450,7 @@ at::Tensor cache_workspace(int64_t need, c10::Device d, hipStream_t st) {
     for(size = 1 << 20; size < need;) size *= 2;
   }
   at::Tensor made = empty({size}, at::kByte, d);
-  call("AttentionOverCache", [&] { return L.cache_attention_workspace_init(made.data_ptr(), (size_t)size, st); });
+  call(where, [&] { return L.cache_attention_workspace_init(made.data_ptr(), (size_t)size, st); });
   if(!once) {
     at::Tensor& held = per_stream[{d.index(), st}].cache;
     if(!held.defined() || held.numel() < size) held = made;   // (another thread may have been here meanwhile)
@@ -1502,6 +1503,172 @@ PyObject* py_cache_keep(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const On on(c.device);
   const hipStream_t st = stream_of(c.device);
   call("keepDrafts", [&] { return L.cache_keep(&c.c, lens, along, path->size(1), accepted, static_cast<int32_t*>(out.data_ptr()), st); });
+  return wrap(std::move(out));
+  MH_END
+}
+
+// verify_drafts(tokens, target, random, draft, parents, counts) -> (path, accepted, next)
+PyObject* py_verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  MH_TRY MH_ARGS(6, "verify_drafts");
+  const at::Tensor *tokens = tensor(args[0]), *target = tensor(args[1]), *random = tensor(args[2]), *draft = none(args[3]) ? nullptr : tensor(args[3]);
+  if(!tokens || !target || !random || tokens->dim() != 2 || target->dim() != 3 || !target->is_cuda() || (!none(args[3]) && !draft)) Py_RETURN_NONE;
+  const c10::Device d = target->device();
+  marian_hip_drafted x{};
+  x.sequences = tokens->size(0);
+  x.n = tokens->size(1);
+  x.vocab = target->size(2);
+  x.type = activation_type(*target);
+  auto rows = [&](const at::Tensor& t, int64_t n, int64_t (&st)[2]) {
+    if(t.size(0) != x.sequences || t.size(1) != n || t.size(2) != x.vocab || (x.vocab > 1 && t.stride(2) != 1)) return false;
+    for(int i = 0; i < 2; ++i) {
+      st[i] = t.stride(i);
+      if(t.size(i) > 1 && st[i] < 0) return false;
+    }
+    return true;
+  };
+  if(x.n < 1 || x.type < 0 || !whole_numbers(args[0], false, x.sequences, x.n, d, &x.tokens) || !rows(*target, x.n, x.target_strides) ||
+     random->scalar_type() != at::kFloat || random->device() != d || !random->is_contiguous() || random->sizes() != tokens->sizes() ||
+     !whole_numbers(args[4], true, x.sequences, x.n, d, &x.parents) || !whole_numbers(args[5], true, x.sequences, -1, d, &x.counts))
+    Py_RETURN_NONE;
+  if(draft && (draft->dim() != 3 || draft->device() != d || draft->scalar_type() != target->scalar_type() || !rows(*draft, x.n - 1, x.draft_strides)))
+    Py_RETURN_NONE;
+  x.target = target->const_data_ptr();
+  x.draft = draft && x.n > 1 ? draft->const_data_ptr() : nullptr;
+  x.random = fptr(random);
+  at::Tensor path = empty({x.sequences, x.n}, at::kInt, d), accepted = empty({x.sequences}, at::kInt, d), next = empty({x.sequences}, at::kInt, d);
+  const On on(d);
+  const hipStream_t st = stream_of(d);
+  const int64_t need = (int64_t)L.verify_drafts_workspace_bytes(x.sequences, x.vocab);
+  at::Tensor ws;
+  if(need > 0) ws = cache_workspace(need, d, st, "verifyDrafts");
+  call("verifyDrafts", [&] {
+    return L.verify_drafts(&x, static_cast<int32_t*>(path.data_ptr()), static_cast<int32_t*>(accepted.data_ptr()), static_cast<int32_t*>(next.data_ptr()),
+                           ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0, st);
+  });
+  Ref a(wrap(std::move(path))), b(wrap(std::move(accepted))), c(wrap(std::move(next)));
+  return PyTuple_Pack(3, a.p, b.p, c.p);
+  MH_END
+}
+
+// ---- a cache in pages ----------------------------------------------------------------------------
+// (table, held, free, freeCount), dense int32 on one device
+struct PageTables {
+  marian_hip_page_tables t;
+  c10::Device device{c10::kCUDA, 0};
+};
+bool tables_of(PyObject* o, PageTables& x) {
+  if(!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+  const at::Tensor* t[4];
+  for(int i = 0; i < 4; ++i) {
+    t[i] = tensor(PyTuple_GET_ITEM(o, i));
+    if(!t[i] || !t[i]->is_cuda() || t[i]->scalar_type() != at::kInt || !t[i]->is_contiguous() || t[i]->device() != t[0]->device() ||
+       t[i]->dim() != (i ? 1 : 2))
+      return false;
+  }
+  if(t[1]->size(0) != t[0]->size(0) || t[3]->size(0) != 1) return false;
+  x.t = marian_hip_page_tables{static_cast<int32_t*>(t[0]->data_ptr()), static_cast<int32_t*>(t[1]->data_ptr()), static_cast<int32_t*>(t[2]->data_ptr()),
+                               static_cast<int32_t*>(t[3]->data_ptr()), t[0]->size(0), t[0]->size(1), t[2]->size(0)};
+  x.device = t[0]->device();
+  return true;
+}
+
+// (k, v), dense, of one type and on one device
+struct PagedCache {
+  marian_hip_pages c;
+  c10::Device device{c10::kCUDA, 0};
+};
+bool pages_of(PyObject* o, PagedCache& x) {
+  if(!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2) return false;
+  const at::Tensor *k = tensor(PyTuple_GET_ITEM(o, 0)), *v = tensor(PyTuple_GET_ITEM(o, 1));
+  if(!k || !v || !k->is_cuda() || k->device() != v->device() || k->dim() != 4 || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() ||
+     !k->is_contiguous() || !v->is_contiguous())
+    return false;
+  x.c = marian_hip_pages{k->data_ptr(), v->data_ptr(), k->size(0), k->size(1), k->size(2), k->size(3), activation_type(*k)};
+  x.device = k->device();
+  return x.c.type >= 0;
+}
+
+// pages_reserve(tables, lens, n, page, counts) -> slots [sequences, n]
+PyObject* py_pages_reserve(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  MH_TRY MH_ARGS(5, "pages_reserve");
+  PageTables t;
+  const int32_t *lens, *counts;
+  if(!tables_of(args[0], t) || !whole_numbers(args[1], false, t.t.sequences, -1, t.device, &lens) ||
+     !whole_numbers(args[4], true, t.t.sequences, -1, t.device, &counts))
+    Py_RETURN_NONE;
+  const int64_t n = whole(args[2]), page = whole(args[3]);
+  if(n < 0) Py_RETURN_NONE;
+  at::Tensor slots = empty({t.t.sequences, n}, at::kInt, t.device);
+  const On on(t.device);
+  const hipStream_t st = stream_of(t.device);
+  call("reservePages", [&] { return L.pages_reserve(&t.t, lens, counts, n, page, static_cast<int32_t*>(slots.data_ptr()), st); });
+  return wrap(std::move(slots));
+  MH_END
+}
+
+// pages_trim(tables, lens, page) -> True
+PyObject* py_pages_trim(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  MH_TRY MH_ARGS(3, "pages_trim");
+  PageTables t;
+  const int32_t* lens;
+  if(!tables_of(args[0], t) || !whole_numbers(args[1], false, t.t.sequences, -1, t.device, &lens)) Py_RETURN_NONE;
+  const int64_t page = whole(args[2]);
+  const On on(t.device);
+  const hipStream_t st = stream_of(t.device);
+  call("trimPages", [&] { return L.pages_trim(&t.t, lens, page, st); });
+  return PyBool_FromLong(1);   // (None: arguments that are not in normal form)
+  MH_END
+}
+
+// pages_write(cache, k, v, slots) -> True
+PyObject* py_pages_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  MH_TRY MH_ARGS(4, "pages_write");
+  PagedCache c;
+  Rows k, v;
+  const int32_t* slots;
+  if(!pages_of(args[0], c) || !rows_of(tensor(args[1]), &c.device, k) || !rows_of(tensor(args[2]), &c.device, v) || k.type != c.c.type ||
+     v.type != c.c.type || k.t->sizes() != v.t->sizes() || k.t->size(1) != c.c.heads || k.t->size(3) != c.c.dk ||
+     !whole_numbers(args[3], false, k.t->size(0), k.t->size(2), c.device, &slots))
+    Py_RETURN_NONE;
+  const On on(c.device);
+  const hipStream_t st = stream_of(c.device);
+  call("writePages", [&] {
+    return L.pages_write(&c.c, k.t->const_data_ptr(), k.strides, v.t->const_data_ptr(), v.strides, k.t->size(0), k.t->size(2), slots, st);
+  });
+  return PyBool_FromLong(1);
+  MH_END
+}
+
+// pages_attention(q, cache, table, lens, counts, scale, out or None) -> out
+PyObject* py_pages_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  MH_TRY MH_ARGS(7, "pages_attention");
+  PagedCache c;
+  Rows q, o;
+  const at::Tensor* table = tensor(args[2]);
+  const int32_t *pages, *lens, *counts;
+  if(!pages_of(args[1], c) || !rows_of(tensor(args[0]), &c.device, q) || q.type != c.c.type || q.t->size(3) != c.c.dk || !table || table->dim() != 2)
+    Py_RETURN_NONE;
+  const int64_t sequences = q.t->size(0), q_heads = q.t->size(1), n = q.t->size(2), row = table->size(1);
+  if(!whole_numbers(args[2], false, sequences, row, c.device, &pages) || !whole_numbers(args[3], false, sequences, -1, c.device, &lens) ||
+     !whole_numbers(args[4], true, sequences, -1, c.device, &counts))
+    Py_RETURN_NONE;
+  const double scale = none(args[5]) ? 1.0 / std::pow((double)c.c.dk, 0.5) : number(args[5]);
+  at::Tensor out;
+  if(none(args[6])) {
+    out = rows_like(q, o.strides);
+  } else {
+    if(!rows_of(tensor(args[6]), &c.device, o) || o.type != q.type || o.t->sizes() != q.t->sizes()) Py_RETURN_NONE;
+    out = *o.t;
+  }
+  const On on(c.device);
+  const hipStream_t st = stream_of(c.device);
+  const int64_t need = (int64_t)L.pages_attention_workspace_bytes(sequences, c.c.heads, q_heads, n, c.c.dk, c.c.type);
+  at::Tensor ws;
+  if(need > 0) ws = cache_workspace(need, c.device, st, "AttentionOverPages");
+  call("AttentionOverPages", [&] {
+    return L.pages_attention(&c.c, pages, sequences, row, lens, counts, n, q.t->const_data_ptr(), q.strides, q_heads, (float)scale, out.data_ptr(), o.strides,
+                             ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0, st);
+  });
   return wrap(std::move(out));
   MH_END
 }
@@ -1568,6 +1735,7 @@ PyMethodDef methods[] = {
     MH_METHOD(embed), MH_METHOD(select_state), MH_METHOD(attention), MH_METHOD(attention_rows), MH_METHOD(split_heads), MH_METHOD(join_heads), MH_METHOD(proj_attention), MH_METHOD(attention_ancestors), MH_METHOD(decoder_layers),
     MH_METHOD(ancestors_advance), MH_METHOD(nbest), MH_METHOD(nbest_words), MH_METHOD(nbest_beams), MH_METHOD(logsoftmax_nbest_beams),
     MH_METHOD(rotary), MH_METHOD(cache_append), MH_METHOD(cache_read), MH_METHOD(cache_attention), MH_METHOD(cache_keep),
+    MH_METHOD(verify_drafts), MH_METHOD(pages_reserve), MH_METHOD(pages_trim), MH_METHOD(pages_write), MH_METHOD(pages_attention),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_calls", "host path of the operators", -1, methods, nullptr, nullptr, nullptr, nullptr};
