@@ -17,8 +17,8 @@
 // the next are under way with the next one's keys and values.  A page that is none, and positions past the end, are
 // read at the start of the cache (one line of memory) and weigh a selected zero: loads need no branches.
 //
-// Weights enter the product with the values in the type of the values: bfloat16 8 bits, float16 11 bits, the sum of them in
-// float32.  They are scaled by a power of two: bfloat16 and float32 2^-24, so that sums over 2^20 positions of values next to the largest stay
+// Weights enter the product with the values in the type of the values, bfloat16 and float16 in two terms, the second of what the first
+// leaves: 16 and 22 bits.  Their sum is of the float32 ones.  They are scaled by a power of two: bfloat16 and float32 2^-24, so that sums over 2^20 positions of values next to the largest stay
 // in range; float16 2^11, so that weights down to 2^-25 of the largest keep their bits.
 #pragma once
 
@@ -65,12 +65,18 @@ __device__ __forceinline__ cache_f4 pages_product(cache_u4 k, cache_u4 q, cache_
   }
 }
 
-// Whether a word of values holds an infinity or NaN.
 template <typename T>
-__device__ __forceinline__ bool pages_not_finite(unsigned w) {
-  constexpr unsigned most = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, _Float16>::value ? 0x7c00u : 0x7f80u;
-  if constexpr(sizeof(T) == 4) return (w & most) == most;
-  else return (w & most) == most || (w >> 16 & most) == most;
+__device__ __forceinline__ float pages_half(unsigned bits) {
+  const uint16_t b = (uint16_t)bits;
+  return to_float(__builtin_bit_cast(T, b));
+}
+
+// A word of values, an infinity or NaN in it as zero.
+template <typename T>
+__device__ __forceinline__ unsigned pages_finite(unsigned w) {
+  if constexpr(sizeof(T) == 4) return (w & 0x7f800000u) == 0x7f800000u ? 0 : w;
+  constexpr unsigned most = std::is_same<T, _Float16>::value ? 0x7c00u : 0x7f80u;
+  return ((w & most) == most ? 0 : w & 0xffffu) | ((w >> 16 & most) == most ? 0 : w & 0xffff0000u);
 }
 
 // The number of the page that an eight of positions is in, and the eight's place in it.
@@ -87,12 +93,11 @@ __device__ __forceinline__ PagesPlace pages_look(const PagesAttentionArgs& a, co
 // (16 (j / kTogether) + 4 g + e) kTogether + j % kTogether as o[t][j][e], unnormalized, the carried maximum and its part of the sum.
 template <typename T, int DP, int QT, int WAVES>
 __device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const CacheTile& x, const cache_f4 (&o)[QT][DP / 16], const float (&top)[QT],
-                                             float (&sum)[QT], CacheJoin<DP, QT, WAVES>& sh) {
+                                             float (&sum)[QT], int wave, CacheJoin<DP, QT, WAVES>& sh) {
   using P = Pages<T, DP>;
   constexpr int kTogether = P::kTogether, kHalf = CacheJoin<DP, QT, WAVES>::kHalf, kPieces = kHalf / (16 * kTogether);
   constexpr float kUnit = P::kUp < 0 ? (float)(1 << -P::kUp * (P::kUp < 0)) : 1.0f / (1 << P::kUp * (P::kUp > 0));   // 2^-kUp
-  const int tid = threadIdx.x, lane = tid & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
   for(int t = 0; t < QT; ++t) {
     sum[t] = over_lanes_sum(sum[t]) * kUnit;
@@ -173,21 +178,22 @@ __device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const 
   if(!out.whole) cache_join_parts<T, DP, 16 * QT, WAVES>(a, x, out, sh.parts);
 }
 
-template <typename T, int DP, int QT, int WAVES>
+template <typename T, int DP, bool WHOLE, int QT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) void pages_attention_kernel(PagesAttentionArgs a) {
   using P = Pages<T, DP>;
   constexpr int kWidth = P::kWidth, kDims = P::kDims, kTogether = P::kTogether, kKeyPieces = P::kKeyPieces, kValuePieces = P::kValuePieces;
   constexpr int kTurn = 32 * WAVES;   // positions that the waves take in one turn
+  constexpr bool kQueriesInLds = DP == 256;   // (which leaves registers to the rest)
   __shared__ CacheJoin<DP, QT, WAVES> sh;
+  __shared__ cache_u4 q_held[kQueriesInLds ? QT : 1][kKeyPieces][kQueriesInLds ? 64 : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   CacheTile x;
   if(!cache_tile<T, DP, 16 * QT, WAVES>(a, tid, x)) return;
-  const int end = x.end, row_bytes = a.dk * kWidth;
+  const int end = x.end, row_bytes = (WHOLE ? DP : a.dk) * kWidth;
   const int* const table = a.table + (long long)x.w.s * a.row;
   const unsigned char* const k_head = a.k_pages + x.head * a.head_bytes;
   const unsigned char* const v_head = a.v_pages + x.head * a.head_bytes;
-  const bool narrow = a.dk < DP;
 
   // A lane's page of the eight positions from `at` on, as an offset; whether there is one.
   auto here = [&](const PagesPlace& y, int at, bool& is) __attribute__((always_inline)) -> long long {
@@ -199,7 +205,7 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
     const unsigned char* const p = k_head + here(place, at + 8 * (c >> 2), is);
 #pragma unroll
     for(int t = 0; t < 2; ++t) {
-      const unsigned char* const key = p + ((is ? c & 3 : 0) + (is ? 4 * t : 0)) * row_bytes;
+      const unsigned char* const key = p + ((c & 3) + 4 * t) * row_bytes;
 #pragma unroll
       for(int i = 0; i < kKeyPieces; ++i) {
         const int d = 64 * i + 16 * g;
@@ -214,7 +220,7 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
 #pragma unroll
       for(int i = 0; i < kValuePieces; ++i) {
         const int d = (16 * i + c) * kTogether * kWidth;
-        const unsigned char* const from = p + (is ? e * row_bytes : 0) + (d < row_bytes ? d : 0);
+        const unsigned char* const from = p + e * row_bytes + (d < row_bytes ? d : 0);
         if constexpr(P::kWords == 4) {
           const cache_u4 w = *reinterpret_cast<const cache_u4*>(from);
 #pragma unroll
@@ -230,15 +236,15 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
   const int begin = x.w.from + 32 * wave;
   auto look_keys = [&](int at) { return pages_look(a, table, (unsigned)(at >> 3) + (c >> 2)); };
   auto look_values = [&](int at) { return pages_look(a, table, (unsigned)(at >> 3) + g); };
-  PagesPlace k_place = look_keys(begin), v_place = look_values(begin);
+  const PagesPlace k_first = look_keys(begin), v_first = look_values(begin);
   PagesPlace k_next = look_keys(begin + kTurn), v_next = look_values(begin + kTurn);
   typename P::Keys key;
   typename P::Values value;
   bool there;   // whether the lane's eight positions have a page
-  fetch_keys(key, k_place, begin);
-  fetch_values(value, v_place, begin, there);
+  fetch_keys(key, k_first, begin);
+  fetch_values(value, v_first, begin, there);
 
-  cache_u4 q[QT][kKeyPieces];
+  cache_u4 q[kQueriesInLds ? 1 : QT][kKeyPieces];
   CacheSight sight[QT];
 #pragma unroll
   for(int t = 0; t < QT; ++t) {
@@ -253,12 +259,19 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
     for(int i = 0; i < kKeyPieces; ++i) {
       const int d = 64 * i + 16 * g;
       const cache_u4 y = *reinterpret_cast<const cache_u4*>(p + (d < row_bytes ? d : 0));
-      q[t][i] = d < row_bytes ? y : cache_u4{0, 0, 0, 0};
+      const cache_u4 z = d < row_bytes ? y : cache_u4{0, 0, 0, 0};
+      if constexpr(kQueriesInLds) {
+        if(wave == t % WAVES) q_held[t][i][lane] = z;
+      } else {
+        q[t][i] = z;
+      }
     }
   }
+  if constexpr(kQueriesInLds) __syncthreads();
 
   cache_f4 o[QT][kDims];
   float top[QT], sum[QT];   // carried maximum (base 2), the lane's part of the sum
+  bool left_out = false;    // whether a value was left out of the product
 #pragma unroll
   for(int t = 0; t < QT; ++t) {
     top[t] = kNone;
@@ -268,12 +281,13 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
   }
 
   for(int at = begin; at < end; at += kTurn) {
-    if(narrow) {   // (what was loaded past a row's end is its start again)
+    if(!WHOLE) {   // (what was loaded past a row's end is its start again)
 #pragma unroll
       for(int i = 0; i < kKeyPieces; ++i)
 #pragma unroll
         for(int t = 0; t < 2; ++t) key.piece[t][i] = 64 * i + 16 * g < row_bytes ? key.piece[t][i] : cache_u4{0, 0, 0, 0};
     }
+    if constexpr(kQueriesInLds) asm volatile("" ::: "memory");   // (or they would be read ahead of all turns, into registers)
     cache_f4 s[QT][2];
 #pragma unroll
     for(int t = 0; t < QT; ++t) s[t][0] = s[t][1] = cache_f4{0, 0, 0, 0};
@@ -282,7 +296,7 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
 #pragma unroll
       for(int b = 0; b < 2; ++b)
 #pragma unroll
-        for(int t = 0; t < QT; ++t) s[t][b] = pages_product<T>(key.piece[b][i], q[t][i], s[t][b]);
+        for(int t = 0; t < QT; ++t) s[t][b] = pages_product<T>(key.piece[b][i], kQueriesInLds ? q_held[t][i][lane] : q[t][i], s[t][b]);
     fetch_keys(key, k_next, at + kTurn);
     const bool is = there;
     const bool masked = at + 32 > x.open || __any(!is);
@@ -334,8 +348,7 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
         sum[t] += p[t][e];
       }
     }
-    // Positions that some rows see and others do not: an infinity or NaN among their values is taken out of the product and
-    // added to the rows that see it.
+    // Positions that some rows see and others do not: infinities and NaN among their values stay out of the product, see below.
     if(masked && end > x.open) {
       bool odd = false;
 #pragma unroll
@@ -343,50 +356,12 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
 #pragma unroll
         for(int i = 0; i < kValuePieces; ++i)
 #pragma unroll
-          for(int w = 0; w < P::kWords; ++w) odd |= pages_not_finite<T>(value.word[e][i][w]) && first + e >= x.open;
-      if(__any(odd)) {
-#pragma unroll
-        for(int e = 0; e < 8; ++e) {
-          if(first + e >= x.open) {
-#pragma unroll
-            for(int i = 0; i < kValuePieces; ++i)
-#pragma unroll
-              for(int w = 0; w < P::kWords; ++w) {
-                unsigned& z = value.word[e][i][w];
-                if constexpr(kWidth == 4) {
-                  z = pages_not_finite<T>(z) ? 0 : z;
-                } else {
-                  const unsigned lo = z & 0xffff, hi = z & 0xffff0000u;
-                  z = (pages_not_finite<T>(lo) ? 0 : lo) | (pages_not_finite<T>(hi) ? 0 : hi);
-                }
-              }
+          for(int w = 0; w < P::kWords; ++w) {
+            const unsigned z = value.word[e][i][w], clean = first + e < x.open ? z : pages_finite<T>(z);
+            odd |= z != clean;
+            value.word[e][i][w] = clean;
           }
-        }
-#pragma unroll 1
-        for(int k = 0; k < 32; ++k) {
-          if(at + k < x.open || at + k >= end) continue;
-          const PagesPlace y = pages_look(a, table, (unsigned)(at + k) >> 3);
-          if((unsigned)y.id >= (unsigned)a.pages) continue;
-          const T* const v = reinterpret_cast<const T*>(v_head + y.id * a.page_bytes + (long long)(8 * y.eight + (k & 7)) * row_bytes);
-#pragma unroll
-          for(int t = 0; t < QT; ++t) {
-            float mine = p[t][0];
-#pragma unroll
-            for(int e = 1; e < 8; ++e) mine = (k & 7) == e ? p[t][e] : mine;
-            const float weight = __shfl(mine, c + 16 * (k >> 3), 64);
-            if(at + k < sight[t].limit) {
-#pragma unroll
-              for(int j = 0; j < kDims; ++j)
-#pragma unroll
-                for(int e = 0; e < 4; ++e) {
-                  const int d = (16 * (j / kTogether) + 4 * g + e) * kTogether + j % kTogether;
-                  const float z = d < a.dk ? to_float(v[d < a.dk ? d : 0]) : 0.0f;
-                  if(!(__builtin_fabsf(z) < __builtin_huge_valf())) o[t][j][e] += weight * z;
-                }
-            }
-          }
-        }
-      }
+      left_out |= __any(odd) != 0;
     }
     // weighted values
     if constexpr(kWidth == 4) {
@@ -398,11 +373,16 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
           for(int t = 0; t < QT; ++t)
             o[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, value.word[e][j / kTogether][j % kTogether]), p[t][e], o[t][j], 0, 0, 0);
     } else {
-      cache_u4 weights[QT];
+      cache_u4 weights[QT][2];
 #pragma unroll
       for(int t = 0; t < QT; ++t)
 #pragma unroll
-        for(int e = 0; e < 4; ++e) weights[t][e] = pack2<T>(p[t][2 * e], p[t][2 * e + 1]);
+        for(int e = 0; e < 4; ++e) {
+          const float lo = settled(p[t][2 * e]), hi = settled(p[t][2 * e + 1]);
+          const unsigned w = pack2<T>(lo, hi);
+          weights[t][0][e] = w;
+          weights[t][1][e] = pack2<T>(lo - pages_half<T>(w & 0xffff), hi - pages_half<T>(w >> 16));
+        }
 #pragma unroll
       for(int j = 0; j < kDims; ++j) {
         constexpr unsigned low = 0x05040100, high_half = 0x07060302;
@@ -412,14 +392,37 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
           d[e] = __builtin_amdgcn_perm(value.word[2 * e + 1][j / kTogether][j % kTogether / 2], value.word[2 * e][j / kTogether][j % kTogether / 2],
                                        j % 2 ? high_half : low);
 #pragma unroll
-        for(int t = 0; t < QT; ++t) o[t][j] = pages_product<T>(d, weights[t], o[t][j]);
+        for(int t = 0; t < QT; ++t)
+#pragma unroll
+          for(int m = 1; m >= 0; --m) o[t][j] = pages_product<T>(d, weights[t][m], o[t][j]);
       }
     }
     fetch_values(value, v_next, at + kTurn, there);
     k_next = look_keys(at + 2 * kTurn);
     v_next = look_values(at + 2 * kTurn);
   }
-  pages_finish<T, DP, QT, WAVES>(a, x, o, top, sum, sh);
+  // What was left out goes to the rows that see it: of any weight an infinity is one, and a NaN is one.
+  if(left_out) {
+#pragma unroll 1
+    for(int at = begin; at < end; at += kTurn)
+#pragma unroll 1
+      for(int k = max(at, x.open); k < min(at + 32, end); ++k) {
+        const PagesPlace y = pages_look(a, table, (unsigned)k >> 3);
+        if((unsigned)y.id >= (unsigned)a.pages) continue;
+        const T* const v = reinterpret_cast<const T*>(v_head + y.id * a.page_bytes + (long long)(8 * y.eight + (k & 7)) * row_bytes);
+#pragma unroll
+        for(int j = 0; j < kDims; ++j)
+#pragma unroll
+          for(int e = 0; e < 4; ++e) {
+            const int d = (16 * (j / kTogether) + 4 * g + e) * kTogether + j % kTogether;
+            const float z = to_float(v[d < a.dk ? d : 0]);
+#pragma unroll
+            for(int t = 0; t < QT; ++t)
+              if(k < sight[t].limit && d < a.dk && !(__builtin_fabsf(z) < __builtin_huge_valf())) o[t][j][e] += z;
+          }
+      }
+  }
+  pages_finish<T, DP, QT, WAVES>(a, x, o, top, sum, wave, sh);
 }
 
 }  // namespace marian_hip

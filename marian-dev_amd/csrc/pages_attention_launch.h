@@ -7,39 +7,42 @@
 
 namespace marian_hip {
 
-template <typename T, int DP, int W>
+template <typename T, int DP, bool WHOLE, int W>
 int launch_pages_attention(const PagesAttentionArgs& a, const PagesAttentionPlan& p, hipStream_t st) {
   constexpr int kMost = pages_most_qt(sizeof(T), DP);
   const dim3 grid((unsigned)p.grid), block(64 * W);
-  if(p.qt == 1) {
-    MH_LAUNCH((pages_attention_kernel<T, DP, 1, W>), grid, block, 0, st, a);
-    return MARIAN_HIP_OK;
+  if constexpr(kMost >= 4) {
+    if(p.qt == 4) {
+      MH_LAUNCH((pages_attention_kernel<T, DP, WHOLE, 4, W>), grid, block, 0, st, a);
+      return MARIAN_HIP_OK;
+    }
   }
   if constexpr(kMost >= 2) {
     if(p.qt == 2) {
-      MH_LAUNCH((pages_attention_kernel<T, DP, 2, W>), grid, block, 0, st, a);
+      MH_LAUNCH((pages_attention_kernel<T, DP, WHOLE, 2, W>), grid, block, 0, st, a);
       return MARIAN_HIP_OK;
     }
   }
-  if constexpr(kMost >= 4) {
-    if(p.qt == 4) {
-      MH_LAUNCH((pages_attention_kernel<T, DP, 4, W>), grid, block, 0, st, a);
-      return MARIAN_HIP_OK;
-    }
-  }
-  return MARIAN_HIP_ERR_SHAPE;
+  MH_LAUNCH((pages_attention_kernel<T, DP, WHOLE, 1, W>), grid, block, 0, st, a);
+  return MARIAN_HIP_OK;
 }
 
-template <typename T, int W>
+template <typename T, int DP, bool WHOLE>
 int launch_pages_attention(const PagesAttentionArgs& a, const PagesAttentionPlan& p, hipStream_t st) {
-  if(p.dp == 64) return launch_pages_attention<T, 64, W>(a, p, st);
-  if(p.dp == 128) return launch_pages_attention<T, 128, W>(a, p, st);
-  return launch_pages_attention<T, 256, W>(a, p, st);
+  return p.waves == 1 ? launch_pages_attention<T, DP, WHOLE, 1>(a, p, st) : launch_pages_attention<T, DP, WHOLE, 4>(a, p, st);
+}
+
+// WHOLE: rows of dp values; their places are constants then.
+template <typename T, int DP>
+int launch_pages_attention(const PagesAttentionArgs& a, const PagesAttentionPlan& p, hipStream_t st) {
+  return a.dk == DP ? launch_pages_attention<T, DP, true>(a, p, st) : launch_pages_attention<T, DP, false>(a, p, st);
 }
 
 template <typename T>
 int launch_pages_attention(const PagesAttentionArgs& a, const PagesAttentionPlan& p, hipStream_t st) {
-  return p.waves == 1 ? launch_pages_attention<T, 1>(a, p, st) : launch_pages_attention<T, 4>(a, p, st);
+  if(p.dp == 64) return launch_pages_attention<T, 64>(a, p, st);
+  if(p.dp == 128) return launch_pages_attention<T, 128>(a, p, st);
+  return launch_pages_attention<T, 256>(a, p, st);
 }
 
 }  // namespace marian_hip

@@ -9,13 +9,18 @@
 
 namespace marian_hip {
 
-// Sixteens of query rows that a wave takes over the same positions, at the most: what 512 registers hold beside 32 positions' keys and values.
+// Registers of a form (an estimate).
+constexpr int pages_registers(int width, int dp, int qt) {
+  const int words = width * dp / 8;   // of keys and of values, each: 32 positions' bytes over 64 lanes
+  return 2 * words + qt * (dp / 4 + words / 2 + 16) + 48;   // results, queries, scores and weights; addresses
+}
+
+// Sixteens of query rows that a wave takes over the same positions, at the most.
 constexpr int pages_most_qt(int width, int dp) { return width == 4 ? (dp == 256 ? 1 : 2) : dp == 256 ? 2 : 4; }
 
 // Waves of a form that fit a SIMD, by its registers.
 constexpr int pages_to_a_simd(int width, int dp, int qt) {
-  const int words = width * dp / 8;   // of keys and of values, each: 32 positions' bytes over 64 lanes
-  const int all = 2 * words + qt * (dp / 4 + words / 2 + 16) + 40;   // results, queries, scores and weights; addresses
+  const int all = pages_registers(width, dp, qt);
   return all <= 128 ? 4 : all <= 168 ? 3 : all <= 256 ? 2 : 1;
 }
 
@@ -23,6 +28,7 @@ struct PagesAttentionPlan {
   int dp;              // values of a row as the kernel holds it: dk rounded up to 64, 128 or 256
   int qt;              // sixteens of query rows to a workgroup
   int waves;           // of a workgroup, which share its rows and take turns of 32 positions
+  int tile_rows;       // of a workgroup
   int64_t row_tiles;   // workgroups that share an entry's positions
   int least;           // blocks of a part
   int64_t target;      // parts that the positions of all sequences together are split into
@@ -36,7 +42,8 @@ inline PagesAttentionPlan pages_attention_plan(int64_t sequences, int64_t heads,
   p.dp = dk <= 64 ? 64 : dk <= 128 ? 128 : 256;
   const int64_t rows = n * (q_heads / heads);
   p.qt = std::min(rows <= 16 ? 1 : rows <= 32 ? 2 : 4, pages_most_qt(width, p.dp));
-  p.row_tiles = (rows + 16 * p.qt - 1) / (16 * p.qt);
+  p.tile_rows = 16 * p.qt;
+  p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const int64_t entries = sequences * heads * p.row_tiles;
   p.waves = entries >= 4096 ? 1 : 4;
   const int64_t at_a_time = 1024 * pages_to_a_simd(width, p.dp, p.qt) / p.waves;
@@ -50,7 +57,7 @@ inline PagesAttentionPlan pages_attention_plan(int64_t sequences, int64_t heads,
 
 // The workspace: counters as in that of the attention over a quantized cache, then the partial results: rows of dp values and a logarithm.
 inline int64_t pages_attention_bytes(const PagesAttentionPlan& p, int64_t heads) {
-  return p.slots == 0 ? 0 : kCacheCounterBytes + p.slots * heads * p.row_tiles * 16 * p.qt * (p.dp + 1) * 4;
+  return p.slots == 0 ? 0 : kCacheCounterBytes + p.slots * heads * p.row_tiles * p.tile_rows * (p.dp + 1) * 4;
 }
 
 }  // namespace marian_hip
