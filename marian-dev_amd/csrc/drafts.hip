@@ -20,13 +20,42 @@ struct VerifyArgs {
   long long t_s, t_n, d_s, d_n;   // values from a sequence and a row of the target's and the draft's to the next
   int *path, *accepted, *next;
   unsigned* counters;
-  double* sums;   // of what is drawn from, and of the target's row, of every part
+  double* sums;   // of what is drawn from, of every share
   int n, vocab, parts;
 };
 
-constexpr int kVerifyThreads = 256, kEach = 16;            // words of a thread
-constexpr int kVerifyPart = kVerifyThreads * kEach;        // ... and of a workgroup
+// Eight waves: a sequence's workgroups judge its tokens each, ahead of all else, and a workgroup's words are summed in 64 bits, five operations a
+// word. With 4, 8 and 16 of them 32000 words of one sequence take 5.7, 6.3 and 9.1 us, 131071 words of 64 sequences 44.0, 20.2 and 22.0.
+constexpr int kVerifyWaves = 8, kVerifyThreads = 64 * kVerifyWaves;
+constexpr int kShare = 2 * kVerifyThreads;                 // words of a wave ...
+constexpr int kVerifyPart = kVerifyWaves * kShare;         // ... and of a workgroup
 constexpr int64_t kVerifySequences = kCacheMost;           // of a launch: a counter each
+
+// x of the lane that a control of lane movement says, zero where there is none.
+template <int CONTROL, int ROWS, bool ZERO>
+__device__ __forceinline__ double moved(double x) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, x);
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, CONTROL, ROWS, 0xf, ZERO);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CONTROL, ROWS, 0xf, ZERO);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+// Inclusive sum over the lanes of a wave: within rows of sixteen lanes, then over the rows, without LDS.
+__device__ __forceinline__ double lanes_sum(double x) {
+  x += moved<0x111, 0xf, true>(x);    // row_shr:1
+  x += moved<0x112, 0xf, true>(x);    // row_shr:2
+  x += moved<0x114, 0xf, true>(x);    // row_shr:4
+  x += moved<0x118, 0xf, true>(x);    // row_shr:8
+  x += moved<0x142, 0xa, false>(x);   // row_bcast:15
+  x += moved<0x143, 0xc, false>(x);   // row_bcast:31
+  return x;
+}
+
+// What became of a sequence's tokens: a bit for each kept one, the last of these, and the ones refused as its children.
+struct Verdict {
+  unsigned long long kept, refused;
+  int last;
+  int token[64];
+};
 
 __device__ __forceinline__ double lane_double(double x, int lane) {
   const unsigned long long b = __builtin_bit_cast(unsigned long long, x);
@@ -34,262 +63,278 @@ __device__ __forceinline__ double lane_double(double x, int lane) {
   return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
 
-// A probability as it counts: nothing where it is below zero or NaN.
-__device__ __forceinline__ double counted(double x) { return x > 0.0 ? x : 0.0; }
-
-// What became of a sequence's tokens: a bit for each kept one, the last of these, and the ones refused as its children.
-struct Verdict {
-  unsigned long long kept, refused;
-  int last, token;   // token: the lane's
-};
-
-// All waves do the same, lanes being tokens.  A token is judged as if its parent were kept - the row that it is held against is known -,
-// and is kept if all that it descends from are.
+// A wave's work, lanes being tokens.  The row that a token is held against is its parent's, so all probabilities are asked for at once; then the
+// kept tokens are followed from the first on.
 template <typename T>
-__device__ __forceinline__ Verdict judge(const VerifyArgs& a, int s, int lane, int count) {
+__device__ __forceinline__ void judge(const VerifyArgs& a, int s, int lane, int count, Verdict& y) {
   const long long at = (long long)s * a.n + lane;
-  const bool there = lane < count;
-  Verdict y;
-  y.token = there ? a.tokens[at] : -1;
-  int parent = !there || !a.parents ? lane - 1 : a.parents[at];
+  const bool inside = lane < a.n, there = lane < count;
+  const int token = inside ? a.tokens[at] : -1;   // (asked for beside the count)
+  int parent = !inside || !a.parents ? lane - 1 : a.parents[at];
+  const double u = inside ? a.random[at] : 0.0;
   if(parent >= lane || parent < 0) parent = -1;
-  const bool judged = there && parent >= 0 && (unsigned)y.token < (unsigned)a.vocab;
+  const bool judged = inside && parent >= 0 && (unsigned)token < (unsigned)a.vocab;
   double p = 0.0, q = 1.0;
-  if(judged) p = counted(to_float(static_cast<const T*>(a.target)[s * a.t_s + parent * a.t_n + y.token]));
-  if(judged && a.draft) q = to_float(static_cast<const T*>(a.draft)[s * a.d_s + parent * a.d_n + y.token]);
-  const double u = there ? a.random[at] : 0.0;
-  unsigned long long siblings = 0;   // that come before
-  double gone = 0.0;                 // their probabilities
-  if(a.parents) {
-    for(int j = 1; j < count; ++j) {
-      const double pj = lane_double(p, j);   // (by now without what a sibling had already)
-      const int parent_j = __builtin_amdgcn_readlane(parent, j), token_j = __builtin_amdgcn_readlane(y.token, j);
-      if(lane > j && parent == parent_j) {
-        siblings |= 1ull << j;
-        if(y.token == token_j) p = 0.0;
-        gone += pj;
-      }
-    }
+  if(judged) {
+    p = fmaxf(to_float(static_cast<const T*>(a.target)[s * a.t_s + parent * a.t_n + token]), 0.0f);
+    if(a.draft) q = fmaxf(to_float(static_cast<const T*>(a.draft)[s * a.d_s + parent * a.d_n + token]), 0.0f);
   }
-  const bool likes = judged && u * (a.draft ? q : 1.0 - gone) < p;
-  const unsigned long long liked = __ballot(likes), chosen = __ballot(likes && !(liked & siblings));
+  unsigned long long kept = count > 0, refused = 0;
+  int last = 0;
   if(a.parents) {
-    int up = parent;
-    unsigned long long line = 1ull << lane;   // itself and what it descends from
-    while(__any(up >= 0)) {   // (a parent is before its child: six rounds at the most, each twice as far up)
-      const unsigned lo = __shfl((unsigned)line, up & 63, 64), hi = __shfl((unsigned)(line >> 32), up & 63, 64);
-      const int next = __shfl(up, up & 63, 64);
-      if(up >= 0) {
-        line |= (unsigned long long)hi << 32 | lo;
-        up = next;
+    for(;;) {
+      unsigned long long children = __ballot(there && parent == last);
+      double gone = 0.0;
+      int next = 0;
+      for(refused = 0; children && !next; children &= children - 1) {
+        const int i = __builtin_ctzll(children);
+        const unsigned long long alike = __ballot(token == __builtin_amdgcn_readlane(token, i));
+        const double its = alike & refused ? 0.0 : lane_double(p, i);   // (a token that a sibling had already has nothing left)
+        if(lane_double(u, i) * (1.0 - gone) < its) {
+          next = i;
+        } else {
+          refused |= 1ull << i;
+          gone += its;
+        }
       }
+      if(!next) break;
+      kept |= 1ull << next;
+      last = next;
     }
-    y.kept = __ballot(there && (line & 1) && !(line & ~1ull & ~chosen));
   } else {
-    const int row = __builtin_ctzll(~(chosen >> 1));   // (the shift leaves a zero on top)
-    y.kept = count > 0 ? (2ull << row) - 1 : 0;
+    const unsigned long long likes = __ballot(there && u * q < p);
+    last = __builtin_ctzll(~(likes >> 1));   // (the shift leaves a zero on top)
+    kept = count > 0 ? (2ull << last) - 1 : 0;
+    refused = last + 1 < count ? 2ull << last : 0;
   }
-  y.last = y.kept ? 63 - __builtin_clzll(y.kept) : 0;
-  y.refused = __ballot(there && lane > 0 && parent == y.last) & ~y.kept;
-  return y;
+  y.token[lane] = token;
+  if(lane == 0) {
+    y.kept = kept;
+    y.refused = refused;
+    y.last = last;
+  }
 }
 
-// What the next token is drawn from: words of the target's row, less the draft's or the refused words.
+// What the next token is drawn from: words of the target's row, less the draft's or the refused words.  Negative numbers and NaN count as nothing.
 template <typename T>
 struct Weights {
-  static constexpr int kTogether = 16 / sizeof(T), kVectors = kEach / kTogether;
+  static constexpr int kTogether = 16 / sizeof(T);
   const T *p, *q;   // q null: not taken away
-  const Verdict& y;
+  const int* token;
   int vocab;
-  // A vector of words from `at` on: what is left, and the target's own.
-  __device__ __forceinline__ void load(int at, double (&left)[kTogether], double (&own)[kTogether]) const {
+  struct Raw {
     T x[kTogether], z[kTogether];
-    const bool whole = at + kTogether <= vocab;
-    if(whole) {
-      __builtin_memcpy(x, p + at, 16);
-      if(q) __builtin_memcpy(z, q + at, 16);
-    }
+  };
+  // Sixteen bytes of words from `at` on; WHOLE: all of them are there.
+  template <bool WHOLE>
+  __device__ __forceinline__ void fetch(Raw& r, int at) const {
+    if constexpr(WHOLE) {
+      __builtin_memcpy(r.x, p + at, 16);
+      if(q) __builtin_memcpy(r.z, q + at, 16);
+    } else {
 #pragma unroll
-    for(int e = 0; e < kTogether; ++e) {
-      const bool is = at + e < vocab;
-      if(!whole && is) {
-        x[e] = p[at + e];
-        if(q) z[e] = q[at + e];
+      for(int e = 0; e < kTogether; ++e) {
+        r.x[e] = at + e < vocab ? p[at + e] : T{};
+        if(q) r.z[e] = at + e < vocab ? q[at + e] : T{};
       }
-      own[e] = is ? counted(to_float(x[e])) : 0.0;
-      left[e] = is && q ? counted((double)to_float(x[e]) - (double)to_float(z[e])) : own[e];
     }
   }
-  // ... without the refused words among `size` from `from` on.
+  // (Differences of two numbers of up to 24 bits and their sums are taken in 64 bits.  A maximum with zero leaves NaN out.)
   template <int COUNT>
-  __device__ __forceinline__ void refuse(double (&left)[COUNT], int at) const {
+  __device__ __forceinline__ void weigh(const T (&x)[COUNT], const T (&z)[COUNT], int at, unsigned long long refused, double (&left)[COUNT]) const {
+#pragma unroll
+    for(int e = 0; e < COUNT; ++e) {
+      const float own = fmaxf(to_float(x[e]), 0.0f);
+      left[e] = q ? fmax((double)own - (double)fmaxf(to_float(z[e]), 0.0f), 0.0) : (double)own;
+    }
 #pragma unroll 1
-    for(unsigned long long bits = q ? 0 : y.refused; bits; bits &= bits - 1) {
-      const int word = __builtin_amdgcn_readlane(y.token, __builtin_ctzll(bits)) - at;
+    for(; refused; refused &= refused - 1) {
+      const int word = token[__builtin_ctzll(refused)] - at;
 #pragma unroll
       for(int e = 0; e < COUNT; ++e) left[e] = word == e ? 0.0 : left[e];
     }
   }
-};
-
-__device__ __forceinline__ double wave_sum_before(double x, int lane, double& all) {   // exclusive, in the lanes' order
-  double sum = x;
+  // Words at and at + 1.
+  __device__ __forceinline__ void two(int at, unsigned long long refused, double (&left)[2]) const {
+    T x[2], z[2];
 #pragma unroll
-  for(int o = 1; o < 64; o <<= 1) {
-    const double other = __shfl_up(sum, o, 64);
-    if(lane >= o) sum += other;
+    for(int e = 0; e < 2; ++e) {
+      x[e] = at + e < vocab ? p[at + e] : T{};
+      z[e] = q && at + e < vocab ? q[at + e] : T{};
+    }
+    weigh(x, z, at, refused, left);
   }
-  all = lane_double(sum, 63);
-  const double before = __shfl_up(sum, 1, 64);
-  return lane == 0 ? 0.0 : before;
-}
+};
 
 struct VerifyShared {
-  double wave[2][kVerifyThreads / 64];
-  double before;
-  int found, last, is_last;
+  Verdict verdict;
+  double wave[kVerifyWaves], share[kVerifyWaves];
+  double before, bar;
+  int found, is_last;
 };
 
-// The exclusive sum over a workgroup's threads, and the sum of all; `which`: a place in LDS that nobody reads any more.
-__device__ __forceinline__ double group_sum_before(VerifyShared& sh, int which, double x, double& all) {
-  const int tid = threadIdx.x, wave = tid >> 6;
-  double mine, before = wave_sum_before(x, tid & 63, mine);
-  if((tid & 63) == 0) sh.wave[which][wave] = mine;
+// The sum of a share that a workgroup's threads have two words each of; in the end all have read it.
+__device__ __forceinline__ double share_sum(VerifyShared& sh, double x) {
+  const double sum = lanes_sum(x);
+  if((threadIdx.x & 63) == 63) sh.wave[threadIdx.x >> 6] = sum;
   __syncthreads();
-  double ahead = 0.0;
-  all = 0.0;
+  double all = 0.0;
 #pragma unroll
-  for(int i = 0; i < kVerifyThreads / 64; ++i) {
-    if(i == wave) ahead = all;
-    all += sh.wave[which][i];
-  }
-  return ahead + before;
+  for(int i = 0; i < kVerifyWaves; ++i) all += sh.wave[i];
+  __syncthreads();
+  return all;
 }
 
-// Every workgroup judges the tokens of a sequence anew - a chain of three loads - and sums its part of the words that the next token is drawn from; the
-// last one to arrive finds the part in which the drawn number lies, and the word in it.  All sums are in 64 bits and in the words' order.
+// A workgroup judges the tokens of a sequence - a chain of three loads - and sums a part of the words that the next token is drawn from, a share
+// to each wave.  The last workgroup of a sequence finds the share in which the drawn number lies, and the word in it.  All sums are in 64
+// bits and in an order of their own, whoever comes last.
 // The kept tokens cost nothing but their own probabilities, so what moves is one row of the target's, and one of the draft's where a
-// token was refused.
+// token was refused.  64 sequences, 131071 words, float32: 20.2 us, 3.3 TB/s; their bytes take 13 us, the judgement ahead of them and the join
+// behind them the rest.  32000 words of one sequence: 6.3 us, a chain of some nine steps through memory.
 template <typename T>
 __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a, int first) {
   using W = Weights<T>;
-  constexpr int kTogether = W::kTogether, kVectors = W::kVectors;
+  constexpr int kTogether = W::kTogether, kTurns = kShare / (64 * kTogether);
   __shared__ VerifyShared sh;
-  const int tid = threadIdx.x, lane = tid & 63, s = first + blockIdx.y, part = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), s = first + blockIdx.y, part = blockIdx.x;
   const int count = a.counts ? clamp_int(a.counts[s], 0, a.n) : a.n;
-  const Verdict y = judge<T>(a, s, lane, count);
   const double u = a.random[(long long)s * a.n];
-  if(part == 0 && tid < 64) {
-    const int accepted = __builtin_popcountll(y.kept);
-    const long long row = (long long)s * a.n;
-    if(lane < a.n && lane >= accepted) a.path[row + lane] = -1;
-    if(y.kept >> lane & 1) a.path[row + __builtin_popcountll(y.kept & ((1ull << lane) - 1))] = lane;
+  if(wave == 0) judge<T>(a, s, lane, count, sh.verdict);
+  __syncthreads();
+  const unsigned long long kept = sh.verdict.kept, refused = sh.verdict.refused;
+  const int row = sh.verdict.last;
+  if(part == 0 && wave == 0) {
+    const int accepted = __builtin_popcountll(kept);
+    const long long to = (long long)s * a.n;
+    if(lane < a.n && lane >= accepted) a.path[to + lane] = -1;
+    if(kept >> lane & 1) a.path[to + __builtin_popcountll(kept & ((1ull << lane) - 1))] = lane;
     if(lane == 0) a.accepted[s] = accepted;
     if(lane == 0 && count == 0) a.next[s] = -1;
   }
   if(count == 0) return;
-  const W w{static_cast<const T*>(a.target) + s * a.t_s + y.last * a.t_n,
-            a.draft && y.refused ? static_cast<const T*>(a.draft) + s * a.d_s + y.last * a.d_n : nullptr, y, a.vocab};
-  if(tid == 0) {
-    sh.found = 0x7fffffff;
-    sh.last = -1;
-  }
-  const int from = part * kVerifyPart;
-  double left_sum = 0.0, own_sum = 0.0;
-  {
-    double left[kVectors][kTogether], own[kVectors][kTogether];
+  W w{static_cast<const T*>(a.target) + s * a.t_s + row * a.t_n,
+      a.draft && refused ? static_cast<const T*>(a.draft) + s * a.d_s + row * a.d_n : nullptr, sh.verdict.token, a.vocab};
+  // The refused words among a share's.
+  auto refused_in = [&](int share) {
+    return a.draft ? 0 : refused & __ballot((unsigned)(sh.verdict.token[lane] - share * kShare) < (unsigned)kShare);
+  };
+  const int mine = part * kVerifyWaves + wave, from = mine * kShare, shares = (a.vocab + kShare - 1) / kShare;
+  double sum = 0.0;
+  if(from < a.vocab) {
+    const unsigned long long out = refused_in(mine);
+    auto add = [&](const typename W::Raw& raw, int at) __attribute__((always_inline)) {
+      double left[kTogether];
+      w.weigh(raw.x, raw.z, at, out, left);
 #pragma unroll
-    for(int v = 0; v < kVectors; ++v) w.load(from + (v * kVerifyThreads + tid) * kTogether, left[v], own[v]);
-#pragma unroll
-    for(int v = 0; v < kVectors; ++v) {
-      w.refuse(left[v], from + (v * kVerifyThreads + tid) * kTogether);
-#pragma unroll
-      for(int e = 0; e < kTogether; ++e) {
-        left_sum += left[v][e];
-        own_sum += own[v][e];
-      }
-    }
-  }
-  double left_all, own_all;
-  group_sum_before(sh, 0, left_sum, left_all);
-  group_sum_before(sh, 1, own_sum, own_all);
-  int found_part = 0;
-  double ahead = 0.0;   // of the part that the word is in
-  if(a.parts > 1) {
-    unsigned long long* const sums = reinterpret_cast<unsigned long long*>(a.sums) + 2 * (long long)blockIdx.y * a.parts;
-    if(tid == 0) {
-      __hip_atomic_store(sums + 2 * part, __builtin_bit_cast(unsigned long long, left_all), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __hip_atomic_store(sums + 2 * part + 1, __builtin_bit_cast(unsigned long long, own_all), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    if(!cache_arrived_last(a.counters + blockIdx.y, a.parts, sh.is_last)) return;
-    const int each = (a.parts + kVerifyThreads - 1) / kVerifyThreads, i0 = tid * each, i1 = min(i0 + each, a.parts);
-    auto sum_of = [&](int i, int which) {
-      return __builtin_bit_cast(double, __hip_atomic_load(sums + 2 * i + which, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+      for(int e = 0; e < kTogether; ++e) sum += left[e];
     };
-    double mine[2] = {0.0, 0.0};
-    for(int i = i0; i < i1; ++i) {
-      mine[0] += sum_of(i, 0);
-      mine[1] += sum_of(i, 1);
-    }
-    double before = group_sum_before(sh, 0, mine[0], left_all);
-    const double before_own = group_sum_before(sh, 1, mine[1], own_all);
-    const int which = left_all > 0.0 ? 0 : 1;
-    if(which) before = before_own;
-    const double bar = u * (which ? own_all : left_all);
-    double sum = before;
-    for(int i = i0; i < i1; ++i) {
-      const double x = sum_of(i, which);
-      sum += x;
-      if(x > 0.0) atomicMax(&sh.last, i);
-      if(x > 0.0 && sum > bar) {
-        atomicMin(&sh.found, i);
-        break;
+    if(from + kShare <= a.vocab) {   // (all are asked for at once)
+      typename W::Raw raw[kTurns];
+#pragma unroll
+      for(int i = 0; i < kTurns; ++i) w.template fetch<true>(raw[i], from + (i * 64 + lane) * kTogether);
+#pragma unroll
+      for(int i = 0; i < kTurns; ++i) add(raw[i], from + (i * 64 + lane) * kTogether);
+    } else {
+#pragma unroll 1
+      for(int at = from + lane * kTogether; at < a.vocab; at += 64 * kTogether) {
+        typename W::Raw raw;
+        w.template fetch<false>(raw, at);
+        add(raw, at);
       }
     }
+    sum = lanes_sum(sum);
+  }
+  unsigned long long* const sums = reinterpret_cast<unsigned long long*>(a.sums) + (long long)blockIdx.y * shares;
+  if(a.parts == 1) {
+    if(lane == 63) sh.share[wave] = sum;
     __syncthreads();
-    // (rounding may leave none where the drawn number is next to one: the last that has anything)
-    found_part = sh.found != 0x7fffffff ? sh.found : max(sh.last, 0);
-    if(found_part >= i0 && found_part < i1) {
-      for(int i = i0; i < found_part; ++i) before += sum_of(i, which);
+  } else {
+    if(lane == 63 && from < a.vocab)
+      __hip_atomic_store(sums + mine, __builtin_bit_cast(unsigned long long, sum), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if(!cache_arrived_last(a.counters + blockIdx.y, a.parts, sh.is_last)) return;
+  }
+  // The share: the first one up to which the sum is above u of all (rounding may leave none where u is next to one: the last that has anything).
+  if(wave == 0) {
+    auto sum_of = [&](int i) {
+      return a.parts == 1 ? sh.share[i] : __builtin_bit_cast(double, __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    };
+    const int each = (shares + 63) / 64, i0 = min(lane * each, shares), i1 = min(i0 + each, shares);
+    double some = 0.0;
+    for(int i = i0; i < i1; ++i) some += sum_of(i);
+    const double upto = lanes_sum(some), bar = u * lane_double(upto, 63), shifted = __shfl_up(upto, 1, 64);
+    const unsigned long long above = __ballot(some > 0.0 && upto > bar), any = __ballot(some > 0.0);
+    const int l = above ? __builtin_ctzll(above) : any ? 63 - __builtin_clzll(any) : -1;
+    if(l < 0 ? lane == 0 : lane == l) {
+      double running = lane == 0 ? 0.0 : shifted, before = running;
+      int found = l < 0 ? -1 : i0;
+      for(int i = i0; i < i1 && l >= 0; ++i) {
+        const double x = sum_of(i);
+        if(x > 0.0) {
+          found = i;
+          before = running;
+          if(running + x > bar) break;
+        }
+        running += x;
+      }
+      sh.found = found;
       sh.before = before;
-    }
-    __syncthreads();
-    ahead = sh.before;
-    if(tid == 0) {
-      sh.found = 0x7fffffff;
-      sh.last = -1;
-    }
-    __syncthreads();
-  }
-  const bool of_left = left_all > 0.0;
-  const double bar = u * (of_left ? left_all : own_all);
-  // sixteen words that follow each other to a thread
-  const int at = found_part * kVerifyPart + tid * kEach;
-  double x[kEach], sum = 0.0;
-#pragma unroll
-  for(int v = 0; v < kVectors; ++v) {
-    double left[kTogether], own[kTogether];
-    w.load(at + v * kTogether, left, own);
-    w.refuse(left, at + v * kTogether);
-#pragma unroll
-    for(int e = 0; e < kTogether; ++e) {
-      x[v * kTogether + e] = of_left ? left[e] : own[e];
-      sum += x[v * kTogether + e];
+      sh.bar = bar;
     }
   }
-  double all;
-  double running = ahead + group_sum_before(sh, 0, sum, all);
-  int found = 0x7fffffff, last = -1;
-#pragma unroll
-  for(int e = 0; e < kEach; ++e) {
-    running += x[e];
-    if(x[e] > 0.0) last = at + e;
-    if(x[e] > 0.0 && running > bar && found == 0x7fffffff) found = at + e;
-  }
-  if(found != 0x7fffffff) atomicMin(&sh.found, found);
-  if(last >= 0) atomicMax(&sh.last, last);
   __syncthreads();
-  if(tid == 0) a.next[s] = sh.found != 0x7fffffff ? sh.found : sh.last;
+  int share = sh.found;
+  double before = sh.before, bar = sh.bar;
+  if(share < 0) {
+    // Nothing is left: the target's own probabilities, summed anew by this workgroup, twice (to be seen only where the draft was not drawn from
+    // its distribution, or probabilities are none).
+    w.q = nullptr;
+    double all = 0.0, left[2];
+    for(int i = 0; i < shares; ++i) {
+      w.two(i * kShare + 2 * tid, 0, left);
+      all += share_sum(sh, left[0] + left[1]);
+    }
+    bar = u * all;
+    double running = 0.0;
+    for(int i = 0; i < shares; ++i) {
+      w.two(i * kShare + 2 * tid, 0, left);
+      const double x = share_sum(sh, left[0] + left[1]);
+      if(x > 0.0) {
+        share = i;
+        before = running;
+        if(running + x > bar) break;
+      }
+      running += x;
+    }
+    if(share < 0) {
+      if(tid == 0) a.next[s] = -1;
+      return;
+    }
+  }
+  // The word, likewise: two that follow each other to a thread.
+  const int at = share * kShare + 2 * tid;
+  double left[2];
+  w.two(at, sh.found < 0 ? 0 : refused_in(share), left);
+  const double upto = lanes_sum(left[0] + left[1]), shifted = __shfl_up(upto, 1, 64);
+  if(lane == 63) sh.wave[wave] = upto;
+  __syncthreads();
+  double ahead = before, running = before;
+  int here = -1;
+#pragma unroll
+  for(int i = 0; i < kVerifyWaves; ++i) {
+    const double x = sh.wave[i];
+    const bool passed = here >= 0 && running > bar;
+    if(x > 0.0 && !passed) {
+      here = i;
+      ahead = running;
+    }
+    if(!passed) running += x;
+  }
+  if(wave != here) return;
+  const double start = lane == 0 ? ahead : ahead + shifted;
+  const bool zero = left[0] > 0.0 && start + left[0] > bar, one = left[1] > 0.0 && start + left[0] + left[1] > bar;
+  const unsigned long long hits = __ballot(zero || one), any = __ballot(left[0] > 0.0 || left[1] > 0.0);
+  const int l = hits ? __builtin_ctzll(hits) : 63 - __builtin_clzll(any);
+  if(lane == l) a.next[s] = hits ? (zero ? at : at + 1) : left[1] > 0.0 ? at + 1 : at;
 }
 
 }  // namespace
@@ -298,7 +343,7 @@ extern "C" {
 
 size_t marian_hip_verify_drafts_workspace_bytes(int64_t sequences, int64_t vocab) {
   if(sequences < 1 || vocab < 1 || sequences > kMaxSequences || vocab >= 1 << 24 || vocab <= kVerifyPart) return 0;
-  return (size_t)(kCacheCounterBytes + std::min(sequences, kVerifySequences) * ((vocab + kVerifyPart - 1) / kVerifyPart) * 16);
+  return (size_t)(kCacheCounterBytes + std::min(sequences, kVerifySequences) * ((vocab + kShare - 1) / kShare) * 8);
 }
 
 int marian_hip_verify_drafts(const marian_hip_drafted* d, int32_t* path, int32_t* accepted, int32_t* next, void* workspace, size_t workspace_bytes,

@@ -115,7 +115,7 @@ def verify(tokens, target, random, draft=None, parents=None, counts=None):
                 continue
             t, u = int(tokens[s][i]), float(random[s][i])
             p = float(mass(target[s, here, t].double())) if 0 <= t < vocab and t not in refused else 0.0
-            q = 1.0 - gone if draft is None else float(draft[s, here, t]) if 0 <= t < vocab else 1.0
+            q = 1.0 - gone if draft is None else float(mass(draft[s, here, t].double())) if 0 <= t < vocab else 1.0
             if p > 0:
                 near = min(near, abs(u * q - p) / p)
             if u * q < p:
@@ -127,7 +127,7 @@ def verify(tokens, target, random, draft=None, parents=None, counts=None):
         own = mass(target[s, here].double())
         left = own.clone()
         if refused and draft is not None:
-            left = mass(target[s, here].double() - draft[s, here].double())
+            left = mass(own - mass(draft[s, here].double()))
         elif refused:
             for t in refused:
                 if 0 <= t < vocab:

@@ -14,7 +14,7 @@ import pages_oracle as oracle
 from conftest import PKG, ROOT, load
 
 GB = 1 << 30
-S, H, HQ, N, PAGES, PAGE, ROW, DK, VOCAB = 3, 2, 4, 5, 12, 16, 4, 64, 5000
+S, H, HQ, N, PAGES, PAGE, ROW, DK, VOCAB = 3, 2, 4, 5, 12, 16, 4, 64, 50000
 NAMES = ("k", "v", "table", "held", "free", "count", "lens", "counts", "slots", "xk", "xv", "xq", "qo", "ws", "tokens", "parents", "target", "draft", "random",
          "path", "accepted", "next")
 PLACES = {n: (i + 1) * GB for i, n in enumerate(NAMES)}

@@ -57,6 +57,7 @@ def check(tokens, target, numbers, draft=None, parents=None, counts=None, on_gpu
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("form", ["drawn", "best", "tree"])
 @pytest.mark.parametrize("S,n,vocab", [(1, 1, 1), (1, 1, 7), (5, 2, 2), (7, 4, 33), (3, 64, 100), (9, 6, 1000), (4, 5, 4095), (4, 5, 4096), (4, 5, 4097),
+                                       (4, 5, 1023), (4, 5, 1024), (4, 5, 1025), (3, 5, 8191), (3, 5, 8192), (3, 5, 8193), (2, 4, 32767), (2, 4, 32768), (2, 4, 32769), (1, 4, 65537),
                                        (2, 3, 50001), (1, 5, 131071)])
 def test_verified(dtype, form, S, n, vocab):
     x = inputs(S + n + vocab, S, n, vocab, dtype, form)
@@ -72,7 +73,12 @@ def test_verified(dtype, form, S, n, vocab):
 
 
 def test_more_sequences_than_counters():
+    torch.manual_seed(3)
     check(*inputs(1, 9000, 2, 4100, BF16, "best"))
+    _, target, _, _, _ = inputs(2, 1, 2, 33000, F16, "best")
+    tokens, numbers = torch.randint(0, 33000, (9000, 2), dtype=torch.int32), torch.rand(9000, 2)
+    tokens[:, 1] = target[0, 0].argmax()
+    check(tokens, target.expand(9000, 2, 33000), numbers, on_gpu=target.cuda().expand(9000, 2, 33000))
 
 
 def test_certain_and_impossible_tokens():
@@ -102,7 +108,7 @@ def test_certain_and_impossible_tokens():
 
 def test_what_is_no_probability_counts_as_none():
     kv = load("cache")
-    for vocab in (100, 9000):
+    for vocab in (100, 9000, 40000):
         target = torch.zeros(4, 2, vocab)
         target[0, 0, 3] = float("nan")
         target[0, 0, 4] = 0.5
@@ -113,6 +119,18 @@ def test_what_is_no_probability_counts_as_none():
         target[3, 0, 8] = float("inf")
         got = kv.verifyDrafts(ints([[0, 3]] * 4), target.cuda(), torch.full((4, 2), 0.3).cuda())
         assert 0 <= got[2][3].item() < vocab
+
+
+@pytest.mark.parametrize("vocab", [40, 5000, 40000])
+def test_a_draft_that_is_no_distribution(vocab):
+    """Nothing left of the target behind a refused draft, over one share of words and many; draft's numbers below zero and NaN"""
+    tokens, target, _, draft, _ = inputs(11, 5, 3, vocab, F32, "drawn")
+    big = draft * 0 + 2.0
+    numbers = torch.tensor([[u, 0.9, 0.9] for u in (0.0, 0.2, 0.5, 0.9, 1 - 2.0 ** -24)])
+    check(tokens, target, numbers, big)
+    big[:, :, ::3] = float("nan")
+    big[:, :, 1::3] = -1.0
+    check(tokens, target, numbers, big)
 
 
 def test_trees_whose_parents_are_odd():
@@ -157,10 +175,11 @@ def test_refusals():
     assert [x.shape[0] for x in kv.verifyDrafts(tokens[:0], target[:0], numbers[:0])] == [0, 0, 0]
 
 
-def test_recorded_and_beside_each_other():
+@pytest.mark.parametrize("vocab", [20000, 70000])
+def test_recorded_and_beside_each_other(vocab):
     """Two graphs on streams of their own, replayed together with eager calls between: a workspace each"""
     kv = load("cache")
-    first, second = ([None if x is None else x.cuda() for x in inputs(s, 8, 5, 20000, F32, "drawn")] for s in (7, 8))
+    first, second = ([None if x is None else x.cuda() for x in inputs(s, 8, 5, vocab, F32, "drawn")] for s in (7, 8))
     want = [[t.clone() for t in kv.verifyDrafts(*x)] for x in (first, second)]
     graphs = []
     for x in (first, second):
