@@ -340,7 +340,7 @@ int marian_hip_pages_attention(const marian_hip_pages* cache, const int32_t* tab
      n * (q_heads / heads) > 1 << 26)
     return MARIAN_HIP_ERR_RANGE;
   if(sequences == 0 || n == 0) return MARIAN_HIP_OK;
-  const PagesAttentionPlan p = pages_attention_plan(sequences, heads, q_heads, n, dk, width);
+  const PagesAttentionPlan p = pages_attention_plan(sequences, heads, q_heads, n, dk, width, row * page);
   if(p.grid > kMostThreads / (64 * p.waves)) return MARIAN_HIP_ERR_RANGE;
   MH_CHECK(check_pages_memory(cache));
   if(!table || !lens) return MARIAN_HIP_ERR_NULL;

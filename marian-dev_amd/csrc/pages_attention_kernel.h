@@ -32,6 +32,7 @@
 namespace marian_hip {
 
 typedef __bf16 pages_b8 __attribute__((ext_vector_type(8)));
+typedef int cache_i4 __attribute__((ext_vector_type(4)));
 
 template <typename T, int DP>
 struct Pages {
@@ -89,6 +90,40 @@ __device__ __forceinline__ PagesPlace pages_look(const PagesAttentionArgs& a, co
   return PagesPlace{table[min(j, (unsigned)a.row - 1)] | (j < (unsigned)a.row ? 0 : (int)0x80000000), (int)within};   // (behind the row: none)
 }
 
+// Adds the infinities and NaN among position k's values to the rows that see it.
+template <typename T, int DP, int QT>
+__device__ __forceinline__ void pages_add_odd(const T* v, int dk, int k, int g, const CacheSight (&sight)[QT], cache_f4 (&o)[QT][DP / 16]) {
+  constexpr int kTogether = Pages<T, DP>::kTogether;
+#pragma unroll
+  for(int j = 0; j < DP / 16; ++j)
+#pragma unroll
+    for(int e = 0; e < 4; ++e) {
+      const int d = (16 * (j / kTogether) + 4 * g + e) * kTogether + j % kTogether;
+      const float z = to_float(v[d < dk ? d : 0]);
+#pragma unroll
+      for(int t = 0; t < QT; ++t)
+        if(k < sight[t].limit && d < dk && !(__builtin_fabsf(z) < __builtin_huge_valf())) o[t][j][e] += z;
+    }
+}
+
+// The weights of a lane's eight scores, 2^(score * scale + from), in two terms of T, and their sum.
+template <typename T>
+__device__ __forceinline__ void pages_weights(const cache_f4 (&s)[2], float scale, float from, float& sum, cache_u4 (&w)[2]) {
+#pragma unroll
+  for(int e = 0; e < 4; ++e) {
+    float y[2];
+#pragma unroll
+    for(int i = 0; i < 2; ++i) {
+      const int at = 2 * e + i;
+      y[i] = settled(__builtin_amdgcn_exp2f(__builtin_fmaf(s[at / 4][at % 4], scale, from)));
+      sum += y[i];
+    }
+    const unsigned both = pack2<T>(y[0], y[1]);
+    w[0][e] = both;
+    w[1][e] = pack2<T>(y[0] - pages_half<T>(both & 0xffff), y[1] - pages_half<T>(both >> 16));
+  }
+}
+
 // The results of waves that share rows, joined and written.  Lane (c, g) holds of row c of each sixteen the values
 // (16 (j / kTogether) + 4 g + e) kTogether + j % kTogether as o[t][j][e], unnormalized, the carried maximum and its part of the sum.
 template <typename T, int DP, int QT, int WAVES>
@@ -128,6 +163,7 @@ __device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const 
     const int up = 5 + 32 - __builtin_clz((unsigned)max(x.end - x.w.from, 1));
     const float over = __builtin_bit_cast(float, (unsigned)(127 - up) << 23) * kUnit, back = __builtin_bit_cast(float, (unsigned)(127 + up) << 23);
     static_assert(kMaximumSlack <= 4.0f, "up counts it");
+    const CacheBuffer part(out.part, CacheOut<T, DP, 16 * QT>::kTileFloats * 4);
     __syncthreads();
 #pragma unroll
     for(int t = 0; t < QT; ++t) {
@@ -169,8 +205,15 @@ __device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const 
             for(int i = 1; i < WAVES; ++i) y[j] += sh.joined[i][r][d + j];
             y[j] *= per;
           }
-          out.emit(16 * t + r, h * kHalf + d, y);
-          if(h == 0 && (tid & 15) == 0) out.emit_log(16 * t + r, top_r, total);
+          if(out.whole) {
+            out.emit(16 * t + r, h * kHalf + d, y);
+          } else if(x.row0 + 16 * t + r < x.rows) {   // (sixteen bytes at a time)
+            const unsigned to = 4u * ((16 * t + r) * DP + h * kHalf + d);
+#pragma unroll
+            for(int j = 0; j < kEach; j += 4) part.store_through(cache_f4{y[j], y[j + 1], y[j + 2], y[j + 3]}, to + 4u * j);
+            if(h == 0 && (tid & 15) == 0)
+              part.store_through(total == 0.0f ? kNone : top_r + __builtin_amdgcn_logf(total), 4u * (16 * QT * DP + 16 * t + r));
+          }
         }
       }
     }
@@ -338,16 +381,6 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
         top[t] = m;
       }
     }
-    float p[QT][8];
-#pragma unroll
-    for(int t = 0; t < QT; ++t) {
-      const float from = (top[t] == kNone ? 0.0f : -top[t]) + P::kUp;   // (nothing seen so far: minus infinity stays that)
-#pragma unroll
-      for(int e = 0; e < 8; ++e) {
-        p[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], a.scale_log2, from));
-        sum[t] += p[t][e];
-      }
-    }
     // Positions that some rows see and others do not: infinities and NaN among their values stay out of the product, see below.
     if(masked && end > x.open) {
       bool odd = false;
@@ -365,6 +398,16 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
     }
     // weighted values
     if constexpr(kWidth == 4) {
+      float p[QT][8];
+#pragma unroll
+      for(int t = 0; t < QT; ++t) {
+        const float from = (top[t] == kNone ? 0.0f : -top[t]) + P::kUp;   // (nothing seen so far: minus infinity stays that)
+#pragma unroll
+        for(int e = 0; e < 8; ++e) {
+          p[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], a.scale_log2, from));
+          sum[t] += p[t][e];
+        }
+      }
 #pragma unroll
       for(int j = 0; j < kDims; ++j)
 #pragma unroll
@@ -375,22 +418,14 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
     } else {
       cache_u4 weights[QT][2];
 #pragma unroll
-      for(int t = 0; t < QT; ++t)
-#pragma unroll
-        for(int e = 0; e < 4; ++e) {
-          const float lo = settled(p[t][2 * e]), hi = settled(p[t][2 * e + 1]);
-          const unsigned w = pack2<T>(lo, hi);
-          weights[t][0][e] = w;
-          weights[t][1][e] = pack2<T>(lo - pages_half<T>(w & 0xffff), hi - pages_half<T>(w >> 16));
-        }
+      for(int t = 0; t < QT; ++t) pages_weights<T>(s[t], a.scale_log2, (top[t] == kNone ? 0.0f : -top[t]) + P::kUp, sum[t], weights[t]);
 #pragma unroll
       for(int j = 0; j < kDims; ++j) {
-        constexpr unsigned low = 0x05040100, high_half = 0x07060302;
         cache_u4 d;
 #pragma unroll
         for(int e = 0; e < 4; ++e)
           d[e] = __builtin_amdgcn_perm(value.word[2 * e + 1][j / kTogether][j % kTogether / 2], value.word[2 * e][j / kTogether][j % kTogether / 2],
-                                       j % 2 ? high_half : low);
+                                       j % 2 ? 0x07060302 : 0x05040100);
 #pragma unroll
         for(int t = 0; t < QT; ++t)
 #pragma unroll
@@ -409,20 +444,351 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
       for(int k = max(at, x.open); k < min(at + 32, end); ++k) {
         const PagesPlace y = pages_look(a, table, (unsigned)k >> 3);
         if((unsigned)y.id >= (unsigned)a.pages) continue;
-        const T* const v = reinterpret_cast<const T*>(v_head + y.id * a.page_bytes + (long long)(8 * y.eight + (k & 7)) * row_bytes);
-#pragma unroll
-        for(int j = 0; j < kDims; ++j)
-#pragma unroll
-          for(int e = 0; e < 4; ++e) {
-            const int d = (16 * (j / kTogether) + 4 * g + e) * kTogether + j % kTogether;
-            const float z = to_float(v[d < a.dk ? d : 0]);
-#pragma unroll
-            for(int t = 0; t < QT; ++t)
-              if(k < sight[t].limit && d < a.dk && !(__builtin_fabsf(z) < __builtin_huge_valf())) o[t][j][e] += z;
-          }
+        pages_add_odd<T, DP, QT>(reinterpret_cast<const T*>(v_head + y.id * a.page_bytes + (long long)(8 * y.eight + (k & 7)) * row_bytes), a.dk, k, g, sight, o);
       }
   }
   pages_finish<T, DP, QT, WAVES>(a, x, o, top, sum, wave, sh);
+}
+
+// ---- more than 32 rows
+// Four waves have 16 * QT rows each and share positions laid out in LDS, 64 at a time, twice: while one is worked on, the next is written and
+// the one after that is on its way to registers.  Keys lie there as they are, values transposed, a dimension's 64 side by side; pieces of 16
+// bytes change places within a row so that eight lanes that read together meet in no bank:
+//   key k, piece i at i ^ k (rows of 256 bytes), i ^ k / 2 (128 bytes); dimension d, eight positions j at j ^ d / kTogether.
+// A wave lays out sixteen positions: sixteen lanes (eight) to a row of keys; of values each lane has DP / 32 dimensions of eight positions.
+// Products, weights and sums are those above.
+template <typename T, int DP>
+struct PagesMany {
+  static constexpr int kTile = 64;                        // positions of a turn
+  static constexpr int kRowPieces = DP / 8;               // pieces of a key
+  static constexpr int kKeyLoads = kRowPieces / 4;        // of a lane: sixteen keys to a wave
+  static constexpr int kDimsEach = DP / 32;               // of a lane's values
+  static constexpr int kValueWords = kDimsEach / 2;
+  // (lanes that read together are, by what was measured, the 16 lanes c, of one half of them with g and of the other with g ^ 1)
+  static __device__ __forceinline__ int key_place(int key, int piece) {
+    const int c = (key >> 1 & 12) | (key & 3);
+    return (key * kRowPieces + (piece ^ (kRowPieces == 16 ? c : c >> 1))) * 16;
+  }
+  static __device__ __forceinline__ int value_place(int dim, int eight) {
+    const int c = dim / Pages<T, DP>::kTogether, j = dim % Pages<T, DP>::kTogether;
+    return (j * 16 + c) * 128 + (eight ^ c >> 1) * 16;
+  }
+  struct Shared {
+    alignas(16) unsigned char keys[2][kTile * DP * 2];
+    alignas(16) unsigned char values[2][kTile * DP * 2];
+    int there[2][8];   // of each eight of positions, whether it has a page
+    int left_out;
+  };
+};
+
+// A barrier for what lies in LDS: loads from memory stay under way, which __syncthreads would wait for.
+__device__ __forceinline__ void pages_lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <typename T, int DP, bool WHOLE, int QT>
+__global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAttentionArgs a) {
+  using P = Pages<T, DP>;
+  using M = PagesMany<T, DP>;
+  constexpr int kDims = P::kDims, kTogether = P::kTogether, kKeyPieces = P::kKeyPieces, kTile = M::kTile;
+  constexpr float kUnit = P::kUp < 0 ? (float)(1 << -P::kUp * (P::kUp < 0)) : 1.0f / (1 << P::kUp * (P::kUp > 0));   // 2^-kUp
+  __shared__ struct {
+    typename M::Shared tile;
+    int is_last;
+  } sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+  CacheTile x;
+  if(!cache_tile<T, DP, 64 * QT, 4>(a, tid, x)) return;
+  const int end = x.end, row_bytes = (WHOLE ? DP : a.dk) * 2;
+  const int* const table = a.table + (long long)x.w.s * a.row;
+  const unsigned char* const k_head = a.k_pages + x.head * a.head_bytes;
+  const unsigned char* const v_head = a.v_pages + x.head * a.head_bytes;
+  if(tid == 0) sh.tile.left_out = 0;
+
+  // ---- what a wave lays out: the eights 2 * wave and 2 * wave + 1 of a tile
+  // (of two tiles, in turn: a tile's 32 KB on their way to each of two workgroups are too few for a memory that answers after some 4 us under load)
+  struct Fetched {
+    cache_u4 key[M::kKeyLoads];
+    unsigned value[8][M::kValueWords];
+    bool there[2];
+    PagesPlace next[2];   // of the tile that is fetched next
+  } even;
+  auto look = [&](Fetched& y, int at) __attribute__((always_inline)) {
+#pragma unroll
+    for(int i = 0; i < 2; ++i) y.next[i] = pages_look(a, table, (unsigned)(at + 16 * wave + 8 * i) >> 3);
+  };
+  auto fetch = [&](Fetched& f, int at) __attribute__((always_inline)) {
+    long long place[2];
+#pragma unroll
+    for(int i = 0; i < 2; ++i) {
+      const int first = at + 16 * wave + 8 * i;
+      const PagesPlace y = f.next[i];
+      f.there[i] = (unsigned)y.id < (unsigned)a.pages && first < end;
+      place[i] = f.there[i] ? y.id * a.page_bytes + (long long)(8 * y.eight) * row_bytes : 0;
+    }
+#pragma unroll
+    for(int i = 0; i < M::kKeyLoads; ++i) {   // (rows past one eight are of the next)
+      constexpr int kAtOnce = 64 / M::kRowPieces;
+      const int row = kAtOnce * i + lane / M::kRowPieces, piece = lane % M::kRowPieces * 16;
+      f.key[i] = *reinterpret_cast<const cache_u4*>(k_head + place[kAtOnce * i / 8] + (row & 7) * row_bytes + (piece < row_bytes ? piece : 0));
+    }
+    const int d = lane % 32 * M::kDimsEach * 2;
+    const unsigned char* const from = v_head + (lane < 32 ? place[0] : place[1]) + (d < row_bytes ? d : 0);
+#pragma unroll
+    for(int e = 0; e < 8; ++e)
+#pragma unroll
+      for(int w = 0; w < M::kValueWords; ++w) f.value[e][w] = reinterpret_cast<const unsigned*>(from + e * row_bytes)[w];
+  };
+  auto lay_out = [&](Fetched& f, int at, int buffer) __attribute__((always_inline)) {
+    constexpr int kAtOnce = 64 / M::kRowPieces;
+#pragma unroll
+    for(int i = 0; i < M::kKeyLoads; ++i) {
+      const int row = 16 * wave + kAtOnce * i + lane / M::kRowPieces, piece = lane % M::kRowPieces;
+      if(!WHOLE) f.key[i] = piece * 16 < row_bytes ? f.key[i] : cache_u4{0, 0, 0, 0};   // (queries are zero there, and so must these be)
+      *reinterpret_cast<cache_u4*>(sh.tile.keys[buffer] + M::key_place(row, piece)) = f.key[i];
+    }
+    const int eight = 2 * wave + (lane >> 5), first = at + 8 * eight;
+    const bool is = lane < 32 ? f.there[0] : f.there[1];
+    if(at + kTile > x.open || !(f.there[0] && f.there[1])) {
+      // Values that no row sees weigh zero, whatever they are; infinities and NaN that some do not see are left out, see below.
+      const int seen = is ? end - first : 0;
+      bool any = false;
+#pragma unroll
+      for(int e = 0; e < 8; ++e)
+#pragma unroll
+        for(int w = 0; w < M::kValueWords; ++w) {
+          const unsigned z = e < seen ? f.value[e][w] : 0, clean = first + e < x.open ? z : pages_finite<T>(z);
+          any |= z != clean;
+          f.value[e][w] = clean;
+        }
+      if(any) sh.tile.left_out = 1;
+    }
+    if((lane & 31) == 0) sh.tile.there[buffer][eight] = is;
+#pragma unroll
+    for(int j = 0; j < M::kDimsEach; ++j) {
+      cache_u4 y;
+#pragma unroll
+      for(int e = 0; e < 4; ++e) y[e] = __builtin_amdgcn_perm(f.value[2 * e + 1][j / 2], f.value[2 * e][j / 2], j % 2 ? 0x07060302 : 0x05040100);
+      *reinterpret_cast<cache_u4*>(sh.tile.values[buffer] + M::value_place(lane % 32 * M::kDimsEach + j, eight)) = y;
+    }
+  };
+
+  const int begin = x.w.from;
+  look(even, begin);
+  fetch(even, begin);
+  look(even, begin + kTile);
+  cache_u4 q[QT][kKeyPieces];
+  CacheSight sight[QT];
+#pragma unroll
+  for(int t = 0; t < QT; ++t) {
+    const int row = min(x.row0 + 16 * (QT * wave + t) + c, x.rows - 1);
+    sight[t] = cache_sight(a, x, row, 0);
+    unsigned of_group;
+    const unsigned token = a.by_group.of((unsigned)row, of_group);
+    const unsigned char* const p =
+        reinterpret_cast<const unsigned char*>(static_cast<const T*>(a.q) + x.w.s * a.q_s + (long long)(x.head * a.G + (int)of_group) * a.q_h +
+                                               (long long)token * a.q_n);
+#pragma unroll
+    for(int i = 0; i < kKeyPieces; ++i) {
+      const int d = 64 * i + 16 * g;
+      const cache_u4 y = *reinterpret_cast<const cache_u4*>(p + (d < row_bytes ? d : 0));
+      q[t][i] = d < row_bytes ? y : cache_u4{0, 0, 0, 0};
+    }
+  }
+  cache_f4 o[QT][kDims];
+  float top[QT], sum[QT];   // carried maximum (base 2), the lane's part of the sum
+#pragma unroll
+  for(int t = 0; t < QT; ++t) {
+    top[t] = kNone;
+    sum[t] = 0.0f;
+#pragma unroll
+    for(int j = 0; j < kDims; ++j) o[t][j] = cache_f4{0, 0, 0, 0};
+  }
+  pages_lds_barrier();   // (left_out is cleared)
+  lay_out(even, begin, 0);
+  fetch(even, begin + kTile);
+  look(even, begin + 2 * kTile);
+  pages_lds_barrier();
+
+  int buffer = 0;
+  for(int at = begin; at < end; at += kTile, buffer ^= 1) {
+    const bool masked = at + kTile > x.open;
+    unsigned none = 0;   // the tile's eights without a page
+    {
+      const cache_i4 lo = *reinterpret_cast<const cache_i4*>(&sh.tile.there[buffer][0]), hi = *reinterpret_cast<const cache_i4*>(&sh.tile.there[buffer][4]);
+#pragma unroll
+      for(int i = 0; i < 4; ++i) none |= (lo[i] ? 0 : 1u << i) | (hi[i] ? 0 : 16u << i);
+    }
+    cache_f4 s[QT][4];   // two and two for 32 positions
+#pragma unroll
+    for(int t = 0; t < QT; ++t)
+#pragma unroll
+      for(int b = 0; b < 4; ++b) s[t][b] = cache_f4{0, 0, 0, 0};
+#pragma unroll
+    for(int i = 0; i < kKeyPieces; ++i)
+#pragma unroll
+      for(int b = 0; b < 4; ++b) {
+        const cache_u4 k = *reinterpret_cast<const cache_u4*>(sh.tile.keys[buffer] + M::key_place(32 * (b / 2) + 8 * (c >> 2) + (c & 3) + 4 * (b % 2), 4 * i + g));
+#pragma unroll
+        for(int t = 0; t < QT; ++t) s[t][b] = pages_product<T>(k, q[t][i], s[t][b]);
+      }
+    if(masked || none) {
+#pragma unroll
+      for(int h = 0; h < 2; ++h) {
+        const int first = at + 32 * h + 8 * g;
+#pragma unroll
+        for(int t = 0; t < QT; ++t) {
+          const int sees = none >> (4 * h + g) & 1 ? 0 : sight[t].limit - first;
+#pragma unroll
+          for(int e = 0; e < 8; ++e) s[t][2 * h + e / 4][e % 4] = e < sees ? s[t][2 * h + e / 4][e % 4] : kNone;
+        }
+      }
+    }
+    float high[QT];
+    bool grown = false;
+#pragma unroll
+    for(int t = 0; t < QT; ++t) {
+      high[t] = kNone;
+#pragma unroll
+      for(int e = 0; e < 16; ++e) high[t] = fmaxf(high[t], s[t][e / 4][e % 4]);
+      high[t] *= a.scale_log2;
+      grown |= high[t] > top[t] + kMaximumSlack;
+    }
+    if(__any(grown)) {
+#pragma unroll
+      for(int t = 0; t < QT; ++t) {
+        const float m = fmaxf(top[t], over_lanes_max(high[t]));
+        const float down = m == top[t] ? 1.0f : __builtin_amdgcn_exp2f(top[t] - m);
+        sum[t] *= down;
+#pragma unroll
+        for(int j = 0; j < kDims; ++j) o[t][j] *= down;
+        top[t] = m;
+      }
+    }
+    // (the second half's weights are made while the first half's products run)
+#pragma unroll
+    for(int h = 0; h < 2; ++h) {
+      cache_u4 weights[QT][2];
+#pragma unroll
+      for(int t = 0; t < QT; ++t) {
+        const cache_f4 mine[2] = {s[t][2 * h], s[t][2 * h + 1]};
+        pages_weights<T>(mine, a.scale_log2, (top[t] == kNone ? 0.0f : -top[t]) + P::kUp, sum[t], weights[t]);
+      }
+#pragma unroll
+      for(int j = 0; j < kDims; ++j) {
+        const int dim = (16 * (j / kTogether) + c) * kTogether + j % kTogether;
+        const cache_u4 v = *reinterpret_cast<const cache_u4*>(sh.tile.values[buffer] + M::value_place(dim, 4 * h + g));
+#pragma unroll
+        for(int t = 0; t < QT; ++t)
+#pragma unroll
+          for(int m = 1; m >= 0; --m) o[t][j] = pages_product<T>(v, weights[t][m], o[t][j]);
+      }
+    }
+    if(at + kTile < end) lay_out(even, at + kTile, buffer ^ 1);
+    fetch(even, at + 2 * kTile);
+    look(even, at + 3 * kTile);
+    pages_lds_barrier();
+  }
+  // What was left out goes to the rows that see it: of any weight an infinity is one, and a NaN is one.
+  if(sh.tile.left_out) {
+#pragma unroll 1
+    for(int k = max(begin, x.open); k < end; ++k) {
+      const PagesPlace y = pages_look(a, table, (unsigned)k >> 3);
+      if((unsigned)y.id >= (unsigned)a.pages) continue;
+      pages_add_odd<T, DP, QT>(reinterpret_cast<const T*>(v_head + y.id * a.page_bytes + (long long)(8 * y.eight + (k & 7)) * row_bytes), a.dk, k, g, sight, o);
+    }
+  }
+  // Rows of a sequence in one part go to the output.  Parts go to the workspace as registers have them, 1 KB at a time, and back: whoever
+  // arrives last joins them, a wave its own rows (16 parts of 64 rows: 20 us less than by rows of 16 threads, which store and load pieces of 8 bytes).
+  const CacheOut<T, DP, 64 * QT> out(a, x);
+  auto write = [&](int t, float factor) __attribute__((always_inline)) {
+    const int row = x.row0 + 16 * (QT * wave + t) + c;
+    if(row >= x.rows) return;
+    T* const to = cache_row_out<T>(a, x, row);
+#pragma unroll
+    for(int i = 0; i < P::kValuePieces; ++i)
+#pragma unroll
+      for(int e = 0; e < 4; ++e) {
+        const int d = (16 * i + 4 * g + e) * kTogether;
+        float y[kTogether];
+#pragma unroll
+        for(int j = 0; j < kTogether; ++j) y[j] = o[t][i * kTogether + j][e] * factor;
+        if(d < a.dk) store_row<kTogether, T>(to + d, y);
+      }
+  };
+#pragma unroll
+  for(int t = 0; t < QT; ++t) sum[t] = over_lanes_sum(sum[t]) * kUnit;
+  if(out.whole) {
+#pragma unroll
+    for(int t = 0; t < QT; ++t) write(t, sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * kUnit);
+    return;
+  }
+  constexpr unsigned kTileBytes = CacheOut<T, DP, 64 * QT>::kTileFloats * 4;
+  const unsigned stride = (unsigned)out.stride * kTileBytes, mine = 16u * (QT * kDims * 64 * wave + lane), my_log = 4u * (64 * QT * DP + 16 * QT * wave + c);
+  const CacheBuffer parts(a.part + out.place * CacheOut<T, DP, 64 * QT>::kTileFloats, stride * x.w.parts);
+#pragma unroll
+  for(int t = 0; t < QT; ++t) {
+    const float factor = sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * kUnit;
+    const unsigned to = stride * x.w.part;
+#pragma unroll
+    for(int j = 0; j < kDims; ++j) parts.store_through(o[t][j] * factor, to + mine + 1024u * (t * kDims + j));
+    if(g == 0) parts.store_through(sum[t] == 0.0f ? kNone : top[t] + __builtin_amdgcn_logf(sum[t]), to + my_log + 64u * t);
+  }
+  if(!cache_arrived_last(a.counters + out.place, x.w.parts, sh.is_last)) return;
+  float weight_sum[QT];
+#pragma unroll
+  for(int t = 0; t < QT; ++t) {
+    top[t] = kNone;
+    weight_sum[t] = 0.0f;
+#pragma unroll
+    for(int j = 0; j < kDims; ++j) o[t][j] = cache_f4{0, 0, 0, 0};
+  }
+  constexpr int kLogs = 8, kBatch = QT == 1 && DP == 64 ? 4 : 2;
+#pragma unroll 1
+  for(int i = 0; i < x.w.parts; i += kLogs) {   // (behind the last part the buffer gives zeros)
+    float l[QT][kLogs];
+#pragma unroll
+    for(int b = 0; b < kLogs; ++b)
+#pragma unroll
+      for(int t = 0; t < QT; ++t) l[t][b] = parts.number_through(stride * (unsigned)(i + b) + my_log + 64u * t);
+#pragma unroll
+    for(int b = 0; b < kLogs; ++b)
+#pragma unroll
+      for(int t = 0; t < QT; ++t) top[t] = i + b < x.w.parts ? fmaxf(top[t], l[t][b]) : top[t];
+  }
+#pragma unroll 1
+  for(int i = 0; i < x.w.parts; i += kBatch) {
+    float l[QT][kBatch];
+    cache_f4 z[kBatch][QT][kDims];
+#pragma unroll
+    for(int b = 0; b < kBatch; ++b) {
+      const unsigned at = stride * (unsigned)(i + b);
+#pragma unroll
+      for(int t = 0; t < QT; ++t) {
+        l[t][b] = parts.number_through(at + my_log + 64u * t);
+#pragma unroll
+        for(int j = 0; j < kDims; ++j) z[b][t][j] = parts.piece_through(at + mine + 1024u * (t * kDims + j));
+      }
+    }
+#pragma unroll
+    for(int b = 0; b < kBatch; ++b) {
+      if(i + b >= x.w.parts) break;
+#pragma unroll
+      for(int t = 0; t < QT; ++t) {
+        // (a part's weight is at most 1, times kPartUnit: sums stay within the largest value)
+        const float weight = l[t][b] == kNone ? 0.0f : __builtin_amdgcn_exp2f(l[t][b] - top[t]) * kPartUnit;
+        weight_sum[t] += weight;
+#pragma unroll
+        for(int j = 0; j < kDims; ++j)
+#pragma unroll
+          for(int e = 0; e < 4; ++e) o[t][j][e] = __builtin_fmaf(weight, z[b][t][j][e], o[t][j][e]);
+      }
+    }
+  }
+#pragma unroll
+  for(int t = 0; t < QT; ++t) write(t, weight_sum[t] == 0.0f ? 0.0f : 1.0f / weight_sum[t]);
 }
 
 }  // namespace marian_hip

@@ -11,12 +11,6 @@ template <typename T, int DP, bool WHOLE, int W>
 int launch_pages_attention(const PagesAttentionArgs& a, const PagesAttentionPlan& p, hipStream_t st) {
   constexpr int kMost = pages_most_qt(sizeof(T), DP);
   const dim3 grid((unsigned)p.grid), block(64 * W);
-  if constexpr(kMost >= 4) {
-    if(p.qt == 4) {
-      MH_LAUNCH((pages_attention_kernel<T, DP, WHOLE, 4, W>), grid, block, 0, st, a);
-      return MARIAN_HIP_OK;
-    }
-  }
   if constexpr(kMost >= 2) {
     if(p.qt == 2) {
       MH_LAUNCH((pages_attention_kernel<T, DP, WHOLE, 2, W>), grid, block, 0, st, a);
@@ -29,6 +23,14 @@ int launch_pages_attention(const PagesAttentionArgs& a, const PagesAttentionPlan
 
 template <typename T, int DP, bool WHOLE>
 int launch_pages_attention(const PagesAttentionArgs& a, const PagesAttentionPlan& p, hipStream_t st) {
+  if constexpr(pages_has_many(sizeof(T), DP)) {
+    if(p.many) {
+      const dim3 grid((unsigned)p.grid), block(256);
+      if(p.qt == 1) MH_LAUNCH((pages_attention_many_kernel<T, DP, WHOLE, 1>), grid, block, 0, st, a);
+      else MH_LAUNCH((pages_attention_many_kernel<T, DP, WHOLE, 2>), grid, block, 0, st, a);
+      return MARIAN_HIP_OK;
+    }
+  }
   return p.waves == 1 ? launch_pages_attention<T, DP, WHOLE, 1>(a, p, st) : launch_pages_attention<T, DP, WHOLE, 4>(a, p, st);
 }
 

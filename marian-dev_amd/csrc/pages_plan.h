@@ -16,7 +16,9 @@ constexpr int pages_registers(int width, int dp, int qt) {
 }
 
 // Sixteens of query rows that a wave takes over the same positions, at the most.
-constexpr int pages_most_qt(int width, int dp) { return width == 4 ? (dp == 256 ? 1 : 2) : dp == 256 ? 2 : 4; }
+constexpr int pages_most_qt(int width, int dp) { return width == 4 && dp == 256 ? 1 : 2; }
+// Whether rows past that have a form in which four waves of 16 * qt rows each share positions in LDS.
+constexpr bool pages_has_many(int width, int dp) { return width == 2 && dp <= 128; }
 
 // Waves of a form that fit a SIMD, by its registers.
 constexpr int pages_to_a_simd(int width, int dp, int qt) {
@@ -27,6 +29,7 @@ constexpr int pages_to_a_simd(int width, int dp, int qt) {
 struct PagesAttentionPlan {
   int dp;              // values of a row as the kernel holds it: dk rounded up to 64, 128 or 256
   int qt;              // sixteens of query rows to a workgroup
+  bool many;           // the waves have these rows each, and share positions laid out in LDS
   int waves;           // of a workgroup, which share its rows and take turns of 32 positions
   int tile_rows;       // of a workgroup
   int64_t row_tiles;   // workgroups that share an entry's positions
@@ -37,17 +40,21 @@ struct PagesAttentionPlan {
   int64_t grid;
 };
 
-inline PagesAttentionPlan pages_attention_plan(int64_t sequences, int64_t heads, int64_t q_heads, int64_t n, int64_t dk, int width) {
+inline PagesAttentionPlan pages_attention_plan(int64_t sequences, int64_t heads, int64_t q_heads, int64_t n, int64_t dk, int width, int64_t capacity = 1 << 30) {
   PagesAttentionPlan p{};
   p.dp = dk <= 64 ? 64 : dk <= 128 ? 128 : 256;
   const int64_t rows = n * (q_heads / heads);
-  p.qt = std::min(rows <= 16 ? 1 : rows <= 32 ? 2 : 4, pages_most_qt(width, p.dp));
-  p.tile_rows = 16 * p.qt;
+  p.many = rows > 32 && pages_has_many(width, p.dp);
+  p.qt = p.many ? (rows > 64 ? 2 : 1) : std::min(rows <= 16 ? 1 : 2, pages_most_qt(width, p.dp));
+  p.tile_rows = p.many ? 64 * p.qt : 16 * p.qt;
   p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const int64_t entries = sequences * heads * p.row_tiles;
-  p.waves = entries >= 4096 ? 1 : 4;
-  const int64_t at_a_time = 1024 * pages_to_a_simd(width, p.dp, p.qt) / p.waves;
+  p.waves = !p.many && entries >= 4096 ? 1 : 4;
+  const int64_t at_a_time = 1024 * (p.many ? 2 : pages_to_a_simd(width, p.dp, p.qt)) / p.waves;
   p.target = std::max<int64_t>(1, at_a_time / (heads * p.row_tiles) - sequences / 2);
+  // A sequence of up to four blocks stays whole, and where no row of the table has room for more nobody looks at the others' lengths.  Nor does he
+  // where these are many: their parts would be few, and a look at them costs every workgroup a load for 64 of them.
+  if(capacity <= kCacheWhole * kCacheBlock || sequences > 1024) p.target = 1;
   p.least = entries <= 32 ? 2 : 4;
   p.items = p.target == 1 ? sequences : p.target + sequences;
   p.slots = p.target == 1 ? 0 : 2 * p.target;

@@ -14,7 +14,7 @@ import pages_oracle as oracle
 from conftest import PKG, ROOT, load
 
 GB = 1 << 30
-S, H, HQ, N, PAGES, PAGE, ROW, DK, VOCAB = 3, 2, 4, 5, 12, 16, 4, 64, 50000
+S, H, HQ, N, PAGES, PAGE, ROW, DK, VOCAB = 3, 2, 4, 5, 12, 16, 64, 64, 50000
 NAMES = ("k", "v", "table", "held", "free", "count", "lens", "counts", "slots", "xk", "xv", "xq", "qo", "ws", "tokens", "parents", "target", "draft", "random",
          "path", "accepted", "next")
 PLACES = {n: (i + 1) * GB for i, n in enumerate(NAMES)}
@@ -165,7 +165,7 @@ int main() {
   long long s, h, hq, n, dk, width;
   while(std::scanf("%lld %lld %lld %lld %lld %lld", &s, &h, &hq, &n, &dk, &width) == 6) {
     const auto p = marian_hip::pages_attention_plan(s, h, hq, n, dk, (int)width);
-    std::printf("%d %d %d %d %lld %lld %lld %lld %lld %lld\n", p.dp, 16 * p.qt, p.waves, p.least, (long long)p.row_tiles, (long long)p.target,
+    std::printf("%d %d %d %d %lld %lld %lld %lld %lld %lld\n", p.dp, p.tile_rows, p.waves, p.least, (long long)p.row_tiles, (long long)p.target,
                 (long long)p.items, (long long)p.slots, (long long)p.grid, (long long)marian_hip::pages_attention_bytes(p, h));
   }
 }
