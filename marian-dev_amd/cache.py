@@ -14,10 +14,11 @@ One step of a decoder with drafted tokens:
         q, k, v = layer.project(x)
         q = appendToCache(cache, k, v, lens, parents, rotary=rotary, q=q)
         x = layer.finish(AttentionOverCache(q, cache, lens, parents))
-    path, accepted, nextTokens = verifyDrafts(tokens, target(x), random, parents=parents)
+    path, accepted = judge(x)
     for cache in caches:   # (each of them from the lengths that its drafts were written behind)
         newLens = keepDrafts(cache, lens, path, accepted)
     lens = newLens
+where judge(x) is path, accepted, nextTokens = verifyDrafts(tokens, target(x), random, parents=parents), or what a program puts in its place.
 For one token, or a prompt, parents is None and lens + n the next step's.  The caches of the surviving hypotheses of
 a beam are gathered like any decoder state: ops.selectState on the tensors' float32 views.
 """

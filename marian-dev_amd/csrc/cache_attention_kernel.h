@@ -67,12 +67,14 @@ __device__ __forceinline__ unsigned lanes_sum(unsigned x) {
   return (unsigned)v;
 }
 
-// Blocks of a part of a sequence of `blocks`.
+// Blocks of a part of a sequence of `blocks`, which has up to MOST parts.
+template <unsigned MOST>
 __device__ __forceinline__ unsigned cache_part_size(unsigned blocks, unsigned each) {
-  return max(blocks <= kCacheWhole ? max(each, kCacheWhole) : each, (blocks + kCacheMostParts - 1) / kCacheMostParts);
+  return max(blocks <= kCacheWhole ? max(each, kCacheWhole) : each, (blocks + MOST - 1) / MOST);
 }
 
 // Finds part `item`; false where there are fewer.  All waves do the same, lanes being sequences.
+template <unsigned MOST>
 __device__ __forceinline__ bool cache_part(const CacheAttentionArgs& a, int item, int lane, CachePart& w) {
   auto blocks_of = [&](int s) -> unsigned {   // of positions that sequence s has in reach
     if(s >= a.S) return 0;
@@ -98,7 +100,7 @@ __device__ __forceinline__ bool cache_part(const CacheAttentionArgs& a, int item
     unsigned before = 0;
     bool found = false;
     auto look = [&](int base, unsigned mine) __attribute__((always_inline)) {
-      const unsigned size = cache_part_size(mine, each), parts = base + lane < a.S ? max(1u, (mine + size - 1) / size) : 0;
+      const unsigned size = cache_part_size<MOST>(mine, each), parts = base + lane < a.S ? max(1u, (mine + size - 1) / size) : 0;
       const unsigned sum = before + lanes_sum(parts > 1 ? parts | parts << 20 : parts);
       const unsigned long long at = __ballot((int)(sum & 0xfffff) > item);
       if(at) {
@@ -123,7 +125,7 @@ __device__ __forceinline__ bool cache_part(const CacheAttentionArgs& a, int item
   w.count = a.counts ? __builtin_amdgcn_readfirstlane(clamp_int(a.counts[w.s], 0, a.n)) : a.n;
   w.used = w.count > 0 ? min(w.len + w.count, a.cap) : 0;
   const unsigned mine = (unsigned)(w.used + kCacheBlock - 1) / kCacheBlock;
-  const int size = (int)cache_part_size(mine, each) * kCacheBlock;
+  const int size = (int)cache_part_size<MOST>(mine, each) * kCacheBlock;
   w.from = a.target > 1 ? w.part * size : 0;
   w.to = a.target > 1 ? min(w.from + size, w.used) : w.used;
   return true;
@@ -279,7 +281,7 @@ __device__ __forceinline__ T* cache_row_out(const CacheAttentionArgs& a, const C
 }
 
 // Finds a workgroup's tile and clears the rows of it that are not there; false where nothing is to be done.
-template <typename T, int DP, int ROWS, int WAVES>
+template <typename T, int DP, int ROWS, int WAVES, unsigned MOST = kCacheMostParts>
 __device__ __forceinline__ bool cache_tile(const CacheAttentionArgs& a, int tid, CacheTile& x) {
   constexpr int kDims = DP / 16;
   // Workgroups with the same positions follow each other on one XCD (a workgroup to each of the eight in turn).
@@ -289,7 +291,7 @@ __device__ __forceinline__ bool cache_tile(const CacheAttentionArgs& a, int tid,
   const int item = (int)a.by_heads.of((unsigned)entry, head);
   x.tile = (int)tile;
   x.head = (int)head;
-  if(!cache_part(a, item, tid & 63, x.w)) return false;
+  if(!cache_part<MOST>(a, item, tid & 63, x.w)) return false;
   x.rows = x.w.count * a.G;
   x.row0 = x.tile * ROWS;
   if(x.w.part == 0 && x.row0 + ROWS > x.rows) {

@@ -34,6 +34,8 @@ namespace marian_hip {
 typedef __bf16 pages_b8 __attribute__((ext_vector_type(8)));
 typedef int cache_i4 __attribute__((ext_vector_type(4)));
 
+static_assert(kPartUnit * kPagesMostParts <= 1.0f, "the parts' weights add up to one at the most");
+
 template <typename T, int DP>
 struct Pages {
   static constexpr int kWidth = sizeof(T);
@@ -232,7 +234,7 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
   const int tid = threadIdx.x, lane = tid & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   CacheTile x;
-  if(!cache_tile<T, DP, 16 * QT, WAVES>(a, tid, x)) return;
+  if(!cache_tile<T, DP, 16 * QT, WAVES, kPagesMostParts>(a, tid, x)) return;
   const int end = x.end, row_bytes = (WHOLE ? DP : a.dk) * kWidth;
   const int* const table = a.table + (long long)x.w.s * a.row;
   const unsigned char* const k_head = a.k_pages + x.head * a.head_bytes;
@@ -500,7 +502,7 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
   } sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   CacheTile x;
-  if(!cache_tile<T, DP, 64 * QT, 4>(a, tid, x)) return;
+  if(!cache_tile<T, DP, 64 * QT, 4, kPagesMostParts>(a, tid, x)) return;
   const int end = x.end, row_bytes = (WHOLE ? DP : a.dk) * 2;
   const int* const table = a.table + (long long)x.w.s * a.row;
   const unsigned char* const k_head = a.k_pages + x.head * a.head_bytes;

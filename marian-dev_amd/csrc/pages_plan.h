@@ -15,6 +15,10 @@ constexpr int pages_registers(int width, int dp, int qt) {
   return 2 * words + qt * (dp / 4 + words / 2 + 16) + 48;   // results, queries, scores and weights; addresses
 }
 
+// Of a sequence.  One token, bfloat16, 128 values, with 48 and with these: a sequence of 100003 positions, 8 heads of keys, 87.1 and 79.9 us; 32000,
+// two heads 17.7 and 16.2; one head of 100000 33.2 and 29.4.
+constexpr unsigned kPagesMostParts = 64;
+
 // Sixteens of query rows that a wave takes over the same positions, at the most.
 constexpr int pages_most_qt(int width, int dp) { return width == 4 && dp == 256 ? 1 : 2; }
 // Whether rows past that have a form in which four waves of 16 * qt rows each share positions in LDS.

@@ -196,13 +196,13 @@ def test_parts_stay_within_grid_and_workspace(tmp_path):
         counters = slots * h * tiles
         assert 4 * counters <= 32768 and size == 32768 + counters * tile * (dp + 1) * 4
         # what the parts are joined through reaches over all of a sequence's, in 32 bits
-        assert 48 * h * tiles * (tile * dp + (tile + 3) // 4 * 4) * 4 < 1 << 32
+        assert 64 * h * tiles * (tile * dp + (tile + 3) // 4 * 4) * 4 < 1 << 32
         for longest in (0, 1, 127, 128, 129, 5000, 1 << 20):
             blocks = [(rng.randint(0, longest) + 127) // 128 for _ in range(s)]
             blocks[rng.randrange(s)] = (longest + 127) // 128
             each = max(least, -(-sum(blocks) // target))
-            # (up to four blocks stay whole, and 48 parts of a sequence are the most)
-            parts = [max(1, -(-b // max(each, 4 if b <= 4 else 0, -(-b // 48)))) for b in blocks]
+            # (up to four blocks stay whole, and 64 parts of a sequence are the most)
+            parts = [max(1, -(-b // max(each, 4 if b <= 4 else 0, -(-b // 64)))) for b in blocks]
             several = sum(p for p in parts if p > 1)
             assert sum(parts) <= items and several <= slots and several < 4096, (s, target, longest)
 
