@@ -500,6 +500,7 @@ typedef struct marian_hip_pages {
  *   held: int32 [sequences]: how many these are;
  *   free: int32 [pages]: a stack of the pages that nobody has, its first free_count[0] entries.
  * sequences <= 65535, row * sequences < 2^31.  A page belongs to one sequence; sequences that share one may read it only.
+ * Calls on the same tables follow each other: on one stream, and of several threads one at a time (a call may be two launches).
  */
 typedef struct marian_hip_page_tables {
   int32_t* table;

@@ -1588,6 +1588,10 @@ bool pages_of(PyObject* o, PagedCache& x) {
   return x.c.type >= 0;
 }
 
+// Held while a call makes its launches on tables: one that moves many pages makes two, and another thread's call on the same stream and
+// tables would come in between.
+std::mutex tables_turn;
+
 // pages_reserve(tables, lens, n, page, counts) -> slots [sequences, n]
 PyObject* py_pages_reserve(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   MH_TRY MH_ARGS(5, "pages_reserve");
@@ -1601,7 +1605,8 @@ PyObject* py_pages_reserve(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   at::Tensor slots = empty({t.t.sequences, n}, at::kInt, t.device);
   const On on(t.device);
   const hipStream_t st = stream_of(t.device);
-  call("reservePages", [&] { return L.pages_reserve(&t.t, lens, counts, n, page, static_cast<int32_t*>(slots.data_ptr()), st); });
+  call("reservePages", [&] { return L.pages_reserve(&t.t, lens, counts, n, page, static_cast<int32_t*>(slots.data_ptr()), st); },
+       nullptr, &tables_turn);
   return wrap(std::move(slots));
   MH_END
 }
@@ -1615,7 +1620,7 @@ PyObject* py_pages_trim(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int64_t page = whole(args[2]);
   const On on(t.device);
   const hipStream_t st = stream_of(t.device);
-  call("trimPages", [&] { return L.pages_trim(&t.t, lens, page, st); });
+  call("trimPages", [&] { return L.pages_trim(&t.t, lens, page, st); }, nullptr, &tables_turn);
   return PyBool_FromLong(1);   // (None: arguments that are not in normal form)
   MH_END
 }

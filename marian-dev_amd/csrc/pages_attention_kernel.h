@@ -92,22 +92,6 @@ __device__ __forceinline__ PagesPlace pages_look(const PagesAttentionArgs& a, co
   return PagesPlace{table[min(j, (unsigned)a.row - 1)] | (j < (unsigned)a.row ? 0 : (int)0x80000000), (int)within};   // (behind the row: none)
 }
 
-// Adds the infinities and NaN among position k's values to the rows that see it.
-template <typename T, int DP, int QT>
-__device__ __forceinline__ void pages_add_odd(const T* v, int dk, int k, int g, const CacheSight (&sight)[QT], cache_f4 (&o)[QT][DP / 16]) {
-  constexpr int kTogether = Pages<T, DP>::kTogether;
-#pragma unroll
-  for(int j = 0; j < DP / 16; ++j)
-#pragma unroll
-    for(int e = 0; e < 4; ++e) {
-      const int d = (16 * (j / kTogether) + 4 * g + e) * kTogether + j % kTogether;
-      const float z = to_float(v[d < dk ? d : 0]);
-#pragma unroll
-      for(int t = 0; t < QT; ++t)
-        if(k < sight[t].limit && d < dk && !(__builtin_fabsf(z) < __builtin_huge_valf())) o[t][j][e] += z;
-    }
-}
-
 // The weights of a lane's eight scores, 2^(score * scale + from), in two terms of T, and their sum.
 template <typename T>
 __device__ __forceinline__ void pages_weights(const cache_f4 (&s)[2], float scale, float from, float& sum, cache_u4 (&w)[2]) {
@@ -221,6 +205,60 @@ __device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const 
     }
   }
   if(!out.whole) cache_join_parts<T, DP, 16 * QT, WAVES>(a, x, out, sh.parts);
+}
+
+// Infinities and NaN among values: a result that sees one is that, of whatever weight, and the sum of them where there are several.  The product
+// does not give that - a weight is in two terms, one of which may be zero or below it -, and what a row does not see must not be in
+// it.  So where the wave left some out, or has a result that is none, it looks at its positions once more: `eights` of them, `step` apart.
+template <typename T, int DP, int QT>
+__device__ __forceinline__ void pages_odd_values(const PagesAttentionArgs& a, const int* table, const unsigned char* v_head, int row_bytes, int begin, int end,
+                                                 int eights, int step, int lane, bool left_out, const CacheSight (&sight)[QT], cache_f4 (&o)[QT][DP / 16]) {
+  constexpr int kTogether = Pages<T, DP>::kTogether, kBits = (DP / 4 + 31) / 32;
+  float none = 0.0f;   // NaN where a result is none
+#pragma unroll
+  for(int t = 0; t < QT; ++t)
+#pragma unroll
+    for(int j = 0; j < DP / 16; ++j)
+#pragma unroll
+      for(int e = 0; e < 4; ++e) none += o[t][j][e] * 0.0f;
+  if(!left_out && !__any(!(none == 0.0f))) return;
+  const int g = lane >> 4;
+  unsigned has[QT][kBits] = {};   // results that have seen one
+#pragma unroll 1
+  for(int at = begin; at < end; at += step)
+#pragma unroll 1
+    for(int first = at; first < min(at + 8 * eights, end); first += 8) {
+      const PagesPlace y = pages_look(a, table, (unsigned)first >> 3);
+      if((unsigned)y.id >= (unsigned)a.pages) continue;
+      const unsigned char* const rows = v_head + y.id * a.page_bytes + (long long)(8 * y.eight) * row_bytes;
+      const int bytes = min(8, end - first) * row_bytes;
+      bool odd = false;
+#pragma unroll 1
+      for(int i = 16 * lane; i < bytes; i += 1024) {
+        const cache_u4 w = *reinterpret_cast<const cache_u4*>(rows + i);
+#pragma unroll
+        for(int e = 0; e < 4; ++e) odd |= pages_finite<T>(w[e]) != w[e];
+      }
+      if(!__any(odd)) continue;
+#pragma unroll 1
+      for(int k = 0; k < min(8, end - first); ++k) {
+        const T* const v = reinterpret_cast<const T*>(rows + k * row_bytes);
+#pragma unroll
+        for(int j = 0; j < DP / 16; ++j)
+#pragma unroll
+          for(int e = 0; e < 4; ++e) {
+            const int d = (16 * (j / kTogether) + 4 * g + e) * kTogether + j % kTogether, bit = 4 * j + e;
+            const float z = to_float(v[d < a.dk ? d : 0]);
+            if(__builtin_fabsf(z) < __builtin_huge_valf() || d >= a.dk) continue;
+#pragma unroll
+            for(int t = 0; t < QT; ++t) {
+              if(first + k >= sight[t].limit) continue;
+              o[t][j][e] = has[t][bit / 32] >> (bit % 32) & 1 ? o[t][j][e] + z : z;
+              has[t][bit / 32] |= 1u << (bit % 32);
+            }
+          }
+      }
+    }
 }
 
 template <typename T, int DP, bool WHOLE, int QT, int WAVES>
@@ -438,17 +476,7 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
     k_next = look_keys(at + 2 * kTurn);
     v_next = look_values(at + 2 * kTurn);
   }
-  // What was left out goes to the rows that see it: of any weight an infinity is one, and a NaN is one.
-  if(left_out) {
-#pragma unroll 1
-    for(int at = begin; at < end; at += kTurn)
-#pragma unroll 1
-      for(int k = max(at, x.open); k < min(at + 32, end); ++k) {
-        const PagesPlace y = pages_look(a, table, (unsigned)k >> 3);
-        if((unsigned)y.id >= (unsigned)a.pages) continue;
-        pages_add_odd<T, DP, QT>(reinterpret_cast<const T*>(v_head + y.id * a.page_bytes + (long long)(8 * y.eight + (k & 7)) * row_bytes), a.dk, k, g, sight, o);
-      }
-  }
+  pages_odd_values<T, DP, QT>(a, table, v_head, row_bytes, begin, end, 4, kTurn, lane, left_out, sight, o);
   pages_finish<T, DP, QT, WAVES>(a, x, o, top, sum, wave, sh);
 }
 
@@ -693,15 +721,7 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
     look(even, at + 3 * kTile);
     pages_lds_barrier();
   }
-  // What was left out goes to the rows that see it: of any weight an infinity is one, and a NaN is one.
-  if(sh.tile.left_out) {
-#pragma unroll 1
-    for(int k = max(begin, x.open); k < end; ++k) {
-      const PagesPlace y = pages_look(a, table, (unsigned)k >> 3);
-      if((unsigned)y.id >= (unsigned)a.pages) continue;
-      pages_add_odd<T, DP, QT>(reinterpret_cast<const T*>(v_head + y.id * a.page_bytes + (long long)(8 * y.eight + (k & 7)) * row_bytes), a.dk, k, g, sight, o);
-    }
-  }
+  pages_odd_values<T, DP, QT>(a, table, v_head, row_bytes, begin, end, kTile / 8, kTile, lane, sh.tile.left_out != 0, sight, o);
   // Rows of a sequence in one part go to the output.  Parts go to the workspace as registers have them, 1 KB at a time, and back: whoever
   // arrives last joins them, a wave its own rows (16 parts of 64 rows: 20 us less than by rows of 16 threads, which store and load pieces of 8 bytes).
   const CacheOut<T, DP, 64 * QT> out(a, x);

@@ -207,6 +207,27 @@ def test_parts_stay_within_grid_and_workspace(tmp_path):
             assert sum(parts) <= items and several <= slots and several < 4096, (s, target, longest)
 
 
+def test_the_shapes_that_are_tested_launch_every_form(tmp_path):
+    """What test_pages_gpu.py takes for all forms, against the launcher's choice: type, values of a row, whole or not, sixteens of rows, waves, and
+    positions shared in LDS"""
+    source = open(os.path.join(ROOT, "tests", "test_pages_gpu.py")).read()
+    names = {}
+    exec(next(l for l in source.splitlines() if l.startswith("FORMS = ")), names)
+    (tmp_path / "plan.cpp").write_text(PLAN.replace('"%d %d %d %d %lld', '"%d %d %d %d %d %d %lld').replace("p.dp, p.tile_rows,", "p.many, p.qt, p.dp, p.tile_rows,"))
+    exe = tmp_path / "plan"
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(ROOT, PKG, "csrc"), "-o", str(exe), str(tmp_path / "plan.cpp")], check=True)
+    cases = [(s, 2 if s < 100 else 4, (2 if s < 100 else 4) * group, n, dk, width) for dk, group, n, s in names["FORMS"] for width in (2, 4)]
+    out = subprocess.run([str(exe)], input="\n".join(" ".join(map(str, c)) for c in cases), capture_output=True, text=True, check=True).stdout
+    got = set()
+    for (s, h, hq, n, dk, width), line in zip(cases, out.splitlines()):
+        many, qt, dp, tile, waves = map(int, line.split()[:5])
+        got.add((width, dp, dk == dp, many, qt, 4 if many else waves))
+    want = {(w, dp, whole, 0, qt, waves) for w in (2, 4) for dp in (64, 128, 256) for whole in (True, False) for qt in (1, 2) for waves in (1, 4)
+            if not (w == 4 and dp == 256 and qt == 2)}
+    want |= {(2, dp, whole, 1, qt, 4) for dp in (64, 128) for whole in (True, False) for qt in (1, 2)}
+    assert got == want
+
+
 # ---- what the verification gives ----------------------------------------------------------------------------
 @pytest.mark.parametrize("form", ["drawn", "best", "tree"])
 def test_verified_words_are_distributed_as_the_targets(form):

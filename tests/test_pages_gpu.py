@@ -115,6 +115,36 @@ def test_attention(dtype, S, heads, group, n, dk, page, lens):
     check(pages.AttentionOverPages(q, kv, wide[:, :row], ints(lens), scale=0.5), want, tol)
 
 
+FORMS = [(dk, group, n, seqs) for dk in (64, 48, 128, 80, 256, 144) for group, n in ((1, 1), (5, 4), (8, 7), (16, 6)) for seqs in (3, 1030)]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dk,group,n,S", FORMS)
+def test_every_form_of_the_attention(dtype, dk, group, n, S):
+    """(tests/test_pages.py asks the plan whether these launch them all); few sequences with long contexts in several parts, or many of one wave"""
+    pages, r = load("pages"), maker(dk + n)
+    heads, page = (2, 32) if S < 100 else (4, 8)
+    lens = [(700, 0, 1400)[s % 3] if S < 100 else s % 12 for s in range(S)]
+    row = 60 if S < 100 else 5
+    table = dealt(7, [l + n for l in lens], page, row, S * row)
+    kv = poisoned(r, table, [l + n for l in lens], page, S * row, heads, dk, dtype) if S < 100 else None
+    if kv is None:   # (written at once: NaN behind the last token of every page)
+        kv = pages.newPagedCache(S * row, heads, page, dk, dtype)
+        kv.k.fill_(float("nan"))
+        kv.v.fill_(float("nan"))
+        longest = max(lens) + n
+        slots = torch.full((S, longest), -1, dtype=torch.int32)
+        for s in range(S):
+            for i in range(lens[s] + n):
+                slots[s, i] = table[s][i // page] * page + i % page
+        pages.writePages(kv, side_by_side(r, S, heads, longest, dk, dtype), side_by_side(r, S, heads, longest, dk, dtype), slots.cuda())
+    q = side_by_side(r, S, heads * group, n, dk, dtype)
+    got = pages.AttentionOverPages(q, kv, ints(table), ints(lens))
+    some = list(range(0, S, 1 if S < 100 else 29))   # (the oracle takes its time)
+    check(got[some], *expected(q[some], kv, ints(table)[some], [lens[s] for s in some]))
+    assert torch.isfinite(got).all()
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_attention_of_many_short_sequences(dtype):
     """(a workgroup of one wave to each)"""
@@ -171,10 +201,11 @@ def test_pages_that_are_none_are_not_seen(dtype):
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("dk", [64, 128, 256])
 @pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
-def test_what_a_token_does_not_see_is_not_in_its_result(dtype, dk, bad):
-    """A chain of five tokens, the fourth of which holds an infinity or NaN in some places: the first three are as without it"""
+@pytest.mark.parametrize("group,n", [(4, 5), (8, 7), (8, 20)])
+def test_what_a_token_does_not_see_is_not_in_its_result(dtype, dk, bad, group, n):
+    """A chain of tokens, the fourth of which holds an infinity or NaN in some places: the first three are as without it"""
     pages, r = load("pages"), maker(6)
-    heads, group, n, page = 2, 4, 5, 8
+    heads, page = 2, 8
     for past in (0, 26, 60, 130):
         row = 20
         table = dealt(4, [past + n], page, row, row)
@@ -189,9 +220,16 @@ def test_what_a_token_does_not_see_is_not_in_its_result(dtype, dk, bad):
         want, tol = expected(q, kv, ints(table), [past])
         assert not torch.isfinite(want[0, :, 3:]).all()
         check(got, want, torch.where(torch.isfinite(want), tol, torch.zeros_like(tol)))
+        if past:   # ... and a settled one, that all see
+            kv.v[table[0][past // 2 // page], 1, past // 2 % page, 7] = bad
+            got = pages.AttentionOverPages(q, kv, ints(table), ints([past]))
+            want, tol = expected(q, kv, ints(table), [past])
+            assert not torch.isfinite(want[0, group:, :, 7]).any()
+            check(got, want, torch.where(torch.isfinite(want), tol, torch.zeros_like(tol)))
+            clean = got
         kv.k[p, :, at] = bad
         got = pages.AttentionOverPages(q, kv, ints(table), ints([past]))
-        assert same(got[:, :, :3], clean[:, :, :3]) and torch.isnan(got[0, :group, 4, 5]).all()
+        assert same(got[:, :, :3].nan_to_num(), clean[:, :, :3].nan_to_num()) and torch.isnan(got[0, :group, 4:, 5]).all()
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
@@ -295,6 +333,9 @@ def test_nothing_to_deal():
     P = load("pages")
     tables = P.newPageTables(3, 2, 4)
     assert P.reservePages(tables, ints([0, 0, 0]), 0, 8).shape == (3, 0)
+    kv, none = P.newPagedCache(4, 2, 8, 64), torch.zeros(3, 2, 0, 64, device="cuda")
+    P.writePages(kv, none, none, P.reservePages(tables, ints([0, 0, 0]), 0, 8))
+    assert P.AttentionOverPages(none, kv, tables.table, ints([0, 0, 0])).shape == (3, 2, 0, 64)
     empty = P.newPageTables(0, 2, 4)
     assert P.reservePages(empty, ints([]), 5, 8).shape == (0, 5)
     P.trimPages(empty, ints([]), 8)
@@ -455,6 +496,27 @@ def test_a_recorded_step_is_replayed():
         step(scratch, *turns[0])
         scratch = fresh()
     assert all(same(a, b) for a, b in zip((*state[0], *state[1], state[2]), end))
+
+
+def test_threads_that_share_tables():
+    """Two threads on one stream and the same tables, calls of two launches: each call is one piece, so no page is dealt twice"""
+    P = load("pages")
+    S, page, pages, row = 700, 8, 20000, 60
+    tables = P.newPageTables(S, row, pages)
+    lens, counts = ints([0] * S), [ints([(31 * s + 7 * t) % 400 for s in range(S)]) for t in range(2)]
+
+    def work(t):
+        for _ in range(30):
+            P.reservePages(tables, lens, 400, page, counts[t])
+            P.trimPages(tables, counts[t] // 2, page)
+    threads = [threading.Thread(target=work, args=(t,)) for t in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    held, free = tables.held.tolist(), tables.free.tolist()[:tables.freeCount.item()]
+    owned = [p for s, line in enumerate(tables.table.tolist()) for p in line[:held[s]]]
+    assert sorted(owned + free) == list(range(pages))
 
 
 def test_calls_of_several_threads_and_streams():
