@@ -9,6 +9,7 @@
 
 #include "abi_common.h"
 #include "cache_args.h"
+#include "cache_attention_kernel.h"
 #include "pages_attention.h"
 
 using namespace marian_hip;
@@ -40,82 +41,70 @@ __device__ __forceinline__ int pages_moved(const TablesArgs& a, int s, int& firs
   }
 }
 
-constexpr int kDealers = 1024;   // threads of a workgroup that deals
+constexpr int kDealers = 1024;   // threads of a workgroup that deals, a sequence each at a time
 
-// Where the pages of all sequences lie in one line of them: an exclusive sum over the sequences, in the workgroup's threads (each has
-// the same number of sequences that follow each other) and in LDS.
+// What a workgroup knows of the sequences it deals for.
 struct Dealt {
-  int before[kDealers + 1];
+  int before[kDealers + 1];   // where their pages lie in one line of all of them
+  int first[kDealers], len[kDealers], count[kDealers];
   int waves[kDealers / 64];
-  int granted;
+  int most;
 };
-template <bool TRIM>
-__device__ __forceinline__ void pages_line(const TablesArgs& a, Dealt& sh, int each) {
-  const int tid = threadIdx.x, lane = tid & 63, s0 = tid * each;
-  int mine = 0, first;
-  for(int s = s0; s < min(s0 + each, a.S); ++s) mine += pages_moved<TRIM>(a, s, first);
-  int sum = mine;
-#pragma unroll
-  for(int o = 1; o < 64; o <<= 1) {
-    const int other = __shfl_up(sum, o, 64);
-    if(lane >= o) sum += other;
-  }
-  if(lane == 63) sh.waves[tid >> 6] = sum;
-  if(tid == 0) sh.granted = 0;
+
+// The sum of x over the threads before this one; all: over all of them.  In the end `waves` has been read.
+__device__ __forceinline__ int dealers_sum_before(Dealt& sh, int x, int& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int sum = (int)lanes_sum((unsigned)x);
+  if(lane == 63) sh.waves[wave] = sum;
   __syncthreads();
   int ahead = 0;
-  for(int i = 0; i < tid >> 6; ++i) ahead += sh.waves[i];
-  sh.before[tid] = ahead + sum - mine;
-  if(tid == kDealers - 1) sh.before[kDealers] = ahead + sum;
-  __syncthreads();
-}
-
-// The number of the line's first pages that are dealt: up to the first sequence that the free ones do not reach for.
-__device__ __forceinline__ void pages_grant(const TablesArgs& a, Dealt& sh, int each, int available) {
-  const int s0 = threadIdx.x * each;
-  int at = sh.before[threadIdx.x], most = 0, first;
-  for(int s = s0; s < min(s0 + each, a.S); ++s) {
-    const int more = pages_moved<false>(a, s, first);
-    at += more;
-    if(more > 0 && at <= available) most = at;
+  all = 0;
+#pragma unroll
+  for(int i = 0; i < kDealers / 64; ++i) {
+    if(i == wave) ahead = all;
+    all += sh.waves[i];
   }
-  if(most > 0) atomicMax(&sh.granted, most);
   __syncthreads();
+  return ahead + sum - x;
 }
 
-__device__ __forceinline__ int slot_of(const TablesArgs& a, unsigned id) {
-  unsigned i, within;
-  const int s = (int)a.by_n.of(id, i);
-  const unsigned at = (unsigned)max(a.lens[s], 0) + i, j = a.by_page.of(at, within);
-  const int count = a.counts ? a.counts[s] : a.n, page = a.table[(long long)s * a.row + min(j, (unsigned)a.row - 1)];
-  return (int)i < count && j < (unsigned)a.row && (unsigned)page < (unsigned)a.pages ? page * a.page + (int)within : -1;
-}
-
-// Moves the pages (MOVE) - a thread to each of the line, found by bisection -, and settles the counts and the map of slots (SETTLE).  One
-// workgroup does all of it where there is little; else many move, each with a line of its own, and a second launch settles, for until
-// all have read the counts none may write them.  Small calls are a launch and a chain of steps (lengths, sum, search, page, store, load of
-// the table, store); the others' time is the slots' stores.
+// Deals pages and maps slots, or takes pages back (MOVE), and settles the counts (SETTLE).  Where there is little one workgroup does all of it; else
+// many move, each finding the sequences' places in the line by itself, and a second launch of one workgroup settles, for until all have
+// read the counts none may write them.  A slot's page comes from the stack where the table does not have it yet, so nothing waits for
+// the table.  Small calls are a launch and a chain of steps (lengths, sum, page, store): 6 sequences 2.8 us, 2.1 to take back.  513 prompts of up to 2047
+// tokens 7.2 us and 4.4 to settle, 3.9 and 2.1 to take back, 256 workgroups (128: 9.1, 512: 8.8); their 4 MB of slots are 1 us of it.
 template <bool TRIM, bool MOVE, bool SETTLE>
 __global__ __launch_bounds__(kDealers) void pages_deal_kernel(TablesArgs a) {
   __shared__ Dealt sh;
-  const int tid = threadIdx.x;
-  if(MOVE || blockIdx.x == 0) {
-    const int each = (a.S + kDealers - 1) / kDealers, available = clamp_int(*a.free_count, 0, a.pages);
-    pages_line<TRIM>(a, sh, each);
-    if(!TRIM) pages_grant(a, sh, each, available);
-    const int all = TRIM ? sh.before[kDealers] : sh.granted;
-    int first;
+  const int tid = threadIdx.x, available = clamp_int(*a.free_count, 0, a.pages);
+  int all = 0, carry = 0, dealt = 0, first;
+  if(TRIM && a.S > kDealers) {   // (the last page of the line goes to the bottom)
+    int mine = 0;
+    for(int s = tid; s < a.S; s += kDealers) mine += pages_moved<TRIM>(a, s, first);
+    dealers_sum_before(sh, mine, all);
+  }
+  for(int base = 0; base < a.S; base += kDealers) {
+    const int s = base + tid, here = min(kDealers, a.S - base);
+    const int more = tid < here ? pages_moved<TRIM>(a, s, first) : 0;
+    int sum;
+    const int mine = carry + dealers_sum_before(sh, more, sum);
+    if(tid < here) {
+      sh.before[tid] = mine;
+      sh.first[tid] = first;
+      if(!TRIM) {
+        sh.len[tid] = max(a.lens[s], 0);
+        sh.count[tid] = a.counts ? a.counts[s] : a.n;
+      }
+    }
+    if(tid == 0) sh.before[here] = carry + sum;
+    if(TRIM && a.S <= kDealers) all = sum;
+    if(!TRIM && mine + more <= available && more > 0) dealt = mine + more;
+    __syncthreads();
     if constexpr(MOVE) {
-      for(int t = blockIdx.x * kDealers + tid; t < all; t += gridDim.x * kDealers) {
-        int u = 0;
-#pragma unroll
-        for(int step = kDealers / 2; step > 0; step >>= 1) u += sh.before[u + step] <= t ? step : 0;
-        int s = u * each, j = t - sh.before[u], more = pages_moved<TRIM>(a, s, first);
-        while(j >= more) {
-          j -= more;
-          more = pages_moved<TRIM>(a, ++s, first);
-        }
-        int* const entry = a.table + (long long)s * a.row + first + j;
+      // A thread to a sequence where each has few pages, or a wave.
+      auto move = [&](int q, int j) __attribute__((always_inline)) {
+        int* const entry = a.table + (long long)(base + q) * a.row + sh.first[q] + j;
+        const int t = sh.before[q] + j;
         if constexpr(TRIM) {
           const long long to = (long long)available + all - 1 - t;
           if(to < a.pages) a.free[to] = *entry;
@@ -123,26 +112,43 @@ __global__ __launch_bounds__(kDealers) void pages_deal_kernel(TablesArgs a) {
         } else {
           *entry = a.free[available - 1 - t];
         }
+      };
+      const int each = TRIM ? 64 : a.n / a.page > 8 ? 64 : 1;
+      for(int q = (blockIdx.x * kDealers + tid) / each; q < here; q += gridDim.x * kDealers / each) {
+        const int pages = sh.before[q + 1] - sh.before[q];
+        if(!TRIM && sh.before[q + 1] > available) continue;
+        for(int j = tid % each; j < pages; j += each) move(q, j);
       }
-      __syncthreads();   // (before anybody's count changes; the slots below read the table)
+      if constexpr(!TRIM) {
+        const unsigned ids = (unsigned)here * a.n;
+        for(unsigned id = blockIdx.x * kDealers + tid; id < ids; id += gridDim.x * kDealers) {
+          unsigned i, within;
+          const int q = (int)a.by_n.of(id, i), j = (int)a.by_page.of((unsigned)sh.len[q] + i, within), k = j - sh.first[q];
+          int page = -1;
+          if((int)i < sh.count[q] && j < a.row) {
+            const bool fresh = k >= 0 && sh.before[q + 1] <= available && k < sh.before[q + 1] - sh.before[q];
+            const int* const from = fresh ? a.free + (available - 1 - sh.before[q] - k) : a.table + (long long)(base + q) * a.row + j;
+            page = *from;
+          }
+          a.slots[(long long)base * a.n + id] = (unsigned)page < (unsigned)a.pages ? page * a.page + (int)within : -1;
+        }
+      }
     }
+    carry += sum;
     if constexpr(SETTLE) {
-      int at = sh.before[tid];
-      for(int s = tid * each; s < min((tid + 1) * each, a.S); ++s) {
-        const int more = pages_moved<TRIM>(a, s, first);
-        at += more;
+      if(tid < here) {
         if(TRIM) a.held[s] = first;
-        else if(more > 0 && at <= available) a.held[s] = first + more;
+        else if(more > 0 && mine + more <= available) a.held[s] = first + more;
       }
-      if(tid == 0) *a.free_count = TRIM ? (int)min((long long)available + all, (long long)a.pages) : available - all;
     }
+    __syncthreads();   // (the places in LDS are read)
   }
-  if constexpr(SETTLE && !TRIM) {
-    const unsigned all = (unsigned)a.S * a.n;
-    // (in a second launch the first workgroup is busy with the counts)
-    const unsigned groups = MOVE ? 1 : gridDim.x - 1, group = MOVE ? 0 : blockIdx.x - 1;
-    if(MOVE || blockIdx.x > 0)
-      for(unsigned id = group * kDealers + tid; id < all; id += groups * kDealers) a.slots[id] = slot_of(a, id);
+  if constexpr(SETTLE) {
+    if(tid == 0) sh.most = 0;
+    __syncthreads();
+    if(!TRIM && dealt > 0) atomicMax(&sh.most, dealt);
+    __syncthreads();
+    if(tid == 0) *a.free_count = TRIM ? (int)min((long long)available + all, (long long)a.pages) : available - sh.most;
   }
 }
 
@@ -158,7 +164,8 @@ struct WriteArgs {
 };
 
 // A thread takes a piece of sixteen bytes of a row of keys and of values, kWriteTurns times, all asked for before the first is stored.  A copy:
-// memory bounds it.
+// memory bounds it.  3 prompts of 2731 tokens, 8 heads of 128 values, bfloat16: 10.8 us, 6.2 TB/s (a large copy: 5.1; these 67 MB stay in the last
+// cache); 128 single tokens of 16 heads of 64 values, float32: 2.6 us, a launch and three steps.
 constexpr int kWriteTurns = 2;
 __global__ __launch_bounds__(256) void pages_write_kernel(const unsigned char* __restrict__ k, const unsigned char* __restrict__ v, WriteArgs a) {
   cache_u4 x[kWriteTurns][2];
@@ -256,13 +263,14 @@ int marian_hip_pages_reserve(const marian_hip_page_tables* tables, const int32_t
   MH_CHECK(check_tables_memory(tables, lens, counts, slots, 4 * tables->sequences * n));
   const TablesArgs a = tables_args(tables, lens, counts, n, page, slots);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t all = tables->sequences * n, moved = tables->sequences * ((n + page - 1) / page + 1);
-  if(all <= 8 * kDealers && moved <= 4 * kDealers) {
+  // One workgroup for up to eight slots a thread: 1024 sequences' two tokens 5.6 us, where two launches take some 9.
+  const int64_t all = std::min<int64_t>(tables->sequences, kDealers) * n;   // (slots of one turn)
+  if(tables->sequences * n <= 8 * kDealers) {
     MH_LAUNCH((pages_deal_kernel<false, true, true>), dim3(1), dim3(kDealers), 0, st, a);
     return MARIAN_HIP_OK;
   }
-  MH_LAUNCH((pages_deal_kernel<false, true, false>), dim3((unsigned)std::min<int64_t>(64, (moved + kDealers - 1) / kDealers)), dim3(kDealers), 0, st, a);
-  MH_LAUNCH((pages_deal_kernel<false, false, true>), dim3((unsigned)(1 + std::min<int64_t>(1024, (all + kDealers - 1) / kDealers))), dim3(kDealers), 0, st, a);
+  MH_LAUNCH((pages_deal_kernel<false, true, false>), dim3((unsigned)std::min<int64_t>(256, (all + kDealers - 1) / kDealers)), dim3(kDealers), 0, st, a);
+  MH_LAUNCH((pages_deal_kernel<false, false, true>), dim3(1), dim3(kDealers), 0, st, a);
   return MARIAN_HIP_OK;
 }
 
@@ -272,12 +280,13 @@ int marian_hip_pages_trim(const marian_hip_page_tables* tables, const int32_t* l
   MH_CHECK(check_tables_memory(tables, lens, nullptr, nullptr, 0));
   const TablesArgs a = tables_args(tables, lens, nullptr, 0, page, nullptr);
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  // (how many pages go back only the device knows: the room for them stands for it)
   const int64_t moved = std::min(tables->sequences * tables->row, tables->pages);
   if(moved <= 4 * kDealers) {
     MH_LAUNCH((pages_deal_kernel<true, true, true>), dim3(1), dim3(kDealers), 0, st, a);
     return MARIAN_HIP_OK;
   }
-  MH_LAUNCH((pages_deal_kernel<true, true, false>), dim3((unsigned)std::min<int64_t>(64, (moved + kDealers - 1) / kDealers)), dim3(kDealers), 0, st, a);
+  MH_LAUNCH((pages_deal_kernel<true, true, false>), dim3((unsigned)std::min<int64_t>(64, (std::min<int64_t>(tables->sequences, kDealers) + 15) / 16)), dim3(kDealers), 0, st, a);
   MH_LAUNCH((pages_deal_kernel<true, false, true>), dim3(1), dim3(kDealers), 0, st, a);
   return MARIAN_HIP_OK;
 }

@@ -54,15 +54,16 @@ inline PagesAttentionPlan pages_attention_plan(int64_t sequences, int64_t heads,
   p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const int64_t entries = sequences * heads * p.row_tiles;
   p.waves = !p.many && entries >= 4096 ? 1 : 4;
-  // Parts for one round of the workgroups that run at a time, by the registers of their form; of 16-bit values for half of them, which have the memory
-  // as busy and fewer parts to join.  One token of 8 heads with four rows each, 128 values, all and half: 100003 positions 79.4 and 75.7 us, 4
-  // sequences of up to 16000 44.8 and 42.2, 16 of up to 32768 264 and 268; 4 drafted tokens, 4 heads with eight rows each, 16 sequences of up
-  // to 8192 51.4 and 45.0.  Not where rows leave many lanes without a load (80 values, 8192: 51.8 and 57.0), nor of float32 (64 values, 16384: 83.4
-  // and 88.2), nor of the form that shares positions in LDS (7 tokens, 24 sequences 75 and 108).
+  // Parts for one round of the workgroups that run at a time, by the registers of their form, half a part for each sequence left out.  Of 16-bit values
+  // half of them have the memory as busy, and leave fewer parts to join: where that makes two parts of a sequence.  One token, 8 heads with four
+  // rows each, 128 values, all and half, over ten sets of lengths: 100003 positions 80.2 and 77.6 us, 4 sequences of up to 16000 44.2 and 42.0, 8
+  // 75.1 and 72.4, but 16 of up to 32768 264 and 291; 4 drafted tokens, 4 heads with eight rows each, 16 of up to 16384 81.3 and 77.2, 40 of up to
+  // 8192 96.9 and 101.  Not where rows leave many lanes without a load (80 values, 16 of up to 8192: 51.8 and 57.0), nor of float32 (64 values,
+  // 16384: 83.4 and 88.2), nor of the form that shares positions in LDS (7 tokens, 24 of up to 8192: 75 and 108).
   const int to_a_simd = p.many ? 2 : pages_to_a_simd(width, p.dp, p.qt);
-  const bool half = width == 2 && !p.many && to_a_simd > 1 && 4 * dk > 3 * p.dp;
-  const int64_t at_a_time = 1024 * (half ? to_a_simd / 2 : to_a_simd) / p.waves;
-  p.target = std::max<int64_t>(1, at_a_time / (heads * p.row_tiles) - sequences / 2);
+  auto parts_of = [&](int64_t at_a_time) { return std::max<int64_t>(1, at_a_time / (heads * p.row_tiles) - sequences / 2); };
+  const int64_t all = parts_of(1024 * to_a_simd / p.waves), half = parts_of(512 * to_a_simd / p.waves);
+  p.target = width == 2 && !p.many && to_a_simd > 1 && 4 * dk > 3 * p.dp && half >= 2 * sequences ? half : all;
   // A sequence of up to four blocks stays whole, and where no row of the table has room for more nobody looks at the others' lengths (6 sequences
   // of up to 120 positions, 8 heads of 64 values, float32: 6.7 and 6.0 us).  Nor where these are many: their parts would be few, and a look at them
   // costs every workgroup a load for 64 of them.
