@@ -244,17 +244,22 @@ __device__ __forceinline__ void pages_odd_values(const PagesAttentionArgs& a, co
       for(int k = 0; k < min(8, end - first); ++k) {
         const T* const v = reinterpret_cast<const T*>(rows + k * row_bytes);
 #pragma unroll
-        for(int j = 0; j < DP / 16; ++j)
+        for(int i = 0; i < DP / 16 / kTogether; ++i)
 #pragma unroll
           for(int e = 0; e < 4; ++e) {
-            const int d = (16 * (j / kTogether) + 4 * g + e) * kTogether + j % kTogether, bit = 4 * j + e;
-            const float z = to_float(v[d < a.dk ? d : 0]);
-            if(__builtin_fabsf(z) < __builtin_huge_valf() || d >= a.dk) continue;
+            const int d = (16 * i + 4 * g + e) * kTogether;
+            float z[kTogether];
+            load_row<kTogether>(v + (d < a.dk ? d : 0), z);
 #pragma unroll
-            for(int t = 0; t < QT; ++t) {
-              if(first + k >= sight[t].limit) continue;
-              o[t][j][e] = has[t][bit / 32] >> (bit % 32) & 1 ? o[t][j][e] + z : z;
-              has[t][bit / 32] |= 1u << (bit % 32);
+            for(int j = 0; j < kTogether; ++j) {
+              const int piece = i * kTogether + j, bit = 4 * piece + e;
+              if(__builtin_fabsf(z[j]) < __builtin_huge_valf() || d >= a.dk) continue;
+#pragma unroll
+              for(int t = 0; t < QT; ++t) {
+                if(first + k >= sight[t].limit) continue;
+                o[t][piece][e] = has[t][bit / 32] >> (bit % 32) & 1 ? o[t][piece][e] + z[j] : z[j];
+                has[t][bit / 32] |= 1u << (bit % 32);
+              }
             }
           }
       }
@@ -481,18 +486,25 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
 }
 
 // ---- more than 32 rows
-// Four waves have 16 * QT rows each and share positions laid out in LDS, 64 at a time, twice: while one is worked on, the next is written and
-// the one after that is on its way to registers.  Keys lie there as they are, values transposed, a dimension's 64 side by side; pieces of 16
-// bytes change places within a row so that eight lanes that read together meet in no bank:
-//   key k, piece i at i ^ k (rows of 256 bytes), i ^ k / 2 (128 bytes); dimension d, eight positions j at j ^ d / kTogether.
-// A wave lays out sixteen positions: sixteen lanes (eight) to a row of keys; of values each lane has DP / 32 dimensions of eight positions.
-// Products, weights and sums are those above.
-template <typename T, int DP>
+// Waves have 16 * QT rows each and share positions laid out in LDS, 64 at a time, twice: while one is worked on, the next is written and the
+// one after that is on its way to registers.  With sixteen rows to a wave (QT == 1) eight waves take 64 rows, four of them the first 32
+// positions of each 64 and four the second (SPLIT == 2); with 32 rows, 128 of them, four waves take all 64 positions (a second half would not fit
+// the registers).  Keys lie in LDS as they are, values transposed, a dimension's 64 side by side; pieces of 16 bytes change places within a
+// row (key_place, value_place) so that few lanes that read together meet in a bank (a third of the cycles that LDS is busy).  A wave lays out one or two eights of positions:
+// sixteen lanes (of rows of 128 bytes eight) to a row of keys; of values a lane has some dimensions of eight positions.  Products, weights and sums are those above.
+//
+// What bounds it: latency, of the memory's answers and of the partial results' way to the workgroup that joins them; LDS is busy less than a third of
+// the time and the matrix units a fifth.  7 drafted tokens, float16, 24 sequences of up to 8192 positions, 4 heads of 128 values with eight
+// rows each (56 rows, 270 MB): 74 us, 3.6 TB/s; four waves that take all positions and join them 80, waves of the form above with a row
+// group each 95.  bfloat16, 64 values, 8 tokens, 16 sequences: 37 and 39.6.  __syncthreads in place of the barrier below waits for the loads too.
+template <typename T, int DP, int SPLIT>
 struct PagesMany {
   static constexpr int kTile = 64;                        // positions of a turn
   static constexpr int kRowPieces = DP / 8;               // pieces of a key
-  static constexpr int kKeyLoads = kRowPieces / 4;        // of a lane: sixteen keys to a wave
-  static constexpr int kDimsEach = DP / 32;               // of a lane's values
+  static constexpr int kEights = 2 / SPLIT;               // of positions that a wave lays out
+  static constexpr int kKeyLoads = kEights * kRowPieces / 8;       // of a lane
+  static constexpr int kLanes = 64 / kEights;             // that have an eight's values, kDimsEach dimensions each
+  static constexpr int kDimsEach = DP / kLanes < 2 ? 2 : DP / kLanes;
   static constexpr int kValueWords = kDimsEach / 2;
   // (lanes that read together are, by what was measured, the 16 lanes c, of one half of them with g and of the other with g ^ 1)
   static __device__ __forceinline__ int key_place(int key, int piece) {
@@ -509,6 +521,10 @@ struct PagesMany {
     int there[2][8];   // of each eight of positions, whether it has a page
     int left_out;
   };
+  struct Halves {   // what either half of the waves has for the other
+    cache_f4 o[2][4][DP / 32][64];
+    float top[2][4][64], sum[2][4][64];
+  };
 };
 
 // A barrier for what lies in LDS: loads from memory stay under way, which __syncthreads would wait for.
@@ -518,42 +534,49 @@ __device__ __forceinline__ void pages_lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// Halves of positions
+constexpr int pages_many_split(int qt) { return qt == 1 ? 2 : 1; }
+
 template <typename T, int DP, bool WHOLE, int QT>
-__global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAttentionArgs a) {
+__global__ __launch_bounds__(256 * pages_many_split(QT), 2 * pages_many_split(QT)) void pages_attention_many_kernel(PagesAttentionArgs a) {
   using P = Pages<T, DP>;
-  using M = PagesMany<T, DP>;
-  constexpr int kDims = P::kDims, kTogether = P::kTogether, kKeyPieces = P::kKeyPieces, kTile = M::kTile;
+  constexpr int SPLIT = pages_many_split(QT);
+  using M = PagesMany<T, DP, SPLIT>;
+  constexpr int kDims = P::kDims, kTogether = P::kTogether, kKeyPieces = P::kKeyPieces, kTile = M::kTile, kEights = M::kEights, kParts = 2 / SPLIT;
   constexpr float kUnit = P::kUp < 0 ? (float)(1 << -P::kUp * (P::kUp < 0)) : 1.0f / (1 << P::kUp * (P::kUp > 0));   // 2^-kUp
   __shared__ struct {
-    typename M::Shared tile;
+    union {
+      typename M::Shared tile;
+      typename M::Halves half;
+    };
     int is_last;
   } sh;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, any_wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+  const int wave = any_wave % 4, half = any_wave / 4;   // of the rows, of the positions
   CacheTile x;
-  if(!cache_tile<T, DP, 64 * QT, 4, kPagesMostParts>(a, tid, x)) return;
+  if(!cache_tile<T, DP, 64 * QT, 4 * SPLIT, kPagesMostParts>(a, tid, x)) return;
   const int end = x.end, row_bytes = (WHOLE ? DP : a.dk) * 2;
   const int* const table = a.table + (long long)x.w.s * a.row;
   const unsigned char* const k_head = a.k_pages + x.head * a.head_bytes;
   const unsigned char* const v_head = a.v_pages + x.head * a.head_bytes;
   if(tid == 0) sh.tile.left_out = 0;
 
-  // ---- what a wave lays out: the eights 2 * wave and 2 * wave + 1 of a tile
-  // (of two tiles, in turn: a tile's 32 KB on their way to each of two workgroups are too few for a memory that answers after some 4 us under load)
+  // ---- what a wave lays out: the eights of a tile from kEights * any_wave on
   struct Fetched {
     cache_u4 key[M::kKeyLoads];
     unsigned value[8][M::kValueWords];
-    bool there[2];
-    PagesPlace next[2];   // of the tile that is fetched next
-  } even;
+    bool there[kEights];
+    PagesPlace next[kEights];   // of the tile that is fetched next
+  } fetched;
   auto look = [&](Fetched& y, int at) __attribute__((always_inline)) {
 #pragma unroll
-    for(int i = 0; i < 2; ++i) y.next[i] = pages_look(a, table, (unsigned)(at + 16 * wave + 8 * i) >> 3);
+    for(int i = 0; i < kEights; ++i) y.next[i] = pages_look(a, table, (unsigned)(at + 8 * (kEights * any_wave + i)) >> 3);
   };
   auto fetch = [&](Fetched& f, int at) __attribute__((always_inline)) {
-    long long place[2];
+    long long place[kEights];
 #pragma unroll
-    for(int i = 0; i < 2; ++i) {
-      const int first = at + 16 * wave + 8 * i;
+    for(int i = 0; i < kEights; ++i) {
+      const int first = at + 8 * (kEights * any_wave + i);
       const PagesPlace y = f.next[i];
       f.there[i] = (unsigned)y.id < (unsigned)a.pages && first < end;
       place[i] = f.there[i] ? y.id * a.page_bytes + (long long)(8 * y.eight) * row_bytes : 0;
@@ -564,8 +587,8 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
       const int row = kAtOnce * i + lane / M::kRowPieces, piece = lane % M::kRowPieces * 16;
       f.key[i] = *reinterpret_cast<const cache_u4*>(k_head + place[kAtOnce * i / 8] + (row & 7) * row_bytes + (piece < row_bytes ? piece : 0));
     }
-    const int d = lane % 32 * M::kDimsEach * 2;
-    const unsigned char* const from = v_head + (lane < 32 ? place[0] : place[1]) + (d < row_bytes ? d : 0);
+    const int d = lane % M::kLanes * M::kDimsEach * 2;
+    const unsigned char* const from = v_head + (lane < M::kLanes ? place[0] : place[kEights - 1]) + (d < row_bytes ? d : 0);
 #pragma unroll
     for(int e = 0; e < 8; ++e)
 #pragma unroll
@@ -575,13 +598,13 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
     constexpr int kAtOnce = 64 / M::kRowPieces;
 #pragma unroll
     for(int i = 0; i < M::kKeyLoads; ++i) {
-      const int row = 16 * wave + kAtOnce * i + lane / M::kRowPieces, piece = lane % M::kRowPieces;
+      const int row = 8 * kEights * any_wave + kAtOnce * i + lane / M::kRowPieces, piece = lane % M::kRowPieces;
       if(!WHOLE) f.key[i] = piece * 16 < row_bytes ? f.key[i] : cache_u4{0, 0, 0, 0};   // (queries are zero there, and so must these be)
       *reinterpret_cast<cache_u4*>(sh.tile.keys[buffer] + M::key_place(row, piece)) = f.key[i];
     }
-    const int eight = 2 * wave + (lane >> 5), first = at + 8 * eight;
-    const bool is = lane < 32 ? f.there[0] : f.there[1];
-    if(at + kTile > x.open || !(f.there[0] && f.there[1])) {
+    const int eight = kEights * any_wave + lane / M::kLanes, first = at + 8 * eight;
+    const bool is = lane < M::kLanes ? f.there[0] : f.there[kEights - 1];
+    if(at + kTile > x.open || !(f.there[0] && f.there[kEights - 1])) {
       // Values that no row sees weigh zero, whatever they are; infinities and NaN that some do not see are left out, see below.
       const int seen = is ? end - first : 0;
       bool any = false;
@@ -595,20 +618,21 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
         }
       if(any) sh.tile.left_out = 1;
     }
-    if((lane & 31) == 0) sh.tile.there[buffer][eight] = is;
+    if(lane % M::kLanes == 0) sh.tile.there[buffer][eight] = is;
 #pragma unroll
     for(int j = 0; j < M::kDimsEach; ++j) {
       cache_u4 y;
 #pragma unroll
       for(int e = 0; e < 4; ++e) y[e] = __builtin_amdgcn_perm(f.value[2 * e + 1][j / 2], f.value[2 * e][j / 2], j % 2 ? 0x07060302 : 0x05040100);
-      *reinterpret_cast<cache_u4*>(sh.tile.values[buffer] + M::value_place(lane % 32 * M::kDimsEach + j, eight)) = y;
+      const int dim = lane % M::kLanes * M::kDimsEach + j;
+      if(M::kLanes * M::kDimsEach == DP || dim < DP) *reinterpret_cast<cache_u4*>(sh.tile.values[buffer] + M::value_place(dim, eight)) = y;
     }
   };
 
   const int begin = x.w.from;
-  look(even, begin);
-  fetch(even, begin);
-  look(even, begin + kTile);
+  look(fetched, begin);
+  fetch(fetched, begin);
+  look(fetched, begin + kTile);
   cache_u4 q[QT][kKeyPieces];
   CacheSight sight[QT];
 #pragma unroll
@@ -637,9 +661,9 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
     for(int j = 0; j < kDims; ++j) o[t][j] = cache_f4{0, 0, 0, 0};
   }
   pages_lds_barrier();   // (left_out is cleared)
-  lay_out(even, begin, 0);
-  fetch(even, begin + kTile);
-  look(even, begin + 2 * kTile);
+  lay_out(fetched, begin, 0);
+  fetch(fetched, begin + kTile);
+  look(fetched, begin + 2 * kTile);
   pages_lds_barrier();
 
   int buffer = 0;
@@ -651,26 +675,26 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
 #pragma unroll
       for(int i = 0; i < 4; ++i) none |= (lo[i] ? 0 : 1u << i) | (hi[i] ? 0 : 16u << i);
     }
-    cache_f4 s[QT][4];   // two and two for 32 positions
+    cache_f4 s[QT][2 * kParts];   // two for 32 positions
 #pragma unroll
     for(int t = 0; t < QT; ++t)
 #pragma unroll
-      for(int b = 0; b < 4; ++b) s[t][b] = cache_f4{0, 0, 0, 0};
+      for(int b = 0; b < 2 * kParts; ++b) s[t][b] = cache_f4{0, 0, 0, 0};
 #pragma unroll
     for(int i = 0; i < kKeyPieces; ++i)
 #pragma unroll
-      for(int b = 0; b < 4; ++b) {
-        const cache_u4 k = *reinterpret_cast<const cache_u4*>(sh.tile.keys[buffer] + M::key_place(32 * (b / 2) + 8 * (c >> 2) + (c & 3) + 4 * (b % 2), 4 * i + g));
+      for(int b = 0; b < 2 * kParts; ++b) {
+        const cache_u4 k = *reinterpret_cast<const cache_u4*>(sh.tile.keys[buffer] + M::key_place(32 * (half + b / 2) + 8 * (c >> 2) + (c & 3) + 4 * (b % 2), 4 * i + g));
 #pragma unroll
         for(int t = 0; t < QT; ++t) s[t][b] = pages_product<T>(k, q[t][i], s[t][b]);
       }
     if(masked || none) {
 #pragma unroll
-      for(int h = 0; h < 2; ++h) {
-        const int first = at + 32 * h + 8 * g;
+      for(int h = 0; h < kParts; ++h) {
+        const int first = at + 32 * (half + h) + 8 * g;
 #pragma unroll
         for(int t = 0; t < QT; ++t) {
-          const int sees = none >> (4 * h + g) & 1 ? 0 : sight[t].limit - first;
+          const int sees = none >> (4 * (half + h) + g) & 1 ? 0 : sight[t].limit - first;
 #pragma unroll
           for(int e = 0; e < 8; ++e) s[t][2 * h + e / 4][e % 4] = e < sees ? s[t][2 * h + e / 4][e % 4] : kNone;
         }
@@ -682,7 +706,7 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
     for(int t = 0; t < QT; ++t) {
       high[t] = kNone;
 #pragma unroll
-      for(int e = 0; e < 16; ++e) high[t] = fmaxf(high[t], s[t][e / 4][e % 4]);
+      for(int e = 0; e < 8 * kParts; ++e) high[t] = fmaxf(high[t], s[t][e / 4][e % 4]);
       high[t] *= a.scale_log2;
       grown |= high[t] > top[t] + kMaximumSlack;
     }
@@ -699,7 +723,7 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
     }
     // (the second half's weights are made while the first half's products run)
 #pragma unroll
-    for(int h = 0; h < 2; ++h) {
+    for(int h = 0; h < kParts; ++h) {
       cache_u4 weights[QT][2];
 #pragma unroll
       for(int t = 0; t < QT; ++t) {
@@ -709,54 +733,91 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
 #pragma unroll
       for(int j = 0; j < kDims; ++j) {
         const int dim = (16 * (j / kTogether) + c) * kTogether + j % kTogether;
-        const cache_u4 v = *reinterpret_cast<const cache_u4*>(sh.tile.values[buffer] + M::value_place(dim, 4 * h + g));
+        const cache_u4 v = *reinterpret_cast<const cache_u4*>(sh.tile.values[buffer] + M::value_place(dim, 4 * (half + h) + g));
 #pragma unroll
         for(int t = 0; t < QT; ++t)
 #pragma unroll
           for(int m = 1; m >= 0; --m) o[t][j] = pages_product<T>(v, weights[t][m], o[t][j]);
       }
     }
-    if(at + kTile < end) lay_out(even, at + kTile, buffer ^ 1);
-    fetch(even, at + 2 * kTile);
-    look(even, at + 3 * kTile);
+    if(at + kTile < end) lay_out(fetched, at + kTile, buffer ^ 1);
+    fetch(fetched, at + 2 * kTile);
+    look(fetched, at + 3 * kTile);
     pages_lds_barrier();
   }
-  pages_odd_values<T, DP, QT>(a, table, v_head, row_bytes, begin, end, kTile / 8, kTile, lane, sh.tile.left_out != 0, sight, o);
+  pages_odd_values<T, DP, QT>(a, table, v_head, row_bytes, begin + 32 * half, end, 4 * kParts, kTile, lane, sh.tile.left_out != 0, sight, o);
   // Rows of a sequence in one part go to the output.  Parts go to the workspace as registers have them, 1 KB at a time, and back: whoever
   // arrives last joins them, a wave its own rows (16 parts of 64 rows: 20 us less than by rows of 16 threads, which store and load pieces of 8 bytes).
   const CacheOut<T, DP, 64 * QT> out(a, x);
+#pragma unroll
+  for(int t = 0; t < QT; ++t) sum[t] = over_lanes_sum(sum[t]) * kUnit;
+  // Two halves exchange results: of its rows each has kOwn of the kDims pieces from here on, `shift` the first of them.
+  constexpr int kOwn = kDims / SPLIT;
+  const int shift = half * kOwn;
+  cache_f4 r[QT][kOwn];
+  if constexpr(SPLIT == 1) {
+#pragma unroll
+    for(int t = 0; t < QT; ++t)
+#pragma unroll
+      for(int j = 0; j < kOwn; ++j) r[t][j] = o[t][j];
+  } else {
+    pages_lds_barrier();   // (left_out has been read)
+    if(half == 0) {
+#pragma unroll
+      for(int j = 0; j < kOwn; ++j) sh.half.o[0][wave][j][lane] = o[0][kOwn + j];
+    } else {
+#pragma unroll
+      for(int j = 0; j < kOwn; ++j) sh.half.o[1][wave][j][lane] = o[0][j];
+    }
+    sh.half.top[half][wave][lane] = top[0];
+    sh.half.sum[half][wave][lane] = sum[0];
+    pages_lds_barrier();
+    const float other = sh.half.top[1 - half][wave][lane], m = fmaxf(top[0], other);
+    const float mine = top[0] == kNone ? 1.0f : __builtin_amdgcn_exp2f(top[0] - m), its = other == kNone ? 1.0f : __builtin_amdgcn_exp2f(other - m);
+    // (of a half without positions both are 0, or NaN)
+#pragma unroll
+    for(int j = 0; j < kOwn; ++j) {
+      const cache_f4 y[2] = {o[0][j], o[0][kOwn + j]}, z = sh.half.o[1 - half][wave][j][lane] * its;
+#pragma unroll
+      for(int e = 0; e < 4; ++e) r[0][j][e] = (half == 0 ? y[0][e] : y[1][e]) * mine + z[e];
+    }
+    sum[0] = sum[0] * mine + sh.half.sum[1 - half][wave][lane] * its;
+    top[0] = m;
+  }
   auto write = [&](int t, float factor) __attribute__((always_inline)) {
     const int row = x.row0 + 16 * (QT * wave + t) + c;
     if(row >= x.rows) return;
     T* const to = cache_row_out<T>(a, x, row);
+    constexpr int kRun = kTogether < kOwn ? kTogether : kOwn;   // values side by side
 #pragma unroll
-    for(int i = 0; i < P::kValuePieces; ++i)
+    for(int i = 0; i < kOwn / kRun; ++i)
 #pragma unroll
       for(int e = 0; e < 4; ++e) {
-        const int d = (16 * i + 4 * g + e) * kTogether;
-        float y[kTogether];
+        const int j0 = shift + i * kRun, d = (16 * (j0 / kTogether) + 4 * g + e) * kTogether + j0 % kTogether;
+        float y[kRun];
 #pragma unroll
-        for(int j = 0; j < kTogether; ++j) y[j] = o[t][i * kTogether + j][e] * factor;
-        if(d < a.dk) store_row<kTogether, T>(to + d, y);
+        for(int j = 0; j < kRun; ++j) y[j] = r[t][i * kRun + j][e] * factor;
+        if(d < a.dk) {
+          if constexpr(kRun == 2) *reinterpret_cast<unsigned*>(to + d) = pack2<T>(y[0], y[1]);
+          else store_row<kRun, T>(to + d, y);
+        }
       }
   };
-#pragma unroll
-  for(int t = 0; t < QT; ++t) sum[t] = over_lanes_sum(sum[t]) * kUnit;
   if(out.whole) {
 #pragma unroll
     for(int t = 0; t < QT; ++t) write(t, sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * kUnit);
     return;
   }
   constexpr unsigned kTileBytes = CacheOut<T, DP, 64 * QT>::kTileFloats * 4;
-  const unsigned stride = (unsigned)out.stride * kTileBytes, mine = 16u * (QT * kDims * 64 * wave + lane), my_log = 4u * (64 * QT * DP + 16 * QT * wave + c);
+  const unsigned stride = (unsigned)out.stride * kTileBytes, mine = 1024u * (QT * kDims * wave + shift) + 16u * lane, my_log = 4u * (64 * QT * DP + 16 * QT * wave + c);
   const CacheBuffer parts(a.part + out.place * CacheOut<T, DP, 64 * QT>::kTileFloats, stride * x.w.parts);
 #pragma unroll
   for(int t = 0; t < QT; ++t) {
     const float factor = sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * kUnit;
     const unsigned to = stride * x.w.part;
 #pragma unroll
-    for(int j = 0; j < kDims; ++j) parts.store_through(o[t][j] * factor, to + mine + 1024u * (t * kDims + j));
-    if(g == 0) parts.store_through(sum[t] == 0.0f ? kNone : top[t] + __builtin_amdgcn_logf(sum[t]), to + my_log + 64u * t);
+    for(int j = 0; j < kOwn; ++j) parts.store_through(r[t][j] * factor, to + mine + 1024u * (t * kDims + j));
+    if(g == 0 && half == 0) parts.store_through(sum[t] == 0.0f ? kNone : top[t] + __builtin_amdgcn_logf(sum[t]), to + my_log + 64u * t);
   }
   if(!cache_arrived_last(a.counters + out.place, x.w.parts, sh.is_last)) return;
   float weight_sum[QT];
@@ -765,9 +826,9 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
     top[t] = kNone;
     weight_sum[t] = 0.0f;
 #pragma unroll
-    for(int j = 0; j < kDims; ++j) o[t][j] = cache_f4{0, 0, 0, 0};
+    for(int j = 0; j < kOwn; ++j) r[t][j] = cache_f4{0, 0, 0, 0};
   }
-  constexpr int kLogs = 8, kBatch = QT == 1 && DP == 64 ? 4 : 2;
+  constexpr int kLogs = 8, kBatch = QT * kOwn > 8 ? 2 : 16 / (QT * kOwn);
 #pragma unroll 1
   for(int i = 0; i < x.w.parts; i += kLogs) {   // (behind the last part the buffer gives zeros)
     float l[QT][kLogs];
@@ -783,7 +844,7 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
 #pragma unroll 1
   for(int i = 0; i < x.w.parts; i += kBatch) {
     float l[QT][kBatch];
-    cache_f4 z[kBatch][QT][kDims];
+    cache_f4 z[kBatch][QT][kOwn];
 #pragma unroll
     for(int b = 0; b < kBatch; ++b) {
       const unsigned at = stride * (unsigned)(i + b);
@@ -791,7 +852,7 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
       for(int t = 0; t < QT; ++t) {
         l[t][b] = parts.number_through(at + my_log + 64u * t);
 #pragma unroll
-        for(int j = 0; j < kDims; ++j) z[b][t][j] = parts.piece_through(at + mine + 1024u * (t * kDims + j));
+        for(int j = 0; j < kOwn; ++j) z[b][t][j] = parts.piece_through(at + mine + 1024u * (t * kDims + j));
       }
     }
 #pragma unroll
@@ -803,9 +864,9 @@ __global__ __launch_bounds__(256, 2) void pages_attention_many_kernel(PagesAtten
         const float weight = l[t][b] == kNone ? 0.0f : __builtin_amdgcn_exp2f(l[t][b] - top[t]) * kPartUnit;
         weight_sum[t] += weight;
 #pragma unroll
-        for(int j = 0; j < kDims; ++j)
+        for(int j = 0; j < kOwn; ++j)
 #pragma unroll
-          for(int e = 0; e < 4; ++e) o[t][j][e] = __builtin_fmaf(weight, z[b][t][j][e], o[t][j][e]);
+          for(int e = 0; e < 4; ++e) r[t][j][e] = __builtin_fmaf(weight, z[b][t][j][e], r[t][j][e]);
       }
     }
   }

@@ -25,7 +25,7 @@ template <typename T, int DP, bool WHOLE>
 int launch_pages_attention(const PagesAttentionArgs& a, const PagesAttentionPlan& p, hipStream_t st) {
   if constexpr(pages_has_many(sizeof(T), DP)) {
     if(p.many) {
-      const dim3 grid((unsigned)p.grid), block(256);
+      const dim3 grid((unsigned)p.grid), block(256 * pages_many_split(p.qt));
       if(p.qt == 1) MH_LAUNCH((pages_attention_many_kernel<T, DP, WHOLE, 1>), grid, block, 0, st, a);
       else MH_LAUNCH((pages_attention_many_kernel<T, DP, WHOLE, 2>), grid, block, 0, st, a);
       return MARIAN_HIP_OK;
