@@ -486,22 +486,27 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
 }
 
 // ---- more than 32 rows
-// Waves have 16 * QT rows each and share positions laid out in LDS, 64 at a time, twice: while one is worked on, the next is written and the
-// one after that is on its way to registers.  With sixteen rows to a wave (QT == 1) eight waves take 64 rows, four of them the first 32
-// positions of each 64 and four the second (SPLIT == 2); with 32 rows, 128 of them, four waves take all 64 positions (a second half would not fit
-// the registers).  Keys lie in LDS as they are, values transposed, a dimension's 64 side by side; pieces of 16 bytes change places within a
+// Waves share positions laid out in LDS, 64 at a time, twice: while one is worked on, the next is written and the one after that is on its way
+// to registers.  64 rows are taken by eight waves of sixteen, four of them for the first 32 positions of each 64 and four for the second.  128
+// rows are taken by eight waves too where rows have 64 values, by four of 32 where they have 128: LDS is read half as often then, and that
+// counts by the length of rows (512 new tokens of 4 sequences, 16 heads of 64 values, 42 us by eight and 45 by four; 1024 of
+// them, 32 heads on 8, 128 values, 200 and 187).  Keys lie in LDS as they are, values transposed, a dimension's 64 side by side; pieces of 16 bytes change places within a
 // row (key_place, value_place) so that few lanes that read together meet in a bank (a third of the cycles that LDS is busy).  A wave lays out one or two eights of positions:
 // sixteen lanes (of rows of 128 bytes eight) to a row of keys; of values a lane has some dimensions of eight positions.  Products, weights and sums are those above.
 //
 // What bounds it: latency, of the memory's answers and of the partial results' way to the workgroup that joins them; LDS is busy less than a third of
 // the time and the matrix units a fifth.  7 drafted tokens, float16, 24 sequences of up to 8192 positions, 4 heads of 128 values with eight
-// rows each (56 rows, 270 MB): 74 us, 3.6 TB/s; four waves that take all positions and join them 80, waves of the form above with a row
+// rows each (56 rows, 270 MB): 70 to 74 us, 3.8 TB/s; four waves that take all positions and join them 80, waves of the form above with a row
 // group each 95.  bfloat16, 64 values, 8 tokens, 16 sequences: 37 and 39.6.  __syncthreads in place of the barrier below waits for the loads too.
-template <typename T, int DP, int SPLIT>
+template <typename T, int DP, int ROWS>
 struct PagesMany {
+  static constexpr int kWaves = pages_many_waves(DP, ROWS);
+  static constexpr int kSixteens = kWaves == 4 && ROWS == 128 ? 2 : 1;   // of rows, to a wave
+  static constexpr int kGroups = ROWS / (16 * kSixteens); // waves that have different rows
+  static constexpr int kSplit = kWaves / kGroups;         // shares of the positions
   static constexpr int kTile = 64;                        // positions of a turn
   static constexpr int kRowPieces = DP / 8;               // pieces of a key
-  static constexpr int kEights = 2 / SPLIT;               // of positions that a wave lays out
+  static constexpr int kEights = 8 / kWaves;               // of positions that a wave lays out
   static constexpr int kKeyLoads = kEights * kRowPieces / 8;       // of a lane
   static constexpr int kLanes = 64 / kEights;             // that have an eight's values, kDimsEach dimensions each
   static constexpr int kDimsEach = DP / kLanes < 2 ? 2 : DP / kLanes;
@@ -534,14 +539,11 @@ __device__ __forceinline__ void pages_lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// Halves of positions
-constexpr int pages_many_split(int qt) { return qt == 1 ? 2 : 1; }
-
-template <typename T, int DP, bool WHOLE, int QT>
-__global__ __launch_bounds__(256 * pages_many_split(QT), 2 * pages_many_split(QT)) void pages_attention_many_kernel(PagesAttentionArgs a) {
+template <typename T, int DP, bool WHOLE, int ROWS>
+__global__ __launch_bounds__(64 * pages_many_waves(DP, ROWS), pages_many_waves(DP, ROWS) / 2) void pages_attention_many_kernel(PagesAttentionArgs a) {
   using P = Pages<T, DP>;
-  constexpr int SPLIT = pages_many_split(QT);
-  using M = PagesMany<T, DP, SPLIT>;
+  using M = PagesMany<T, DP, ROWS>;
+  constexpr int QT = M::kSixteens, SPLIT = M::kSplit;
   constexpr int kDims = P::kDims, kTogether = P::kTogether, kKeyPieces = P::kKeyPieces, kTile = M::kTile, kEights = M::kEights, kParts = 2 / SPLIT;
   constexpr float kUnit = P::kUp < 0 ? (float)(1 << -P::kUp * (P::kUp < 0)) : 1.0f / (1 << P::kUp * (P::kUp > 0));   // 2^-kUp
   __shared__ struct {
@@ -552,9 +554,9 @@ __global__ __launch_bounds__(256 * pages_many_split(QT), 2 * pages_many_split(QT
     int is_last;
   } sh;
   const int tid = threadIdx.x, lane = tid & 63, any_wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
-  const int wave = any_wave % 4, half = any_wave / 4;   // of the rows, of the positions
+  const int wave = any_wave % M::kGroups, half = any_wave / M::kGroups;   // of the rows, of the positions
   CacheTile x;
-  if(!cache_tile<T, DP, 64 * QT, 4 * SPLIT, kPagesMostParts>(a, tid, x)) return;
+  if(!cache_tile<T, DP, ROWS, M::kWaves, kPagesMostParts>(a, tid, x)) return;
   const int end = x.end, row_bytes = (WHOLE ? DP : a.dk) * 2;
   const int* const table = a.table + (long long)x.w.s * a.row;
   const unsigned char* const k_head = a.k_pages + x.head * a.head_bytes;
@@ -748,7 +750,7 @@ __global__ __launch_bounds__(256 * pages_many_split(QT), 2 * pages_many_split(QT
   pages_odd_values<T, DP, QT>(a, table, v_head, row_bytes, begin + 32 * half, end, 4 * kParts, kTile, lane, sh.tile.left_out != 0, sight, o);
   // Rows of a sequence in one part go to the output.  Parts go to the workspace as registers have them, 1 KB at a time, and back: whoever
   // arrives last joins them, a wave its own rows (16 parts of 64 rows: 20 us less than by rows of 16 threads, which store and load pieces of 8 bytes).
-  const CacheOut<T, DP, 64 * QT> out(a, x);
+  const CacheOut<T, DP, ROWS> out(a, x);
 #pragma unroll
   for(int t = 0; t < QT; ++t) sum[t] = over_lanes_sum(sum[t]) * kUnit;
   // Two halves exchange results: of its rows each has kOwn of the kDims pieces from here on, `shift` the first of them.
@@ -808,9 +810,9 @@ __global__ __launch_bounds__(256 * pages_many_split(QT), 2 * pages_many_split(QT
     for(int t = 0; t < QT; ++t) write(t, sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * kUnit);
     return;
   }
-  constexpr unsigned kTileBytes = CacheOut<T, DP, 64 * QT>::kTileFloats * 4;
-  const unsigned stride = (unsigned)out.stride * kTileBytes, mine = 1024u * (QT * kDims * wave + shift) + 16u * lane, my_log = 4u * (64 * QT * DP + 16 * QT * wave + c);
-  const CacheBuffer parts(a.part + out.place * CacheOut<T, DP, 64 * QT>::kTileFloats, stride * x.w.parts);
+  constexpr unsigned kTileBytes = CacheOut<T, DP, ROWS>::kTileFloats * 4;
+  const unsigned stride = (unsigned)out.stride * kTileBytes, mine = 1024u * (QT * kDims * wave + shift) + 16u * lane, my_log = 4u * (ROWS * DP + 16 * QT * wave + c);
+  const CacheBuffer parts(a.part + out.place * CacheOut<T, DP, ROWS>::kTileFloats, stride * x.w.parts);
 #pragma unroll
   for(int t = 0; t < QT; ++t) {
     const float factor = sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * kUnit;

@@ -25,9 +25,9 @@ template <typename T, int DP, bool WHOLE>
 int launch_pages_attention(const PagesAttentionArgs& a, const PagesAttentionPlan& p, hipStream_t st) {
   if constexpr(pages_has_many(sizeof(T), DP)) {
     if(p.many) {
-      const dim3 grid((unsigned)p.grid), block(256 * pages_many_split(p.qt));
-      if(p.qt == 1) MH_LAUNCH((pages_attention_many_kernel<T, DP, WHOLE, 1>), grid, block, 0, st, a);
-      else MH_LAUNCH((pages_attention_many_kernel<T, DP, WHOLE, 2>), grid, block, 0, st, a);
+      const dim3 grid((unsigned)p.grid), block(64 * p.waves);
+      if(p.tile_rows == 64) MH_LAUNCH((pages_attention_many_kernel<T, DP, WHOLE, 64>), grid, block, 0, st, a);
+      else MH_LAUNCH((pages_attention_many_kernel<T, DP, WHOLE, 128>), grid, block, 0, st, a);
       return MARIAN_HIP_OK;
     }
   }

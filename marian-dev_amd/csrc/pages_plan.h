@@ -21,8 +21,9 @@ constexpr unsigned kPagesMostParts = 64;
 
 // Sixteens of query rows that a wave takes over the same positions, at the most.
 constexpr int pages_most_qt(int width, int dp) { return width == 4 && dp == 256 ? 1 : 2; }
-// Whether rows past that have a form in which four waves of 16 * qt rows each share positions in LDS.
+// Whether rows past that have a form in which waves with rows of their own share positions in LDS, for 64 or 128 rows.
 constexpr bool pages_has_many(int width, int dp) { return width == 2 && dp <= 128; }
+constexpr int pages_many_waves(int dp, int rows) { return dp == 128 && rows == 128 ? 4 : 8; }
 
 // Waves of a form that fit a SIMD, by its registers.
 constexpr int pages_to_a_simd(int width, int dp, int qt) {
@@ -32,9 +33,9 @@ constexpr int pages_to_a_simd(int width, int dp, int qt) {
 
 struct PagesAttentionPlan {
   int dp;              // values of a row as the kernel holds it: dk rounded up to 64, 128 or 256
-  int qt;              // sixteens of query rows to a workgroup
-  bool many;           // the waves have these rows each, and share positions laid out in LDS
-  int waves;           // of a workgroup, which share its rows and take turns of 32 positions
+  bool many;           // the waves have rows of their own and share positions laid out in LDS
+  int qt;              // if not: sixteens of query rows to a workgroup
+  int waves;           // of a workgroup; if not, they share its rows and take turns of 32 positions
   int tile_rows;       // of a workgroup
   int64_t row_tiles;   // workgroups that share an entry's positions
   int least;           // blocks of a part
@@ -49,18 +50,18 @@ inline PagesAttentionPlan pages_attention_plan(int64_t sequences, int64_t heads,
   p.dp = dk <= 64 ? 64 : dk <= 128 ? 128 : 256;
   const int64_t rows = n * (q_heads / heads);
   p.many = rows > 32 && pages_has_many(width, p.dp);
-  p.qt = p.many ? (rows > 64 ? 2 : 1) : std::min(rows <= 16 ? 1 : 2, pages_most_qt(width, p.dp));
-  p.tile_rows = p.many ? 64 * p.qt : 16 * p.qt;
+  p.qt = std::min(rows <= 16 ? 1 : 2, pages_most_qt(width, p.dp));
+  p.tile_rows = p.many ? (rows > 64 ? 128 : 64) : 16 * p.qt;
   p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const int64_t entries = sequences * heads * p.row_tiles;
-  p.waves = !p.many && entries >= 4096 ? 1 : 4;
+  p.waves = p.many ? pages_many_waves(p.dp, p.tile_rows) : entries >= 4096 ? 1 : 4;
   // Parts for one round of the workgroups that run at a time, by the registers of their form, half a part for each sequence left out.  Of 16-bit values
   // half of them have the memory as busy, and leave fewer parts to join: where that makes two parts of a sequence.  One token, 8 heads with four
   // rows each, 128 values, all and half, over ten sets of lengths: 100003 positions 80.2 and 77.6 us, 4 sequences of up to 16000 44.2 and 42.0, 8
   // 75.1 and 72.4, but 16 of up to 32768 264 and 291; 4 drafted tokens, 4 heads with eight rows each, 16 of up to 16384 81.3 and 77.2, 40 of up to
   // 8192 96.9 and 101.  Not where rows leave many lanes without a load (80 values, 16 of up to 8192: 51.8 and 57.0), nor of float32 (64 values,
   // 16384: 83.4 and 88.2), nor of the form that shares positions in LDS (7 tokens, 24 of up to 8192: 75 and 108).
-  const int to_a_simd = p.many ? 2 : pages_to_a_simd(width, p.dp, p.qt);
+  const int to_a_simd = p.many ? p.waves / 2 : pages_to_a_simd(width, p.dp, p.qt);
   auto parts_of = [&](int64_t at_a_time) { return std::max<int64_t>(1, at_a_time / (heads * p.row_tiles) - sequences / 2); };
   const int64_t all = parts_of(1024 * to_a_simd / p.waves), half = parts_of(512 * to_a_simd / p.waves);
   p.target = width == 2 && !p.many && to_a_simd > 1 && 4 * dk > 3 * p.dp && half >= 2 * sequences ? half : all;
