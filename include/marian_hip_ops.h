@@ -542,13 +542,15 @@ int marian_hip_pages_write(const marian_hip_pages* cache, const void* k, const i
  *   out = softmax(scale * q . key) value
  * over the lens[s] positions before the new tokens, the token itself and the new ones before it.  table: int32 [sequences, row]; rows may share
  * pages.  Positions of a page that is none (below 0, or at or past `pages`), and past the row, are not seen.  What a token does not see is
- * not read into its result, infinities and NaN included.  A token that sees nothing, or whose scores are all minus infinity, gives zeros,
- * and so do rows at or past counts[s] (counts: null, or int32 [sequences]).  out shares no memory with anything else.  scale: finite, above zero.
- * Products and sums are float32; weights enter the product with the values in the cache's type (bfloat16: 8 bits, float16 11), their sum in float32.
+ * not read into its result, infinities and NaN included; an infinity among the values that it sees is its result (NaN if there are both, or
+ * if its weight is below 2^-126 of the largest, and NaN if there is one).  A token that sees nothing, or whose scores are all minus infinity,
+ * gives zeros, and so do rows at or past counts[s] (counts: null, or int32 [sequences]).  out shares no memory with anything else.
+ * scale: finite, above zero.
+ * Products and sums are float32; weights enter the product with the values with 16 bits (bfloat16), 22 (float16) or 24, their sum in float32.
  * Values (bfloat16 and float32) below 2^-100 lose bits to the scale of the weights.
  * The last bits of a result depend on the batch's lengths and the table's width, which say how positions are split over workgroups, and not on
- * the order of anything.  Made for few rows a head of keys, n * q_heads / heads up to 64; more are taken 64 (or fewer, see the sources) at a time, each time
- * reading keys and values again.
+ * the order of anything.  Made for few rows a head of keys, n * q_heads / heads: keys and values are read once for every 128 of them (16-bit
+ * types with up to 128 values a row), 32, or 16 (float32 with more than 128).
  * lens outside 0 .. row * page are taken as the nearer end.  row * page < 2^30; n up to 2^20.
  *   workspace: at least marian_hip_pages_attention_workspace_bytes(...) bytes, cleared once by marian_hip_cache_attention_workspace_init; as for
  *   marian_hip_cache_attention, whose workspace serves this call too where it is large enough.

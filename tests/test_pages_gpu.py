@@ -233,6 +233,27 @@ def test_what_a_token_does_not_see_is_not_in_its_result(dtype, dk, bad, group, n
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dk", [64, 128, 256])
+@pytest.mark.parametrize("group,n", [(4, 1), (8, 4), (8, 7), (8, 16)])
+def test_infinities_in_long_sequences(dtype, dk, group, n):
+    """Settled positions of every turn's both halves, in one part of a sequence or another: an infinity that all see is their result, NaN
+    where a later position has one of the other sign or NaN; all else is as without"""
+    pages, r = load("pages"), maker(9)
+    heads, page, past = 2, 16, 2500
+    row = -(-(past + n) // page)
+    table = dealt(6, [past + n], page, row, row)
+    kv = poisoned(r, table, [past + n], page, row, heads, dk, dtype)
+    q = side_by_side(r, 1, heads * group, n, dk, dtype)
+    inf = float("inf")
+    for at, d, x in ((3, 0, inf), (40, 1, -inf), (700, 2, inf), (1333, 3, -inf), (64, 4, inf), (2100, 4, -inf), (95, 5, inf), (2499, 5, float("nan"))):
+        kv.v[table[0][at // page], 1, at % page, d] = x
+    got = pages.AttentionOverPages(q, kv, ints(table), ints([past]))
+    want, tol = expected(q, kv, ints(table), [past])
+    assert torch.isinf(want[0, group:, :, :4]).all() and torch.isnan(want[0, group:, :, 4:6]).all() and torch.isfinite(want[0, :group]).all()
+    check(got, want, torch.where(torch.isfinite(want), tol, torch.zeros_like(tol)))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("share", [1.0, 0.99])
 def test_values_next_to_the_largest(dtype, share):
     """Results are means of values, and stay in range where what they may be off by does: the mean of values that are all the largest number M
