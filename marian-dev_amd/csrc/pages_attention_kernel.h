@@ -21,7 +21,7 @@
 // leaves: 16 and 22 bits.  Their sum is of the float32 ones.  They are scaled by a power of two: bfloat16 and float32 2^-24, so that sums over
 // 2^20 positions of values next to the largest stay in range; float16 2^11, so that weights down to 2^-25 of the largest keep their bits.
 //
-// What bounds it: the memory.  One token of 128 sequences of up to 512 positions, 16 heads of 64 values, float32 (360 MB): 73 us, 4.9 TB/s; of 16
+// What bounds it: the memory.  One token of 128 sequences of up to 512 positions, 16 heads of 64 values, float32 (360 MB): 72 to 75 us, 4.9 TB/s; of 16
 // sequences of up to 32768, 8 heads of 128 values with four rows each, bfloat16 (1.4 GB): 264 us, 5.4 TB/s; one sequence of 100003 (410 MB) 78
 // us, 5.3 TB/s.  Where there is little to read, 6 sequences of up to 120 positions: 6.0 us, a workgroup's start, three dependent loads (length,
 // page, keys and values) and its end.
@@ -50,6 +50,7 @@ struct Pages {
   static constexpr int kValuePieces = kDims / kTogether;
   static constexpr int kWords = kTogether * kWidth / 4;            // of a piece of values
   static constexpr int kUp = std::is_same<T, _Float16>::value ? 11 : -24;   // exponent that weights are held with
+  static constexpr float kUnit = kUp < 0 ? (float)(1 << -kUp * (kUp < 0)) : 1.0f / (1 << kUp * (kUp > 0));   // 2^-kUp
   struct Keys {
     cache_u4 piece[2][kKeyPieces];
   };
@@ -122,11 +123,10 @@ __device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const 
                                              float (&sum)[QT], int wave, CacheJoin<DP, QT, WAVES>& sh) {
   using P = Pages<T, DP>;
   constexpr int kTogether = P::kTogether, kHalf = CacheJoin<DP, QT, WAVES>::kHalf, kPieces = kHalf / (16 * kTogether);
-  constexpr float kUnit = P::kUp < 0 ? (float)(1 << -P::kUp * (P::kUp < 0)) : 1.0f / (1 << P::kUp * (P::kUp > 0));   // 2^-kUp
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
   for(int t = 0; t < QT; ++t) {
-    sum[t] = over_lanes_sum(sum[t]) * kUnit;
+    sum[t] = over_lanes_sum(sum[t]) * P::kUnit;
     if(WAVES > 1 && g == 0) {
       sh.row_max[wave][16 * t + c] = top[t];
       sh.row_sum[wave][16 * t + c] = sum[t];
@@ -136,7 +136,7 @@ __device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const 
   if constexpr(WAVES == 1) {
 #pragma unroll
     for(int t = 0; t < QT; ++t) {
-      const float factor = sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * kUnit;
+      const float factor = sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * P::kUnit;
 #pragma unroll
       for(int i = 0; i < P::kValuePieces; ++i)
 #pragma unroll
@@ -152,7 +152,7 @@ __device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const 
     // A row's weights of N positions add up to 2^kMaximumSlack N at the most, and their values to that many times the largest, which may be next
     // to the largest float32: they are summed over a power of two above it, twice as large for the roundings.  (It changes no bit of a result.)
     const int up = 5 + 32 - __builtin_clz((unsigned)max(x.end - x.w.from, 1));
-    const float over = __builtin_bit_cast(float, (unsigned)(127 - up) << 23) * kUnit, back = __builtin_bit_cast(float, (unsigned)(127 + up) << 23);
+    const float over = __builtin_bit_cast(float, (unsigned)(127 - up) << 23) * P::kUnit, back = __builtin_bit_cast(float, (unsigned)(127 + up) << 23);
     static_assert(kMaximumSlack <= 4.0f, "up counts it");
     const CacheBuffer part(out.part, CacheOut<T, DP, 16 * QT>::kTileFloats * 4);
     __syncthreads();
@@ -451,10 +451,12 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
       float p[QT][8];
 #pragma unroll
       for(int t = 0; t < QT; ++t) {
-        const float from = (top[t] == kNone ? 0.0f : -top[t]) + P::kUp;   // (nothing seen so far: minus infinity stays that)
+        const float from = top[t] == kNone ? 0.0f : -top[t];   // (nothing seen so far: minus infinity stays that)
+        // (Scaled behind the exponential: a weight next to one has an exponent next to zero then, in all its bits.  128 sequences of 513 positions, 64
+        // values, are 3.5e-7 off 64 bits, and 6.0e-7 with the scale in the exponent, which takes 1 to 2 us less of 75.)
 #pragma unroll
         for(int e = 0; e < 8; ++e) {
-          p[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], a.scale_log2, from));
+          p[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], a.scale_log2, from)) * (1.0f / P::kUnit);
           sum[t] += p[t][e];
         }
       }
@@ -503,7 +505,7 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
 //
 // What bounds it: latency, of the memory's answers and of the partial results' way to the workgroup that joins them; LDS is busy less than a third of
 // the time and the matrix units a fifth.  7 drafted tokens, float16, 24 sequences of up to 8192 positions, 4 heads of 128 values with eight
-// rows each (56 rows, 270 MB): 70 to 74 us, 3.8 TB/s; four waves that take all positions and join them 80, waves of the form above with a row
+// rows each (56 rows, 270 MB): 67 to 73 us, 3.9 TB/s; four waves that take all positions and join them 80, waves of the form above with a row
 // group each 95.  bfloat16, 64 values, 8 tokens, 16 sequences: 37 and 39.6.  __syncthreads in place of the barrier below waits for the loads too.
 template <typename T, int DP, int ROWS>
 struct PagesMany {
@@ -552,7 +554,6 @@ __global__ __launch_bounds__(64 * pages_many_waves(DP, ROWS), pages_many_waves(D
   using M = PagesMany<T, DP, ROWS>;
   constexpr int QT = M::kSixteens, SPLIT = M::kSplit;
   constexpr int kDims = P::kDims, kTogether = P::kTogether, kKeyPieces = P::kKeyPieces, kTile = M::kTile, kEights = M::kEights, kParts = 2 / SPLIT;
-  constexpr float kUnit = P::kUp < 0 ? (float)(1 << -P::kUp * (P::kUp < 0)) : 1.0f / (1 << P::kUp * (P::kUp > 0));   // 2^-kUp
   __shared__ struct {
     union {
       typename M::Shared tile;
@@ -759,7 +760,7 @@ __global__ __launch_bounds__(64 * pages_many_waves(DP, ROWS), pages_many_waves(D
   // arrives last joins them, a wave its own rows (16 parts of 64 rows: 20 us less than by rows of 16 threads, which store and load pieces of 8 bytes).
   const CacheOut<T, DP, ROWS> out(a, x);
 #pragma unroll
-  for(int t = 0; t < QT; ++t) sum[t] = over_lanes_sum(sum[t]) * kUnit;
+  for(int t = 0; t < QT; ++t) sum[t] = over_lanes_sum(sum[t]) * P::kUnit;
   // Two halves exchange results: of its rows each has kOwn of the kDims pieces from here on, `shift` the first of them.
   constexpr int kOwn = kDims / SPLIT;
   const int shift = half * kOwn;
@@ -814,7 +815,7 @@ __global__ __launch_bounds__(64 * pages_many_waves(DP, ROWS), pages_many_waves(D
   };
   if(out.whole) {
 #pragma unroll
-    for(int t = 0; t < QT; ++t) write(t, sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * kUnit);
+    for(int t = 0; t < QT; ++t) write(t, sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * P::kUnit);
     return;
   }
   constexpr unsigned kTileBytes = CacheOut<T, DP, ROWS>::kTileFloats * 4;
@@ -822,7 +823,7 @@ __global__ __launch_bounds__(64 * pages_many_waves(DP, ROWS), pages_many_waves(D
   const CacheBuffer parts(a.part + out.place * CacheOut<T, DP, ROWS>::kTileFloats, stride * x.w.parts);
 #pragma unroll
   for(int t = 0; t < QT; ++t) {
-    const float factor = sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * kUnit;
+    const float factor = sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * P::kUnit;
     const unsigned to = stride * x.w.part;
 #pragma unroll
     for(int j = 0; j < kOwn; ++j) parts.store_through(r[t][j] * factor, to + mine + 1024u * (t * kDims + j));
