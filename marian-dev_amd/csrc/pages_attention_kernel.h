@@ -116,39 +116,48 @@ __device__ __forceinline__ void pages_weights(const cache_f4 (&s)[2], float scal
   }
 }
 
-// The results of waves that share rows, joined and written.  Lane (c, g) holds of row c of each sixteen the values
-// (16 (j / kTogether) + 4 g + e) kTogether + j % kTogether as o[t][j][e], unnormalized, the carried maximum and its part of the sum.
+// A wave's results, written: lane (c, g) holds of row c of each sixteen the values (16 (j / kTogether) + 4 g + e) kTogether + j % kTogether as
+// o[t][j][e], unnormalized, the carried maximum and the sum.
+template <typename T, int DP, int QT>
+__device__ __forceinline__ void pages_write(const CacheOut<T, DP, 16 * QT>& out, const cache_f4 (&o)[QT][DP / 16], const float (&top)[QT],
+                                            const float (&sum)[QT], int c, int g) {
+  using P = Pages<T, DP>;
+#pragma unroll
+  for(int t = 0; t < QT; ++t) {
+    const float factor = sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * P::kUnit;
+#pragma unroll
+    for(int i = 0; i < P::kValuePieces; ++i)
+#pragma unroll
+      for(int e = 0; e < 4; ++e) {
+        float y[P::kTogether];
+#pragma unroll
+        for(int j = 0; j < P::kTogether; ++j) y[j] = o[t][i * P::kTogether + j][e] * factor;
+        out.emit(16 * t + c, (16 * i + 4 * g + e) * P::kTogether, y);
+      }
+    if(g == 0) out.emit_log(16 * t + c, top[t], sum[t]);
+  }
+}
+
+// The results of waves that share rows, joined and written; alone: one wave has all of them, and the others have ended.
 template <typename T, int DP, int QT, int WAVES>
 __device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const CacheTile& x, const cache_f4 (&o)[QT][DP / 16], const float (&top)[QT],
-                                             float (&sum)[QT], int wave, CacheJoin<DP, QT, WAVES>& sh) {
+                                             float (&sum)[QT], int wave, bool alone, CacheJoin<DP, QT, WAVES>& sh) {
   using P = Pages<T, DP>;
   constexpr int kTogether = P::kTogether, kHalf = CacheJoin<DP, QT, WAVES>::kHalf, kPieces = kHalf / (16 * kTogether);
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
-  for(int t = 0; t < QT; ++t) {
-    sum[t] = over_lanes_sum(sum[t]) * P::kUnit;
-    if(WAVES > 1 && g == 0) {
-      sh.row_max[wave][16 * t + c] = top[t];
-      sh.row_sum[wave][16 * t + c] = sum[t];
-    }
-  }
+  for(int t = 0; t < QT; ++t) sum[t] = over_lanes_sum(sum[t]) * P::kUnit;
   const CacheOut<T, DP, 16 * QT> out(a, x);
-  if constexpr(WAVES == 1) {
+  if(alone) {
+    pages_write<T, DP, QT>(out, o, top, sum, c, g);
+    if(WAVES > 1) return;
+  } else if constexpr(WAVES > 1) {
 #pragma unroll
-    for(int t = 0; t < QT; ++t) {
-      const float factor = sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * P::kUnit;
-#pragma unroll
-      for(int i = 0; i < P::kValuePieces; ++i)
-#pragma unroll
-        for(int e = 0; e < 4; ++e) {
-          float y[kTogether];
-#pragma unroll
-          for(int j = 0; j < kTogether; ++j) y[j] = o[t][i * kTogether + j][e] * factor;
-          out.emit(16 * t + c, (16 * i + 4 * g + e) * kTogether, y);
-        }
-      if(g == 0) out.emit_log(16 * t + c, top[t], sum[t]);
-    }
-  } else {
+    for(int t = 0; t < QT; ++t)
+      if(g == 0) {
+        sh.row_max[wave][16 * t + c] = top[t];
+        sh.row_sum[wave][16 * t + c] = sum[t];
+      }
     // A row's weights of N positions add up to 2^kMaximumSlack N at the most, and their values to that many times the largest, which may be next
     // to the largest float32: they are summed over a power of two above it, twice as large for the roundings.  (It changes no bit of a result.)
     const int up = 5 + 32 - __builtin_clz((unsigned)max(x.end - x.w.from, 1));
@@ -284,6 +293,9 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
   CacheTile x;
   if(!cache_tile<T, DP, 16 * QT, WAVES, kPagesMostParts>(a, tid, x)) return;
   const int end = x.end, row_bytes = (WHOLE ? DP : a.dk) * kWidth;
+  // A sequence of one turn of one wave is that wave's: no join, and the others make room (236 of three positions, 16 heads of 64 values, 11 us and 20).
+  const bool alone = WAVES == 1 || (x.w.parts == 1 && end - x.w.from <= 32);
+  if(alone && wave > 0) return;
   const int* const table = a.table + (long long)x.w.s * a.row;
   const unsigned char* const k_head = a.k_pages + x.head * a.head_bytes;
   const unsigned char* const v_head = a.v_pages + x.head * a.head_bytes;
@@ -354,13 +366,13 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
       const cache_u4 y = *reinterpret_cast<const cache_u4*>(p + (d < row_bytes ? d : 0));
       const cache_u4 z = d < row_bytes ? y : cache_u4{0, 0, 0, 0};
       if constexpr(kQueriesInLds) {
-        if(wave == t % WAVES) q_held[t][i][lane] = z;
+        if(alone || wave == t % WAVES) q_held[t][i][lane] = z;
       } else {
         q[t][i] = z;
       }
     }
   }
-  if constexpr(kQueriesInLds) __syncthreads();
+  if(kQueriesInLds && !alone) __syncthreads();
 
   cache_f4 o[QT][kDims];
   float top[QT], sum[QT];   // carried maximum (base 2), the lane's part of the sum
@@ -489,7 +501,7 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
     v_next = look_values(at + 2 * kTurn);
   }
   pages_odd_values<T, DP, QT>(a, table, v_head, row_bytes, begin, end, 4, kTurn, lane, left_out, sight, o);
-  pages_finish<T, DP, QT, WAVES>(a, x, o, top, sum, wave, sh);
+  pages_finish<T, DP, QT, WAVES>(a, x, o, top, sum, wave, alone, sh);
 }
 
 // ---- more than 32 rows

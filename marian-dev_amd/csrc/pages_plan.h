@@ -25,6 +25,11 @@ constexpr int pages_most_qt(int width, int dp) { return width == 4 && dp == 256 
 constexpr bool pages_has_many(int width, int dp) { return width == 2 && dp <= 128; }
 constexpr int pages_many_waves(int dp, int rows) { return dp == 128 && rows == 128 ? 4 : 8; }
 
+// Positions up to which a sequence is short: eight turns of a wave.
+constexpr int64_t kPagesShort = 256;
+// Positions up to which sequences are taken to differ little.
+constexpr int64_t kPagesEven = 1024;
+
 // Waves of a form that fit a SIMD, by its registers.
 constexpr int pages_to_a_simd(int width, int dp, int qt) {
   const int all = pages_registers(width, dp, qt);
@@ -54,15 +59,27 @@ inline PagesAttentionPlan pages_attention_plan(int64_t sequences, int64_t heads,
   p.tile_rows = p.many ? (rows > 64 ? 128 : 64) : 16 * p.qt;
   p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const int64_t entries = sequences * heads * p.row_tiles;
-  p.waves = p.many ? pages_many_waves(p.dp, p.tile_rows) : entries >= 4096 ? 1 : 4;
+  const int form = pages_to_a_simd(width, p.dp, p.qt);
+  // One wave to an entry where the entries fill the card with that, or in four rounds and are short for certain: four waves of which most find no
+  // position cost a start and a join for it.  One token, four waves and one: 241 sequences of one position, 16 heads of 256 values, float16 103
+  // and 34 us; 182 of up to 192, 16 of 80, float32 96 and 82; 250 of up to 60, 8 of 128 with four rows each, bfloat16 24 and 15; but in room for
+  // 512, 128 of up to 512, 16 of 64, float32 74 and 84.
+  const bool one = entries >= 1024 * form || (entries >= 256 * form && capacity <= kPagesShort);
+  p.waves = p.many ? pages_many_waves(p.dp, p.tile_rows) : one ? 1 : 4;
   // Parts for one round of the workgroups that run at a time, by the registers of their form, half a part for each sequence left out.  Of 16-bit values
   // half of them have the memory as busy, and leave fewer parts to join: where that makes two parts of a sequence.  One token, 8 heads with four
   // rows each, 128 values, all and half, over ten sets of lengths: 100003 positions 80.2 and 77.6 us, 4 sequences of up to 16000 44.2 and 42.0, 8
   // 75.1 and 72.4, but 16 of up to 32768 264 and 291; 4 drafted tokens, 4 heads with eight rows each, 16 of up to 16384 81.3 and 77.2, 40 of up to
   // 8192 96.9 and 101.  Not where rows leave many lanes without a load (80 values, 16 of up to 8192: 51.8 and 57.0), nor of float32 (64 values,
   // 16384: 83.4 and 88.2), nor of the form that shares positions in LDS (7 tokens, 24 of up to 8192: 75 and 108).
-  const int to_a_simd = p.many ? p.waves / 2 : pages_to_a_simd(width, p.dp, p.qt);
-  auto parts_of = [&](int64_t at_a_time) { return std::max<int64_t>(1, at_a_time / (heads * p.row_tiles) - sequences / 2); };
+  const int to_a_simd = p.many ? p.waves / 2 : form;
+  // Many sequences leave few parts or none, and one of them may still have most of the positions: half of the parts there are anyway, where a row of
+  // the table has room for that to show.  8 heads of 128 values with four rows each, 128 sequences, one of 4096 positions and the others of
+  // 80: 55 and 22 us, all of up to 4096 269 and 269; but 200 of up to 700 76 and 79, by the look at all lengths.
+  auto parts_of = [&](int64_t at_a_time) {
+    const int64_t parts = at_a_time / (heads * p.row_tiles);
+    return std::max<int64_t>({1, parts - sequences / 2, capacity > kPagesEven ? parts / 2 : 0});
+  };
   const int64_t all = parts_of(1024 * to_a_simd / p.waves), half = parts_of(512 * to_a_simd / p.waves);
   p.target = width == 2 && !p.many && to_a_simd > 1 && 4 * dk > 3 * p.dp && half >= 2 * sequences ? half : all;
   // A sequence of up to four blocks stays whole, and where no row of the table has room for more nobody looks at the others' lengths (6 sequences
