@@ -549,8 +549,8 @@ int marian_hip_pages_write(const marian_hip_pages* cache, const void* k, const i
  * Products and sums are float32; weights enter the product with the values with 16 bits (bfloat16), 22 (float16) or 24, their sum in float32.
  * Values (bfloat16 and float32) below 2^-100 lose bits to the scale of the weights.
  * The last bits of a result depend on the batch's lengths and the table's width, which say how positions are split over workgroups, and not on
- * the order of anything.  Made for few rows a head of keys, n * q_heads / heads: keys and values are read once for every 128 of them (16-bit
- * types with up to 128 values a row), 32, or 16 (float32 with more than 128).
+ * the order of anything.  Made for few rows a head of keys, n * q_heads / heads: keys and values are read once for every 128 of them (up to 128
+ * values a row, float32 more than 64), 32 (float32 up to 64 values, 16-bit types past 128), or 16 (float32 past 128).
  * lens outside 0 .. row * page are taken as the nearer end.  row * page < 2^30; n up to 2^20.
  *   workspace: at least marian_hip_pages_attention_workspace_bytes(...) bytes, cleared once by marian_hip_cache_attention_workspace_init; as for
  *   marian_hip_cache_attention, whose workspace serves this call too where it is large enough.

@@ -513,37 +513,40 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
 // Keys lie in LDS as they are, values transposed, a dimension's 64 side by side; pieces of 16 bytes change places within a row (key_place,
 // value_place) so that few lanes that read together meet in a bank (a third of the cycles that LDS is busy).  A wave lays out one or two eights
 // of positions: sixteen lanes (of rows of 128 bytes eight) to a row of keys; of values a lane has some dimensions of eight positions.
-// Products, weights and sums are those above.
+// Products, weights and sums are those above.  float32 is taken by eight waves for 64 and for 128 rows; its values lie in LDS as they are, too, a
+// product takes one of them at a time.
 //
 // What bounds it: latency, of the memory's answers and of the partial results' way to the workgroup that joins them; LDS is busy less than a third of
 // the time and the matrix units a fifth.  7 drafted tokens, float16, 24 sequences of up to 8192 positions, 4 heads of 128 values with eight
 // rows each (56 rows, 270 MB): 67 to 73 us, 3.9 TB/s; four waves that take all positions and join them 80, waves of the form above with a row
-// group each 95.  bfloat16, 64 values, 8 tokens, 16 sequences: 37 and 39.6.  __syncthreads in place of the barrier below waits for the loads too.
+// group each 95.  bfloat16, 64 values, 8 tokens, 16 sequences: 37 and 39.6.  float32, the 56 rows above: 220 us,
+// of which the matrix products alone take 110 (17 GFLOP).  __syncthreads in place of the barrier below waits for the loads too.
 template <typename T, int DP, int ROWS>
 struct PagesMany {
-  static constexpr int kWaves = pages_many_waves(DP, ROWS);
+  static constexpr int kWidth = sizeof(T);
+  static constexpr int kWaves = pages_many_waves(kWidth, DP, ROWS);
   static constexpr int kSixteens = kWaves == 4 && ROWS == 128 ? 2 : 1;   // of rows, to a wave
   static constexpr int kGroups = ROWS / (16 * kSixteens); // waves that have different rows
   static constexpr int kSplit = kWaves / kGroups;         // shares of the positions
   static constexpr int kTile = 64;                        // positions of a turn
-  static constexpr int kRowPieces = DP / 8;               // pieces of a key
+  static constexpr int kRowPieces = DP * kWidth / 16;     // pieces of a row
   static constexpr int kEights = 8 / kWaves;               // of positions that a wave lays out
-  static constexpr int kKeyLoads = kEights * kRowPieces / 8;       // of a lane
+  static constexpr int kRowLoads = kEights * kRowPieces / 8;       // of a lane, of keys (float32: of values too)
   static constexpr int kLanes = 64 / kEights;             // that have an eight's values, kDimsEach dimensions each
   static constexpr int kDimsEach = DP / kLanes < 2 ? 2 : DP / kLanes;
   static constexpr int kValueWords = kDimsEach / 2;
   // (lanes that read together are, by what was measured, the 16 lanes c, of one half of them with g and of the other with g ^ 1)
   static __device__ __forceinline__ int key_place(int key, int piece) {
     const int c = (key >> 1 & 12) | (key & 3);
-    return (key * kRowPieces + (piece ^ (kRowPieces == 16 ? c : c >> 1))) * 16;
+    return (key * kRowPieces + (piece ^ (kRowPieces >= 16 ? c : c >> 1))) * 16;
   }
-  static __device__ __forceinline__ int value_place(int dim, int eight) {
+  static __device__ __forceinline__ int value_place(int dim, int eight) {   // (16-bit types)
     const int c = dim / Pages<T, DP>::kTogether, j = dim % Pages<T, DP>::kTogether;
     return (j * 16 + c) * 128 + (eight ^ c >> 1) * 16;
   }
   struct Shared {
-    alignas(16) unsigned char keys[2][kTile * DP * 2];
-    alignas(16) unsigned char values[2][kTile * DP * 2];
+    alignas(16) unsigned char keys[2][kTile * DP * kWidth];
+    alignas(16) unsigned char values[2][kTile * DP * kWidth];
     int there[2][8];   // of each eight of positions, whether it has a page
     int left_out;
   };
@@ -561,11 +564,11 @@ __device__ __forceinline__ void pages_lds_barrier() {
 }
 
 template <typename T, int DP, bool WHOLE, int ROWS>
-__global__ __launch_bounds__(64 * pages_many_waves(DP, ROWS), pages_many_waves(DP, ROWS) / 2) void pages_attention_many_kernel(PagesAttentionArgs a) {
+__global__ __launch_bounds__(64 * pages_many_waves(sizeof(T), DP, ROWS), pages_many_to_a_simd(sizeof(T), DP, ROWS)) void pages_attention_many_kernel(PagesAttentionArgs a) {
   using P = Pages<T, DP>;
   using M = PagesMany<T, DP, ROWS>;
   constexpr int QT = M::kSixteens, SPLIT = M::kSplit;
-  constexpr int kDims = P::kDims, kTogether = P::kTogether, kKeyPieces = P::kKeyPieces, kTile = M::kTile, kEights = M::kEights, kParts = 2 / SPLIT;
+  constexpr int kDims = P::kDims, kTogether = P::kTogether, kKeyPieces = P::kKeyPieces, kTile = M::kTile, kEights = M::kEights, kParts = 2 / SPLIT, kWidth = M::kWidth;
   __shared__ struct {
     union {
       typename M::Shared tile;
@@ -577,7 +580,7 @@ __global__ __launch_bounds__(64 * pages_many_waves(DP, ROWS), pages_many_waves(D
   const int wave = any_wave % M::kGroups, half = any_wave / M::kGroups;   // of the rows, of the positions
   CacheTile x;
   if(!cache_tile<T, DP, ROWS, M::kWaves, kPagesMostParts>(a, tid, x)) return;
-  const int end = x.end, row_bytes = (WHOLE ? DP : a.dk) * 2;
+  const int end = x.end, row_bytes = (WHOLE ? DP : a.dk) * kWidth;
   const int* const table = a.table + (long long)x.w.s * a.row;
   const unsigned char* const k_head = a.k_pages + x.head * a.head_bytes;
   const unsigned char* const v_head = a.v_pages + x.head * a.head_bytes;
@@ -585,8 +588,9 @@ __global__ __launch_bounds__(64 * pages_many_waves(DP, ROWS), pages_many_waves(D
 
   // ---- what a wave lays out: the eights of a tile from kEights * any_wave on
   struct Fetched {
-    cache_u4 key[M::kKeyLoads];
-    unsigned value[8][M::kValueWords];
+    cache_u4 key[M::kRowLoads];
+    unsigned value[8][M::kValueWords];   // 16-bit types: some dimensions of an eight ...
+    cache_u4 value_row[M::kRowLoads];    // ... float32: pieces as of keys
     bool there[kEights];
     PagesPlace next[kEights];   // of the tile that is fetched next
   } fetched;
@@ -604,11 +608,14 @@ __global__ __launch_bounds__(64 * pages_many_waves(DP, ROWS), pages_many_waves(D
       place[i] = f.there[i] ? y.id * a.page_bytes + (long long)(8 * y.eight) * row_bytes : 0;
     }
 #pragma unroll
-    for(int i = 0; i < M::kKeyLoads; ++i) {   // (rows past one eight are of the next)
+    for(int i = 0; i < M::kRowLoads; ++i) {   // (rows past one eight are of the next)
       constexpr int kAtOnce = 64 / M::kRowPieces;
       const int row = kAtOnce * i + lane / M::kRowPieces, piece = lane % M::kRowPieces * 16;
-      f.key[i] = *reinterpret_cast<const cache_u4*>(k_head + place[kAtOnce * i / 8] + (row & 7) * row_bytes + (piece < row_bytes ? piece : 0));
+      const long long from = place[kAtOnce * i / 8] + (row & 7) * row_bytes + (piece < row_bytes ? piece : 0);
+      f.key[i] = *reinterpret_cast<const cache_u4*>(k_head + from);
+      if(kWidth == 4) f.value_row[i] = *reinterpret_cast<const cache_u4*>(v_head + from);
     }
+    if constexpr(kWidth == 4) return;
     const int d = lane % M::kLanes * M::kDimsEach * 2;
     const unsigned char* const from = v_head + (lane < M::kLanes ? place[0] : place[kEights - 1]) + (d < row_bytes ? d : 0);
 #pragma unroll
@@ -619,10 +626,26 @@ __global__ __launch_bounds__(64 * pages_many_waves(DP, ROWS), pages_many_waves(D
   auto lay_out = [&](Fetched& f, int at, int buffer) __attribute__((always_inline)) {
     constexpr int kAtOnce = 64 / M::kRowPieces;
 #pragma unroll
-    for(int i = 0; i < M::kKeyLoads; ++i) {
+    for(int i = 0; i < M::kRowLoads; ++i) {
       const int row = 8 * kEights * any_wave + kAtOnce * i + lane / M::kRowPieces, piece = lane % M::kRowPieces;
       if(!WHOLE) f.key[i] = piece * 16 < row_bytes ? f.key[i] : cache_u4{0, 0, 0, 0};   // (queries are zero there, and so must these be)
       *reinterpret_cast<cache_u4*>(sh.tile.keys[buffer] + M::key_place(row, piece)) = f.key[i];
+      if constexpr(kWidth == 4) {
+        if(at + kTile > x.open || !f.there[0]) {   // (as below)
+          const bool seen = f.there[0] && at + row < end;
+#pragma unroll
+          for(int w = 0; w < 4; ++w) {
+            const unsigned z = seen ? f.value_row[i][w] : 0, clean = at + row < x.open ? z : pages_finite<T>(z);
+            if(z != clean) sh.tile.left_out = 1;
+            f.value_row[i][w] = clean;
+          }
+        }
+        *reinterpret_cast<cache_u4*>(sh.tile.values[buffer] + (row * M::kRowPieces + piece) * 16) = f.value_row[i];
+      }
+    }
+    if constexpr(kWidth == 4) {
+      if(lane == 0) sh.tile.there[buffer][any_wave] = f.there[0];
+      return;
     }
     const int eight = kEights * any_wave + lane / M::kLanes, first = at + 8 * eight;
     const bool is = lane < M::kLanes ? f.there[0] : f.there[kEights - 1];
@@ -744,22 +767,44 @@ __global__ __launch_bounds__(64 * pages_many_waves(DP, ROWS), pages_many_waves(D
       }
     }
     // (the second half's weights are made while the first half's products run)
+    if constexpr(kWidth == 4) {
 #pragma unroll
-    for(int h = 0; h < kParts; ++h) {
-      cache_u4 weights[QT][2];
+      for(int h = 0; h < kParts; ++h) {
+        float p[8];
+        const float from = top[0] == kNone ? 0.0f : -top[0];
 #pragma unroll
-      for(int t = 0; t < QT; ++t) {
-        const cache_f4 mine[2] = {s[t][2 * h], s[t][2 * h + 1]};
-        pages_weights<T>(mine, a.scale_log2, (top[t] == kNone ? 0.0f : -top[t]) + P::kUp, sum[t], weights[t]);
+        for(int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][2 * h + e / 4][e % 4], a.scale_log2, from)) * (1.0f / P::kUnit);
+          sum[0] += p[e];
+        }
+#pragma unroll
+        for(int i = 0; i < P::kValuePieces; ++i)
+#pragma unroll
+          for(int e = 0; e < 8; ++e) {
+            const cache_f4 v = *reinterpret_cast<const cache_f4*>(sh.tile.values[buffer] + ((32 * (half + h) + 8 * g + e) * M::kRowPieces + 16 * i + c) * 16);
+#pragma unroll
+            for(int j = 0; j < kTogether; ++j)
+              o[0][i * kTogether + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j], p[e], o[0][i * kTogether + j], 0, 0, 0);
+          }
       }
+    } else {
 #pragma unroll
-      for(int j = 0; j < kDims; ++j) {
-        const int dim = (16 * (j / kTogether) + c) * kTogether + j % kTogether;
-        const cache_u4 v = *reinterpret_cast<const cache_u4*>(sh.tile.values[buffer] + M::value_place(dim, 4 * (half + h) + g));
+      for(int h = 0; h < kParts; ++h) {
+        cache_u4 weights[QT][2];
 #pragma unroll
-        for(int t = 0; t < QT; ++t)
+        for(int t = 0; t < QT; ++t) {
+          const cache_f4 mine[2] = {s[t][2 * h], s[t][2 * h + 1]};
+          pages_weights<T>(mine, a.scale_log2, (top[t] == kNone ? 0.0f : -top[t]) + P::kUp, sum[t], weights[t]);
+        }
 #pragma unroll
-          for(int m = 1; m >= 0; --m) o[t][j] = pages_product<T>(v, weights[t][m], o[t][j]);
+        for(int j = 0; j < kDims; ++j) {
+          const int dim = (16 * (j / kTogether) + c) * kTogether + j % kTogether;
+          const cache_u4 v = *reinterpret_cast<const cache_u4*>(sh.tile.values[buffer] + M::value_place(dim, 4 * (half + h) + g));
+#pragma unroll
+          for(int t = 0; t < QT; ++t)
+#pragma unroll
+            for(int m = 1; m >= 0; --m) o[t][j] = pages_product<T>(v, weights[t][m], o[t][j]);
+        }
       }
     }
     if(at + kTile < end) lay_out(fetched, at + kTile, buffer ^ 1);
@@ -820,7 +865,8 @@ __global__ __launch_bounds__(64 * pages_many_waves(DP, ROWS), pages_many_waves(D
 #pragma unroll
         for(int j = 0; j < kRun; ++j) y[j] = r[t][i * kRun + j][e] * factor;
         if(d < a.dk) {
-          if constexpr(kRun == 2) *reinterpret_cast<unsigned*>(to + d) = pack2<T>(y[0], y[1]);
+          if constexpr(kRun == 2 && kWidth == 4) *reinterpret_cast<cache_u2*>(to + d) = cache_u2{__builtin_bit_cast(unsigned, y[0]), __builtin_bit_cast(unsigned, y[1])};
+          else if constexpr(kRun == 2) *reinterpret_cast<unsigned*>(to + d) = pack2<T>(y[0], y[1]);
           else store_row<kRun, T>(to + d, y);
         }
       }

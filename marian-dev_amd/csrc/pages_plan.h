@@ -21,9 +21,13 @@ constexpr unsigned kPagesMostParts = 64;
 
 // Sixteens of query rows that a wave takes over the same positions, at the most.
 constexpr int pages_most_qt(int width, int dp) { return width == 4 && dp == 256 ? 1 : 2; }
-// Whether rows past that have a form in which waves with rows of their own share positions in LDS, for 64 or 128 rows.
-constexpr bool pages_has_many(int width, int dp) { return width == 2 && dp <= 128; }
-constexpr int pages_many_waves(int dp, int rows) { return dp == 128 && rows == 128 ? 4 : 8; }
+// Whether rows past that have a form in which waves with rows of their own share positions in LDS, for 64 or 128 rows.  float32 without and with it: 7
+// tokens of 24 sequences of up to 8192 positions, 4 heads with eight rows each, 128 values 268 and 220 us, 64 values 118 and 117; 9 of 11 of
+// up to 64, 16 heads with four rows, 128 values 24 and 18; 256 of 4 of up to 512, 16 heads, 64 values 39 and 48.
+constexpr bool pages_has_many(int width, int dp) { return dp == 128 || (width == 2 && dp == 64); }
+constexpr int pages_many_waves(int width, int dp, int rows) { return width == 2 && dp == 128 && rows == 128 ? 4 : 8; }
+// (a workgroup of float32, 128 values, has 128 KB of LDS)
+constexpr int pages_many_to_a_simd(int width, int dp, int rows) { return width == 4 && dp == 128 ? 2 : pages_many_waves(width, dp, rows) / 2; }
 
 // Positions up to which a sequence is short: eight turns of a wave.
 constexpr int64_t kPagesShort = 256;
@@ -65,14 +69,14 @@ inline PagesAttentionPlan pages_attention_plan(int64_t sequences, int64_t heads,
   // and 34 us; 182 of up to 192, 16 of 80, float32 96 and 82; 250 of up to 60, 8 of 128 with four rows each, bfloat16 24 and 15; but in room for
   // 512, 128 of up to 512, 16 of 64, float32 74 and 84.
   const bool one = entries >= 1024 * form || (entries >= 256 * form && capacity <= kPagesShort);
-  p.waves = p.many ? pages_many_waves(p.dp, p.tile_rows) : one ? 1 : 4;
+  p.waves = p.many ? pages_many_waves(width, p.dp, p.tile_rows) : one ? 1 : 4;
   // Parts for one round of the workgroups that run at a time, by the registers of their form, half a part for each sequence left out.  Of 16-bit values
   // half of them have the memory as busy, and leave fewer parts to join: where that makes two parts of a sequence.  One token, 8 heads with four
   // rows each, 128 values, all and half, over ten sets of lengths: 100003 positions 80.2 and 77.6 us, 4 sequences of up to 16000 44.2 and 42.0, 8
   // 75.1 and 72.4, but 16 of up to 32768 264 and 291; 4 drafted tokens, 4 heads with eight rows each, 16 of up to 16384 81.3 and 77.2, 40 of up to
   // 8192 96.9 and 101.  Not where rows leave many lanes without a load (80 values, 16 of up to 8192: 51.8 and 57.0), nor of float32 (64 values,
   // 16384: 83.4 and 88.2), nor of the form that shares positions in LDS (7 tokens, 24 of up to 8192: 75 and 108).
-  const int to_a_simd = p.many ? p.waves / 2 : form;
+  const int to_a_simd = p.many ? pages_many_to_a_simd(width, p.dp, p.tile_rows) : form;
   // Many sequences leave few parts or none, and one of them may still have most of the positions: half of the parts there are anyway, where a row of
   // the table has room for that to show.  8 heads of 128 values with four rows each, 128 sequences, one of 4096 positions and the others of
   // 80: 55 and 22 us, all of up to 4096 269 and 269; but 200 of up to 700 76 and 79, by the look at all lengths.

@@ -127,8 +127,8 @@ def AttentionOverPages(q, cache, table, lens, counts=None, scale=None, out=None)
     row]; scale None: 1 / sqrt(dk).  A token sees the lens[s] positions before the new ones, itself and the new tokens before it.  Rows of
     the table may share pages; positions of pages that are none (-1), or past the row, are not seen, and a token that sees nothing gives zeros, as do
     rows at or past counts[s].  The last bits of a result depend on the batch's lengths and the table's width.  Made for few rows a head of keys
-    (n times the heads that share it): 128 of them read the pages once (16-bit types with dk up to 128), 32, or 16 (float32 with dk past 128).
-    The output lies in memory as q does."""
+    (n times the heads that share it): 128 of them read the pages once, or 32 (float32 with dk up to
+    64, 16-bit types with dk past 128), or 16 (float32 with dk past 128).  The output lies in memory as q does."""
     res = _host.pages_attention(q, cache, table, lens, counts, scale, out)
     if res is not None:
         return res

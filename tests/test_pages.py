@@ -224,7 +224,7 @@ def test_the_shapes_that_are_tested_launch_every_form(tmp_path):
         got.add((width, dp, dk == dp, many, tile // 64 if many else qt, 4 if many else waves))
     want = {(w, dp, whole, 0, qt, waves) for w in (2, 4) for dp in (64, 128, 256) for whole in (True, False) for qt in (1, 2) for waves in (1, 4)
             if not (w == 4 and dp == 256 and qt == 2)}
-    want |= {(2, dp, whole, 1, qt, 4) for dp in (64, 128) for whole in (True, False) for qt in (1, 2)}
+    want |= {(w, dp, whole, 1, qt, 4) for w, dp in ((2, 64), (2, 128), (4, 128)) for whole in (True, False) for qt in (1, 2)}
     assert got == want
 
 
