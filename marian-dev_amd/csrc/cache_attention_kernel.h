@@ -280,8 +280,9 @@ __device__ __forceinline__ T* cache_row_out(const CacheAttentionArgs& a, const C
   return static_cast<T*>(a.out) + x.w.s * a.o_s + (long long)(x.head * a.G + (int)of_group) * a.o_h + (long long)token * a.o_n;
 }
 
-// Finds a workgroup's tile and clears the rows of it that are not there; false where nothing is to be done.
-template <typename T, int DP, int ROWS, int WAVES, unsigned MOST = kCacheMostParts>
+// Finds a workgroup's tile and clears the rows of it that are not there; false where nothing is to be done.  LAST_FIRST: the last rows, which see
+// the most positions, go first.
+template <typename T, int DP, int ROWS, int WAVES, unsigned MOST = kCacheMostParts, bool LAST_FIRST = false>
 __device__ __forceinline__ bool cache_tile(const CacheAttentionArgs& a, int tid, CacheTile& x) {
   constexpr int kDims = DP / 16;
   // Workgroups with the same positions follow each other on one XCD (a workgroup to each of the eight in turn).
@@ -289,7 +290,7 @@ __device__ __forceinline__ bool cache_tile(const CacheAttentionArgs& a, int tid,
   const int entry = (int)a.by_tiles.of(blockIdx.x >> 3, tile) * 8 + (blockIdx.x & 7);
   if(entry >= a.items * a.Hk) return false;
   const int item = (int)a.by_heads.of((unsigned)entry, head);
-  x.tile = (int)tile;
+  x.tile = LAST_FIRST ? a.row_tiles - 1 - (int)tile : (int)tile;
   x.head = (int)head;
   if(!cache_part<MOST>(a, item, tid & 63, x.w)) return false;
   x.rows = x.w.count * a.G;

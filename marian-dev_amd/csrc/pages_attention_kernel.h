@@ -291,7 +291,7 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
   const int tid = threadIdx.x, lane = tid & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   CacheTile x;
-  if(!cache_tile<T, DP, 16 * QT, WAVES, kPagesMostParts>(a, tid, x)) return;
+  if(!cache_tile<T, DP, 16 * QT, WAVES, kPagesMostParts, true>(a, tid, x)) return;
   const int end = x.end, row_bytes = (WHOLE ? DP : a.dk) * kWidth;
   // A sequence of one turn of one wave is that wave's: no join, and the others make room (236 of three positions, 16 heads of 64 values, 11 us and 20).
   const bool alone = WAVES == 1 || (x.w.parts == 1 && end - x.w.from <= 32);
@@ -509,7 +509,7 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
 // to registers.  64 rows are taken by eight waves of sixteen, four of them for the first 32 positions of each 64 and four for the second.  128
 // rows are taken by eight waves too where rows have 64 values, by four of 32 where they have 128: LDS is read half as often then, and that
 // counts by the length of rows (512 new tokens of 4 sequences, 16 heads of 64 values, 42 us by eight and 45 by four; 1024 of them, 32 heads on
-// 8, 128 values, 200 and 187).
+// 8, 128 values, 200 and 187).  The last rows go first: a prompt of 4096 tokens, 32 heads on 8, 128 values 262 us and 290, 525 TFLOP/s of what they see.
 // Keys lie in LDS as they are, values transposed, a dimension's 64 side by side; pieces of 16 bytes change places within a row (key_place,
 // value_place) so that few lanes that read together meet in a bank (a third of the cycles that LDS is busy).  A wave lays out one or two eights
 // of positions: sixteen lanes (of rows of 128 bytes eight) to a row of keys; of values a lane has some dimensions of eight positions.
@@ -579,7 +579,7 @@ __global__ __launch_bounds__(64 * pages_many_waves(sizeof(T), DP, ROWS), pages_m
   const int tid = threadIdx.x, lane = tid & 63, any_wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   const int wave = any_wave % M::kGroups, half = any_wave / M::kGroups;   // of the rows, of the positions
   CacheTile x;
-  if(!cache_tile<T, DP, ROWS, M::kWaves, kPagesMostParts>(a, tid, x)) return;
+  if(!cache_tile<T, DP, ROWS, M::kWaves, kPagesMostParts, true>(a, tid, x)) return;
   const int end = x.end, row_bytes = (WHOLE ? DP : a.dk) * kWidth;
   const int* const table = a.table + (long long)x.w.s * a.row;
   const unsigned char* const k_head = a.k_pages + x.head * a.head_bytes;
