@@ -542,9 +542,10 @@ int marian_hip_pages_write(const marian_hip_pages* cache, const void* k, const i
  *   out = softmax(scale * q . key) value
  * over the lens[s] positions before the new tokens, the token itself and the new ones before it.  table: int32 [sequences, row]; rows may share
  * pages.  Positions of a page that is none (below 0, or at or past `pages`), and past the row, are not seen.  What a token does not see is
- * not read into its result, infinities and NaN included; an infinity among the values that it sees is its result (NaN if there are both, or
- * if its weight is below 2^-126 of the largest, and NaN if there is one).  A token that sees nothing, or whose scores are all minus infinity,
- * gives zeros, and so do rows at or past counts[s] (counts: null, or int32 [sequences]).  out shares no memory with anything else.
+ * not read into its result, infinities and NaN included; an infinity among the values that it sees is its result, whatever its weight, also where its
+ * score is minus infinity (NaN if there are both, or one; a score that is plus infinity or NaN makes the row NaN).  A token that sees nothing, or whose
+ * scores are all minus infinity, gives zeros but for that, and so do rows at or past counts[s] (counts: null, or int32 [sequences]).  out shares no
+ * memory with anything else.
  * scale: finite, above zero.
  * Products and sums are float32; weights enter the product with the values with 16 bits (bfloat16), 22 (float16) or 24, their sum in float32.
  * Values (bfloat16 and float32) below 2^-100 lose bits to the scale of the weights.

@@ -429,8 +429,16 @@ struct CacheParts {
 constexpr float kPartUnit = 1.0f / 64;
 static_assert(kPartUnit * kCacheMostParts <= 1.0f, "the parts' weights add up to one at the most");
 
-// The parts of a sequence: the workgroup that arrives last joins them, in their order.
-template <typename T, int DP, int ROWS, int WAVES>
+// A weighted value, and a sum of them, in which infinities and NaN count whatever their weight, zero included.
+__device__ __forceinline__ bool is_odd(float z) { return !(__builtin_fabsf(z) < __builtin_huge_valf()); }
+__device__ __forceinline__ float times_odd(float z, float weight) { return weight == 0.0f && is_odd(z) ? z : z * weight; }
+__device__ __forceinline__ float add_odd(float y, float weight, float z) {
+  return weight == 0.0f && is_odd(z) ? y + z : __builtin_fmaf(weight, z, y);
+}
+
+// The parts of a sequence: the workgroup that arrives last joins them, in their order.  ODD: an infinity or NaN among a part's results is the
+// result, whatever the part weighs; sums that are none are made once more for it.
+template <typename T, int DP, int ROWS, int WAVES, bool ODD = false>
 __device__ __forceinline__ void cache_join_parts(const CacheAttentionArgs& a, const CacheTile& x, const CacheOut<T, DP, ROWS>& out,
                                                  CacheParts<DP, WAVES>& sh) {
   using Out = CacheOut<T, DP, ROWS>;
@@ -480,6 +488,27 @@ __device__ __forceinline__ void cache_join_parts(const CacheAttentionArgs& a, co
         for(int j = 0; j < kDims; ++j) y[j] = __builtin_fmaf(weight, z[b][j / 4][j % 4], y[j]);
       }
     }
+    float none = 0.0f;
+    if constexpr(ODD) {
+#pragma unroll
+      for(int j = 0; j < kDims; ++j) none += y[j] * 0.0f;
+    }
+    if(ODD && __builtin_expect(!(none == 0.0f), 0)) {
+      float again[kDims] = {};
+#pragma unroll 1
+      for(int i = group % share; i < x.w.parts; i += share) {
+        const unsigned at = 4u * stride * (unsigned)i;
+        const float log = from.number_through(at + my_log), weight = log == kNone ? 0.0f : __builtin_amdgcn_exp2f(log - m) * kPartUnit;
+#pragma unroll
+        for(int j = 0; j < kDims / 4; ++j) {
+          const cache_f4 z = from.piece_through(at + mine + 16u * j);
+#pragma unroll
+          for(int e = 0; e < 4; ++e) again[4 * j + e] = add_odd(again[4 * j + e], weight, z[e]);
+        }
+      }
+#pragma unroll
+      for(int j = 0; j < kDims; ++j) y[j] = is_odd(y[j]) ? again[j] : y[j];
+    }
     if(share > 1) {   // (r is the only row of all threads: sixteens beyond the rows have left)
       float* const rest = &sh.rest[group][(tid & 15) * kDims];
 #pragma unroll
@@ -490,7 +519,7 @@ __device__ __forceinline__ void cache_join_parts(const CacheAttentionArgs& a, co
       }
     }
     if(share == 1 && d_mine < a.dk) {
-      const float per = total == 0.0f ? 0.0f : 1.0f / total;
+      const float per = total == 0.0f ? ODD : 1.0f / total;   // (without weights: zeros, infinities and NaN)
 #pragma unroll
       for(int j = 0; j < kDims; ++j) y[j] *= per;
       store_row<kDims, T>(cache_row_out<T>(a, x, x.row0 + r) + d_mine, y);
@@ -509,7 +538,23 @@ __device__ __forceinline__ void cache_join_parts(const CacheAttentionArgs& a, co
 #pragma unroll
     for(int j = 0; j < kDims; ++j) y[j] = __builtin_fmaf(rest[j], weight, y[j]);
   }
-  const float per = total == 0.0f ? 0.0f : 1.0f / total;
+  float none = 0.0f;
+  if constexpr(ODD) {
+#pragma unroll
+    for(int j = 0; j < kDims; ++j) none += y[j] * 0.0f;
+  }
+  if(ODD && __builtin_expect(!(none == 0.0f), 0)) {
+    float again[kDims] = {};
+#pragma unroll 1
+    for(int i = 0; i < share; ++i) {
+      const float from = sh.top[group + i], weight = from == kNone ? 0.0f : __builtin_amdgcn_exp2f(from - m);
+#pragma unroll
+      for(int j = 0; j < kDims; ++j) again[j] = add_odd(again[j], weight, sh.rest[group + i][(tid & 15) * kDims + j]);
+    }
+#pragma unroll
+    for(int j = 0; j < kDims; ++j) y[j] = is_odd(y[j]) ? again[j] : y[j];
+  }
+  const float per = total == 0.0f ? ODD : 1.0f / total;
 #pragma unroll
   for(int j = 0; j < kDims; ++j) y[j] *= per;
   store_row<kDims, T>(cache_row_out<T>(a, x, x.row0 + r) + d_mine, y);

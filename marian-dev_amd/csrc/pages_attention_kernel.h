@@ -124,7 +124,7 @@ __device__ __forceinline__ void pages_write(const CacheOut<T, DP, 16 * QT>& out,
   using P = Pages<T, DP>;
 #pragma unroll
   for(int t = 0; t < QT; ++t) {
-    const float factor = sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * P::kUnit;
+    const float factor = sum[t] == 0.0f ? 1.0f : 1.0f / sum[t] * P::kUnit;   // (without weights: zeros, infinities and NaN)
 #pragma unroll
     for(int i = 0; i < P::kValuePieces; ++i)
 #pragma unroll
@@ -138,10 +138,11 @@ __device__ __forceinline__ void pages_write(const CacheOut<T, DP, 16 * QT>& out,
   }
 }
 
-// The results of waves that share rows, joined and written; alone: one wave has all of them, and the others have ended.
+// The results of waves that share rows, joined and written; alone: one wave has all of them, and the others have ended; odd: the wave has infinities
+// or NaN among them.
 template <typename T, int DP, int QT, int WAVES>
-__device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const CacheTile& x, const cache_f4 (&o)[QT][DP / 16], const float (&top)[QT],
-                                             float (&sum)[QT], int wave, bool alone, CacheJoin<DP, QT, WAVES>& sh) {
+__device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const CacheTile& x, cache_f4 (&o)[QT][DP / 16], const float (&top)[QT],
+                                             float (&sum)[QT], int wave, bool alone, bool odd, CacheJoin<DP, QT, WAVES>& sh) {
   using P = Pages<T, DP>;
   constexpr int kTogether = P::kTogether, kHalf = CacheJoin<DP, QT, WAVES>::kHalf, kPieces = kHalf / (16 * kTogether);
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
@@ -170,7 +171,14 @@ __device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const 
       float m = sh.row_max[0][16 * t + c];
 #pragma unroll
       for(int i = 1; i < WAVES; ++i) m = fmaxf(m, sh.row_max[i][16 * t + c]);
-      const float mine = top[t] == kNone ? 0.0f : __builtin_amdgcn_exp2f(top[t] - m) * over;
+      float mine = top[t] == kNone ? 0.0f : __builtin_amdgcn_exp2f(top[t] - m) * over;
+      if(__builtin_expect(odd, 0)) {
+#pragma unroll
+        for(int j = 0; j < DP / 16; ++j)
+#pragma unroll
+          for(int e = 0; e < 4; ++e) o[t][j][e] = times_odd(o[t][j][e], mine);
+        mine = 1.0f;
+      }
 #pragma unroll
       for(int h = 0; h < DP / kHalf; ++h) {
         if(h || t) __syncthreads();
@@ -197,7 +205,7 @@ __device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const 
             const float from = sh.row_max[i][16 * t + r];   // (of a wave that saw nothing the sum is 0, or NaN)
             total += sh.row_sum[i][16 * t + r] * (from == kNone ? 1.0f : __builtin_amdgcn_exp2f(from - top_r));
           }
-          const float per = total == 0.0f ? 0.0f : 1.0f / total * back;
+          const float per = total == 0.0f ? 1.0f : 1.0f / total * back;
 #pragma unroll
           for(int j = 0; j < kEach; ++j) {
             y[j] = sh.joined[0][r][d + j];
@@ -218,14 +226,16 @@ __device__ __forceinline__ void pages_finish(const PagesAttentionArgs& a, const 
       }
     }
   }
-  if(!out.whole) cache_join_parts<T, DP, 16 * QT, WAVES>(a, x, out, sh.parts);
+  if(!out.whole) cache_join_parts<T, DP, 16 * QT, WAVES, true>(a, x, out, sh.parts);
 }
 
 // Infinities and NaN among values: a result that sees one is that, of whatever weight, and the sum of them where there are several.  The product
 // does not give that - a weight is in two terms, one of which may be zero or below it -, and what a row does not see must not be in
-// it.  So where the wave left some out, or has a result that is none, it looks at its positions once more: `eights` of them, `step` apart.
+// it.  So where the wave left some out, or has a result that is none, it looks at its positions once more: `eights` of them, `step` apart.  Where
+// waves, halves and parts are joined, times_odd and add_odd have them outlive a weight that is zero there: a result does not depend on where
+// positions come to lie.  Returns whether it looked.
 template <typename T, int DP, int QT>
-__device__ __forceinline__ void pages_odd_values(const PagesAttentionArgs& a, const int* table, const unsigned char* v_head, int row_bytes, int begin, int end,
+__device__ __forceinline__ bool pages_odd_values(const PagesAttentionArgs& a, const int* table, const unsigned char* v_head, int row_bytes, int begin, int end,
                                                  int eights, int step, int lane, bool left_out, const CacheSight (&sight)[QT], cache_f4 (&o)[QT][DP / 16]) {
   constexpr int kTogether = Pages<T, DP>::kTogether, kBits = (DP / 4 + 31) / 32;
   float none = 0.0f;   // NaN where a result is none
@@ -235,7 +245,7 @@ __device__ __forceinline__ void pages_odd_values(const PagesAttentionArgs& a, co
     for(int j = 0; j < DP / 16; ++j)
 #pragma unroll
       for(int e = 0; e < 4; ++e) none += o[t][j][e] * 0.0f;
-  if(!left_out && !__any(!(none == 0.0f))) return;
+  if(!left_out && !__any(!(none == 0.0f))) return false;
   const int g = lane >> 4;
   unsigned has[QT][kBits] = {};   // results that have seen one
 #pragma unroll 1
@@ -278,6 +288,7 @@ __device__ __forceinline__ void pages_odd_values(const PagesAttentionArgs& a, co
           }
       }
     }
+  return true;
 }
 
 template <typename T, int DP, bool WHOLE, int QT, int WAVES>
@@ -505,8 +516,8 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
     k_next = look_keys(at + 2 * kTurn);
     v_next = look_values(at + 2 * kTurn);
   }
-  pages_odd_values<T, DP, QT>(a, table, v_head, row_bytes, begin, end, 4, kTurn, lane, left_out, sight, o);
-  pages_finish<T, DP, QT, WAVES>(a, x, o, top, sum, wave, alone, sh);
+  const bool odd = pages_odd_values<T, DP, QT>(a, table, v_head, row_bytes, begin, end, 4, kTurn, lane, left_out, sight, o);
+  pages_finish<T, DP, QT, WAVES>(a, x, o, top, sum, wave, alone, odd, sh);
 }
 
 // ---- more than 32 rows
@@ -827,6 +838,14 @@ __global__ __launch_bounds__(64 * pages_many_waves(sizeof(T), DP, ROWS), pages_m
   constexpr int kOwn = kDims / SPLIT;
   const int shift = half * kOwn;
   cache_f4 r[QT][kOwn];
+  auto none_of = [](const cache_f4 (&y)[kOwn]) {   // whether one of these is an infinity or NaN
+    float none = 0.0f;
+#pragma unroll
+    for(int j = 0; j < kOwn; ++j)
+#pragma unroll
+      for(int e = 0; e < 4; ++e) none += y[j][e] * 0.0f;
+    return !(none == 0.0f);
+  };
   if constexpr(SPLIT == 1) {
 #pragma unroll
     for(int t = 0; t < QT; ++t)
@@ -853,6 +872,14 @@ __global__ __launch_bounds__(64 * pages_many_waves(sizeof(T), DP, ROWS), pages_m
 #pragma unroll
       for(int e = 0; e < 4; ++e) r[0][j][e] = (half == 0 ? y[0][e] : y[1][e]) * mine + z[e];
     }
+    if(__builtin_expect(none_of(r[0]), 0)) {
+#pragma unroll
+      for(int j = 0; j < kOwn; ++j) {
+        const cache_f4 z = sh.half.o[1 - half][wave][j][lane];
+#pragma unroll
+        for(int e = 0; e < 4; ++e) r[0][j][e] = times_odd(half == 0 ? o[0][j][e] : o[0][kOwn + j][e], mine) + times_odd(z[e], its);
+      }
+    }
     sum[0] = sum[0] * mine + sh.half.sum[1 - half][wave][lane] * its;
     top[0] = m;
   }
@@ -878,7 +905,7 @@ __global__ __launch_bounds__(64 * pages_many_waves(sizeof(T), DP, ROWS), pages_m
   };
   if(out.whole) {
 #pragma unroll
-    for(int t = 0; t < QT; ++t) write(t, sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * P::kUnit);
+    for(int t = 0; t < QT; ++t) write(t, sum[t] == 0.0f ? 1.0f : 1.0f / sum[t] * P::kUnit);   // (without weights: zeros, infinities and NaN)
     return;
   }
   constexpr unsigned kTileBytes = CacheOut<T, DP, ROWS>::kTileFloats * 4;
@@ -886,7 +913,7 @@ __global__ __launch_bounds__(64 * pages_many_waves(sizeof(T), DP, ROWS), pages_m
   const CacheBuffer parts(a.part + out.place * CacheOut<T, DP, ROWS>::kTileFloats, stride * x.w.parts);
 #pragma unroll
   for(int t = 0; t < QT; ++t) {
-    const float factor = sum[t] == 0.0f ? 0.0f : 1.0f / sum[t] * P::kUnit;
+    const float factor = sum[t] == 0.0f ? 1.0f : 1.0f / sum[t] * P::kUnit;
     const unsigned to = stride * x.w.part;
 #pragma unroll
     for(int j = 0; j < kOwn; ++j) parts.store_through(r[t][j] * factor, to + mine + 1024u * (t * kDims + j));
@@ -914,6 +941,8 @@ __global__ __launch_bounds__(64 * pages_many_waves(sizeof(T), DP, ROWS), pages_m
 #pragma unroll
       for(int t = 0; t < QT; ++t) top[t] = i + b < x.w.parts ? fmaxf(top[t], l[t][b]) : top[t];
   }
+  // (a part's weight is at most 1, times kPartUnit: sums stay within the largest value)
+  auto weight_of = [](float l, float high) { return l == kNone ? 0.0f : __builtin_amdgcn_exp2f(l - high) * kPartUnit; };
 #pragma unroll 1
   for(int i = 0; i < x.w.parts; i += kBatch) {
     float l[QT][kBatch];
@@ -933,8 +962,7 @@ __global__ __launch_bounds__(64 * pages_many_waves(sizeof(T), DP, ROWS), pages_m
       if(i + b >= x.w.parts) break;
 #pragma unroll
       for(int t = 0; t < QT; ++t) {
-        // (a part's weight is at most 1, times kPartUnit: sums stay within the largest value)
-        const float weight = l[t][b] == kNone ? 0.0f : __builtin_amdgcn_exp2f(l[t][b] - top[t]) * kPartUnit;
+        const float weight = weight_of(l[t][b], top[t]);
         weight_sum[t] += weight;
 #pragma unroll
         for(int j = 0; j < kOwn; ++j)
@@ -944,7 +972,24 @@ __global__ __launch_bounds__(64 * pages_many_waves(sizeof(T), DP, ROWS), pages_m
     }
   }
 #pragma unroll
-  for(int t = 0; t < QT; ++t) write(t, weight_sum[t] == 0.0f ? 0.0f : 1.0f / weight_sum[t]);
+  for(int t = 0; t < QT; ++t) {
+    if(__builtin_expect(none_of(r[t]), 0)) {
+#pragma unroll
+      for(int j = 0; j < kOwn; ++j) r[t][j] = cache_f4{0, 0, 0, 0};
+#pragma unroll 1
+      for(int i = 0; i < x.w.parts; ++i) {
+        const unsigned at = stride * (unsigned)i;
+        const float weight = weight_of(parts.number_through(at + my_log + 64u * t), top[t]);
+#pragma unroll
+        for(int j = 0; j < kOwn; ++j) {
+          const cache_f4 z = parts.piece_through(at + mine + 1024u * (t * kDims + j));
+#pragma unroll
+          for(int e = 0; e < 4; ++e) r[t][j][e] = add_odd(r[t][j][e], weight, z[e]);
+        }
+      }
+    }
+    write(t, weight_sum[t] == 0.0f ? 1.0f : 1.0f / weight_sum[t]);
+  }
 }
 
 }  // namespace marian_hip
