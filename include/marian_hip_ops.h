@@ -515,7 +515,8 @@ typedef struct marian_hip_page_tables {
  * sequence gets the pages that it lacks up to position lens[s] + counts[s], in the sequences' order from the top of the stack.  A sequence that the free
  * pages do not reach for, or whose row of the table is too short, gets none; so does every later one that lacks some, in the first case.
  *   slots: int32 [sequences, n]: where token i of sequence s lies, page number * page + place in it; -1 for tokens that are not
- *   there or have no page (and so the sign of a sequence that got none).
+ *   there or have no page.  A sequence's tokens that have a slot come first: how many these are is what the rest of the step takes as counts, so that
+ *   no length grows past what is written.
  * Lengths below 0 are taken as 0, counts into 0 .. n, held into 0 .. row, free_count into 0 .. pages.
  * Replays of a recorded call go on from what the table holds then.
  */

@@ -9,16 +9,18 @@ a step needs no synchronisation, and may be recorded into a graph.  There is no 
 
 One step of a decoder, n tokens a sequence (a prompt, one token, or a chain of drafted ones behind the last):
     slots = reservePages(tables, lens, n, pageSize)
+    counts = (slots >= 0).sum(1, dtype=torch.int32)     # the tokens that have a place: fewer than n, or none, where the free pages do not reach
     for layer, cache in zip(layers, caches):     # (all layers have the same pages)
         q, k, v = layer.project(x)
         q, k = rotaryPositions(q, lens, rotary), rotaryPositions(k, lens, rotary)
         writePages(cache, k, v, slots)
-        x = layer.finish(AttentionOverPages(q, cache, tables.table, lens))
-    path, accepted, nextTokens = verifyDrafts(tokens, target(x), random, draft)      # (cache.py; one token: accepted is 1)
+        x = layer.finish(AttentionOverPages(q, cache, tables.table, lens, counts))
+    path, accepted, nextTokens = verifyDrafts(tokens, target(x), random, draft, counts=counts)     # (cache.py; of a prompt, all counts are accepted)
     lens = lens + accepted
     trimPages(tables, lens, pageSize)     # the refused drafts' pages; with lens 0 those of a sequence that is done
-Accepted tokens of a chain lie where they are to stay.  A sequence whose slots are -1 found no free pages: what it writes is dropped, and
-its step has to be repeated when others are done.
+Accepted tokens of a chain lie where they are to stay.  Where slots are -1 a sequence found no free pages, and its length must not grow past the
+tokens that have a place: with counts as above these are all that is written, seen and verified.  A sequence without any stays where it is
+(accepted is 0, its next token -1), and its step is repeated when others are done.
 """
 from typing import NamedTuple
 
