@@ -499,7 +499,8 @@ typedef struct marian_hip_pages {
  *   table: int32 [sequences, row]: the pages of a sequence in the order of its positions, -1 behind them;
  *   held: int32 [sequences]: how many these are;
  *   free: int32 [pages]: a stack of the pages that nobody has, its first free_count[0] entries.
- * sequences <= 65535, row * sequences < 2^31.  A page belongs to one sequence; sequences that share one may read it only.
+ * sequences <= 65535, row * sequences < 2^31.  A page belongs to one sequence; sequences that share one may read it only: one that two of them hold
+ * would go back twice, and be dealt twice.
  * Calls on the same tables follow each other: on one stream, and of several threads one at a time (a call may be two launches).
  */
 typedef struct marian_hip_page_tables {
@@ -525,7 +526,8 @@ int marian_hip_pages_reserve(const marian_hip_page_tables* tables, const int32_t
 
 /*
  * Gives the pages behind lens[s] positions back, of every sequence (lens[s] = 0: all of them): what a refused draft or a finished
- * sequence leaves.  Undoes a marian_hip_pages_reserve with the same lens, the order of the stack included.
+ * sequence leaves.  Undoes a marian_hip_pages_reserve with the same lens, the order of the stack included, where no sequence held pages behind its lens
+ * before.
  */
 int marian_hip_pages_trim(const marian_hip_page_tables* tables, const int32_t* lens, int64_t page, void* stream);
 

@@ -21,6 +21,11 @@ One step of a decoder, n tokens a sequence (a prompt, one token, or a chain of d
 Accepted tokens of a chain lie where they are to stay.  Where slots are -1 a sequence found no free pages, and its length must not grow past the
 tokens that have a place: with counts as above these are all that is written, seen and verified.  A sequence without any stays where it is
 (accepted is 0, its next token -1), and its step is repeated when others are done.
+
+A page belongs to one sequence.  Rows of a table may be copied to read the same pages - hypotheses of a beam that begin alike, say - but
+only one of them may be reserved for, written to or trimmed: trimPages would put the pages of each on the stack, and they would be dealt twice.  There is
+no move or copy of pages: a beam search whose hypotheses take each other's place has its cache in cache.py, or copies rows itself.  Chains of tokens only: trees
+of drafts are for cache.py, too.
 """
 from typing import NamedTuple
 
@@ -101,7 +106,8 @@ def reservePages(tables, lens, n, pageSize, counts=None):
 
 
 def trimPages(tables, lens, pageSize):
-    """Takes back the pages that lie behind the sequences' lens (0: all of a sequence's).  With the lens of a reservePages it undoes that."""
+    """Takes back the pages that lie behind the sequences' lens (0: all of a sequence's).  With the lens of a reservePages it undoes that, if no
+    sequence held pages behind its lens before.  No page may be in two sequences' rows (their held pages): it would be dealt twice."""
     if _host.pages_trim(tables, lens, pageSize) is None:
         what = "trimPages"
         tables = _tables(tables, what)
