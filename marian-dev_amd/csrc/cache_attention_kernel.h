@@ -280,9 +280,9 @@ __device__ __forceinline__ T* cache_row_out(const CacheAttentionArgs& a, const C
   return static_cast<T*>(a.out) + x.w.s * a.o_s + (long long)(x.head * a.G + (int)of_group) * a.o_h + (long long)token * a.o_n;
 }
 
-// Finds a workgroup's tile and clears the rows of it that are not there; false where nothing is to be done.  LAST_FIRST: the last rows, which see
-// the most positions, go first.
-template <typename T, int DP, int ROWS, int WAVES, unsigned MOST = kCacheMostParts, bool LAST_FIRST = false>
+// Finds a workgroup's tile and clears the rows of it that are not there; false where nothing is to be done.  PAGES: an entry's keys and values have no
+// place of their own, and the last rows, which see the most positions, go first.
+template <typename T, int DP, int ROWS, int WAVES, unsigned MOST = kCacheMostParts, bool PAGES = false>
 __device__ __forceinline__ bool cache_tile(const CacheAttentionArgs& a, int tid, CacheTile& x) {
   constexpr int kDims = DP / 16;
   // Workgroups with the same positions follow each other on one XCD (a workgroup to each of the eight in turn).
@@ -290,7 +290,7 @@ __device__ __forceinline__ bool cache_tile(const CacheAttentionArgs& a, int tid,
   const int entry = (int)a.by_tiles.of(blockIdx.x >> 3, tile) * 8 + (blockIdx.x & 7);
   if(entry >= a.items * a.Hk) return false;
   const int item = (int)a.by_heads.of((unsigned)entry, head);
-  x.tile = LAST_FIRST ? a.row_tiles - 1 - (int)tile : (int)tile;
+  x.tile = PAGES ? a.row_tiles - 1 - (int)tile : (int)tile;
   x.head = (int)head;
   if(!cache_part<MOST>(a, item, tid & 63, x.w)) return false;
   x.rows = x.w.count * a.G;
@@ -306,11 +306,13 @@ __device__ __forceinline__ bool cache_tile(const CacheAttentionArgs& a, int tid,
   const int last_token = (int)a.by_group.of((unsigned)min(x.rows - 1, x.row0 + ROWS - 1));
   x.end = min(x.w.to, x.w.len + last_token + 1);
   x.open = min(x.end, x.w.len + (a.parents ? 0 : (int)a.by_group.of((unsigned)x.row0) + 1));
-  const long long first = ((long long)x.w.s * a.Hk + x.head) * a.cap;
-  x.k = a.k + first * a.dk;
-  x.v = a.v + first * a.dk;
-  x.ks = a.ks + first;
-  x.vs = a.vs + first;
+  if constexpr(!PAGES) {
+    const long long first = ((long long)x.w.s * a.Hk + x.head) * a.cap;
+    x.k = a.k + first * a.dk;
+    x.v = a.v + first * a.dk;
+    x.ks = a.ks + first;
+    x.vs = a.vs + first;
+  }
   return true;
 }
 
