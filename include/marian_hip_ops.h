@@ -518,7 +518,7 @@ typedef struct marian_hip_page_tables {
  *   slots: int32 [sequences, n]: where token i of sequence s lies, page number * page + place in it; -1 for tokens that are not
  *   there or have no page.  A sequence's tokens that have a slot come first: how many these are is what the rest of the step takes as counts, so that
  *   no length grows past what is written.
- * Lengths below 0 are taken as 0, counts into 0 .. n, held into 0 .. row, free_count into 0 .. pages.
+ * Lengths below 0 are taken as 0, counts into 0 .. n, held into 0 .. row, free_count into 0 .. pages.  n up to 2^20, sequences * n < 2^31.
  * Replays of a recorded call go on from what the table holds then.
  */
 int marian_hip_pages_reserve(const marian_hip_page_tables* tables, const int32_t* lens, const int32_t* counts, int64_t n, int64_t page,
@@ -534,7 +534,7 @@ int marian_hip_pages_trim(const marian_hip_page_tables* tables, const int32_t* l
 /*
  * Writes keys and values of n tokens a sequence, [sequences, heads, n, dk] of the cache's type by strides (as for
  * marian_hip_cache_append), to their slots: int32 [sequences, n]; a slot below 0 or past the last page writes nothing.  No two tokens of a call
- * have the same slot.  n up to 2^20.
+ * have the same slot.  n up to 2^20, sequences * n * heads rows of less than 2^36 bytes in all.
  */
 int marian_hip_pages_write(const marian_hip_pages* cache, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
                            int64_t sequences, int64_t n, const int32_t* slots, void* stream);
@@ -554,8 +554,12 @@ int marian_hip_pages_write(const marian_hip_pages* cache, const void* k, const i
  * Values (bfloat16 and float32) below 2^-100 lose bits to the scale of the weights.
  * The last bits of a result depend on the batch's lengths and the table's width, which say how positions are split over workgroups, and not on
  * the order of anything.  Made for few rows a head of keys, n * q_heads / heads: keys and values are read once for every 128 of them (up to 128
- * values a row, float32 more than 64), 32 (float32 up to 64 values, 16-bit types past 128), or 16 (float32 past 128).
- * lens outside 0 .. row * page are taken as the nearer end.  row * page < 2^30; n up to 2^20.
+ * values a row, float32 more than 64), 32 (float32 up to 64 values, 16-bit types past 128), or 16 (float32 past 128).  A long sequence is
+ * split over workgroups in calls of up to 1024 sequences, and the less so the more new tokens a call has room for: a long one among more sequences, or
+ * beside a prompt, is better given a call of its own.
+ * lens outside 0 .. row * page are taken as the nearer end.  sequences <= 65535, row * page < 2^30, sequences * row < 2^31, n up to 2^20,
+ * q_heads / heads <= 4096, n * q_heads / heads <= 2^26, and sequences * heads times the workgroups that share an entry's rows (one to 16, 32, 64 or
+ * 128 of them) less than 2^23.
  *   workspace: at least marian_hip_pages_attention_workspace_bytes(...) bytes, cleared once by marian_hip_cache_attention_workspace_init; as for
  *   marian_hip_cache_attention, whose workspace serves this call too where it is large enough.
  */

@@ -25,7 +25,7 @@ struct VerifyArgs {
 };
 
 // Eight waves: a sequence's workgroups judge its tokens each, ahead of all else, and a workgroup's words are summed in 64 bits, five operations a
-// word. With 4, 8 and 16 of them 32000 words of one sequence take 5.7, 6.3 and 9.1 us, 131071 words of 64 sequences 44.0, 20.2 and 22.0.
+// word. With 4, 8 and 16 of them 32000 words of one sequence took 5.7, 6.3 and 9.1 us, 131071 words of 64 sequences 44.0, 20.2 and 22.0.
 constexpr int kVerifyWaves = 8, kVerifyThreads = 64 * kVerifyWaves;
 constexpr int kShare = 2 * kVerifyThreads;                 // words of a wave ...
 constexpr int kVerifyPart = kVerifyWaves * kShare;         // ... and of a workgroup
@@ -189,7 +189,7 @@ __device__ __forceinline__ double share_sum(VerifyShared& sh, double x) {
 // to each wave.  The last workgroup of a sequence finds the share in which the drawn number lies, and the word in it.  All sums are in 64
 // bits and in an order of their own, whoever comes last.
 // The kept tokens cost nothing but their own probabilities, so what moves is one row of the target's, and one of the draft's where a
-// token was refused.  64 sequences, 131071 words, float32: 20.2 us, 3.3 TB/s; their bytes take 13 us, the judgement ahead of them and the join
+// token was refused.  64 sequences, 131071 words, float32: 18.5 us, 3.6 TB/s; their bytes take 13 us, the judgement ahead of them and the join
 // behind them the rest.  32000 words of one sequence: 6.3 us, a chain of some nine steps through memory.
 template <typename T>
 __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a, int first) {

@@ -21,9 +21,9 @@
 // leaves: 16 and 22 bits.  Their sum is of the float32 ones.  They are scaled by a power of two: bfloat16 and float32 2^-24, so that sums over
 // 2^20 positions of values next to the largest stay in range; float16 2^11, so that weights down to 2^-25 of the largest keep their bits.
 //
-// What bounds it: the memory.  One token of 128 sequences of up to 512 positions, 16 heads of 64 values, float32 (360 MB): 72 to 75 us, 4.9 TB/s; of 16
-// sequences of up to 32768, 8 heads of 128 values with four rows each, bfloat16 (1.4 GB): 264 us, 5.4 TB/s; one sequence of 100003 (410 MB) 78
-// us, 5.3 TB/s.  Where there is little to read, 6 sequences of up to 120 positions: 6.0 us, a workgroup's start, three dependent loads (length,
+// What bounds it: the memory.  One token of 128 sequences of up to 512 positions, 16 heads of 64 values, float32 (360 MB): 71 to 72 us, 5.0 TB/s; of 16
+// sequences of up to 32768, 8 heads of 128 values with four rows each, bfloat16 (1.4 GB): 257 to 264 us, 5.4 TB/s; one sequence of 100003 (410 MB) 75
+// us, 5.4 TB/s.  Where there is little to read, 6 sequences of up to 120 positions: 5.9 us, a workgroup's start, three dependent loads (length,
 // page, keys and values) and its end.
 #pragma once
 
@@ -525,7 +525,7 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
 // to registers.  64 rows are taken by eight waves of sixteen, four of them for the first 32 positions of each 64 and four for the second.  128
 // rows are taken by eight waves too where rows have 64 values, by four of 32 where they have 128: LDS is read half as often then, and that
 // counts by the length of rows (512 new tokens of 4 sequences, 16 heads of 64 values, 42 us by eight and 45 by four; 1024 of them, 32 heads on
-// 8, 128 values, 200 and 187).  The last rows go first: a prompt of 4096 tokens, 32 heads on 8, 128 values 262 us and 290, 525 TFLOP/s of what they see.
+// 8, 128 values, 200 and 187).  The last rows go first: a prompt of 4096 tokens, 32 heads on 8, 128 values 262 us and 290; now 225 us, 610 TFLOP/s of what they see.
 // Keys lie in LDS as they are, values transposed, a dimension's 64 side by side; pieces of 16 bytes change places within a row (key_place,
 // value_place) so that few lanes that read together meet in a bank (a third of the cycles that LDS is busy).  A wave lays out one or two eights
 // of positions: sixteen lanes (of rows of 128 bytes eight) to a row of keys; of values a lane has some dimensions of eight positions.
@@ -534,8 +534,8 @@ __global__ __launch_bounds__(64 * WAVES, pages_to_a_simd(sizeof(T), DP, QT)) voi
 //
 // What bounds it: latency, of the memory's answers and of the partial results' way to the workgroup that joins them; LDS is busy less than a third of
 // the time and the matrix units a fifth.  7 drafted tokens, float16, 24 sequences of up to 8192 positions, 4 heads of 128 values with eight
-// rows each (56 rows, 270 MB): 67 to 73 us, 3.9 TB/s; four waves that take all positions and join them 80, waves of the form above with a row
-// group each 95.  bfloat16, 64 values, 8 tokens, 16 sequences: 37 and 39.6.  float32, the 56 rows above: 220 us,
+// rows each (56 rows, 270 MB): 65 to 71 us, 3.9 TB/s; four waves that take all positions and join them 80, waves of the form above with a row
+// group each 95.  bfloat16, 64 values, 8 tokens, 16 sequences: 35, by four waves 39.6.  float32, the 56 rows above: 217 us,
 // of which the matrix products alone take 110 (17 GFLOP).  __syncthreads in place of the barrier below waits for the loads too.
 template <typename T, int DP, int ROWS>
 struct PagesMany {

@@ -9,7 +9,9 @@
 
 namespace marian_hip {
 
-// Registers of a form (an estimate).
+// Registers of a form (an estimate).  Of float32 rows of 65 to 127 values, up to sixteen rows, it is nine too low, and as many go to memory ahead of the
+// loop; with one wave to a SIMD none do: one token, 16 sequences of up to 2000 positions, 16 heads of 80 values 74.1 us so and 78.3, of up to 8192, 8 of
+// 112 with four rows each 140.4 and 138.1.
 constexpr int pages_registers(int width, int dp, int qt) {
   const int words = width * dp / 8;   // of keys and of values, each: 32 positions' bytes over 64 lanes
   return 2 * words + qt * (dp / 4 + words / 2 + 16) + 48;   // results, queries, scores and weights; addresses
@@ -29,8 +31,10 @@ constexpr int pages_many_waves(int width, int dp, int rows) { return width == 2 
 // (a workgroup of float32, 128 values, has 128 KB of LDS)
 constexpr int pages_many_to_a_simd(int width, int dp, int rows) { return width == 4 && dp == 128 ? 2 : pages_many_waves(width, dp, rows) / 2; }
 
-// Positions up to which a sequence is short: eight turns of a wave.
+// Positions up to which a sequence is short: eight turns of a wave.  (Where rows of the table have no room for more, sequences are not split: so one wave
+// to an entry, which leaves room for more parts, never needs a larger workspace than what is asked for without knowing the rows.)
 constexpr int64_t kPagesShort = 256;
+static_assert(kPagesShort <= (int64_t)kCacheWhole * kCacheBlock, "short sequences have one part");
 // Positions up to which sequences are taken to differ little.
 constexpr int64_t kPagesEven = 1024;
 
@@ -65,9 +69,9 @@ inline PagesAttentionPlan pages_attention_plan(int64_t sequences, int64_t heads,
   const int64_t entries = sequences * heads * p.row_tiles;
   const int form = pages_to_a_simd(width, p.dp, p.qt);
   // One wave to an entry where the entries fill the card with that, or in four rounds and are short for certain: four waves of which most find no
-  // position cost a start and a join for it.  One token, four waves and one: 241 sequences of one position, 16 heads of 256 values, float16 103
-  // and 34 us; 182 of up to 192, 16 of 80, float32 96 and 82; 250 of up to 60, 8 of 128 with four rows each, bfloat16 24 and 15; but in room for
-  // 512, 128 of up to 512, 16 of 64, float32 74 and 84.
+  // position cost a start and a join for it.  One token, four waves - of which three end at once where positions are 32 at the most - and one:
+  // 241 sequences of two positions, 16 heads of 256 values, float16 102 and 30 us; 182 of up to 192, 16 of 80, float32 97 and 82; 250 of up to 60, 8
+  // of 128 with four rows each, bfloat16 19.8 and 12.4; but in room for 512, 128 of up to 512, 16 of 64, float32 74 and 84.
   const bool one = entries >= 1024 * form || (entries >= 256 * form && capacity <= kPagesShort);
   p.waves = p.many ? pages_many_waves(width, p.dp, p.tile_rows) : one ? 1 : 4;
   // Parts for one round of the workgroups that run at a time, by the registers of their form, half a part for each sequence left out.  Of 16-bit values
@@ -88,7 +92,9 @@ inline PagesAttentionPlan pages_attention_plan(int64_t sequences, int64_t heads,
   p.target = width == 2 && !p.many && to_a_simd > 1 && 4 * dk > 3 * p.dp && half >= 2 * sequences ? half : all;
   // A sequence of up to four blocks stays whole, and where no row of the table has room for more nobody looks at the others' lengths (6 sequences
   // of up to 120 positions, 8 heads of 64 values, float32: 6.7 and 6.0 us).  Nor where these are many: their parts would be few, and a look at them
-  // costs every workgroup a load for 64 of them.
+  // costs every workgroup a load for 64 of them (8 heads of 128 values with four rows each, all of 80 positions: 1024 sequences 95 us, 1025 72).  That is
+  // wrong where one of many is long (one of 32768: 173 us, and 1729), and so is row_tiles where only one sequence has many new tokens: in a
+  // batch with a prompt of 4096 tokens no sequence has parts (16 sequences, one token behind 80 positions 301 us, of one of them behind 32768 1538).
   if(capacity <= kCacheWhole * kCacheBlock || sequences > 1024) p.target = 1;
   p.least = entries <= 32 ? 2 : 4;
   p.items = p.target == 1 ? sequences : p.target + sequences;

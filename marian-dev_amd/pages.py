@@ -136,7 +136,9 @@ def AttentionOverPages(q, cache, table, lens, counts=None, scale=None, out=None)
     the table may share pages; positions of pages that are none (-1), or past the row, are not seen, and a token that sees nothing gives zeros, as do
     rows at or past counts[s].  The last bits of a result depend on the batch's lengths and the table's width.  Made for few rows a head of keys
     (n times the heads that share it): 128 of them read the pages once, or 32 (float32 with dk up to
-    64, 16-bit types with dk past 128), or 16 (float32 with dk past 128).  The output lies in memory as q does."""
+    64, 16-bit types with dk past 128), or 16 (float32 with dk past 128).  A long sequence among more than 1024, or beside a prompt in the
+    same call, is not split over the card: it is better given a call of its own.  An infinity among the values that a token sees is its result,
+    whatever its weight.  The output lies in memory as q does."""
     res = _host.pages_attention(q, cache, table, lens, counts, scale, out)
     if res is not None:
         return res
