@@ -9,8 +9,8 @@
 
 namespace marian_hip {
 
-// Registers of a form (an estimate).  Of float32 rows of 65 to 127 values, up to sixteen rows, it is nine too low, and as many go to memory ahead of the
-// loop; with one wave to a SIMD none do: one token, 16 sequences of up to 2000 positions, 16 heads of 80 values 74.1 us so and 78.3, of up to 8192, 8 of
+// Registers of a form (an estimate).  Of float32 rows of 65 to 127 values, up to sixteen rows, it is nine too low, and as many go to memory;
+// with one wave to a SIMD none do: one token, 16 sequences of up to 2000 positions, 16 heads of 80 values 74.1 us so and 78.3, of up to 8192, 8 of
 // 112 with four rows each 140.4 and 138.1.
 constexpr int pages_registers(int width, int dp, int qt) {
   const int words = width * dp / 8;   // of keys and of values, each: 32 positions' bytes over 64 lanes
